@@ -251,6 +251,68 @@ size_t mgq_argmax_workspace(void);
 int mgq_argmax(const float *logits, uint32_t n, void *workspace, uint32_t *out_token, uint32_t *next_token, uint32_t *kv_pos,
                uint32_t *history, uint32_t history_cap, void *stream);
 
+/* ---- many sequences over one cache (no reference counterpart: the reference serves one sequence per session).
+ *
+ * A layer's cache is k[pages][page_size][kv_heads][head_dim] and v likewise, page_size a power of two from 8 to 1024.  Sequence s holds
+ * held[s] pages, named in order by its row of the block table, table[s * table_width + j]; token i of it lies in page
+ * table[s][i / page_size] at place i % page_size, so that its slot, the row of the cache seen as [pages * page_size][kv_heads * head_dim],
+ * is page * page_size + place.  All layers share one table.  Pages that nobody holds are a stack: free_pages[0 .. *free_count), the top last.
+ * A step takes new tokens of many sequences, packed: rows [starts[s], starts[s + 1]) are sequence s's, the last of its lengths[s] tokens.
+ * All lengths live in device memory, so a step is a fixed launch sequence that can be captured in a CUDA graph and replayed.
+ * Words that are out of range are never followed: rows behind `rows` and lengths behind the table are cut off, a page that is not
+ * below `pages` holds no tokens, a slot that is not below pages * page_size is not written.
+ *
+ * mgq_paged_plan: from cached[s] (tokens in the cache) and fresh[s] (new ones) the step's starts[sequences + 1] and lengths, and for
+ *   each of `rows` rows its position (cached + place among the new tokens) and slot; rows behind the last sequence get
+ *   position 0 and slot MGQ_NO_SLOT.  Sequences that hold too few pages take them from the stack in order (table, held and *free_count are
+ *   updated).  A sequence gets all that it needs or none: if the stack does not reach for it and those before it that need pages, or its
+ *   table row is too narrow, its slots are MGQ_NO_SLOT and its length stays cached[s].  *lacking: pages that the stack was short of.
+ * mgq_paged_trim: pages beyond the first lengths[s] tokens return to the stack, and their table entries become MGQ_NO_PAGE: 0 ends a
+ *   sequence, the kept length takes back rejected drafts, the lengths before a plan undo it (the stack is then as before).
+ * mgq_paged_append: rows of k and v into the cache rows slots[r] (MGQ_NO_SLOT: not written), with theta > 0 k rotated by positions[r]
+ *   (half-split pairs, angle = position * theta^(-2i/head_dim) in 64 bits), and rows of q likewise into q_out [rows, q_heads * head_dim]
+ *   (q may be NULL: keys and values only).  Sources are f32 or of the cache's type; their rows are `pitch` elements apart.  Values
+ *   are rounded to nearest.  Slots must differ from one another, else which row stays is open.
+ * mgq_paged_attention: each new token's query heads over the tokens of its sequence up to itself, with window > 0 over the last
+ *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  What a row does not
+ *   see has no part in it, whatever it holds; a row that sees nothing is zero; rows behind the last sequence are left as they are.  max_fresh: no sequence has more
+ *   new tokens in this step (it chooses kernels; more are not computed).  head_dim at most 256.  `workspace`: mgq_paged_attention_workspace(...) bytes for
+ *   the same arguments, 16-byte aligned, in any state; calls that may run at the same time (two streams, two graphs) need one each.
+ * All need table_width * page_size and the number of rows below 2^31, and at most MGQ_PAGED_MAX_SEQUENCES sequences. */
+#define MGQ_NO_SLOT  0xFFFFFFFFu
+#define MGQ_NO_PAGE  0xFFFFFFFFu
+#define MGQ_NO_TOKEN 0xFFFFFFFFu
+#define MGQ_PAGED_MAX_SEQUENCES 4096
+#define MGQ_PAGED_MAX_HEAD 256
+int mgq_paged_plan(const uint32_t *cached, const uint32_t *fresh, uint32_t sequences, uint32_t page_size, uint32_t *table, uint32_t table_width, uint32_t *held,
+                   const uint32_t *free_pages, uint32_t pages, uint32_t *free_count, uint32_t rows, uint32_t *starts, uint32_t *lengths, uint32_t *positions,
+                   uint32_t *slots, uint32_t *lacking, void *stream);
+int mgq_paged_trim(const uint32_t *lengths, uint32_t sequences, uint32_t page_size, uint32_t *table, uint32_t table_width, uint32_t *held, uint32_t *free_pages,
+                   uint32_t pages, uint32_t *free_count, void *stream);
+int mgq_paged_append(const void *q, const void *k, const void *v, int src_dtype, const uint32_t *positions, const uint32_t *slots, void *q_out, void *k_cache,
+                     void *v_cache, int cache_dtype, uint32_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_pitch, uint32_t k_pitch,
+                     uint32_t v_pitch, uint32_t page_size, uint32_t pages, float theta, void *stream);
+size_t mgq_paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh, int dtype);
+int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
+                        void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,
+                        uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
+
+/* mgq_token_probs: out[r, :] = softmax(logits[r, :] / temperature[r]); a temperature that is not above 0 gives 1 to the lowest index among the
+ *   largest logits (temperature NULL: 1 everywhere).  NaN logits count as -inf; a row of them alone is zero.  Where the largest is +inf those that are share the row.
+ * mgq_verify_drafts: speculative sampling.  Sequence s fed its last token and then its drafts: rows [starts[s], starts[s + 1]), tokens[r] the
+ *   token of row r.  target[r, :] are the target's probabilities behind row r, draft[r, :] those that tokens[r + 1] was drawn from (the
+ *   last row of a sequence is not read), or draft NULL where drafts were chosen outright.  Draft by draft, tokens[r + 1] is kept while
+ *   accept[r] * draft[r, it] < target[r, it] (draft NULL: accept[r] < target[r, it]); accepted[s] counts them.  Then next[s] is drawn: behind a draft
+ *   that is not kept from max(target - draft, 0) (draft NULL: from target without it; where nothing is left from target), behind the
+ *   last one from target: the lowest index at which the running sum exceeds sample[s] times the whole.  out[r] has the kept tokens, then next,
+ *   then MGQ_NO_TOKEN.  Sums are in 64 bits; entries that are negative, infinite or NaN count as 0; rows need not sum to 1.  next is MGQ_NO_TOKEN where target has no mass, and
+ *   for a sequence without rows.  A sequence of one row has no drafts: its next token is sampled.
+ * Rows are `pitch` elements apart; all values f32. */
+int mgq_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream);
+int mgq_verify_drafts(const float *target, uint32_t target_pitch, const float *draft, uint32_t draft_pitch, const uint32_t *tokens, const uint32_t *starts,
+                      const float *accept, const float *sample, uint32_t *accepted, uint32_t *next, uint32_t *out, uint32_t sequences, uint32_t rows, uint32_t vocab,
+                      void *stream);
+
 /* Routing wrapper.  f32 activations with m <= MGQ_GEMV_MAX_M go to mgq_gemv, unless that would need more passes over the
  * weights than mgq_gemm takes time: from 5 rows on (8 or 12 for few columns) where k % 256 != 0, from 9 rows on for large
  * Q8 weights, and where no streaming kernel takes the shape (k < 256, k > 32768, Q8 with k / 32 odd and above 256, packed

@@ -77,6 +77,14 @@ SIGNATURES = {
     "mgq_cached_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp]),
     "mgq_argmax_workspace": (_sz, []),
     "mgq_argmax": (_int, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _vp]),
+    "mgq_paged_plan": (_int, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mgq_paged_trim": (_int, [_vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _vp]),
+    "mgq_paged_append": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, ctypes.c_float, _vp]),
+    "mgq_paged_attention_workspace": (_sz, [_u32, _u32, _u32, _u32, _int]),
+    "mgq_paged_attention": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, ctypes.c_float, _u32,
+                                   _vp, _vp]),
+    "mgq_token_probs": (_int, [_vp, _u32, _vp, _vp, _u32, _u32, _u32, _vp]),
+    "mgq_verify_drafts": (_int, [_vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
     "mgq_gemv_exchange": (_int, [_int, _vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp]),
     "mgq_exchange_finish": (_int, [_vp, _u32, _vp, _vp, _vp, _vp]),
     "mgq_exchange_all_gather": (_int, [_vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _vp]),

@@ -1,0 +1,231 @@
+// Attention of new tokens over a paged cache, any types and sizes: the form that the others stand beside, and the one for f32.
+#include <cstdint>
+
+#include "mgq_paged.cuh"
+
+namespace mgq {
+namespace {
+
+constexpr int kThreads = 128, kWarps = 4;
+constexpr int kRows = 16, kKeys = 32;                    // pairs of token and head, keys of a block
+constexpr int kRowsPerWarp = kRows / kWarps;
+
+// out[row, col] (+)= over a tile of 32 keys: a warp scores four rows with a key per lane, a thread sums one or two columns for all rows.
+template <typename T, int COLS>                          // COLS: columns per thread, heads of up to 128 * COLS
+__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
+{
+    extern __shared__ __align__(16) float s_mem[];
+    __shared__ unsigned long long s_walk[40];
+    __shared__ float s_p[kRows][kKeys], s_scale[kRows];
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, d = a.d, d4 = (d + 3) / 4 * 4, pitch = d4 + 4;
+    float *s_q = s_mem, *s_k = s_q + kRows * d4, *s_v = s_k + kKeys * pitch;
+    pdl_launch_dependents();
+    pdl_wait();
+    Walk<kRows, kKeys> walk(a);
+    walk.begin(blockIdx.x, gridDim.x, 1, s_walk);
+    if (t == 0) clear_parts(a, blockIdx.x);
+
+    Segment g;
+    while (walk.next(g)) {
+        const uint32_t pairs = g.tokens * g.heads;
+        __syncthreads();
+        for (uint32_t i = t; i < kRows * d4; i += kThreads) {
+            const uint32_t r = i / d4, c = i - r * d4, token = r / g.heads, head = r - token * g.heads;
+            s_q[i] = r < pairs && c < d ? to_f32(static_cast<const T *>(a.q)[(size_t)(g.row0 + token) * a.q_pitch + (g.head0 + head) * d + c]) : 0.f;
+        }
+        float m[kRowsPerWarp], l[kRowsPerWarp], acc[COLS][kRows];
+        int pos[kRowsPerWarp];
+#pragma unroll
+        for (int i = 0; i < kRowsPerWarp; i++) {
+            const uint32_t r = warp * kRowsPerWarp + i;
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+            pos[i] = r < pairs ? g.pos0 + (int)(r / g.heads) : -1;
+        }
+#pragma unroll
+        for (int c = 0; c < COLS; c++)
+#pragma unroll
+            for (int r = 0; r < kRows; r++) acc[c][r] = 0.f;
+
+        for (uint32_t kb = g.begin; kb < g.end; kb++) {
+            __syncthreads();                             // the tile before has been used
+            for (uint32_t i = t; i < kKeys * d4; i += kThreads) {
+                const uint32_t j = i / d4, c = i - j * d4, key = kb * kKeys + j;
+                float kv = 0.f, vv = 0.f;
+                if ((int)key < g.len && c < d) {
+                    const uint32_t page = g.table[key >> a.page_shift];
+                    if (page < a.pages) {
+                        const size_t at = (((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads * d + (size_t)g.kv * d + c;
+                        kv = to_f32(static_cast<const T *>(a.k)[at]);
+                        vv = to_f32(static_cast<const T *>(a.v)[at]);
+                    }
+                }
+                s_k[j * pitch + c] = kv;
+                s_v[j * pitch + c] = vv;
+            }
+            __syncthreads();
+            const int key = (int)(kb * kKeys + lane);
+            const bool there = key < g.len && g.table[(uint32_t)key >> a.page_shift] < a.pages;
+            float s[kRowsPerWarp];
+#pragma unroll
+            for (int i = 0; i < kRowsPerWarp; i++) s[i] = 0.f;
+            for (uint32_t c = 0; c < d4; c += 4) {
+                const float4 kv = *reinterpret_cast<const float4 *>(s_k + lane * pitch + c);
+#pragma unroll
+                for (int i = 0; i < kRowsPerWarp; i++) {
+                    const float4 qv = *reinterpret_cast<const float4 *>(s_q + (warp * kRowsPerWarp + i) * d4 + c);
+                    s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[i]))));
+                }
+            }
+            bool hidden = false;                         // some pair of this tile is masked
+#pragma unroll
+            for (int i = 0; i < kRowsPerWarp; i++) {
+                const bool seen = there && key <= pos[i] && (!a.window || key > pos[i] - (int)a.window);
+                hidden |= !seen;
+                const float x = seen ? s[i] * a.scale_log2 : -INFINITY, top = fmaxf(m[i], warp_max(x));
+                // a row whose seen scores are all -inf has no weight, like one that sees nothing; NaN stays NaN
+                const float w = !seen ? 0.f : x != x ? x : top > -INFINITY ? exp2f(x - top) : 0.f, keep = top > -INFINITY ? exp2f(m[i] - top) : 1.f;
+                l[i] = l[i] * keep + warp_sum(w);
+                m[i] = top;
+                s_p[warp * kRowsPerWarp + i][lane] = w;
+                if (lane == 0) s_scale[warp * kRowsPerWarp + i] = keep;
+            }
+            const bool masked = __syncthreads_or(hidden);
+#pragma unroll
+            for (int c = 0; c < COLS; c++) {
+                const uint32_t col = t + c * kThreads;
+                if (col >= d) continue;
+#pragma unroll
+                for (int r = 0; r < kRows; r++) acc[c][r] *= s_scale[r];
+                for (int j = 0; j < kKeys; j += 4) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = s_v[(j + e) * pitch + col];
+#pragma unroll
+                    for (int r = 0; r < kRows; r++) {
+                        const float4 p = *reinterpret_cast<const float4 *>(&s_p[r][j]);
+                        if (masked) {                    // what a row does not see stays out, infinities and NaN too
+                            acc[c][r] += (p.x != 0.f ? p.x * v[0] : 0.f) + (p.y != 0.f ? p.y * v[1] : 0.f) + (p.z != 0.f ? p.z * v[2] : 0.f) + (p.w != 0.f ? p.w * v[3] : 0.f);
+                        } else {
+                            acc[c][r] = fmaf(p.x, v[0], fmaf(p.y, v[1], fmaf(p.z, v[2], fmaf(p.w, v[3], acc[c][r]))));
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = g.first && g.last;
+        if (whole) {
+            if (lane == 0)
+#pragma unroll
+                for (int i = 0; i < kRowsPerWarp; i++) s_scale[warp * kRowsPerWarp + i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+            __syncthreads();
+        }
+        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kRows * (d + 2);
+#pragma unroll
+        for (int c = 0; c < COLS; c++) {
+            const uint32_t col = t + c * kThreads;
+            if (col >= d) continue;
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; r++) {
+                if (r >= pairs) break;
+                const uint32_t token = r / g.heads, head = r - token * g.heads;
+                if (whole) static_cast<T *>(a.out)[(size_t)(g.row0 + token) * a.out_pitch + (g.head0 + head) * d + col] = rounded<T>(acc[c][r] * s_scale[r]);
+                else       part[r * (d + 2) + col] = acc[c][r];
+            }
+        }
+        if (!whole) {
+            if (lane == 0)
+#pragma unroll
+                for (int i = 0; i < kRowsPerWarp; i++) {
+                    part[(warp * kRowsPerWarp + i) * (d + 2) + d] = m[i];
+                    part[(warp * kRowsPerWarp + i) * (d + 2) + d + 1] = l[i];
+                }
+            if (t == 0) name_part(a, blockIdx.x, g);
+        }
+    }
+}
+
+// Joins the parts of the unit that CTA blockIdx.x of the attention kernel began and did not end: with M the largest of the parts' maxima
+// o = sum 2^(m - M) o_part / sum 2^(m - M) l_part.  The parts are those of the CTAs that follow, up to the one that ends the
+// unit, added in this order.
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(128) merge_kernel(const AttendArgs a, uint32_t ctas)
+{
+    __shared__ uint32_t s_end;
+    const uint32_t t = threadIdx.x, c0 = blockIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
+    const PartHead h = a.heads[2 * c0 + 1];
+    if (h.state != kOpens) return;
+    if (t == 0) s_end = ctas;
+    __syncthreads();
+    for (uint32_t c = c0 + 1 + t; c < ctas; c += 128)
+        if (a.heads[2 * c].state == kCloses) {
+            atomicMin(&s_end, c);
+            break;
+        }
+    __syncthreads();
+    const uint32_t end = min(s_end, ctas - 1), d = a.d, step = d + 2;          // the part that closes
+    auto part = [&](uint32_t c) { return a.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS * step; };
+    for (uint32_t r = blockIdx.y; r < h.tokens * h.heads; r += gridDim.y) {
+        float top = -INFINITY, l = 0.f;
+        for (uint32_t c = c0; c <= end; c++) top = fmaxf(top, part(c)[r * step + d]);
+        auto weight = [&](uint32_t c) { return part(c)[r * step + d + 1] != 0.f ? exp2f(part(c)[r * step + d] - top) : 0.f; };    // a NaN is a weight
+        for (uint32_t c = c0; c <= end; c++) l += weight(c) * part(c)[r * step + d + 1];
+        const float scale = l == 0.f ? 0.f : 1.f / l;
+        const uint32_t token = r / h.heads, head = r - token * h.heads;
+        for (uint32_t col = t; col < d; col += 128) {
+            float o = 0.f;
+            for (uint32_t c = c0; c <= end; c++) o += weight(c) * part(c)[r * step + col];
+            static_cast<T *>(a.out)[(size_t)(h.row0 + token) * a.out_pitch + (h.head0 + head) * d + col] = rounded<T>(o * scale);
+        }
+    }
+}
+
+constexpr uint32_t kCtas = 148 * 3;
+
+template <typename T>
+int launch_attend(AttendArgs a, cudaStream_t stream)
+{
+    const uint32_t d4 = (a.d + 3) / 4 * 4;
+    const size_t smem = ((size_t)kRows * d4 + 2 * kKeys * (d4 + 4)) * sizeof(float);
+    auto *kernel = a.d <= 128 ? attend_kernel<T, 1> : attend_kernel<T, 2>;
+    if (int rc = allow_smem(kernel, smem)) return rc;
+    if (int rc = launch(kernel, dim3(kCtas), dim3(kThreads), smem, stream, a)) return rc;
+    return launch(merge_kernel<T, kRows>, dim3(kCtas, 4), dim3(128), 0, stream, a, kCtas);
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh, int dtype)
+{
+    (void)heads; (void)kv_heads; (void)max_fresh; (void)dtype;
+    return kCtas * 2 * (sizeof(PartHead) + (size_t)kRows * (head_dim + 2) * sizeof(float));
+}
+
+int launch_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
+                           void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,
+                           uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream)
+{
+    (void)max_fresh;
+    AttendArgs a{};
+    a.q = q; a.k = k_cache; a.v = v_cache; a.out = out;
+    a.starts = starts; a.lengths = lengths; a.table = table;
+    a.sequences = sequences; a.rows = rows; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.d = head_dim;
+    a.page_shift = page_shift(page_size); a.pages = pages; a.table_width = table_width;
+    a.window = window < (1u << 31) ? window : 0u;                      // no sequence is longer
+    a.q_pitch = q_pitch; a.out_pitch = out_pitch;
+    a.rows_from = 1; a.rows_to = 0xFFFFFFFFu;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.heads = static_cast<PartHead *>(workspace);
+    a.parts = reinterpret_cast<float *>(a.heads + 2 * kCtas);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case MGQ_FMT_F32: return launch_attend<float>(a, s);
+        case MGQ_FMT_F16: return launch_attend<__half>(a, s);
+        default: return launch_attend<__nv_bfloat16>(a, s);
+    }
+}
+
+}  // namespace mgq

@@ -1,0 +1,359 @@
+// From logits to tokens for rows of many sequences: probabilities with a temperature per row (mgq_token_probs) and the verification
+// of drafted tokens against the target's probabilities with given random numbers (mgq_verify_drafts).
+//
+// Both stream rows of a vocabulary (150000 f32, 0.6 MB) and are bound by HBM when there are many rows, by latency when there are few.
+// A row is shared out over a cluster of up to eight CTAs whose sums meet through distributed shared memory, so that its
+// values are read once and stay in registers between the passes.
+#include <cfloat>
+#include <cstdint>
+
+#include "mgq_launch.cuh"
+
+namespace mgq {
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kHold = 10;                                // groups of four values a thread keeps: 8 CTAs hold a row of 163840
+constexpr uint32_t kGroup = 4 * kThreads, kSlice = kHold * kGroup;
+
+template <typename T>
+__device__ __forceinline__ T cluster_read(const T *p, uint32_t rank)
+{
+    uint32_t addr;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    if constexpr (sizeof(T) == 8) {
+        unsigned long long v;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+        return *reinterpret_cast<T *>(&v);
+    } else {
+        uint32_t v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+        return *reinterpret_cast<T *>(&v);
+    }
+}
+
+// Four values of a row from column c on; `fill` behind its end.
+template <bool WIDE>
+__device__ __forceinline__ void read4(const float *row, uint32_t c, uint32_t end, float fill, float (&v)[4])
+{
+    if (WIDE) {
+        float4 q = make_float4(fill, fill, fill, fill);
+        if (c < end) q = __ldcs(reinterpret_cast<const float4 *>(row + c));
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = c + e < end ? __ldcs(row + c + e) : fill;
+    }
+}
+
+// ---------------------------------------------------------------- probabilities
+// p_i = exp((l_i - m) / t) / sum; t <= 0 (or NaN): 1 for the lowest index among the largest logits.  NaN logits count as -inf; where
+// the largest is +inf, those that are share the row.  Rows without a finite or +inf logit are all zero.
+// The values of a CTA's slice stay in registers; a vocabulary beyond 8 slices is read again for each pass (HELD false).
+template <bool WIDE, bool HELD>
+__global__ void __launch_bounds__(kThreads, 2) probs_kernel(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t vocab)
+{
+    __shared__ float s_max[kWarps], s_sum[kWarps];
+    __shared__ uint32_t s_at[kWarps];
+    __shared__ float x_max, x_sum;
+    __shared__ uint32_t x_at;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, part = blockIdx.y, parts = gridDim.y;
+    const uint32_t each = ((vocab + parts - 1) / parts + 3) / 4 * 4, begin = min(part * each, vocab), end = min(begin + each, vocab);
+    pdl_launch_dependents();
+    pdl_wait();
+    const float *row = logits + (size_t)blockIdx.x * pitch;
+    float *dst = out + (size_t)blockIdx.x * out_pitch;
+    const float temp = temperature ? temperature[blockIdx.x] : 1.f;
+    const bool greedy = !(temp > 0.f);
+
+    float v[kHold][4];
+    float m = -INFINITY;
+    uint32_t at = 0xFFFFFFFFu;
+    auto largest = [&](float x, uint32_t i) {
+        if (x > m || (x == m && i < at && x > -INFINITY)) { m = x; at = i; }
+    };
+    if (HELD) {
+#pragma unroll
+        for (int k = 0; k < kHold; k++) read4<WIDE>(row, begin + k * kGroup + 4 * t, end, -INFINITY, v[k]);
+#pragma unroll
+        for (int k = 0; k < kHold; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) largest(v[k][e], begin + k * kGroup + 4 * t + e);
+    } else {
+        for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
+            read4<WIDE>(row, c, end, -INFINITY, v[0]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) largest(v[0][e], c + e);
+        }
+    }
+    auto merge = [&](float om, uint32_t oat) {
+        if (om > m || (om == m && oat < at)) { m = om; at = oat; }
+    };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) merge(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
+    if (lane == 0) { s_max[warp] = m; s_at[warp] = at; }
+    __syncthreads();
+    for (int w = 0; w < kWarps; w++) merge(s_max[w], s_at[w]);
+    if (parts > 1) {
+        if (t == 0) { x_max = m; x_at = at; }
+        cluster_sync();
+        for (uint32_t p = 0; p < parts; p++) merge(cluster_read(&x_max, p), cluster_read(&x_at, p));
+    }
+
+    const float inv = greedy ? 0.f : 1.f / temp;
+    auto weight = [&](float x, uint32_t i) {
+        if (greedy) return x == m && i == at ? 1.f : 0.f;          // an index behind the slice's end is another CTA's
+        return x == m ? (m > -INFINITY ? 1.f : 0.f) : x < m ? expf((x - m) * inv) : 0.f;
+    };
+    float sum = 0.f;
+    if (HELD) {
+#pragma unroll
+        for (int k = 0; k < kHold; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[k][e] = weight(v[k][e], begin + k * kGroup + 4 * t + e);
+                sum += v[k][e];
+            }
+    } else {
+        for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
+            read4<WIDE>(row, c, end, -INFINITY, v[0]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += weight(v[0][e], c + e);
+        }
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < kWarps; w++) sum += s_sum[w];
+    if (parts > 1) {
+        if (t == 0) x_sum = sum;
+        cluster_sync();
+        sum = 0.f;
+        for (uint32_t p = 0; p < parts; p++) sum += cluster_read(&x_sum, p);
+    }
+    const float scale = sum > 0.f ? 1.f / sum : 0.f;
+    auto store = [&](uint32_t c, const float (&p)[4]) {
+        if (WIDE) {
+            if (c < end) __stcs(reinterpret_cast<float4 *>(dst + c), make_float4(p[0] * scale, p[1] * scale, p[2] * scale, p[3] * scale));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c + e < end) __stcs(dst + c + e, p[e] * scale);
+        }
+    };
+    if (HELD) {
+#pragma unroll
+        for (int k = 0; k < kHold; k++) store(begin + k * kGroup + 4 * t, v[k]);
+    } else {
+        for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
+            read4<WIDE>(row, c, end, -INFINITY, v[0]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[0][e] = weight(v[0][e], c + e);
+            store(c, v[0]);
+        }
+    }
+    if (parts > 1) cluster_sync();                       // nobody leaves while its sums are being read
+}
+
+// ---------------------------------------------------------------- verification
+// Draft i of a sequence (fed as row start + i) is kept while u q(d) < p(d), with p and q from row start + i - 1: the products of
+// two f32 are exact in 64 bits.  At the first draft that is not kept the next token is drawn from max(p - q, 0), behind the last
+// one from p: the lowest index whose running sum exceeds u times the whole.  Running sums are in 64 bits, because with 150000
+// entries an f32 sum is wrong by more than many an entry: per thread and group of four, then warps in order, then CTAs in order.
+struct VerifyArgs {
+    const float *target, *draft;
+    const uint32_t *tokens, *starts;
+    const float *accept, *sample;
+    uint32_t *accepted, *next, *out;
+    uint32_t target_pitch, draft_pitch, rows, vocab;
+};
+
+__device__ __forceinline__ double mass(float p) { return p > 0.f && p <= FLT_MAX ? (double)p : 0.0; }
+
+template <bool WIDE>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
+{
+    __shared__ double s_sum[kWarps];
+    __shared__ double x_sum;
+    __shared__ uint32_t s_kept, s_warp;
+    __shared__ double s_x;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, seq = blockIdx.x, part = blockIdx.y, parts = gridDim.y;
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t first = min(a.starts[seq], a.rows), last = max(min(a.starts[seq + 1], a.rows), first), n = last - first;
+    if (n == 0) {                                        // uniform over the cluster
+        if (part == 0 && t == 0) {
+            a.accepted[seq] = 0;
+            a.next[seq] = MGQ_NO_TOKEN;
+        }
+        return;
+    }
+    if (t == 0) s_kept = n - 1;
+    __syncthreads();
+    for (uint32_t i = t; i + 1 < n; i += kThreads) {
+        const uint32_t row = first + i, d = a.tokens[row + 1];
+        bool keep = false;
+        if (d < a.vocab) {
+            const double p = a.target[(size_t)row * a.target_pitch + d], q = a.draft ? (double)a.draft[(size_t)row * a.draft_pitch + d] : 1.0;
+            keep = (double)a.accept[row] * q < p;
+        }
+        if (!keep) {
+            atomicMin(&s_kept, i);
+            break;
+        }
+    }
+    __syncthreads();
+    const uint32_t kept = s_kept, row = first + kept;
+    const bool all = kept + 1 == n;
+    if (part == 0) {
+        if (t == 0) a.accepted[seq] = kept;
+        for (uint32_t i = t; i < n; i += kThreads)
+            if (i != kept) a.out[first + i] = i < kept ? a.tokens[first + i + 1] : MGQ_NO_TOKEN;
+    }
+    const uint32_t each = ((a.vocab + parts - 1) / parts + 3) / 4 * 4, begin = min(part * each, a.vocab), end = min(begin + each, a.vocab);
+    // a warp takes a contiguous piece of the slice, so that the pieces are in order
+    const uint32_t piece = ((end - begin + kWarps - 1) / kWarps + 127) / 128 * 128, w0 = min(begin + warp * piece, end), w1 = min(w0 + piece, end);
+    const float *p = a.target + (size_t)row * a.target_pitch, *q = a.draft ? a.draft + (size_t)row * a.draft_pitch : nullptr;
+    const uint32_t taboo = !all && !q ? a.tokens[row + 1] : MGQ_NO_TOKEN;
+    double total = 0.0, tot[8];
+    // first the rest that the draft leaves over; where that is nothing, the target's own row
+    for (int pass = all ? 1 : 0; pass < 2; pass++) {
+        const bool rest = pass == 0;
+        auto weights = [&](uint32_t c, double (&w)[4]) {
+            float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
+            read4<WIDE>(p, c, w1, 0.f, x);
+            if (rest && q) read4<WIDE>(q, c, w1, 0.f, y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                w[e] = mass(x[e]);
+                if (rest) w[e] = q ? fmax(w[e] - mass(y[e]), 0.0) : c + e == taboo ? 0.0 : w[e];
+            }
+        };
+        double sum = 0.0;
+#pragma unroll 4
+        for (uint32_t c = w0 + 4 * lane; c < w1; c += 128) {
+            double w[4];
+            weights(c, w);
+            sum += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        __syncthreads();                                 // the pass before has read these
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        double whole = 0.0;
+        for (int w = 0; w < kWarps; w++) whole += s_sum[w];
+        if (parts > 1) {
+            if (t == 0) x_sum = whole;
+            cluster_sync();
+        }
+        total = 0.0;
+        double base = 0.0;
+        for (uint32_t i = 0; i < 8; i++) {
+            tot[i] = i < parts ? (parts > 1 ? cluster_read(&x_sum, i) : whole) : 0.0;
+            if (i == part) base = total;
+            total += tot[i];
+        }
+        if (parts > 1) cluster_sync();                   // read before the next pass writes, and before anybody leaves
+        if (!(total > 0.0)) continue;
+        // u times the whole lies in exactly one CTA's share; at the whole itself (u = 1) it is the last one with any
+        float u = a.sample[seq];
+        u = u > 0.f ? fminf(u, 1.f) : 0.f;
+        const double x = (double)u * total;
+        uint32_t owner = 0;
+        double run = 0.0;
+        bool found = false;
+        for (uint32_t i = 0; i < 8; i++) {
+            if (tot[i] > 0.0 && !found) {
+                owner = i;
+                found = x < run + tot[i];
+            }
+            run += tot[i];
+        }
+        if (owner != part) return;
+        if (t == 0) {
+            double left = x - base;
+            uint32_t pick = 0;
+            for (int w = 0; w < kWarps; w++)
+                if (s_sum[w] > 0.0) pick = w;            // the last with any, should rounding leave `left` at the end
+            for (int w = 0; w < kWarps; w++) {
+                if (s_sum[w] > 0.0 && left < s_sum[w]) { pick = w; break; }
+                if ((uint32_t)w < pick) left -= s_sum[w];
+            }
+            s_warp = pick;
+            s_x = left;
+        }
+        __syncthreads();
+        if (warp != s_warp) return;
+        double left = s_x;
+        uint32_t token = MGQ_NO_TOKEN, highest = MGQ_NO_TOKEN;
+        for (uint32_t c0 = w0; c0 < w1 && token == MGQ_NO_TOKEN; c0 += 128) {
+            double w[4];
+            weights(c0 + 4 * lane, w);                   // zeros behind the piece
+            const double own = (w[0] + w[1]) + (w[2] + w[3]);
+            double upto = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double below = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += below;
+            }
+            double at = upto - own;                      // exclusive
+            uint32_t mine = MGQ_NO_TOKEN, top = MGQ_NO_TOKEN;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                at += w[e];
+                if (w[e] > 0.0) {
+                    top = c0 + 4 * lane + e;
+                    if (mine == MGQ_NO_TOKEN && at > left) mine = top;
+                }
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, mine != MGQ_NO_TOKEN), any = __ballot_sync(0xffffffffu, top != MGQ_NO_TOKEN);
+            if (any) highest = __shfl_sync(0xffffffffu, top, 31 - __clz(any));
+            if (hit) token = __shfl_sync(0xffffffffu, mine, __ffs(hit) - 1);
+            left -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) {
+            const uint32_t pick = token != MGQ_NO_TOKEN ? token : highest;
+            a.next[seq] = pick;
+            a.out[row] = pick;
+        }
+        return;
+    }
+    if (part == 0 && t == 0) {                           // neither the rest nor the row has any mass
+        a.next[seq] = MGQ_NO_TOKEN;
+        a.out[row] = MGQ_NO_TOKEN;
+    }
+}
+
+bool aligned16(const void *p, uint32_t pitch) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % 4 == 0; }
+
+// CTAs per row: few rows are spread over more of them.
+uint32_t row_parts(uint32_t rows, uint32_t vocab)
+{
+    uint32_t parts = 1;
+    while (parts < 8 && (vocab > parts * kSlice || (rows * parts * 2 <= 296 && vocab > parts * kGroup))) parts *= 2;
+    return parts;
+}
+
+}  // namespace
+
+int launch_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream)
+{
+    const uint32_t parts = row_parts(rows, vocab);
+    const bool wide = vocab % 4 == 0 && aligned16(logits, pitch) && aligned16(out, out_pitch), held = vocab <= parts * kSlice;
+    auto *kernel = wide ? (held ? probs_kernel<true, true> : probs_kernel<true, false>) : (held ? probs_kernel<false, true> : probs_kernel<false, false>);
+    return launch_clustered(kernel, dim3(rows, parts), dim3(kThreads), parts, 0, static_cast<cudaStream_t>(stream), logits, pitch, temperature, out, out_pitch, vocab);
+}
+
+int launch_verify_drafts(const float *target, uint32_t target_pitch, const float *draft, uint32_t draft_pitch, const uint32_t *tokens, const uint32_t *starts,
+                         const float *accept, const float *sample, uint32_t *accepted, uint32_t *next, uint32_t *out, uint32_t sequences, uint32_t rows,
+                         uint32_t vocab, void *stream)
+{
+    const VerifyArgs a{target, draft, tokens, starts, accept, sample, accepted, next, out, target_pitch, draft_pitch, rows, vocab};
+    const uint32_t parts = row_parts(sequences, vocab);
+    const bool wide = vocab % 4 == 0 && aligned16(target, target_pitch) && (!draft || aligned16(draft, draft_pitch));
+    return launch_clustered(wide ? verify_kernel<true> : verify_kernel<false>, dim3(sequences, parts), dim3(kThreads), parts, 0, static_cast<cudaStream_t>(stream), a);
+}
+
+}  // namespace mgq
