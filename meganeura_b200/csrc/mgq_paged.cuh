@@ -54,20 +54,13 @@ struct Segment {
 
 template <int ROWS, int KEYS>
 struct Walk {
-    const AttendArgs &a;
     uint32_t slice, slices, per_tile;               // heads of a unit, units per key / value head, tokens of a unit
-    uint32_t s = 0, head = 0, tile = 0, off = 0;    // the next segment: sequence, head block, token block, key blocks behind
-    uint32_t r0 = 0, n = 0, tiles = 0;
-    int len = 0;
-    unsigned long long left = 0;
+    uint32_t s, head, tile, off;                    // the next segment: sequence, head block, token block, key blocks behind
+    uint32_t r0, n, tiles;
+    int len;
+    unsigned long long left;
 
-    __device__ __forceinline__ explicit Walk(const AttendArgs &args) : a(args)
-    {
-        slice = min(a.group, (uint32_t)ROWS);
-        slices = (a.group + slice - 1) / slice;
-        per_tile = ROWS / slice;
-    }
-    __device__ __forceinline__ void open(uint32_t seq)
+    __device__ __forceinline__ void open(const AttendArgs &a, uint32_t seq)
     {
         s = seq;
         r0 = min(a.starts[s], a.rows);
@@ -76,36 +69,40 @@ struct Walk {
         const unsigned long long pairs = (unsigned long long)n * a.group;
         tiles = pairs >= a.rows_from && pairs <= a.rows_to ? (n + per_tile - 1) / per_tile : 0;
     }
-    __device__ __forceinline__ void keys(uint32_t t, uint32_t &lo, uint32_t &hi) const
+    __device__ __forceinline__ void keys(const AttendArgs &a, uint32_t t, uint32_t &lo, uint32_t &hi) const
     {
         const int first = len - (int)n + (int)(t * per_tile), last = min(len - 1, first + (int)per_tile - 1);
         hi = last < 0 ? 0u : (uint32_t)last / KEYS + 1;
         lo = a.window && first >= (int)a.window ? min((uint32_t)(first - (int)a.window + 1) / KEYS, hi) : 0u;
     }
     // Key blocks of a unit; one without any still costs a block, because its rows have to be written.
-    __device__ __forceinline__ uint32_t cost(uint32_t t) const
+    __device__ __forceinline__ uint32_t cost(const AttendArgs &a, uint32_t t) const
     {
         uint32_t lo, hi;
-        keys(t, lo, hi);
+        keys(a, t, lo, hi);
         return max(1u, hi - lo);
     }
-    __device__ __forceinline__ unsigned long long head_cost() const
+    __device__ __forceinline__ unsigned long long head_cost(const AttendArgs &a) const
     {
         unsigned long long c = 0;
-        for (uint32_t t = 0; t < tiles; t++) c += cost(t);
+        for (uint32_t t = 0; t < tiles; t++) c += cost(a, t);
         return c;
     }
 
     // Every thread of the block: this CTA's piece.  `scratch`: 40 words of shared memory, free again when the call returns.  Pieces have
     // at least `least` key blocks where there are that many.
-    __device__ __forceinline__ void begin(uint32_t cta, uint32_t ctas, uint32_t least, unsigned long long *scratch)
+    __device__ __forceinline__ void begin(const AttendArgs &a, uint32_t cta, uint32_t ctas, uint32_t least, unsigned long long *scratch)
     {
+        slice = min(a.group, (uint32_t)ROWS);
+        slices = (a.group + slice - 1) / slice;
+        per_tile = ROWS / slice;
+        s = head = tile = off = 0;
         const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, warps = blockDim.x >> 5, each = (a.sequences + blockDim.x - 1) / blockDim.x;
         const uint32_t s0 = min(t * each, a.sequences), s1 = min(s0 + each, a.sequences), heads = a.kv_heads * slices;
         unsigned long long mine = 0;
         for (uint32_t i = s0; i < s1; i++) {
-            open(i);
-            mine += head_cost() * heads;
+            open(a, i);
+            mine += head_cost(a) * heads;
         }
         unsigned long long upto = mine;
 #pragma unroll
@@ -125,15 +122,15 @@ struct Walk {
         if (w0 >= base && w0 < base + mine) {            // one thread at most
             unsigned long long rest = w0 - base, c = 0;
             for (uint32_t i = s0; i < s1; i++) {
-                open(i);
-                c = head_cost();
+                open(a, i);
+                c = head_cost(a);
                 if (rest < c * heads) break;
                 rest -= c * heads;
             }
             head = (uint32_t)(rest / c);
             rest %= c;
             tile = 0;
-            while (rest >= cost(tile)) rest -= cost(tile++);
+            while (rest >= cost(a, tile)) rest -= cost(a, tile++);
             scratch[32] = s;
             scratch[33] = head;
             scratch[34] = tile;
@@ -146,22 +143,22 @@ struct Walk {
             head = (uint32_t)scratch[33];
             tile = (uint32_t)scratch[34];
             off = (uint32_t)scratch[35];
-            open(at);
+            open(a, at);
         }
         __syncthreads();
     }
 
-    __device__ __forceinline__ bool next(Segment &g)
+    __device__ __forceinline__ bool next(const AttendArgs &a, Segment &g)
     {
         if (!left) return false;
         while (tile == tiles) {                          // behind the last unit of a head, or a sequence without any
             tile = 0;
             if (tiles && ++head < a.kv_heads * slices) break;
             head = 0;
-            open(s + 1);                                 // `left` says that there is one
+            open(a, s + 1);                              // `left` says that there is one
         }
         uint32_t lo, hi;
-        keys(tile, lo, hi);
+        keys(a, tile, lo, hi);
         const uint32_t all = max(1u, hi - lo), take = (uint32_t)min((unsigned long long)(all - off), left);
         g.row0 = r0 + tile * per_tile;
         g.tokens = min(per_tile, n - tile * per_tile);
@@ -202,5 +199,70 @@ __device__ __forceinline__ void name_part(const AttendArgs &a, uint32_t cta, con
     h.heads = g.heads;
     h.state = g.first ? kOpens : g.last ? kCloses : kGoesOn;
 }
+
+// Joins the parts of the unit that CTA blockIdx.x of an attention kernel began and did not end: with M the largest of the parts' maxima
+// o = sum 2^(m - M) o_part / sum 2^(m - M) l_part.  The parts are those of the CTAs that follow, up to the one that ends the
+// unit, added in this order.  Grid: (CTAs, anything): the rows are shared out over y.  Round trips to L2 bound it: states first, then
+// a row's maxima and weights by all threads, then its sums, several parts in flight.
+constexpr int kMergeThreads = 128, kMaxCtas = 148 * 4;
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a, uint32_t ctas)
+{
+    __shared__ float s_weight[kMaxCtas], s_warp[2][kMergeThreads / 32];
+    __shared__ uint32_t s_end;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, c0 = blockIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
+    const PartHead h = a.heads[2 * c0 + 1];
+    if (h.state != kOpens) return;
+    if (t == 0) s_end = ctas - 1;
+    __syncthreads();
+    for (uint32_t c = c0 + 1 + t; c < ctas; c += kMergeThreads)
+        if (a.heads[2 * c].state == kCloses) {
+            atomicMin(&s_end, c);
+            break;
+        }
+    __syncthreads();
+    const uint32_t parts = s_end - c0 + 1, d = a.d, step = d + 2;
+    auto part = [&](uint32_t i) { return a.parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * ROWS * step; };
+    for (uint32_t r = blockIdx.y; r < h.tokens * h.heads; r += gridDim.y) {
+        float top = -INFINITY;
+        for (uint32_t i = t; i < parts; i += kMergeThreads) top = fmaxf(top, part(i)[r * step + d]);
+        top = warp_max(top);
+        if (lane == 0) s_warp[0][warp] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(s_warp[0][0], s_warp[0][1]), fmaxf(s_warp[0][2], s_warp[0][3]));
+        float l = 0.f;
+        for (uint32_t i = t; i < parts; i += kMergeThreads) {
+            const float m = part(i)[r * step + d], mine = part(i)[r * step + d + 1];
+            const float w = mine != 0.f ? exp2f(m - top) : 0.f;      // a NaN is a weight
+            s_weight[i] = w;
+            l += w * mine;
+        }
+        l = warp_sum(l);
+        if (lane == 0) s_warp[1][warp] = l;
+        __syncthreads();
+        l = (s_warp[1][0] + s_warp[1][1]) + (s_warp[1][2] + s_warp[1][3]);
+        const float scale = l == 0.f ? 0.f : 1.f / l;
+        const uint32_t token = r / h.heads, head = r - token * h.heads;
+        T *out = static_cast<T *>(a.out) + (size_t)(h.row0 + token) * a.out_pitch + (size_t)(h.head0 + head) * d;
+        for (uint32_t col = t; col < d; col += kMergeThreads) {
+            float o = 0.f;
+#pragma unroll 8
+            for (uint32_t i = 0; i < parts; i++) {
+                const float w = s_weight[i], v = part(i)[r * step + col];
+                o += w != 0.f ? w * v : 0.f;                         // a part without weight may hold anything
+            }
+            out[col] = rounded<T>(o * scale);
+        }
+        __syncthreads();
+    }
+}
+
+// 16-bit types with heads of a multiple of 8 elements on 16-byte boundaries: few new tokens (mgq_paged_decode.cu).
+bool decode_takes(const AttendArgs &a, int dtype);
+uint32_t decode_ctas(uint32_t head_dim);
+constexpr int kDecodeRows = 32;
+int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream);      // pairs: a bound of a sequence's tokens * heads per key / value head
 
 }  // namespace mgq

@@ -21,12 +21,12 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     float *s_q = s_mem, *s_k = s_q + kRows * d4, *s_v = s_k + kKeys * pitch;
     pdl_launch_dependents();
     pdl_wait();
-    Walk<kRows, kKeys> walk(a);
-    walk.begin(blockIdx.x, gridDim.x, 1, s_walk);
+    Walk<kRows, kKeys> walk;
+    walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 
     Segment g;
-    while (walk.next(g)) {
+    while (walk.next(a, g)) {
         const uint32_t pairs = g.tokens * g.heads;
         __syncthreads();
         for (uint32_t i = t; i < kRows * d4; i += kThreads) {
@@ -146,43 +146,6 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     }
 }
 
-// Joins the parts of the unit that CTA blockIdx.x of the attention kernel began and did not end: with M the largest of the parts' maxima
-// o = sum 2^(m - M) o_part / sum 2^(m - M) l_part.  The parts are those of the CTAs that follow, up to the one that ends the
-// unit, added in this order.
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(128) merge_kernel(const AttendArgs a, uint32_t ctas)
-{
-    __shared__ uint32_t s_end;
-    const uint32_t t = threadIdx.x, c0 = blockIdx.x;
-    pdl_launch_dependents();
-    pdl_wait();
-    const PartHead h = a.heads[2 * c0 + 1];
-    if (h.state != kOpens) return;
-    if (t == 0) s_end = ctas;
-    __syncthreads();
-    for (uint32_t c = c0 + 1 + t; c < ctas; c += 128)
-        if (a.heads[2 * c].state == kCloses) {
-            atomicMin(&s_end, c);
-            break;
-        }
-    __syncthreads();
-    const uint32_t end = min(s_end, ctas - 1), d = a.d, step = d + 2;          // the part that closes
-    auto part = [&](uint32_t c) { return a.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS * step; };
-    for (uint32_t r = blockIdx.y; r < h.tokens * h.heads; r += gridDim.y) {
-        float top = -INFINITY, l = 0.f;
-        for (uint32_t c = c0; c <= end; c++) top = fmaxf(top, part(c)[r * step + d]);
-        auto weight = [&](uint32_t c) { return part(c)[r * step + d + 1] != 0.f ? exp2f(part(c)[r * step + d] - top) : 0.f; };    // a NaN is a weight
-        for (uint32_t c = c0; c <= end; c++) l += weight(c) * part(c)[r * step + d + 1];
-        const float scale = l == 0.f ? 0.f : 1.f / l;
-        const uint32_t token = r / h.heads, head = r - token * h.heads;
-        for (uint32_t col = t; col < d; col += 128) {
-            float o = 0.f;
-            for (uint32_t c = c0; c <= end; c++) o += weight(c) * part(c)[r * step + col];
-            static_cast<T *>(a.out)[(size_t)(h.row0 + token) * a.out_pitch + (h.head0 + head) * d + col] = rounded<T>(o * scale);
-        }
-    }
-}
-
 constexpr uint32_t kCtas = 148 * 3;
 
 template <typename T>
@@ -193,22 +156,24 @@ int launch_attend(AttendArgs a, cudaStream_t stream)
     auto *kernel = a.d <= 128 ? attend_kernel<T, 1> : attend_kernel<T, 2>;
     if (int rc = allow_smem(kernel, smem)) return rc;
     if (int rc = launch(kernel, dim3(kCtas), dim3(kThreads), smem, stream, a)) return rc;
-    return launch(merge_kernel<T, kRows>, dim3(kCtas, 4), dim3(128), 0, stream, a, kCtas);
+    return launch(merge_kernel<T, kRows>, dim3(kCtas, 4), dim3(kMergeThreads), 0, stream, a, kCtas);
 }
 
 }  // namespace
 
+// Parts of the kernel that serves these arguments (the largest of them where the alignment decides).
 size_t paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh, int dtype)
 {
-    (void)heads; (void)kv_heads; (void)max_fresh; (void)dtype;
-    return kCtas * 2 * (sizeof(PartHead) + (size_t)kRows * (head_dim + 2) * sizeof(float));
+    (void)heads; (void)kv_heads; (void)max_fresh;
+    auto bytes = [&](uint32_t ctas, size_t rows) { return ctas * 2 * (sizeof(PartHead) + rows * (head_dim + 2) * sizeof(float)); };
+    const size_t plain = bytes(kCtas, kRows);
+    return dtype == MGQ_FMT_F32 ? plain : max(plain, bytes(decode_ctas(head_dim), kDecodeRows));
 }
 
 int launch_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
                            void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,
                            uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream)
 {
-    (void)max_fresh;
     AttendArgs a{};
     a.q = q; a.k = k_cache; a.v = v_cache; a.out = out;
     a.starts = starts; a.lengths = lengths; a.table = table;
@@ -218,9 +183,16 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
     a.q_pitch = q_pitch; a.out_pitch = out_pitch;
     a.rows_from = 1; a.rows_to = 0xFFFFFFFFu;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.heads = static_cast<PartHead *>(workspace);
-    a.parts = reinterpret_cast<float *>(a.heads + 2 * kCtas);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    auto room = [&](uint32_t ctas) {
+        a.heads = static_cast<PartHead *>(workspace);
+        a.parts = reinterpret_cast<float *>(a.heads + 2 * ctas);
+    };
+    if (decode_takes(a, dtype)) {
+        room(decode_ctas(head_dim));
+        return launch_decode(a, dtype, (uint32_t)min((unsigned long long)max_fresh * a.group, 0xFFFFFFFFull), s);
+    }
+    room(kCtas);
     switch (dtype) {
         case MGQ_FMT_F32: return launch_attend<float>(a, s);
         case MGQ_FMT_F16: return launch_attend<__half>(a, s);
