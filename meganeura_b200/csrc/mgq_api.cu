@@ -80,7 +80,11 @@ int mgq_set_option(const char *name, long value)
     return set_gemv_option(name, value);
 }
 
-int mgq_device_status(void) { return tc_device_status(); }
+int mgq_device_status(void)
+{
+    if (int rc = tc_device_status()) return rc;
+    return decode_status();
+}
 
 int mgq_gemv(int fmt, const float *x, const void *w, const float *addend, float *y,
              uint32_t m, uint32_t k, uint32_t n, void *stream)

@@ -2,31 +2,33 @@
 // once, so HBM bounds it, and all that matters is that loads never pause.
 //
 // A unit's pairs of token and head (16 or 32: heads of one key / value head share its keys) are the rows of m16n8k16 products.  The
-// four warps of a CTA split the keys: each takes 16 of a block of 64, has a ring of its own for their keys and values, filled with
-// 16-byte cp.async that run across the borders of units, and an online softmax of its own; nothing in the loop waits for another warp.  At a unit's end the
-// four sums are joined in shared memory.  Scores, maxima and sums are f32; a weight enters its product as the sum of two 16-bit values (the tensor
-// cores have time for both), so only the result is rounded.
-// Rows in shared memory are padded by 16 bytes, which keeps ldmatrix free of bank conflicts for every head size.
+// four warps of a CTA split the keys: each takes 16 of a block of 64, has a ring of its own for their keys and values, filled by
+// TMA boxes of 16 keys by 64 elements that run across the borders of units, and an online softmax of its own; nothing in the loop waits for another warp.  At a
+// unit's end the four sums are joined in shared memory.  Scores, maxima and sums are f32; a weight enters its product as the sum of two 16-bit values (the
+// tensor cores have time for both), so only the result is rounded.
+// With 16-byte cp.async instead of boxes a step took 627 instructions and 64 single tokens of the Qwen3-8B shape 242 us.
 #include <cstdint>
 
 #include "mgq_paged.cuh"
+#include "mgq_tcgen05.cuh"
 
 namespace mgq {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kBlock = 64, kStep = 16;      // keys of a block, of a warp's step
 constexpr int kChunk = 16, kPitch = kChunk + 2;                         // columns joined at a time
-
-template <int D> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 3 : D == 128 ? 2 : 1; }
-template <int D> __host__ __device__ constexpr int row_bytes() { return D * 2 + 16; }
 constexpr int kStages = 3;
-template <int D, int MT> constexpr size_t smem_bytes() { return (size_t)kWarps * kStages * 2 * kStep * row_bytes<D>() + (size_t)kWarps * 16 * MT * kPitch * 4; }
+constexpr uint32_t kTile = kStep * 128;                                 // 16 keys by 64 elements, as one swizzled box lies in shared memory
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real)
-{
-    const uint32_t bytes = real ? 16 : 0;                // the rest is zero-filled
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
+// Stages of 16 keys and values fill the SM's shared memory, three per warp.
+template <int D> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 3 : D == 128 ? 2 : 1; }
+template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return 2 * D / 64 * kTile; }
+// Queries (two blocks of rows do not fit into the registers) and, behind a unit's last key, the warps' sums.
+template <int D, int MT> __host__ __device__ constexpr uint32_t rows_bytes() { return MT == 2 ? 32 * (D * 2 + 16) > kWarps * 32 * kPitch * 4 ? 32 * (D * 2 + 16) : kWarps * 32 * kPitch * 4 : kWarps * 16 * kPitch * 4; }
+template <int D, int MT> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * kStages * stage_bytes<D>() + rows_bytes<D, MT>(); }
+
+__device__ unsigned int g_decode_error;
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -49,10 +51,16 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 template <typename T>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t &high, uint32_t &low)
 {
-    const T hx = rounded<T>(x), hy = rounded<T>(y);
-    const T lx = rounded<T>(x - to_f32(hx)), ly = rounded<T>(y - to_f32(hy));
-    high = (uint32_t)*reinterpret_cast<const uint16_t *>(&hx) | (uint32_t)*reinterpret_cast<const uint16_t *>(&hy) << 16;
-    low = (uint32_t)*reinterpret_cast<const uint16_t *>(&lx) | (uint32_t)*reinterpret_cast<const uint16_t *>(&ly) << 16;
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y), l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+        high = *reinterpret_cast<const uint32_t *>(&h);
+        low = *reinterpret_cast<const uint32_t *>(&l);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        high = *reinterpret_cast<const uint32_t *>(&h);
+        const __nv_bfloat162 l = __floats2bfloat162_rn(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xFFFF0000u));
+        low = *reinterpret_cast<const uint32_t *>(&l);
+    }
 }
 __device__ __forceinline__ float exp2_fast(float x)
 {
@@ -72,20 +80,34 @@ __device__ __forceinline__ bool not_finite8(const uint4 &v)
     return bad;
 }
 
+struct CacheMaps {
+    CUtensorMap k, v;                                    // {head_dim, kv_heads, pages * page_size}, boxes of 64 elements by 16 (or 8) tokens
+};
+
 template <typename T, int D, int MT>                     // D: head size rounded up to 64, 128 or 256; MT: blocks of 16 rows
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const AttendArgs a)
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const __grid_constant__ CacheMaps maps, const AttendArgs a)
 {
-    constexpr int ROWS = 16 * MT, RB = row_bytes<D>(), NT = D / 8, KT = D / 16, CH = D / 8;     // CH: 16-byte pieces of a row
+    constexpr int ROWS = 16 * MT, NT = D / 8, KT = D / 16, PARTS = D / 64, QB = D * 2 + 16;
+    constexpr uint32_t kStage = stage_bytes<D>();
     using Way = Walk<ROWS, kBlock>;
-    extern __shared__ __align__(16) uint8_t s_mem[];
+    extern __shared__ uint8_t s_raw[];
     __shared__ unsigned long long s_walk[40];
+    __shared__ __align__(8) unsigned long long s_full[kWarps][kStages];
     __shared__ Way s_way[kWarps];
     __shared__ Segment s_seg[kWarps][8];
     __shared__ uint32_t s_there[kWarps][kStages];
     __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
-    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, d = a.d;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_mem) + warp * (kStages * 2 * kStep * RB);
-    float *s_join = reinterpret_cast<float *>(s_mem + (size_t)kWarps * kStages * 2 * kStep * RB);
+    __shared__ volatile int s_failed;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = __shfl_sync(0xffffffffu, t >> 5, 0), d = a.d;
+    uint8_t *s_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t ring = smem_u32(s_mem) + warp * (kStages * kStage);
+    uint8_t *s_rows = s_mem + (size_t)kWarps * kStages * kStage;
+    float *s_join = reinterpret_cast<float *>(s_rows);
+    if (t == 0) {
+        for (int i = 0; i < kWarps * kStages; i++) mbar_init(&s_full[i / kStages][i % kStages], 1);
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     pdl_launch_dependents();
     pdl_wait();
     {
@@ -97,12 +119,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
     __syncwarp();
 
     // ---- the producer's side of a warp: one step of 16 keys at a time, a segment without keys is a step without loads
-    uint32_t p_seg = 0, p_block = 0, p_end = 0, p_slot = 0, p_steps = 0;      // segments begun, its next and last block, ring slot, steps issued
+    uint32_t p_seg = 0, p_block = 0, p_end = 0, p_slot = 0;      // segments begun, its next and last block, ring slot
     bool p_live = true;
     const uint32_t *p_table = nullptr;
-    int p_len = 0;
-    const uint8_t *p_k = nullptr, *p_v = nullptr;
-    const size_t row_stride = (size_t)a.kv_heads * d * sizeof(T);
+    int p_len = 0, p_kv = 0;
     auto produce = [&]() {
         if (p_live && p_block >= p_end) {                // the next segment
             if (lane == 0) {
@@ -117,59 +137,71 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             if (p_live) {
                 p_seg++;
                 p_table = g.table;
-                p_len = g.len;
+                p_len = g.end <= g.begin ? 0 : g.len;
+                p_kv = (int)g.kv;
                 p_block = g.begin;
                 p_end = max(g.end, g.begin + 1);
-                const size_t head = ((size_t)g.kv * d + (lane % CH) * 8) * sizeof(T);
-                p_k = static_cast<const uint8_t *>(a.k) + head;
-                p_v = static_cast<const uint8_t *>(a.v) + head;
-                if (g.end <= g.begin) p_len = 0;
             }
         }
         if (p_live) {
-            const uint32_t key0 = p_block * kBlock + warp * kStep, slot = p_slot;
-            uint32_t page[2];
-            bool real[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {                // pages have at least 8 tokens
-                const uint32_t key = key0 + 8 * h;
-                page[h] = (int)key < p_len ? p_table[key >> a.page_shift] : 0xFFFFFFFFu;
-                real[h] = page[h] < a.pages;
-            }
-            const uint32_t within = (1u << a.page_shift) - 1, dst = ring + slot * (2 * kStep * RB) + (lane % CH) * 16;
-            const bool column = (lane % CH) * 8 < d;
-#pragma unroll
-            for (int i = 0; i < kStep * CH / 32; i++) {
-                const uint32_t r = i * (32 / CH) + lane / CH, h = r / 8;
-                const uint32_t pg = h ? page[1] : page[0];
-                const bool ok = (h ? real[1] : real[0]) && (int)(key0 + r) < p_len && column;
-                const size_t at = ok ? (((size_t)pg << a.page_shift) + ((key0 + r) & within)) * row_stride : 0;
-                copy16(dst + r * RB, p_k + at, ok);
-                copy16(dst + (kStep + r) * RB, p_v + at, ok);
-            }
             if (lane == 0) {
-                uint32_t there = (real[0] ? 0xFFu : 0u) | (real[1] ? 0xFF00u : 0u);
-                const int upto = p_len - (int)key0;
-                if (upto < kStep) there &= upto > 0 ? (1u << upto) - 1 : 0u;
-                s_there[warp][slot] = there;
+                const uint32_t key0 = p_block * kBlock + warp * kStep, within = (1u << a.page_shift) - 1;
+                uint32_t there = 0;                                             // written before the arrival that publishes it
+                if ((int)key0 < p_len) {
+                    const uint32_t gone = a.pages << a.page_shift;              // a slot behind the last one: the box is filled with zeros
+                    uint32_t page = p_table[key0 >> a.page_shift], slot[2];
+                    const bool real = page < a.pages;
+                    slot[0] = real ? (page << a.page_shift) + (key0 & within) : gone;
+                    there = real ? 0xFFFFu : 0u;
+                    if (a.page_shift == 3) {                                    // 16 keys of two pages
+                        page = (int)key0 + 8 < p_len ? p_table[(key0 >> 3) + 1] : 0xFFFFFFFFu;
+                        slot[1] = page < a.pages ? page << 3 : gone;
+                        there = (real ? 0xFFu : 0u) | (page < a.pages ? 0xFF00u : 0u);
+                    }
+                    const int upto = p_len - (int)key0;
+                    if (upto < kStep) there &= (1u << upto) - 1;
+                    s_there[warp][p_slot] = there;
+                    unsigned long long *bar = &s_full[warp][p_slot];
+                    const uint32_t dst = ring + p_slot * kStage;
+                    mbar_arrive_expect_tx(bar, kStage);
+#pragma unroll
+                    for (int c = 0; c < PARTS; c++) {
+                        tma_load_3d(dst + c * kTile, &maps.k, c * 64, p_kv, (int)slot[0], bar);
+                        tma_load_3d(dst + (PARTS + c) * kTile, &maps.v, c * 64, p_kv, (int)slot[0], bar);
+                        if (a.page_shift == 3) {
+                            tma_load_3d(dst + c * kTile + kTile / 2, &maps.k, c * 64, p_kv, (int)slot[1], bar);
+                            tma_load_3d(dst + (PARTS + c) * kTile + kTile / 2, &maps.v, c * 64, p_kv, (int)slot[1], bar);
+                        }
+                    }
+                } else {
+                    s_there[warp][p_slot] = 0;
+                    mbar_arrive(&s_full[warp][p_slot]);
+                }
             }
             p_block++;
-            p_steps++;
+            p_slot = p_slot == kStages - 1 ? 0 : p_slot + 1;
         }
-        p_slot = p_slot == kStages - 1 ? 0 : p_slot + 1;
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kStages - 1; i++) produce();
 
     // ---- the consumer's side
-    uint32_t c_seg = 0, slot = 0;
+    uint32_t c_seg = 0, slot = 0, parity = 0;
+    bool ok = true;
     const uint32_t row = lane >> 2, quad = lane & 3u;
+    // a lane's ldmatrix row in a box, and the 16-byte piece it starts with in each group of 16 elements (the swizzle XORs it with the row)
+    const uint32_t krow = ((lane & 7u) + (lane >> 4) * 8) * 128, vrow = (lane & 15u) * 128;
+    uint32_t kpiece[4], vpiece[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        kpiece[i] = krow + (((2 * i + ((lane >> 3) & 1u)) ^ (lane & 7u)) << 4);
+        vpiece[i] = vrow + (((2 * i + (lane >> 4)) ^ (lane & 7u)) << 4);
+    }
     while (c_seg < p_seg) {
         const Segment g = s_seg[warp][c_seg & 7u];
         c_seg++;
         const uint32_t pairs = g.tokens * g.heads;
-        uint32_t q[MT][KT][4];
+        uint32_t q[MT == 1 ? KT : 1][4];
         int pos[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
@@ -179,12 +211,24 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 const bool live = r < pairs;
                 pos[mt][half] = live ? g.pos0 + (int)token : -1;
                 const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d + 2 * quad;
+                if constexpr (MT == 1) {
 #pragma unroll
-                for (int k = 0; k < KT; k++)
+                    for (int k = 0; k < KT; k++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        q[mt][k][half + 2 * j] = live && k * 16 + j * 8 + 2 * quad < d ? *reinterpret_cast<const uint32_t *>(src + k * 16 + j * 8) : 0u;
+                        for (int j = 0; j < 2; j++)
+                            q[k][half + 2 * j] = live && k * 16 + j * 8 + 2 * quad < d ? *reinterpret_cast<const uint32_t *>(src + k * 16 + j * 8) : 0u;
+                }
             }
+        if constexpr (MT == 2) {
+            for (uint32_t i = t; i < ROWS * D / 2; i += kThreads) {
+                const uint32_t r = i / (D / 2), c = i % (D / 2) * 2, token = r / g.heads, head = r - token * g.heads;
+                uint32_t x = 0;
+                if (r < pairs && c < d) x = *reinterpret_cast<const uint32_t *>(static_cast<const T *>(a.q) + (size_t)(g.row0 + token) * a.q_pitch + (size_t)(g.head0 + head) * d + c);
+                *reinterpret_cast<uint32_t *>(s_rows + r * QB + c * 2) = x;
+            }
+            __syncthreads();
+        }
+        const uint32_t qaddr = smem_u32(s_rows) + (lane & 15u) * QB + (lane >> 4) * 16;
         float o[MT][NT][4], m[MT][2], l[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
@@ -196,28 +240,44 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
         const uint32_t blocks = max(g.end, g.begin + 1) - g.begin;
         const int last_pos = g.pos0 + (int)g.tokens - 1;
         for (uint32_t b = 0; b < blocks; b++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            __syncwarp();
-            const uint32_t there = s_there[warp][slot];
-            const uint32_t kbase = ring + slot * (2 * kStep * RB), vbase = kbase + kStep * RB;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode_error)))) break;
+            uint32_t there = s_there[warp][slot];
+            const uint32_t kbase = ring + slot * kStage, vbase = kbase + PARTS * kTile;
             slot = slot == kStages - 1 ? 0 : slot + 1;
+            parity ^= slot == 0;
             produce();
+            const int key0 = (int)((g.begin + b) * kBlock + warp * kStep), upto = last_pos - key0 + 1, behind = a.window ? g.pos0 - (int)a.window + 1 - key0 : 0;
+            if (upto < kStep) there &= upto > 0 ? (1u << upto) - 1 : 0u;
+            if (behind > 0) there &= behind < kStep ? ~0u << behind : 0u;
             if (!there) continue;
-            const int key0 = (int)((g.begin + b) * kBlock + warp * kStep);
+            if (there != 0xFFFFu) {                      // values that no row sees, whatever the page holds there, become zeros
+#pragma unroll
+                for (uint32_t i = 0; i < PARTS * kTile / 512; i++)
+                    if (!(there >> (i % 4 * 4 + lane / 8) & 1u))
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vbase + i * 512 + lane * 16), "r"(0) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // before the stage is filled again
+                __syncwarp();
+            }
             float s[MT][2][4];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int n = 0; n < 2; n++) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
-            const uint32_t kaddr = kbase + ((lane & 7u) + (lane >> 4) * 8) * RB + ((lane >> 3) & 1u) * 16;
 #pragma unroll
             for (int k = 0; k < KT; k++) {
                 uint32_t kf[4];
-                ldmatrix4(kf, kaddr + k * 32);
+                ldmatrix4(kf, kbase + k / 4 * kTile + kpiece[k % 4]);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    mma<T>(s[mt][0], q[mt][k], kf[0], kf[1]);
-                    mma<T>(s[mt][1], q[mt][k], kf[2], kf[3]);
+                    uint32_t qf[4];
+                    if constexpr (MT == 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) qf[i] = q[k][i];
+                    } else {
+                        ldmatrix4(qf, qaddr + mt * 16 * QB + k * 32);
+                    }
+                    mma<T>(s[mt][0], qf, kf[0], kf[1]);
+                    mma<T>(s[mt][1], qf, kf[2], kf[3]);
                 }
             }
             const bool whole = there == 0xFFFFu && key0 + kStep - 1 <= g.pos0 && (!a.window || key0 > last_pos - (int)a.window);
@@ -235,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                             if (!whole) {
                                 const int key = key0 + n * 8 + 2 * (int)quad + e, p = pos[mt][half];
                                 const bool seen = key <= p && (there >> (n * 8 + 2 * quad + e) & 1u) && (!a.window || key > p - (int)a.window);
-                                hidden |= !seen && (there >> (n * 8 + 2 * quad + e) & 1u);
+                                hidden |= !seen;
                                 x = seen ? x : -INFINITY;
                             }
                             s[mt][n][2 * half + e] = x;
@@ -263,14 +323,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                             l[mt][half] += p;
                         }
                 }
-            // where some row does not see a value that is infinite or NaN, its product with a weight of 0 must not be formed
+            // where some row does not see a value that another one sees and that is infinite or NaN, its product with a weight of 0 must not be formed
             if (!whole && __any_sync(0xffffffffu, hidden)) {
                 bool bad = false;
 #pragma unroll
-                for (int i = 0; i < kStep * CH / 32; i++) {
+                for (uint32_t i = 0; i < PARTS * kTile / 512; i++) {
                     uint4 v;
-                    const uint32_t at = vbase + (i * (32 / CH) + lane / CH) * RB + (lane % CH) * 16;
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(vbase + i * 512 + lane * 16) : "memory");
                     bad |= not_finite8<T>(v);
                 }
                 if (__any_sync(0xffffffffu, bad)) {
@@ -287,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             uint32_t w;
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vbase + j * RB + n * 16 + quad * 4) : "memory");
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vbase + n / 8 * kTile + j * 128 + (((n % 8) ^ (j & 7u)) << 4) + quad * 4) : "memory");
                             const T *v = reinterpret_cast<const T *>(&w);
 #pragma unroll
                             for (int mt = 0; mt < MT; mt++)
@@ -306,11 +365,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) split_pair<T>(s[mt][i >> 1][2 * (i & 1)], s[mt][i >> 1][2 * (i & 1) + 1], high[mt][i], low[mt][i]);
-            const uint32_t vaddr = vbase + (lane & 15u) * RB + (lane >> 4) * 16;
 #pragma unroll
             for (int n = 0; n < NT; n += 2) {
                 uint32_t vf[4];
-                ldmatrix4_t(vf, vaddr + n * 16);
+                ldmatrix4_t(vf, vbase + n / 8 * kTile + vpiece[n / 2 % 4]);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
                     mma<T>(o[mt][n], high[mt], vf[0], vf[1]);
@@ -320,6 +378,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 }
             }
         }
+
+        if (!ok) break;
 
         // ---- the four warps' sums
 #pragma unroll
@@ -403,26 +463,43 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             __syncthreads();                             // before the next unit's maxima
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // given up: the copies in flight land before the CTA exits
+    if (!ok && lane == 0)
+        for (int i = 0; i < kStages - 1; i++) {
+            for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&s_full[warp][slot], parity); w++) { }
+            slot = slot == kStages - 1 ? 0 : slot + 1;
+            parity ^= slot == 0;
+        }
+}
+
+// Tokens of one head by 64 elements, 128-byte swizzle; what lies outside the cache reads as zero.
+int encode_cache(EncodeTiledFn encode, CUtensorMap &map, const void *base, int dtype, const AttendArgs &a, uint32_t tokens)
+{
+    const cuuint64_t dims[3] = {a.d, a.kv_heads, (cuuint64_t)a.pages << a.page_shift};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.d * 2, (cuuint64_t)a.kv_heads * a.d * 2};
+    const cuuint32_t box[3] = {64, 1, tokens}, elem[3] = {1, 1, 1};
+    const CUresult cr = encode(&map, dtype == MGQ_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box,
+                               elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? MGQ_OK : fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
 }
 
 template <typename T, int D, int MT>
-int launch_sized(const AttendArgs &a, cudaStream_t stream)
+int launch_sized(const AttendArgs &a, const CacheMaps &maps, cudaStream_t stream)
 {
     constexpr uint32_t ctas = 148 * ctas_per_sm<D>();
     auto *kernel = decode_kernel<T, D, MT>;
     if (int rc = allow_smem(kernel, smem_bytes<D, MT>())) return rc;
-    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, MT>(), stream, a)) return rc;
+    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, MT>(), stream, maps, a)) return rc;
     return launch(merge_kernel<T, 16 * MT>, dim3(ctas, 8), dim3(kMergeThreads), 0, stream, a, ctas);
 }
 
 template <typename T>
-int launch_typed(const AttendArgs &a, uint32_t pairs, cudaStream_t stream)
+int launch_typed(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cudaStream_t stream)
 {
     const bool two = pairs > 16;
-    if (a.d <= 64) return two ? launch_sized<T, 64, 2>(a, stream) : launch_sized<T, 64, 1>(a, stream);
-    if (a.d <= 128) return two ? launch_sized<T, 128, 2>(a, stream) : launch_sized<T, 128, 1>(a, stream);
-    return launch_sized<T, 256, 1>(a, stream);
+    if (a.d <= 64) return two ? launch_sized<T, 64, 2>(a, maps, stream) : launch_sized<T, 64, 1>(a, maps, stream);
+    if (a.d <= 128) return two ? launch_sized<T, 128, 2>(a, maps, stream) : launch_sized<T, 128, 1>(a, maps, stream);
+    return launch_sized<T, 256, 1>(a, maps, stream);
 }
 
 }  // namespace
@@ -430,14 +507,31 @@ int launch_typed(const AttendArgs &a, uint32_t pairs, cudaStream_t stream)
 bool decode_takes(const AttendArgs &a, int dtype)
 {
     auto on = [](const void *p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
-    return dtype != MGQ_FMT_F32 && a.d % 8 == 0 && on(a.k, 16) && on(a.v, 16) && on(a.q, 4) && on(a.out, 4) && a.q_pitch % 2 == 0 && a.out_pitch % 2 == 0;
+    return dtype != MGQ_FMT_F32 && a.d % 8 == 0 && on(a.k, 16) && on(a.v, 16) && on(a.q, 4) && on(a.out, 4) && a.q_pitch % 2 == 0 && a.out_pitch % 2 == 0 &&
+           (unsigned long long)a.pages << a.page_shift < (1ull << 31);
 }
 
 uint32_t decode_ctas(uint32_t head_dim) { return 148 * (head_dim <= 64 ? ctas_per_sm<64>() : head_dim <= 128 ? ctas_per_sm<128>() : ctas_per_sm<256>()); }
 
 int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream)
 {
-    return dtype == MGQ_FMT_F16 ? launch_typed<__half>(a, pairs, stream) : launch_typed<__nv_bfloat16>(a, pairs, stream);
+    EncodeTiledFn encode = nullptr;
+    if (int rc = encode_fn(encode)) return rc;
+    CacheMaps maps;
+    const uint32_t tokens = a.page_shift == 3 ? 8 : kStep;
+    if (int rc = encode_cache(encode, maps.k, a.k, dtype, a, tokens)) return rc;
+    if (int rc = encode_cache(encode, maps.v, a.v, dtype, a, tokens)) return rc;
+    return dtype == MGQ_FMT_F16 ? launch_typed<__half>(a, maps, pairs, stream) : launch_typed<__nv_bfloat16>(a, maps, pairs, stream);
+}
+
+int decode_status()
+{
+    unsigned int err = 0;
+    MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_decode_error, sizeof err));
+    if (!err) return MGQ_OK;
+    const unsigned int zero = 0;
+    MGQ_CUDA(cudaMemcpyToSymbol(g_decode_error, &zero, sizeof zero));
+    return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the paged attention kernel ran out");
 }
 
 }  // namespace mgq

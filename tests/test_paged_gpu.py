@@ -126,7 +126,7 @@ def test_append_keeps_infinities_and_nan_as_a_cast_does():
 
 # ---------------------------------------------------------------------------------------------- attention
 
-SHAPES = [(9, 3, 64), (32, 8, 128), (4, 4, 80), (16, 2, 96), (8, 1, 128), (6, 2, 256), (3, 1, 20), (5, 5, 33), (40, 1, 64)]
+SHAPES = [(9, 3, 64), (32, 8, 128), (4, 4, 80), (16, 2, 96), (8, 1, 128), (6, 2, 256), (3, 1, 20), (5, 5, 33), (40, 1, 64), (4, 2, 40), (2, 1, 8), (6, 3, 136)]
 BATCHES = {
     "one": (16, [0], [1]), "two": (16, [1], [1]), "tile": (16, [31], [1]), "decode": (16, [5, 130, 0, 64, 63, 65, 700], [1] * 7),
     "drafts": (8, [3, 40, 257, 0], [5, 2, 4, 3]), "ragged": (32, [0, 77, 300, 12, 0], [40, 0, 3, 1, 129]), "chunk": (64, [200, 0], [150, 300]), "wide page": (1024, [900, 100], [9, 33]),
