@@ -278,7 +278,7 @@ int mgq_argmax(const float *logits, uint32_t n, void *workspace, uint32_t *out_t
  *   see has no part in it, whatever it holds; a row that sees nothing is zero; rows behind the last sequence are left as they are.  max_fresh: no sequence has more
  *   new tokens in this step (it chooses kernels; more are not computed).  head_dim at most 256.  `workspace`: mgq_paged_attention_workspace(...) bytes for
  *   the same arguments, 16-byte aligned, in any state; calls that may run at the same time (two streams, two graphs) need one each.
- * All need table_width * page_size and the number of rows below 2^31, and at most MGQ_PAGED_MAX_SEQUENCES sequences. */
+ * All need table_width * page_size below 2^30, the number of rows below 2^31, and at most MGQ_PAGED_MAX_SEQUENCES sequences. */
 #define MGQ_NO_SLOT  0xFFFFFFFFu
 #define MGQ_NO_PAGE  0xFFFFFFFFu
 #define MGQ_NO_TOKEN 0xFFFFFFFFu

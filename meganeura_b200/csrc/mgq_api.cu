@@ -83,7 +83,7 @@ int mgq_set_option(const char *name, long value)
 int mgq_device_status(void)
 {
     if (int rc = tc_device_status()) return rc;
-    return decode_status();
+    return paged_status();
 }
 
 int mgq_gemv(int fmt, const float *x, const void *w, const float *addend, float *y,

@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "mgq_launch.cuh"
+#include "mgq_tcgen05.cuh"
 
 namespace mgq {
 
@@ -36,7 +37,7 @@ struct AttendArgs {
     uint32_t rows_from, rows_to;         // sequences with this many pairs of token and head of a key / value head are this kernel's
     float scale_log2;                    // scale * log2(e): scores are exponents of 2
     struct PartHead *heads;              // [CTAs][2]
-    float *parts;                        // [CTAs][2][ROWS][d + 2]: sums, maximum, weight
+    float *parts;                        // [CTAs][2]: sums [ROWS][d], then maximum and weight of each row [ROWS][2]
 };
 
 enum PartState : uint32_t { kNoPart = 0, kOpens = 1, kGoesOn = 2, kCloses = 3 };
@@ -202,13 +203,13 @@ __device__ __forceinline__ void name_part(const AttendArgs &a, uint32_t cta, con
 
 // Joins the parts of the unit that CTA blockIdx.x of an attention kernel began and did not end: with M the largest of the parts' maxima
 // o = sum 2^(m - M) o_part / sum 2^(m - M) l_part.  The parts are those of the CTAs that follow, up to the one that ends the
-// unit, added in this order.  Grid: (CTAs, anything): the rows are shared out over y.  Round trips to L2 bound it: states first, then
-// a row's maxima and weights by all threads, then its sums, several parts in flight.
-constexpr int kMergeThreads = 128, kMaxCtas = 148 * 4;
+// unit, added in this order.  Grid: (CTAs, anything): the rows are shared out over y, a warp takes a row.  Round trips to L2 bound it: states first,
+// then a row's maxima and weights by all lanes, then its sums, several parts in flight.
+constexpr int kMergeThreads = 128, kMergeWarps = kMergeThreads / 32, kMaxCtas = 148 * 3;
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a, uint32_t ctas)
 {
-    __shared__ float s_weight[kMaxCtas], s_warp[2][kMergeThreads / 32];
+    __shared__ float s_weight[kMergeWarps][kMaxCtas];
     __shared__ uint32_t s_end;
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, c0 = blockIdx.x;
     pdl_launch_dependents();
@@ -223,39 +224,36 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a
             break;
         }
     __syncthreads();
-    const uint32_t parts = s_end - c0 + 1, d = a.d, step = d + 2;
-    auto part = [&](uint32_t i) { return a.parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * ROWS * step; };
-    for (uint32_t r = blockIdx.y; r < h.tokens * h.heads; r += gridDim.y) {
+    const uint32_t parts = s_end - c0 + 1, d = a.d;
+    const size_t size = (size_t)ROWS * (d + 2);
+    const float *first = a.parts + (2 * (size_t)c0 + 1) * size, *rest = a.parts + 2 * (size_t)c0 * size;     // part i > 0 at rest + 2 i size
+    auto part = [&](uint32_t i) { return i == 0 ? first : rest + 2 * i * size; };
+    for (uint32_t r = blockIdx.y * kMergeWarps + warp; r < h.tokens * h.heads; r += gridDim.y * kMergeWarps) {
         float top = -INFINITY;
-        for (uint32_t i = t; i < parts; i += kMergeThreads) top = fmaxf(top, part(i)[r * step + d]);
+        for (uint32_t i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[ROWS * d + 2 * r]);
         top = warp_max(top);
-        if (lane == 0) s_warp[0][warp] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(s_warp[0][0], s_warp[0][1]), fmaxf(s_warp[0][2], s_warp[0][3]));
         float l = 0.f;
-        for (uint32_t i = t; i < parts; i += kMergeThreads) {
-            const float m = part(i)[r * step + d], mine = part(i)[r * step + d + 1];
+        for (uint32_t i = lane; i < parts; i += 32) {
+            const float m = part(i)[ROWS * d + 2 * r], mine = part(i)[ROWS * d + 2 * r + 1];
             const float w = mine != 0.f ? exp2f(m - top) : 0.f;      // a NaN is a weight
-            s_weight[i] = w;
+            s_weight[warp][i] = w;
             l += w * mine;
         }
         l = warp_sum(l);
-        if (lane == 0) s_warp[1][warp] = l;
-        __syncthreads();
-        l = (s_warp[1][0] + s_warp[1][1]) + (s_warp[1][2] + s_warp[1][3]);
+        __syncwarp();
         const float scale = l == 0.f ? 0.f : 1.f / l;
         const uint32_t token = r / h.heads, head = r - token * h.heads;
         T *out = static_cast<T *>(a.out) + (size_t)(h.row0 + token) * a.out_pitch + (size_t)(h.head0 + head) * d;
-        for (uint32_t col = t; col < d; col += kMergeThreads) {
+        for (uint32_t col = lane; col < d; col += 32) {
             float o = 0.f;
 #pragma unroll 8
             for (uint32_t i = 0; i < parts; i++) {
-                const float w = s_weight[i], v = part(i)[r * step + col];
+                const float w = s_weight[warp][i], v = part(i)[r * d + col];
                 o += w != 0.f ? w * v : 0.f;                         // a part without weight may hold anything
             }
             out[col] = rounded<T>(o * scale);
         }
-        __syncthreads();
+        __syncwarp();
     }
 }
 
@@ -264,5 +262,17 @@ bool decode_takes(const AttendArgs &a, int dtype);
 uint32_t decode_ctas(uint32_t head_dim);
 constexpr int kDecodeRows = 32;
 int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream);      // pairs: a bound of a sequence's tokens * heads per key / value head
+
+// The same types with heads of up to 128, everything on 16-byte boundaries: many new tokens (mgq_paged_prefill.cu).
+bool prefill_takes(const AttendArgs &a, int dtype);
+constexpr uint32_t kPrefillCtas = 148, kPrefillRows = 256;
+int launch_prefill(const AttendArgs &a, int dtype, cudaStream_t stream);
+
+// {head_dim, kv_heads, pages * page_size} of a cache, for boxes of 64 elements by `tokens` tokens of one head in the 128-byte swizzle.  What
+// lies outside the cache reads as zero.
+struct CacheMaps {
+    CUtensorMap k, v;
+};
+int encode_caches(CacheMaps &maps, int dtype, const AttendArgs &a, uint32_t tokens);         // mgq_paged_decode.cu
 
 }  // namespace mgq

@@ -19,7 +19,7 @@ int check_table(const char *what, uint32_t sequences, uint32_t page_size, uint32
 {
     if (int rc = check_pages(what, page_size, pages)) return rc;
     if (sequences == 0 || sequences > MGQ_PAGED_MAX_SEQUENCES) return fail(MGQ_ERR_SHAPE, "%s: %u sequences (1 to %d)", what, sequences, MGQ_PAGED_MAX_SEQUENCES);
-    if (table_width == 0 || (unsigned long long)table_width * page_size >= (1ull << 31))
+    if (table_width == 0 || (unsigned long long)table_width * page_size >= (1ull << 30))
         return fail(MGQ_ERR_SHAPE, "%s: a table of %u pages of %u tokens per sequence", what, table_width, page_size);
     return MGQ_OK;
 }

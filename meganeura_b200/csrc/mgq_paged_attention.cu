@@ -131,15 +131,15 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
                 if (r >= pairs) break;
                 const uint32_t token = r / g.heads, head = r - token * g.heads;
                 if (whole) static_cast<T *>(a.out)[(size_t)(g.row0 + token) * a.out_pitch + (g.head0 + head) * d + col] = rounded<T>(acc[c][r] * s_scale[r]);
-                else       part[r * (d + 2) + col] = acc[c][r];
+                else       part[r * d + col] = acc[c][r];
             }
         }
         if (!whole) {
             if (lane == 0)
 #pragma unroll
                 for (int i = 0; i < kRowsPerWarp; i++) {
-                    part[(warp * kRowsPerWarp + i) * (d + 2) + d] = m[i];
-                    part[(warp * kRowsPerWarp + i) * (d + 2) + d + 1] = l[i];
+                    part[kRows * d + 2 * (warp * kRowsPerWarp + i)] = m[i];
+                    part[kRows * d + 2 * (warp * kRowsPerWarp + i) + 1] = l[i];
                 }
             if (t == 0) name_part(a, blockIdx.x, g);
         }
@@ -167,7 +167,7 @@ size_t paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t hea
     (void)heads; (void)kv_heads; (void)max_fresh;
     auto bytes = [&](uint32_t ctas, size_t rows) { return ctas * 2 * (sizeof(PartHead) + rows * (head_dim + 2) * sizeof(float)); };
     const size_t plain = bytes(kCtas, kRows);
-    return dtype == MGQ_FMT_F32 ? plain : max(plain, bytes(decode_ctas(head_dim), kDecodeRows));
+    return dtype == MGQ_FMT_F32 ? plain : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
 }
 
 int launch_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
@@ -188,9 +188,18 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
         a.heads = static_cast<PartHead *>(workspace);
         a.parts = reinterpret_cast<float *>(a.heads + 2 * ctas);
     };
+    const uint32_t pairs = (uint32_t)min((unsigned long long)max_fresh * a.group, 0xFFFFFFFFull);
     if (decode_takes(a, dtype)) {
         room(decode_ctas(head_dim));
-        return launch_decode(a, dtype, (uint32_t)min((unsigned long long)max_fresh * a.group, 0xFFFFFFFFull), s);
+        if (pairs <= kDecodeRows || !prefill_takes(a, dtype)) return launch_decode(a, dtype, pairs, s);
+        // both kinds of sequences may be there
+        a.rows_to = kDecodeRows;
+        if (int rc = launch_decode(a, dtype, kDecodeRows, s)) return rc;
+        a.rows_from = kDecodeRows + 1;
+        a.rows_to = 0xFFFFFFFFu;
+        a.heads = reinterpret_cast<PartHead *>(a.parts + (size_t)decode_ctas(head_dim) * 2 * kDecodeRows * (head_dim + 2));
+        a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);
+        return launch_prefill(a, dtype, s);
     }
     room(kCtas);
     switch (dtype) {

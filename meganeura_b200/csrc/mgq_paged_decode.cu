@@ -80,10 +80,6 @@ __device__ __forceinline__ bool not_finite8(const uint4 &v)
     return bad;
 }
 
-struct CacheMaps {
-    CUtensorMap k, v;                                    // {head_dim, kv_heads, pages * page_size}, boxes of 64 elements by 16 (or 8) tokens
-};
-
 template <typename T, int D, int MT>                     // D: head size rounded up to 64, 128 or 256; MT: blocks of 16 rows
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const __grid_constant__ CacheMaps maps, const AttendArgs a)
 {
@@ -447,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                     *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d + c * kChunk + col) =
                         *reinterpret_cast<const uint32_t *>(pair);
                 } else {
-                    *reinterpret_cast<float2 *>(part + r * (d + 2) + c * kChunk + col) = make_float2(x, y);
+                    *reinterpret_cast<float2 *>(part + r * d + c * kChunk + col) = make_float2(x, y);
                 }
             }
             __syncthreads();
@@ -456,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             if (t < pairs) {
                 float top;
                 const float sum = total(t, top);
-                part[t * (d + 2) + d] = top;
-                part[t * (d + 2) + d + 1] = sum;
+                part[ROWS * d + 2 * t] = top;
+                part[ROWS * d + 2 * t + 1] = sum;
             }
             if (t == 0) name_part(a, blockIdx.x, g);
             __syncthreads();                             // before the next unit's maxima
@@ -470,17 +466,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             slot = slot == kStages - 1 ? 0 : slot + 1;
             parity ^= slot == 0;
         }
-}
-
-// Tokens of one head by 64 elements, 128-byte swizzle; what lies outside the cache reads as zero.
-int encode_cache(EncodeTiledFn encode, CUtensorMap &map, const void *base, int dtype, const AttendArgs &a, uint32_t tokens)
-{
-    const cuuint64_t dims[3] = {a.d, a.kv_heads, (cuuint64_t)a.pages << a.page_shift};
-    const cuuint64_t strides[2] = {(cuuint64_t)a.d * 2, (cuuint64_t)a.kv_heads * a.d * 2};
-    const cuuint32_t box[3] = {64, 1, tokens}, elem[3] = {1, 1, 1};
-    const CUresult cr = encode(&map, dtype == MGQ_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box,
-                               elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return cr == CUDA_SUCCESS ? MGQ_OK : fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
 }
 
 template <typename T, int D, int MT>
@@ -513,25 +498,37 @@ bool decode_takes(const AttendArgs &a, int dtype)
 
 uint32_t decode_ctas(uint32_t head_dim) { return 148 * (head_dim <= 64 ? ctas_per_sm<64>() : head_dim <= 128 ? ctas_per_sm<128>() : ctas_per_sm<256>()); }
 
-int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream)
+int encode_caches(CacheMaps &maps, int dtype, const AttendArgs &a, uint32_t tokens)
 {
     EncodeTiledFn encode = nullptr;
     if (int rc = encode_fn(encode)) return rc;
+    const cuuint64_t dims[3] = {a.d, a.kv_heads, (cuuint64_t)a.pages << a.page_shift};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.d * 2, (cuuint64_t)a.kv_heads * a.d * 2};
+    const cuuint32_t box[3] = {64, 1, tokens}, elem[3] = {1, 1, 1};
+    const CUtensorMapDataType type = dtype == MGQ_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < 2; i++) {
+        const CUresult cr = encode(i ? &maps.v : &maps.k, type, 3, const_cast<void *>(i ? a.v : a.k), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) return fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    }
+    return MGQ_OK;
+}
+
+int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream)
+{
     CacheMaps maps;
-    const uint32_t tokens = a.page_shift == 3 ? 8 : kStep;
-    if (int rc = encode_cache(encode, maps.k, a.k, dtype, a, tokens)) return rc;
-    if (int rc = encode_cache(encode, maps.v, a.v, dtype, a, tokens)) return rc;
+    if (int rc = encode_caches(maps, dtype, a, a.page_shift == 3 ? 8 : kStep)) return rc;
     return dtype == MGQ_FMT_F16 ? launch_typed<__half>(a, maps, pairs, stream) : launch_typed<__nv_bfloat16>(a, maps, pairs, stream);
 }
 
-int decode_status()
+int paged_status()
 {
     unsigned int err = 0;
     MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_decode_error, sizeof err));
-    if (!err) return MGQ_OK;
+    if (!err) return prefill_status();
     const unsigned int zero = 0;
     MGQ_CUDA(cudaMemcpyToSymbol(g_decode_error, &zero, sizeof zero));
-    return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the paged attention kernel ran out");
+    return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the paged attention of few tokens ran out");
 }
 
 }  // namespace mgq

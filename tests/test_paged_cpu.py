@@ -51,7 +51,7 @@ def verify(**change):
     *[(plan, {name: None}, NULL) for name in ("cached", "fresh", "table", "held", "free", "count", "starts", "lengths", "positions", "slots", "lacking")],
     (plan, dict(page_size=12), SHAPE), (plan, dict(page_size=4), SHAPE), (plan, dict(page_size=2048), SHAPE), (plan, dict(pages=0), SHAPE),
     (plan, dict(pages=1 << 28), SHAPE), (plan, dict(sequences=0), SHAPE), (plan, dict(sequences=4097), SHAPE), (plan, dict(width=0), SHAPE),
-    (plan, dict(width=1 << 27), SHAPE), (plan, dict(rows=0), SHAPE), (plan, dict(rows=1 << 31), SHAPE),
+    (plan, dict(width=1 << 26), SHAPE), (plan, dict(rows=0), SHAPE), (plan, dict(rows=1 << 31), SHAPE),
     *[(trim, {name: None}, NULL) for name in ("lengths", "table", "held", "free", "count")],
     (trim, dict(page_size=24), SHAPE), (trim, dict(sequences=5000), SHAPE), (trim, dict(width=0), SHAPE),
     *[(append, {name: None}, NULL) for name in ("k", "v", "positions", "slots", "k_cache", "v_cache", "q_out")],

@@ -135,7 +135,9 @@ BATCHES = {
 
 def run(q, k, v, table, starts, lengths, most, **kw):
     from meganeura_b200 import ops
-    return ops.paged_attention(q, k, v, words(table), words(starts), words(lengths), most, **kw)
+    out = ops.paged_attention(q, k, v, words(table), words(starts), words(lengths), most, **kw)
+    ops.device_status()                                            # no wait inside the kernels ran out
+    return out
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -267,6 +269,19 @@ def test_attention_of_long_sequences_is_split_and_joined():
                                                      ("bf16", 2, 1, 128, [7000], [100])):
         q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 32, cached, fresh, gain=2.0)
         check_attention(dtype, q, k, v, table, starts, lengths, run(q, k, v, table, starts, lengths, max(fresh)), d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,window", [("bf16", 8, 2, 128, 0), ("f16", 6, 3, 64, 0), ("bf16", 8, 2, 80, 700), ("f16", 3, 1, 64, 100)])
+def test_attention_of_long_portions(dtype, heads, kv_heads, d, window):
+    """Enough work for several units per CTA and many blocks of keys per unit.  The oracle takes a sample of the rows."""
+    rng = np.random.default_rng(17)
+    cached, fresh = [3000, 0, 900, 5000], [2100, 2500, 1300, 1000]
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 32, cached, fresh, gain=1.5)
+    got = run(q, k, v, table, starts, lengths, 2500, window=window)
+    for s in range(4):
+        for i in sorted({0, 1, 63, 64, 127, 128, fresh[s] - 1} | set(rng.integers(0, fresh[s], 12).tolist())):
+            r, n = int(starts[s]) + i, int(lengths[s]) - fresh[s] + i + 1               # the row alone, as the last token of its sequence
+            check_attention(dtype, q[r:r + 1], k, v, table[s:s + 1], [0, 1], [n], got[r:r + 1], d ** -0.5, window)
 
 
 def test_attention_with_many_sequences():
