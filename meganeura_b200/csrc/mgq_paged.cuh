@@ -53,7 +53,7 @@ struct Segment {
     bool first, last;                               // of its unit
 };
 
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, int EXTRA>
 struct Walk {
     uint32_t slice, slices, per_tile;               // heads of a unit, units per key / value head, tokens of a unit
     uint32_t s, head, tile, off;                    // the next segment: sequence, head block, token block, key blocks behind
@@ -81,7 +81,7 @@ struct Walk {
     {
         uint32_t lo, hi;
         keys(a, t, lo, hi);
-        return max(1u, hi - lo);
+        return EXTRA + max(1u, hi - lo);
     }
     __device__ __forceinline__ unsigned long long head_cost(const AttendArgs &a) const
     {
@@ -151,36 +151,39 @@ struct Walk {
 
     __device__ __forceinline__ bool next(const AttendArgs &a, Segment &g)
     {
-        if (!left) return false;
-        while (tile == tiles) {                          // behind the last unit of a head, or a sequence without any
-            tile = 0;
-            if (tiles && ++head < a.kv_heads * slices) break;
-            head = 0;
-            open(a, s + 1);                              // `left` says that there is one
+        while (left) {
+            while (tile == tiles) {                      // behind the last unit of a head, or a sequence without any
+                tile = 0;
+                if (tiles && ++head < a.kv_heads * slices) break;
+                head = 0;
+                open(a, s + 1);                          // `left` says that there is one
+            }
+            uint32_t lo, hi;
+            keys(a, tile, lo, hi);
+            const uint32_t all = EXTRA + max(1u, hi - lo), take = (uint32_t)min((unsigned long long)(all - off), left);
+            const uint32_t from = max(off, (uint32_t)EXTRA) - EXTRA, to = max(off + take, (uint32_t)EXTRA) - EXTRA;       // its own blocks
+            g.row0 = r0 + tile * per_tile;
+            g.tokens = min(per_tile, n - tile * per_tile);
+            g.kv = head / slices;
+            const uint32_t sub = head - g.kv * slices;
+            g.head0 = g.kv * a.group + sub * slice;
+            g.heads = min(slice, a.group - sub * slice);
+            g.pos0 = len - (int)n + (int)(tile * per_tile);
+            g.len = len;
+            g.table = a.table + (size_t)s * a.table_width;
+            g.begin = lo + from;
+            g.end = min(lo + to, hi);                    // none where no row sees a key
+            g.first = from == 0;
+            off += take;
+            left -= take;
+            g.last = off == all;
+            if (g.last) {
+                off = 0;
+                tile++;
+            }
+            if (to > from) return true;                  // else the piece ends in front of the unit's first block
         }
-        uint32_t lo, hi;
-        keys(a, tile, lo, hi);
-        const uint32_t all = max(1u, hi - lo), take = (uint32_t)min((unsigned long long)(all - off), left);
-        g.row0 = r0 + tile * per_tile;
-        g.tokens = min(per_tile, n - tile * per_tile);
-        g.kv = head / slices;
-        const uint32_t sub = head - g.kv * slices;
-        g.head0 = g.kv * a.group + sub * slice;
-        g.heads = min(slice, a.group - sub * slice);
-        g.pos0 = len - (int)n + (int)(tile * per_tile);
-        g.len = len;
-        g.table = a.table + (size_t)s * a.table_width;
-        g.begin = lo + off;
-        g.end = min(lo + off + take, hi);                // none where no row sees a key
-        g.first = off == 0;
-        off += take;
-        left -= take;
-        g.last = off == all;
-        if (g.last) {
-            off = 0;
-            tile++;
-        }
-        return true;
+        return false;
     }
 };
 

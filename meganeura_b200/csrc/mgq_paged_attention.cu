@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     float *s_q = s_mem, *s_k = s_q + kRows * d4, *s_v = s_k + kKeys * pitch;
     pdl_launch_dependents();
     pdl_wait();
-    Walk<kRows, kKeys> walk;
+    Walk<kRows, kKeys, 1> walk;
     walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 {
     constexpr int ROWS = 16 * MT, NT = D / 8, KT = D / 16, PARTS = D / 64, QB = D * 2 + 16;
     constexpr uint32_t kStage = stage_bytes<D>();
-    using Way = Walk<ROWS, kBlock>;
+    using Way = Walk<ROWS, kBlock, 1>;
     extern __shared__ uint8_t s_raw[];
     __shared__ unsigned long long s_walk[40];
     __shared__ __align__(8) unsigned long long s_full[kWarps][kStages];
