@@ -5,11 +5,12 @@
 // and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.
 //   warps 0-7, 8-15 softmax of tile 0 and 1, two threads per row with 64 keys of a block each (one per row took 3200 cycles per block, most of them
 //                   waiting for its own results): S from TMEM, running maximum and sum in f32, P back into TMEM over S (as the
-//                   16-bit left operand of the second product); queries into shared memory, results out of TMEM.
+//                   16-bit left operand of the second product), results out of TMEM.
 //   warp 16         keys and values: TMA boxes of a page's tokens (128 at most) by 64 elements, a lane each, into a ring of stages that hold
 //                   128 keys or 128 values.
 //   warp 17         issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
-//                   S(j + 1) done knows that O(j) is.
+//                   S(j + 1) done knows that O(j) is.  O(j) begins when the first half of either thread's weights is there.
+//   warp 18         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
 // Sums are kept relative to a maximum that may be 2^8 too low: only where a row's maximum grows by more do its threads agree on a new one and scale O.  Weights are
 // rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.
 // TMEM: S0, S1 (128 columns each, P in the first 32 of either half), O0, O1.
@@ -21,7 +22,8 @@
 namespace mgq {
 namespace {
 
-constexpr int kThreads = 576;
+constexpr int kThreads = 608;
+constexpr int kSoft = 2;                                 // of eight pairs of exponentials, those that go to the multiply-add units
 constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
@@ -33,12 +35,11 @@ __device__ unsigned int g_prefill_error;
 using Way = Walk<kPrefillRows, kKeys, kExtra>;
 struct __align__(16) Shared {
     float top[2][2][kTile];                              // of a row's two threads: maximum, at the end sum of weights
-    unsigned long long full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2];
-    Way way[4];                                          // of the tiles' warps, the producer, the issuer
-    Segment seg[6];                                      // two of either tile's warps, then the producer's and the issuer's
+    unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2];
+    Way way[2];                                          // of the producers of keys and of queries
+    Segment kv_seg, seg[2];                              // of the producer of keys; of everybody else, two units in turn, no tokens behind the last
     uint32_t there[8][4];                                // keys of a block that exist, for the last eight blocks
     uint32_t tmem;
-    int more[2];
     volatile int failed;
 };
 template <int D> constexpr size_t smem_bytes() { return (size_t)(2 + stages<D>()) * stage_bytes<D>() + sizeof(Shared); }
@@ -61,10 +62,11 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The largest; NaN if one is NaN.
 __device__ __forceinline__ float max3(float x, float y, float z)
 {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
 // (x, y) * s - b and (x, y) += (z, w), two elements per instruction.
@@ -81,6 +83,41 @@ __device__ __forceinline__ void add_pair(float &x, float &y, float z, float w)
         "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
         "add.rn.f32x2 a, a, b;\n\t"
         "mov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(z), "f"(w));
+}
+// 2^x and 2^y of finite x and y <= 127 on the multiply-add units: 16 exponentials per cycle leave an SM idle for half of attention's time
+// (heads of 128).  x = n + f with n whole and f in [-1/2, 1/2]: 2^f by a polynomial fitted to the least relative error (7.5e-5 of degree 3 for
+// bf16 weights, 2.6e-6 of degree 4 for f16 ones), n added to its exponent.  Below 2^-126 the result stays there.
+template <typename T>
+__device__ __forceinline__ void exp2_pair(float &x, float &y)
+{
+    constexpr bool kFour = std::is_same<T, __half>::value;
+    const float c0 = kFour ? 0.9999992847442627f : 0.9999280571937561f, c1 = kFour ? 0.6931217908859253f : 0.6932609677314758f;
+    const float c2 = kFour ? 0.240247443318367f : 0.2426111251115799f, c3 = kFour ? 0.05591785907745361f : 0.0551716685295105f, c4 = 0.009570102207362652f;
+    x = fmaxf(x, -126.f);
+    y = fmaxf(y, -126.f);
+    const float magic = 12582912.f;                      // 1.5 * 2^23: the sum's last bits are the rounded value
+    float rx, ry;
+    if constexpr (kFour)
+        asm("{\n\t.reg .b64 v, r, f, p, m, c;\n\t"
+            "mov.b64 v, {%0, %1};\n\tmov.b64 m, {%4, %4};\n\tadd.rn.f32x2 r, v, m;\n\tmov.b64 {%2, %3}, r;\n\t"
+            "sub.rn.f32x2 f, r, m;\n\tsub.rn.f32x2 f, v, f;\n\t"
+            "mov.b64 p, {%9, %9};\n\tmov.b64 c, {%8, %8};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 {%0, %1}, p;\n\t}"
+            : "+f"(x), "+f"(y), "=&f"(rx), "=&f"(ry) : "f"(magic), "f"(c0), "f"(c1), "f"(c2), "f"(c3), "f"(c4));
+    else
+        asm("{\n\t.reg .b64 v, r, f, p, m, c;\n\t"
+            "mov.b64 v, {%0, %1};\n\tmov.b64 m, {%4, %4};\n\tadd.rn.f32x2 r, v, m;\n\tmov.b64 {%2, %3}, r;\n\t"
+            "sub.rn.f32x2 f, r, m;\n\tsub.rn.f32x2 f, v, f;\n\t"
+            "mov.b64 p, {%8, %8};\n\tmov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 {%0, %1}, p;\n\t}"
+            : "+f"(x), "+f"(y), "=&f"(rx), "=&f"(ry) : "f"(magic), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+    x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(rx) << 23));
+    y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ry) << 23));
 }
 // 64 columns of this lane's row, one wait for all of them.
 __device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&y)[64])
@@ -115,12 +152,11 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int base)
     return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - hi + lo)) << lo;
 }
 
-// Key blocks of one tile of a segment: [g.begin, what is returned).
-__device__ __forceinline__ uint32_t tile_end(const Segment &g, uint32_t tile)
+// Key blocks of one tile of a segment: [g.begin, what is returned).  last_token: that of the tile's last row, were all tokens there.
+__device__ __forceinline__ uint32_t tile_end(const Segment &g, uint32_t tile, uint32_t last_token)
 {
-    const uint32_t pairs = g.tokens * g.heads;
-    if (tile * kTile >= pairs) return g.begin;
-    const int last = min(g.pos0 + (int)((min(pairs, (tile + 1) * kTile) - 1) / g.heads), g.len - 1);
+    if (tile * kTile >= g.tokens * g.heads) return g.begin;
+    const int last = min(g.pos0 + (int)min(last_token, g.tokens - 1), g.len - 1);
     return last < 0 ? g.begin : max(g.begin, min(g.end, (uint32_t)last / kKeys + 1));
 }
 
@@ -161,7 +197,7 @@ __device__ __noinline__ void row_again(const AttendArgs &a, const Segment &g, ui
 }
 
 template <typename T, int D>                             // D: head size rounded up to 64 or 128
-__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ CacheMaps maps, const AttendArgs a)
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ CacheMaps maps, const __grid_constant__ CUtensorMap q_map, const AttendArgs a)
 {
     constexpr int S = stages<D>(), PARTS = D / 64;
     constexpr uint32_t kStage = stage_bytes<D>();
@@ -182,9 +218,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             mbar_init(&sh.full[s], 1);
             mbar_init(&sh.empty[s], 1);
         }
+        mbar_init(&sh.q_full, 1);
+        mbar_init(&sh.q_empty, 3);                                        // the issuer, both tiles' warps
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.q_full[i], 8);
             mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_half[i], 8);
             mbar_init(&sh.p_full[i], 8);
             mbar_init(&sh.o_full[i], 1);
         }
@@ -198,33 +236,38 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t role = warp < 16 ? warp >> 3 : warp - 14;              // 0, 1: softmax of a tile, 2: producer, 3: issuer
+    const uint32_t slice = min(a.group, kPrefillRows), rows = kPrefillRows / slice * slice;       // heads of a unit, rows that TMA fills
     {
         Way way;
         way.begin(a, blockIdx.x, gridDim.x, 1, reinterpret_cast<unsigned long long *>(s_q));
-        if (lane == 0 && (warp & 7u) == (role < 2 ? 0 : role - 2)) sh.way[role] = way;
+        if (lane == 0 && (warp == 16 || warp == 18)) sh.way[warp == 18] = way;
+    }
+    for (uint32_t i = tid; i < (kPrefillRows - rows) * PARTS * 8; i += kThreads) {            // the others are zero for good
+        const uint32_t part = i / ((kPrefillRows - rows) * 8), at = i - part * (kPrefillRows - rows) * 8;
+        *reinterpret_cast<uint4 *>(s_q + part * 2 * kHalf + rows * 128 + at * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
     if (tid == 0) clear_parts(a, blockIdx.x);
-    __syncwarp();
-    // The next segment of the producer or the issuer, if there is one.
-    auto fetch = [&]() {
-        int more = 0;
-        if (lane == 0) more = sh.way[role].next(a, sh.seg[role + 2]);
-        __syncwarp();
-        return __shfl_sync(0xffffffffu, more, 0) != 0;
-    };
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    // the tokens of the tiles' last rows
+    const uint32_t last_token[2] = {(kTile - 1) / slice, (2 * kTile - 1) / slice};
     auto wait = [&](unsigned long long *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh.failed, &g_prefill_error)) != 0; };
 
-    if (role == 2) {
+    if (warp == 16) {
         const uint32_t shift = a.page_shift, page_keys = 1u << shift, box = min(page_keys, kKeys), boxes = kKeys / box, gone = a.pages << shift;
         uint32_t slot = 0, round = 0, block = 0;
         int armed = 0;
         bool ok = true;
-        while (ok && fetch()) {
-            const Segment &g = sh.seg[4];
+        while (ok) {
+            int more_units = 0;
+            if (lane == 0) more_units = sh.way[0].next(a, sh.kv_seg);
+            __syncwarp();
+            if (!__shfl_sync(0xffffffffu, more_units, 0)) break;
+            const Segment &g = sh.kv_seg;
             const int len = g.len, kv = (int)g.kv;
             const uint32_t *table = g.table;
-            for (uint32_t kb = g.begin; ok && kb < g.end; kb++, block++) {
+            const uint32_t kb_end = g.end;
+            for (uint32_t kb = g.begin; ok && kb < kb_end; kb++, block++) {
                 // lane = box of the block + boxes * group of 64 elements
                 const uint32_t b = lane % boxes, part = lane / boxes, key = kb * kKeys + b * box;
                 uint32_t y = gone, have = 0;
@@ -261,48 +304,75 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (slot-- == 0) { slot = S - 1; round--; }
                 for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.full[slot], round & 1u); w++) { }
             }
-    } else if (role == 3) {
+    } else if (warp == 18) {
+        uint32_t unit = 0;
+        bool ok = true, more = true;
+        for (; more; unit++) {
+            if (!(ok = wait(&sh.q_empty, (unit & 1u) ^ 1u))) break;
+            if (lane == 0) {
+                Segment &g = sh.seg[unit & 1u];
+                more = sh.way[1].next(a, g);
+                if (!more) g.tokens = 0;
+                if (more && g.end > g.begin) {
+                    mbar_arrive_expect_tx(&sh.q_full, PARTS * rows * 128);
+                    for (int c = 0; c < PARTS; c++) tma_load_3d(smem_u32(s_q) + c * 2 * kHalf, &q_map, c * 64, (int)g.head0, (int)g.row0, &sh.q_full);
+                } else {
+                    mbar_arrive(&sh.q_full);
+                }
+            }
+            more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+        }
+        if (!ok && lane == 0 && unit > 0)                // given up: the copy in flight lands before the CTA exits
+            for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.q_full, (unit - 1) & 1u); w++) { }
+    } else if (warp == 17) {
         const bool leader = elect_one();
         const uint32_t q16 = smem_u32(s_q) >> 4, ring16 = smem_u32(ring) >> 4;
-        uint32_t slot = 0, round = 0, q_seen = 0, p_seen = 0;             // parities of the two tiles in bits 0 and 1
+        uint32_t slot = 0, round = 0, p_seen = 0;                         // p_seen: parities of the two tiles in bits 0 and 1
         bool ok = true;
         auto advance = [&]() {
             if (++slot == S) { slot = 0; round++; }
         };
         auto scores = [&](uint32_t tile, uint32_t at) {
             if (leader) {
-                const uint32_t q = q16 + tile * (kStage / 16), k = ring16 + at * (kStage / 16);
+                const uint32_t q = q16 + tile * (kHalf / 16), k = ring16 + at * (kStage / 16);
                 umma_step<false>(tmem + tile * 128, q, k, kInstrS);
 #pragma unroll
-                for (uint32_t i = 1; i < D / 16; i++) umma_step<true>(tmem + tile * 128, q + i / 4 * (kHalf / 16) + i % 4 * 2, k + i / 4 * (kHalf / 16) + i % 4 * 2, kInstrS);
+                for (uint32_t i = 1; i < D / 16; i++) umma_step<true>(tmem + tile * 128, q + i / 4 * (2 * kHalf / 16) + i % 4 * 2, k + i / 4 * (kHalf / 16) + i % 4 * 2, kInstrS);
                 umma_commit(&sh.s_full[tile]);
             }
             __syncwarp();
         };
-        auto values = [&](uint32_t tile, uint32_t at, bool first) {
+        // 16 keys per product; the quarters 0 and 2 of the block's keys first, whose weights come first
+        auto values = [&](uint32_t tile, uint32_t at, uint32_t part, bool first) {
             if (leader) {
                 const uint32_t v = ring16 + at * (kStage / 16), o = tmem + 256 + tile * D, p = tmem + tile * 128;
 #pragma unroll
-                for (uint32_t i = 0; i < kKeys / 16; i++) umma_f16_ts_mn(o, p + i / 4 * 64 + i % 4 * 8, v + i * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0);
+                for (uint32_t i = 0; i < kKeys / 32; i++) {
+                    const uint32_t step = i / 2 * 4 + part * 2 + i % 2;
+                    umma_f16_ts_mn(o, p + step / 4 * 64 + step % 4 * 8, v + step * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0 || part > 0);
+                }
             }
             __syncwarp();
         };
-        while (ok && fetch()) {
-            const Segment &g = sh.seg[5];
-            const uint32_t begin = g.begin, end = g.end, stop[2] = {tile_end(g, 0), tile_end(g, 1)};
-            if (end <= begin) continue;
+        for (uint32_t unit = 0;; unit++) {
+            if (!(ok = wait(&sh.q_full, unit & 1u))) break;
+            const Segment &g = sh.seg[unit & 1u];
+            if (g.tokens == 0) break;
+            const uint32_t begin = g.begin, end = g.end, stop[2] = {tile_end(g, 0, last_token[0]), tile_end(g, 1, last_token[1])};
+            __syncwarp();
+            if (end <= begin) {
+                if (leader) mbar_arrive(&sh.q_empty);
+                continue;
+            }
             if (!(ok = wait(&sh.full[slot], round & 1u))) break;
             tc_fence_after();
 #pragma unroll
             for (uint32_t tile = 0; tile < 2; tile++)
-                if (ok && stop[tile] > begin) {
-                    if (!(ok = wait(&sh.q_full[tile], q_seen >> tile & 1u))) break;
-                    q_seen ^= 1u << tile;
-                    tc_fence_after();
-                    scores(tile, slot);
-                }
-            if (!ok) break;
-            if (leader) umma_commit(&sh.empty[slot]);
+                if (stop[tile] > begin) scores(tile, slot);
+            if (leader) {
+                umma_commit(&sh.empty[slot]);
+                if (begin + 1 == end) umma_commit(&sh.q_empty);
+            }
             __syncwarp();
             advance();
             for (uint32_t kb = begin; ok && kb < end; kb++) {
@@ -315,10 +385,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
 #pragma unroll
                 for (uint32_t tile = 0; tile < 2; tile++) {
                     if (stop[tile] > kb) {
+                        if (!(ok = wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
+                        tc_fence_after();
+                        values(tile, v_slot, 0, kb == begin);
                         if (!(ok = wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
                         p_seen ^= 1u << tile;
                         tc_fence_after();
-                        values(tile, v_slot, kb == begin);
+                        values(tile, v_slot, 1, false);
                         if (kb + 1 == stop[tile] && leader) umma_commit(&sh.o_full[tile]);
                         __syncwarp();
                     }
@@ -335,54 +408,34 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (leader) umma_commit(&sh.empty[v_slot]);
                 if (more) {
                     if (!waited && !(ok = wait(&sh.full[slot], round & 1u))) break;
-                    if (leader) umma_commit(&sh.empty[slot]);
+                    if (leader) {
+                        umma_commit(&sh.empty[slot]);
+                        if (kb + 2 == end) umma_commit(&sh.q_empty);      // no more scores of this unit
+                    }
                     advance();
                 }
                 __syncwarp();
             }
+            if (!ok) break;
         }
     } else {
         // thread = row of the tile and half of a block's keys, of O's columns, of the query's pieces
-        const uint32_t tile = role, half = warp >> 2 & 1u, quad = warp & 3u, r_tile = quad * 32 + lane, row = tile * kTile + r_tile;
+        const uint32_t tile = warp >> 3, half = warp >> 2 & 1u, quad = warp & 3u, r_tile = quad * 32 + lane, row = tile * kTile + r_tile;
         const uint32_t lanes = (quad * 32u) << 16, s_at = tmem + tile * 128 + half * 64 + lanes, o_at = tmem + 256 + tile * D + half * (D / 2) + lanes, d = a.d;
-        const float scale = fabsf(a.scale_log2);
-        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;      // a negative scale turns the queries' signs
+        const float scale = a.scale_log2;
+        const uint32_t token = row / slice, head = row - token * slice, first_token = tile * kTile / slice;     // of this row, of the tile's first
         uint32_t slot = 0, round = 0, block = 0;         // of the ring, as the producer counts
-        uint32_t s_seen = 0, o_seen = 0, turn = 0;
+        uint32_t s_seen = 0, o_seen = 0;
         bool ok = true;
-        // the tile's next segment: one thread looks for it, all meet
-        auto fetch_tile = [&]() {
-            if (half == 0 && r_tile == 0) sh.more[tile] = sh.way[tile].next(a, sh.seg[2 * tile + (turn & 1u)]);
-            turn++;
-            any_of_tile(tile, false);
-            return sh.more[tile] != 0;
-        };
-        // this thread's half of a query into the swizzled tile; heads beyond d and rows behind the last pair are zero
-        auto load_q = [&](const Segment &g) {
-            if (tile_end(g, tile) <= g.begin) return;
-            const uint32_t token = row / g.heads, head = row - token * g.heads;
-            const bool live = row < g.tokens * g.heads;
-            const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d);
-#pragma unroll
-            for (uint32_t i = 0; i < D / 16; i++) {
-                const uint32_t c = half * (D / 16) + i;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (live && c * 8 < d) v = src[c];
-                v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-                *reinterpret_cast<uint4 *>(s_q + tile * kStage + c / 8 * kHalf + r_tile * 128 + ((c % 8) ^ (r_tile & 7u)) * 16) = v;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.q_full[tile]);
-        };
         // A wait that runs out is noted and carried to the next meeting of the tile's warps, where all of them leave.
-        bool live_seg = fetch_tile();
-        if (live_seg) load_q(sh.seg[2 * tile]);
-        while (live_seg) {
-            const Segment &g = sh.seg[2 * tile + ((turn - 1) & 1u)];
-            const uint32_t begin = g.begin, end = g.end, stop = tile_end(g, tile), pairs = g.tokens * g.heads;
-            const int pos = row < pairs ? g.pos0 + (int)(row / g.heads) : -1, first_pos = g.pos0 + (int)(tile * kTile / g.heads);
-            const int last_pos = g.pos0 + (int)((min(pairs, (tile + 1) * kTile) - 1) / g.heads), window = (int)a.window;
+        for (uint32_t unit = 0;; unit++) {
+            ok = wait(&sh.q_full, unit & 1u);
+            const Segment &g = sh.seg[unit & 1u];
+            if (any_of_tile(tile, !ok)) break;
+            if (g.tokens == 0) break;
+            const uint32_t begin = g.begin, end = g.end, stop = tile_end(g, tile, last_token[tile]), pairs = g.tokens * g.heads;
+            const int pos = row < pairs ? g.pos0 + (int)token : -1, first_pos = g.pos0 + (int)first_token;
+            const int last_pos = g.pos0 + (int)min(last_token[tile], g.tokens - 1), window = (int)a.window;
             float m = -INFINITY, l = 0.f;
             for (uint32_t kb = begin; kb < end; kb++, block++) {
                 if (++slot == S) { slot = 0; round++; }
@@ -402,7 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 tmem_ld64(s_at, s);
                 const int key0 = (int)(kb * kKeys);
                 const bool every = (there[0] & there[1] & there[2] & there[3]) == 0xFFFFFFFFu;
-                if (!every || key0 + (int)kKeys - 1 > first_pos || (window && key0 <= last_pos - window)) {
+                bool plain = every && key0 + (int)kKeys - 1 <= first_pos && !(window && key0 <= last_pos - window);      // nothing is masked
+                if (!plain) {
 #pragma unroll
                     for (int w = 0; w < 2; w++) {
                         const uint32_t seen = (half ? there[2 + w] : there[w]) & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 64 * (int)half + 32 * w);
@@ -417,7 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 for (int e = 12; e < 60; e += 8)
 #pragma unroll
                     for (int i = 0; i < 4; i++) tops[i] = max3(tops[i], s[e + i], s[e + 4 + i]);
-                float top = fmaxf(max3(tops[0], tops[1], s[60]), max3(max3(tops[2], tops[3], s[61]), s[62], s[63])) * scale;
+                float top = max3(max3(tops[0], tops[1], s[60]), max3(tops[2], tops[3], s[61]), max3(s[62], s[62], s[63])) * scale;
+                plain = plain && __all_sync(0xffffffffu, fabsf(top) <= FLT_MAX);       // and all rows are finite
                 if (any_of_tile(tile, !ok || (!(top <= m + 8.f) && top > -INFINITY))) {
                     sh.top[tile][half][r_tile] = top;
                     if (any_of_tile(tile, !ok)) {
@@ -442,21 +497,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 }
                 const float base = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        float x = s[32 * c + 2 * e], y = s[32 * c + 2 * e + 1];
-                        scaled_pair(x, y, scale, -base);
-                        x = exp2_fast(x);
-                        y = exp2_fast(y);
-                        add_pair(sum[e % 2 * 2], sum[e % 2 * 2 + 1], x, y);
-                        p[e] = pack<T>(x, y);
-                    }
-                    tmem_st16(s_at + 16 * c, p);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (!every) {                            // values that nobody sees, whatever the page holds there, become zeros
                     uint8_t *v = ring + v_slot * kStage;
                     for (uint32_t i = half * 128 + r_tile; i < kKeys * PARTS * 8; i += 256) {
@@ -464,30 +504,56 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                         if (!(word >> (key % 32) & 1u)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    any_of_tile(tile, false);            // the product takes keys of both threads' halves from the first signal on
                 }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[tile]);
+                auto weights = [&](int c, bool soft) {   // 32 keys: exponentials, sums, P
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        float x = s[32 * c + 2 * e], y = s[32 * c + 2 * e + 1];
+                        scaled_pair(x, y, scale, -base);
+                        if (soft && e % 8 < kSoft) {
+                            exp2_pair<T>(x, y);
+                        } else {
+                            x = exp2_fast(x);
+                            y = exp2_fast(y);
+                        }
+                        add_pair(sum[e % 2 * 2], sum[e % 2 * 2 + 1], x, y);
+                        p[e] = pack<T>(x, y);
+                    }
+                    tmem_st16(s_at + 16 * c, p);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c ? &sh.p_full[tile] : &sh.p_half[tile]);
+                };
+                if (plain) {
+                    weights(0, true);
+                    weights(1, true);
+                } else {
+                    weights(0, false);
+                    weights(1, false);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             if (!ok) break;
-            // the next unit's queries, while the last product runs: the scores of this one are done with them
-            const bool more = fetch_tile();
-            if (more) load_q(sh.seg[2 * tile + ((turn - 1) & 1u)]);
+            // this tile's scores are done with the queries (its warps have met in this unit)
+            if (half == 0 && r_tile == 0) mbar_arrive(&sh.q_empty);
             if (stop > begin) {
                 ok = wait(&sh.o_full[tile], o_seen & 1u);
                 o_seen++;
                 tc_fence_after();
             }
-            sh.top[tile][half][r_tile] = l;
-            if (any_of_tile(tile, !ok)) {
+            if (any_of_tile(tile, !ok)) {                // everybody has read the last maxima
                 ok = false;
                 break;
             }
+            sh.top[tile][half][r_tile] = l;
+            any_of_tile(tile, false);
             l += sh.top[tile][half ^ 1u][r_tile];
             if (tile * kTile < pairs) {
                 const bool alone = g.first && g.last;
-                const uint32_t token = row / g.heads, head = row - token * g.heads, c0 = half * (D / 2);
+                const uint32_t c0 = half * (D / 2);
                 T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d + c0;
                 float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kPrefillRows * (d + 2);
                 const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -548,7 +614,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             any_of_tile(tile, false);                    // sums read, before the next unit's maxima
             tc_fence_before();
             __syncwarp();
-            live_seg = more;
         }
     }
     tc_fence_before();
@@ -561,12 +626,26 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
 }
 
 template <typename T, int D>
-int launch_sized(const AttendArgs &a, const CacheMaps &maps, cudaStream_t stream)
+int launch_sized(const AttendArgs &a, const CacheMaps &maps, const CUtensorMap &q_map, cudaStream_t stream)
 {
     auto *kernel = prefill_kernel<T, D>;
     if (int rc = allow_smem(kernel, smem_bytes<D>())) return rc;
-    if (int rc = launch(kernel, dim3(kPrefillCtas), dim3(kThreads), smem_bytes<D>(), stream, maps, a)) return rc;
+    if (int rc = launch(kernel, dim3(kPrefillCtas), dim3(kThreads), smem_bytes<D>(), stream, maps, q_map, a)) return rc;
     return launch(merge_kernel<T, (int)kPrefillRows>, dim3(kPrefillCtas, 16), dim3(kMergeThreads), 0, stream, a, kPrefillCtas);
+}
+
+// {head_dim, heads, rows} of the queries, for boxes of 64 elements by the heads of a key / value head by the tokens of a unit: as they lie in
+// shared memory then, the pairs of token and head are the rows.
+int encode_queries(CUtensorMap &map, int dtype, const AttendArgs &a)
+{
+    EncodeTiledFn encode = nullptr;
+    if (int rc = encode_fn(encode)) return rc;
+    const cuuint64_t dims[3] = {a.d, (cuuint64_t)a.kv_heads * a.group, a.rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.d * 2, (cuuint64_t)a.q_pitch * 2};
+    const cuuint32_t box[3] = {64, a.group, kPrefillRows / a.group}, elem[3] = {1, 1, 1};
+    const CUresult cr = encode(&map, dtype == MGQ_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(a.q), dims, strides, box,
+                               elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? MGQ_OK : fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
 }
 
 }  // namespace
@@ -574,16 +653,18 @@ int launch_sized(const AttendArgs &a, const CacheMaps &maps, cudaStream_t stream
 bool prefill_takes(const AttendArgs &a, int dtype)
 {
     auto on = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    // masked scores are -inf before they are scaled: a scale of 0 would make them NaN
-    return decode_takes(a, dtype) && a.d <= 128 && fabsf(a.scale_log2) >= 1e-30f && on(a.q) && on(a.out) && a.q_pitch % 8 == 0 && a.out_pitch % 8 == 0;
+    // scores are masked and compared before they are scaled: a scale of 0 would make -inf NaN, a negative one turn the order around
+    return decode_takes(a, dtype) && a.d <= 128 && a.group <= kPrefillRows && a.scale_log2 >= 1e-30f && on(a.q) && on(a.out) && a.q_pitch % 8 == 0 && a.out_pitch % 8 == 0;
 }
 
 int launch_prefill(const AttendArgs &a, int dtype, cudaStream_t stream)
 {
     CacheMaps maps;
     if (int rc = encode_caches(maps, dtype, a, min(1u << a.page_shift, kKeys))) return rc;
-    if (dtype == MGQ_FMT_F16) return a.d <= 64 ? launch_sized<__half, 64>(a, maps, stream) : launch_sized<__half, 128>(a, maps, stream);
-    return a.d <= 64 ? launch_sized<__nv_bfloat16, 64>(a, maps, stream) : launch_sized<__nv_bfloat16, 128>(a, maps, stream);
+    CUtensorMap q_map;
+    if (int rc = encode_queries(q_map, dtype, a)) return rc;
+    if (dtype == MGQ_FMT_F16) return a.d <= 64 ? launch_sized<__half, 64>(a, maps, q_map, stream) : launch_sized<__half, 128>(a, maps, q_map, stream);
+    return a.d <= 64 ? launch_sized<__nv_bfloat16, 64>(a, maps, q_map, stream) : launch_sized<__nv_bfloat16, 128>(a, maps, q_map, stream);
 }
 
 int prefill_status()
