@@ -3,17 +3,17 @@
 // A unit is 256 pairs of token and query head of one key / value head, two tiles of 128 rows that share the keys and values of a block
 // of 128.  Per block and tile S = Q K^T and O += P V are four to eight products of K = 16 each way; the tensor cores need 512 cycles for either (heads of 128),
 // and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.
-//   warps 0-7, 8-15 softmax of tile 0 and 1, two threads per row with 64 keys of a block each (one per row took 3200 cycles per block, most of them
-//                   waiting for its own results): S from TMEM, running maximum and sum in f32, P back into TMEM over S (as the
-//                   16-bit left operand of the second product), results out of TMEM.
+//   warps 0-7, 8-15 softmax of tile 0 and 1, 16 rows per warp and four lanes per row, as the 16-lane TMEM shapes lay them out (two shuffles join a
+//                   row's maximum; with two warps per row a barrier of 280 cycles did): S from TMEM, running maximum and sum in f32, P back into
+//                   TMEM over S (as the 16-bit left operand of the second product), results out of TMEM.
 //   warp 16         keys and values: TMA boxes of a page's tokens (128 at most) by 64 elements, a lane each, into a ring of stages that hold
 //                   128 keys or 128 values.
 //   warp 17         issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
-//                   S(j + 1) done knows that O(j) is.  O(j) begins when the first half of either thread's weights is there.
+//                   S(j + 1) done knows that O(j) is.  O(j) begins when the weights of the first 64 keys are there.
 //   warp 18         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
-// Sums are kept relative to a maximum that may be 2^8 too low: only where a row's maximum grows by more do its threads agree on a new one and scale O.  Weights are
+// Sums are kept relative to a maximum that may be 2^8 too low: only where a row's maximum grows by more is O scaled.  Weights are
 // rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.
-// TMEM: S0, S1 (128 columns each, P in the first 32 of either half), O0, O1.
+// TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
 #include <cfloat>
 #include <cstdint>
 
@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kThreads = 608;
 constexpr int kSoft = 2;                                 // of eight pairs of exponentials, those that go to the multiply-add units
-constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
+constexpr int kExtra = 4;                                // blocks of keys that starting and ending a unit take as long as
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return D / 64 * kHalf; }
@@ -34,11 +34,13 @@ __device__ unsigned int g_prefill_error;
 
 using Way = Walk<kPrefillRows, kKeys, kExtra>;
 struct __align__(16) Shared {
-    float top[2][2][kTile];                              // of a row's two threads: maximum, at the end sum of weights
+    float sum[2][2][kTile];                              // of a unit's rows: weights and maxima, then whether they are to be computed again
     unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2];
     Way way[2];                                          // of the producers of keys and of queries
-    Segment kv_seg, seg[2];                              // of the producer of keys; of everybody else, two units in turn, no tokens behind the last
+    Segment kv_seg, next, seg[2];                        // of the producer of keys; of that of queries; of everybody else, two units in turn, no tokens behind the last
+    int more;
     uint32_t there[8][4];                                // keys of a block that exist, for the last eight blocks
+    uint32_t holes[2];                                   // whether the unit's keys have pages that do not exist
     uint32_t tmem;
     volatile int failed;
 };
@@ -119,22 +121,48 @@ __device__ __forceinline__ void exp2_pair(float &x, float &y)
     x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(rx) << 23));
     y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ry) << 23));
 }
-// 64 columns of this lane's row, one wait for all of them.
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&y)[64])
+// 16 TMEM lanes as accumulators of products lie in registers: thread 4 r + c holds of each 8 columns 2 c and 2 c + 1 of the lanes r (y[4 n], y[4 n + 1])
+// and r + 8 (y[4 n + 2], y[4 n + 3]).  128 columns, with one wait.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, float (&y)[64])
 {
 #pragma unroll
     for (int c = 0; c < 64; c += 32)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 "
                      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
                      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                      : "=f"(y[c + 0]), "=f"(y[c + 1]), "=f"(y[c + 2]), "=f"(y[c + 3]), "=f"(y[c + 4]), "=f"(y[c + 5]), "=f"(y[c + 6]), "=f"(y[c + 7]),
                        "=f"(y[c + 8]), "=f"(y[c + 9]), "=f"(y[c + 10]), "=f"(y[c + 11]), "=f"(y[c + 12]), "=f"(y[c + 13]), "=f"(y[c + 14]), "=f"(y[c + 15]),
                        "=f"(y[c + 16]), "=f"(y[c + 17]), "=f"(y[c + 18]), "=f"(y[c + 19]), "=f"(y[c + 20]), "=f"(y[c + 21]), "=f"(y[c + 22]), "=f"(y[c + 23]),
                        "=f"(y[c + 24]), "=f"(y[c + 25]), "=f"(y[c + 26]), "=f"(y[c + 27]), "=f"(y[c + 28]), "=f"(y[c + 29]), "=f"(y[c + 30]), "=f"(y[c + 31])
-                     : "r"(addr + c) : "memory");
+                     : "r"(addr + c * 2) : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int c = 0; c < 64; c++) asm volatile("" : "+f"(y[c]));     // nothing that uses them moves in front of the wait
+    for (int c = 0; c < 64; c++) asm volatile("" : "+f"(y[c]));      // nothing that uses them moves in front of the wait
+}
+// The same of 32 columns, each row scaled.
+__device__ __forceinline__ void tmem_scale_rows(uint32_t addr, float low, float high)
+{
+    float y[16];
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]), "=f"(y[4]), "=f"(y[5]), "=f"(y[6]), "=f"(y[7]), "=f"(y[8]), "=f"(y[9]), "=f"(y[10]), "=f"(y[11]),
+                   "=f"(y[12]), "=f"(y[13]), "=f"(y[14]), "=f"(y[15])
+                 : "r"(addr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        asm volatile("" : "+f"(y[i]));
+        y[i] *= i & 2 ? high : low;
+    }
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(addr), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]), "f"(y[8]), "f"(y[9]), "f"(y[10]), "f"(y[11]),
+                   "f"(y[12]), "f"(y[13]), "f"(y[14]), "f"(y[15]) : "memory");
+}
+// 32 columns of pairs: thread 4 r + c holds column 4 n + c of the lanes r (v[2 n]) and r + 8 (v[2 n + 1]).
+__device__ __forceinline__ void tmem_st_rows(uint32_t addr, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+                   "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
 // All 256 threads of a tile's warps: whether any of them says so.
 __device__ __forceinline__ bool any_of_tile(uint32_t tile, bool mine)
@@ -251,7 +279,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     __syncthreads();
     // the tokens of the tiles' last rows
     const uint32_t last_token[2] = {(kTile - 1) / slice, (2 * kTile - 1) / slice};
-    auto wait = [&](unsigned long long *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh.failed, &g_prefill_error)) != 0; };
+    // Each lane by itself: false where the limit ran out, or another role has given up.
+    auto lane_wait = [&](unsigned long long *bar, uint32_t parity) {
+        return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, &sh.failed, &g_prefill_error);
+    };
+    auto wait = [&](unsigned long long *bar, uint32_t parity) {
+        const bool done = lane_wait(bar, parity);
+        __syncwarp();
+        return done;
+    };
+    auto wait_all = [&](unsigned long long *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
     if (warp == 16) {
         const uint32_t shift = a.page_shift, page_keys = 1u << shift, box = min(page_keys, kKeys), boxes = kKeys / box, gone = a.pages << shift;
@@ -283,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 for (int w = 0; w < 4; w++) there[w] = __reduce_or_sync(0xffffffffu, bits(b * box, b * box + have, 32 * w));
 #pragma unroll
                 for (int what = 0; what < 2 && ok; what++) {
-                    if (!(ok = wait(&sh.empty[slot], (round & 1u) ^ 1u))) break;
+                    if (!(ok = wait_all(&sh.empty[slot], (round & 1u) ^ 1u))) break;
                     if (lane == 0) {
                         if (what == 0)
                             for (int w = 0; w < 4; w++) sh.there[block & 7u][w] = there[w];
@@ -308,11 +345,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         uint32_t unit = 0;
         bool ok = true, more = true;
         for (; more; unit++) {
-            if (!(ok = wait(&sh.q_empty, (unit & 1u) ^ 1u))) break;
+            if (lane == 0) {
+                sh.next.tokens = 0;
+                sh.more = sh.way[1].next(a, sh.next);
+            }
+            __syncwarp();
+            more = sh.more != 0;
+            bool holes = false;
+            if (more && sh.next.end > sh.next.begin) {
+                const uint32_t first = sh.next.begin * kKeys >> a.page_shift, last = (min(sh.next.end * kKeys, (uint32_t)sh.next.len) - 1) >> a.page_shift;
+                for (uint32_t j = first + lane; j <= last; j += 32) holes |= sh.next.table[j] >= a.pages;
+            }
+            holes = __any_sync(0xffffffffu, holes);
+            if (!(ok = wait_all(&sh.q_empty, (unit & 1u) ^ 1u))) break;
             if (lane == 0) {
                 Segment &g = sh.seg[unit & 1u];
-                more = sh.way[1].next(a, g);
+                g = sh.next;
                 if (!more) g.tokens = 0;
+                sh.holes[unit & 1u] = holes;
                 if (more && g.end > g.begin) {
                     mbar_arrive_expect_tx(&sh.q_full, PARTS * rows * 128);
                     for (int c = 0; c < PARTS; c++) tma_load_3d(smem_u32(s_q) + c * 2 * kHalf, &q_map, c * 64, (int)g.head0, (int)g.row0, &sh.q_full);
@@ -320,11 +370,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     mbar_arrive(&sh.q_full);
                 }
             }
-            more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+            __syncwarp();
         }
         if (!ok && lane == 0 && unit > 0)                // given up: the copy in flight lands before the CTA exits
             for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.q_full, (unit - 1) & 1u); w++) { }
     } else if (warp == 17) {
+        // All lanes run along, one issues; nothing in here needs them together.
         const bool leader = elect_one();
         const uint32_t q16 = smem_u32(s_q) >> 4, ring16 = smem_u32(ring) >> 4;
         uint32_t slot = 0, round = 0, p_seen = 0;                         // p_seen: parities of the two tiles in bits 0 and 1
@@ -340,31 +391,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 for (uint32_t i = 1; i < D / 16; i++) umma_step<true>(tmem + tile * 128, q + i / 4 * (2 * kHalf / 16) + i % 4 * 2, k + i / 4 * (kHalf / 16) + i % 4 * 2, kInstrS);
                 umma_commit(&sh.s_full[tile]);
             }
-            __syncwarp();
         };
-        // 16 keys per product; the quarters 0 and 2 of the block's keys first, whose weights come first
+        // 64 keys, 16 per product
         auto values = [&](uint32_t tile, uint32_t at, uint32_t part, bool first) {
             if (leader) {
                 const uint32_t v = ring16 + at * (kStage / 16), o = tmem + 256 + tile * D, p = tmem + tile * 128;
 #pragma unroll
                 for (uint32_t i = 0; i < kKeys / 32; i++) {
-                    const uint32_t step = i / 2 * 4 + part * 2 + i % 2;
-                    umma_f16_ts_mn(o, p + step / 4 * 64 + step % 4 * 8, v + step * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0 || part > 0);
+                    const uint32_t step = part * 4 + i;
+                    umma_f16_ts_mn(o, p + step * 8, v + step * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0 || part > 0);
                 }
             }
-            __syncwarp();
         };
         for (uint32_t unit = 0;; unit++) {
-            if (!(ok = wait(&sh.q_full, unit & 1u))) break;
+            if (!(ok = lane_wait(&sh.q_full, unit & 1u))) break;
             const Segment &g = sh.seg[unit & 1u];
             if (g.tokens == 0) break;
             const uint32_t begin = g.begin, end = g.end, stop[2] = {tile_end(g, 0, last_token[0]), tile_end(g, 1, last_token[1])};
-            __syncwarp();
             if (end <= begin) {
                 if (leader) mbar_arrive(&sh.q_empty);
                 continue;
             }
-            if (!(ok = wait(&sh.full[slot], round & 1u))) break;
+            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
             tc_fence_after();
 #pragma unroll
             for (uint32_t tile = 0; tile < 2; tile++)
@@ -373,11 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 umma_commit(&sh.empty[slot]);
                 if (begin + 1 == end) umma_commit(&sh.q_empty);
             }
-            __syncwarp();
             advance();
             for (uint32_t kb = begin; ok && kb < end; kb++) {
                 const uint32_t v_slot = slot;
-                if (!(ok = wait(&sh.full[slot], round & 1u))) break;
+                if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
                 tc_fence_after();
                 advance();
                 const bool more = kb + 1 < end;
@@ -385,19 +432,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
 #pragma unroll
                 for (uint32_t tile = 0; tile < 2; tile++) {
                     if (stop[tile] > kb) {
-                        if (!(ok = wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
+                        if (!(ok = lane_wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
                         tc_fence_after();
                         values(tile, v_slot, 0, kb == begin);
-                        if (!(ok = wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
+                        if (!(ok = lane_wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
                         p_seen ^= 1u << tile;
                         tc_fence_after();
                         values(tile, v_slot, 1, false);
                         if (kb + 1 == stop[tile] && leader) umma_commit(&sh.o_full[tile]);
-                        __syncwarp();
                     }
                     if (stop[tile] > kb + 1) {
                         if (!waited) {
-                            if (!(ok = wait(&sh.full[slot], round & 1u))) break;
+                            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
                             tc_fence_after();
                             waited = true;
                         }
@@ -407,125 +453,147 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (!ok) break;
                 if (leader) umma_commit(&sh.empty[v_slot]);
                 if (more) {
-                    if (!waited && !(ok = wait(&sh.full[slot], round & 1u))) break;
+                    if (!waited && !(ok = lane_wait(&sh.full[slot], round & 1u))) break;
                     if (leader) {
                         umma_commit(&sh.empty[slot]);
                         if (kb + 2 == end) umma_commit(&sh.q_empty);      // no more scores of this unit
                     }
                     advance();
                 }
-                __syncwarp();
             }
             if (!ok) break;
         }
     } else {
-        // thread = row of the tile and half of a block's keys, of O's columns, of the query's pieces
-        const uint32_t tile = warp >> 3, half = warp >> 2 & 1u, quad = warp & 3u, r_tile = quad * 32 + lane, row = tile * kTile + r_tile;
-        const uint32_t lanes = (quad * 32u) << 16, s_at = tmem + tile * 128 + half * 64 + lanes, o_at = tmem + 256 + tile * D + half * (D / 2) + lanes, d = a.d;
+        const uint32_t tile = warp >> 3, quad = warp & 3u, half = warp >> 2 & 1u, d = a.d;
+        // softmax: rows r and r + 8 of 16, four lanes each
+        const uint32_t row16 = tile * kTile + quad * 32 + half * 16 + lane / 4, pair = lane & 3u, lanes16 = (quad * 32u + half * 16u) << 16;
+        const uint32_t s_at = tmem + tile * 128 + lanes16, o16_at = tmem + 256 + tile * D + lanes16;
+        // results: a row of 32 and half of its columns
+        const uint32_t r_tile = quad * 32 + lane, row = tile * kTile + r_tile, o_at = tmem + 256 + tile * D + half * (D / 2) + ((quad * 32u) << 16);
         const float scale = a.scale_log2;
         const uint32_t token = row / slice, head = row - token * slice, first_token = tile * kTile / slice;     // of this row, of the tile's first
+        const uint32_t token16[2] = {row16 / slice, (row16 + 8) / slice};
         uint32_t slot = 0, round = 0, block = 0;         // of the ring, as the producer counts
         uint32_t s_seen = 0, o_seen = 0;
-        bool ok = true;
-        // A wait that runs out is noted and carried to the next meeting of the tile's warps, where all of them leave.
+        // Where a wait runs out the tile's warps run on without waiting, and leave together at the next unit.
         for (uint32_t unit = 0;; unit++) {
-            ok = wait(&sh.q_full, unit & 1u);
+            const bool there_is = wait(&sh.q_full, unit & 1u);
             const Segment &g = sh.seg[unit & 1u];
-            if (any_of_tile(tile, !ok)) break;
+            if (any_of_tile(tile, !there_is)) break;
             if (g.tokens == 0) break;
             const uint32_t begin = g.begin, end = g.end, stop = tile_end(g, tile, last_token[tile]), pairs = g.tokens * g.heads;
-            const int pos = row < pairs ? g.pos0 + (int)token : -1, first_pos = g.pos0 + (int)first_token;
+            const int first_pos = g.pos0 + (int)first_token, len = g.len;
             const int last_pos = g.pos0 + (int)min(last_token[tile], g.tokens - 1), window = (int)a.window;
-            float m = -INFINITY, l = 0.f;
+            const int pos[2] = {row16 < pairs ? g.pos0 + (int)token16[0] : -1, row16 + 8 < pairs ? g.pos0 + (int)token16[1] : -1};
+            const bool holes = sh.holes[unit & 1u] != 0;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
             for (uint32_t kb = begin; kb < end; kb++, block++) {
                 if (++slot == S) { slot = 0; round++; }
                 const uint32_t v_slot = slot, v_round = round;
                 if (++slot == S) { slot = 0; round++; }
                 if (kb >= stop) continue;
-                ok = wait(&sh.s_full[tile], s_seen & 1u);
+                wait(&sh.s_full[tile], s_seen & 1u);
                 s_seen++;
                 tc_fence_after();
-                // For sight of `there`, and to write into the values below.  Not the keys' barrier: their stage is free by now and may have been filled
-                // again, two phases on, where this parity would wait for a third.  The values' stage is free behind this tile's product only.
-                ok = wait(&sh.full[v_slot], v_round & 1u) && ok;
-                uint32_t there[4];
-#pragma unroll
-                for (int w = 0; w < 4; w++) there[w] = sh.there[block & 7u][w];
                 float s[64];
-                tmem_ld64(s_at, s);
+                tmem_ld_rows(s_at, s);
                 const int key0 = (int)(kb * kKeys);
-                const bool every = (there[0] & there[1] & there[2] & there[3]) == 0xFFFFFFFFu;
+                const bool every = !holes && key0 + (int)kKeys <= len;
                 bool plain = every && key0 + (int)kKeys - 1 <= first_pos && !(window && key0 <= last_pos - window);      // nothing is masked
                 if (!plain) {
+                    uint32_t there[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                    if (!every) {
+                        // For sight of `there`, and to write into the values.  Not the keys' barrier: their stage is free by now and may have been
+                        // filled again, two phases on, where this parity would wait for a third.  The values' stage is free behind this tile's product only.
+                        wait(&sh.full[v_slot], v_round & 1u);
 #pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const uint32_t seen = (half ? there[2 + w] : there[w]) & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 64 * (int)half + 32 * w);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) s[32 * w + e] = seen >> e & 1u ? s[32 * w + e] : -INFINITY;
-                    }
-                }
-                float tops[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) tops[i] = max3(s[i], s[4 + i], s[8 + i]);
-#pragma unroll
-                for (int e = 12; e < 60; e += 8)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) tops[i] = max3(tops[i], s[e + i], s[e + 4 + i]);
-                float top = max3(max3(tops[0], tops[1], s[60]), max3(tops[2], tops[3], s[61]), max3(s[62], s[62], s[63])) * scale;
-                plain = plain && __all_sync(0xffffffffu, fabsf(top) <= FLT_MAX);       // and all rows are finite
-                if (any_of_tile(tile, !ok || (!(top <= m + 8.f) && top > -INFINITY))) {
-                    sh.top[tile][half][r_tile] = top;
-                    if (any_of_tile(tile, !ok)) {
-                        ok = false;
-                        break;
-                    }
-                    top = fmaxf(top, sh.top[tile][half ^ 1u][r_tile]);
-                    const bool up = !(top <= m + 8.f) && top > -INFINITY;             // also where m is still -inf
-                    const float keep = up ? exp2_fast(m - top) : 1.f;
-                    l *= keep;
-                    m = up ? top : m;
-                    if (kb != begin && __any_sync(0xffffffffu, up)) {
-#pragma unroll 1
-                        for (uint32_t c = 0; c < D / 2; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o_at + c, o);
-#pragma unroll
-                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_st16(o_at + c, o);
+                        for (int w = 0; w < 4; w++) there[w] = sh.there[block & 7u][w];
+                        // values that nobody sees, whatever the page holds there, become zeros
+                        uint8_t *v = ring + v_slot * kStage;
+                        for (uint32_t i = half * 128 + r_tile; i < kKeys * PARTS * 8; i += 256) {
+                            const uint32_t key = i / 8 % kKeys, w = key / 32, word = w == 0 ? there[0] : w == 1 ? there[1] : w == 2 ? there[2] : there[3];
+                            if (!(word >> (key % 32) & 1u)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                         }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            const uint32_t seen = (there[w] & bits(window ? pos[h] - window + 1 : 0, pos[h] + 1, key0 + 32 * w)) >> (2 * pair);
+#pragma unroll
+                            for (int n = 0; n < 4; n++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++) {
+                                    float &x = s[4 * (4 * w + n) + 2 * h + e];
+                                    x = seen >> (8 * n + e) & 1u ? x : -INFINITY;
+                                }
+                        }
+                    __syncwarp();
+                }
+                float top[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float t0 = max3(s[2 * h], s[2 * h + 1], s[4 + 2 * h]), t1 = max3(s[5 + 2 * h], s[8 + 2 * h], s[9 + 2 * h]);
+#pragma unroll
+                    for (int n = 3; n < 15; n += 2) {
+                        t0 = max3(t0, s[4 * n + 2 * h], s[4 * n + 1 + 2 * h]);
+                        t1 = max3(t1, s[4 * n + 4 + 2 * h], s[4 * n + 5 + 2 * h]);
+                    }
+                    t0 = max3(t0, s[60 + 2 * h], s[61 + 2 * h]);
+                    top[h] = max3(t0, t1, t1);
+                }
+#pragma unroll
+                for (int o = 1; o < 4; o *= 2)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float other = __shfl_xor_sync(0xffffffffu, top[h], o);
+                        top[h] = max3(top[h], other, other);
+                    }
+                top[0] *= scale;
+                top[1] *= scale;
+                plain = plain && __all_sync(0xffffffffu, fmaxf(fabsf(top[0]), fabsf(top[1])) <= FLT_MAX && top[0] == top[0] && top[1] == top[1]);     // and all rows are finite
+                // also where m is still -inf
+                const bool up[2] = {!(top[0] <= m[0] + 8.f) && top[0] > -INFINITY, !(top[1] <= m[1] + 8.f) && top[1] > -INFINITY};
+                if (__any_sync(0xffffffffu, up[0] || up[1])) {
+                    float keep[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        keep[h] = up[h] ? exp2_fast(m[h] - top[h]) : 1.f;
+                        l[h] *= keep[h];
+                        m[h] = up[h] ? top[h] : m[h];
+                    }
+                    if (kb != begin) {
+#pragma unroll 1
+                        for (uint32_t c = 0; c < D; c += 32) tmem_scale_rows(o16_at + c, keep[0], keep[1]);
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                if (!every) {                            // values that nobody sees, whatever the page holds there, become zeros
-                    uint8_t *v = ring + v_slot * kStage;
-                    for (uint32_t i = half * 128 + r_tile; i < kKeys * PARTS * 8; i += 256) {
-                        const uint32_t key = i / 8 % kKeys, w = key / 32, word = w == 0 ? there[0] : w == 1 ? there[1] : w == 2 ? there[2] : there[3];
-                        if (!(word >> (key % 32) & 1u)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    any_of_tile(tile, false);            // the product takes keys of both threads' halves from the first signal on
-                }
-                auto weights = [&](int c, bool soft) {   // 32 keys: exponentials, sums, P
+                const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+                if (!every) any_of_tile(tile, false);    // all values that become zeros have
+                auto weights = [&](int c, bool soft) {   // 64 keys: exponentials, sums, P
                     uint32_t p[16];
+                    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
+                        const int h = e & 1;
                         float x = s[32 * c + 2 * e], y = s[32 * c + 2 * e + 1];
-                        scaled_pair(x, y, scale, -base);
+                        scaled_pair(x, y, scale, -base[h]);
                         if (soft && e % 8 < kSoft) {
                             exp2_pair<T>(x, y);
                         } else {
                             x = exp2_fast(x);
                             y = exp2_fast(y);
                         }
-                        add_pair(sum[e % 2 * 2], sum[e % 2 * 2 + 1], x, y);
+                        add_pair(sum[h][0], sum[h][1], x, y);
                         p[e] = pack<T>(x, y);
                     }
-                    tmem_st16(s_at + 16 * c, p);
+                    tmem_st_rows(s_at + 32 * c, p);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(c ? &sh.p_full[tile] : &sh.p_half[tile]);
+                    l[0] += sum[0][0] + sum[0][1];
+                    l[1] += sum[1][0] + sum[1][1];
                 };
                 if (plain) {
                     weights(0, true);
@@ -534,29 +602,33 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     weights(0, false);
                     weights(1, false);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            if (!ok) break;
             // this tile's scores are done with the queries (its warps have met in this unit)
             if (half == 0 && r_tile == 0) mbar_arrive(&sh.q_empty);
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2)
+#pragma unroll
+                for (int h = 0; h < 2; h++) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+            if (pair == 0) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    sh.sum[tile][0][row16 - tile * kTile + 8 * h] = l[h];
+                    sh.sum[tile][1][row16 - tile * kTile + 8 * h] = m[h];
+                }
+            }
             if (stop > begin) {
-                ok = wait(&sh.o_full[tile], o_seen & 1u);
+                wait(&sh.o_full[tile], o_seen & 1u);
                 o_seen++;
                 tc_fence_after();
             }
-            if (any_of_tile(tile, !ok)) {                // everybody has read the last maxima
-                ok = false;
-                break;
-            }
-            sh.top[tile][half][r_tile] = l;
             any_of_tile(tile, false);
-            l += sh.top[tile][half ^ 1u][r_tile];
+            const float row_l = sh.sum[tile][0][r_tile], row_m = sh.sum[tile][1][r_tile];
             if (tile * kTile < pairs) {
                 const bool alone = g.first && g.last;
                 const uint32_t c0 = half * (D / 2);
                 T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d + c0;
                 float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kPrefillRows * (d + 2);
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = row_l == 0.f ? 0.f : 1.f / row_l;
                 bool bad = false;
 #pragma unroll 1
                 for (uint32_t c = 0; c < D / 2; c += 16) {
@@ -588,12 +660,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     }
                     __syncwarp();                        // the next columns are read by the whole warp
                 }
-                if (!alone && half == 0 && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(m, l);
+                if (!alone && half == 0 && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(row_m, row_l);
                 // a row that either thread finds spoilt is computed again by the first one's warp, behind both threads' stores
                 if (any_of_tile(tile, bad)) {
-                    sh.top[tile][half][r_tile] = bad ? 1.f : 0.f;
+                    sh.sum[tile][half][r_tile] = bad ? 1.f : 0.f;
                     any_of_tile(tile, false);
-                    const bool redo = half == 0 && (sh.top[tile][0][r_tile] != 0.f || sh.top[tile][1][r_tile] != 0.f);
+                    const bool redo = half == 0 && (sh.sum[tile][0][r_tile] != 0.f || sh.sum[tile][1][r_tile] != 0.f);
                     for (uint32_t left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
                         const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
                         float rm, rl, acc[D / 32];
@@ -611,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 }
                 if (!alone && tid == 0) name_part(a, blockIdx.x, g);
             }
-            any_of_tile(tile, false);                    // sums read, before the next unit's maxima
+            any_of_tile(tile, false);                    // sums read, before the next unit's; O read by all warps, before it is written again
             tc_fence_before();
             __syncwarp();
         }
