@@ -3,14 +3,14 @@
 // A unit is 256 pairs of token and query head of one key / value head, two tiles of 128 rows that share the keys and values of a block
 // of 128.  Per block and tile S = Q K^T and O += P V are four to eight products of K = 16 each way; the tensor cores need 512 cycles for either (heads of 128),
 // and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.
-//   warps 0-7, 8-15 softmax of tile 0 and 1, 16 rows per warp and four lanes per row, as the 16-lane TMEM shapes lay them out (two shuffles join a
-//                   row's maximum; with two warps per row a barrier of 280 cycles did): S from TMEM, running maximum and sum in f32, P back into
-//                   TMEM over S (as the 16-bit left operand of the second product), results out of TMEM.
-//   warp 16         keys and values: TMA boxes of a page's tokens (128 at most) by 64 elements, a lane each, into a ring of stages that hold
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a row per thread: S from TMEM, running maximum and sum in f32, P back into TMEM over S (as the
+//                   16-bit left operand of the second product), results out of TMEM.  Two warps per row need a barrier per block (280 cycles, 671 us for
+//                   4 x 2048 tokens); four lanes per row read TMEM at half the rate (500 cycles of a block, 653 us).
+//   warp 8          keys and values: TMA boxes of a page's tokens (128 at most) by 64 elements, a lane each, into a ring of stages that hold
 //                   128 keys or 128 values.
-//   warp 17         issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
+//   warp 9          issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
 //                   S(j + 1) done knows that O(j) is.  O(j) begins when the weights of the first 64 keys are there.
-//   warp 18         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
+//   warp 10         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
 // Sums are kept relative to a maximum that may be 2^8 too low: only where a row's maximum grows by more is O scaled.  Weights are
 // rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.
 // TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
@@ -22,8 +22,8 @@
 namespace mgq {
 namespace {
 
-constexpr int kThreads = 608;
-constexpr int kSoft = 2;                                 // of eight pairs of exponentials, those that go to the multiply-add units
+constexpr int kThreads = 384;
+constexpr int kSoft = 0;                                 // of eight pairs of exponentials, those that go to the multiply-add units
 constexpr int kExtra = 4;                                // blocks of keys that starting and ending a unit take as long as
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
@@ -34,7 +34,6 @@ __device__ unsigned int g_prefill_error;
 
 using Way = Walk<kPrefillRows, kKeys, kExtra>;
 struct __align__(16) Shared {
-    float sum[2][2][kTile];                              // of a unit's rows: weights and maxima, then whether they are to be computed again
     unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2];
     Way way[2];                                          // of the producers of keys and of queries
     Segment kv_seg, next, seg[2];                        // of the producer of keys; of that of queries; of everybody else, two units in turn, no tokens behind the last
@@ -71,104 +70,76 @@ __device__ __forceinline__ float max3(float x, float y, float z)
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
-// (x, y) * s - b and (x, y) += (z, w), two elements per instruction.
-__device__ __forceinline__ void scaled_pair(float &x, float &y, float s, float minus_b)
+// Two f32 side by side, for instructions that take two.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair_of(float x, float y)
 {
-    asm("{\n\t.reg .b64 v, s, b;\n\t"
-        "mov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 b, {%3, %3};\n\t"
-        "fma.rn.f32x2 v, v, s, b;\n\t"
-        "mov.b64 {%0, %1}, v;\n\t}" : "+f"(x), "+f"(y) : "f"(s), "f"(minus_b));
+    pair_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
 }
-__device__ __forceinline__ void add_pair(float &x, float &y, float z, float w)
+__device__ __forceinline__ void parts_of(pair_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ pair_t pair_fma(pair_t x, pair_t y, pair_t z)
 {
-    asm("{\n\t.reg .b64 a, b;\n\t"
-        "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
-        "add.rn.f32x2 a, a, b;\n\t"
-        "mov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(z), "f"(w));
+    pair_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
 }
-// 2^x and 2^y of finite x and y <= 127 on the multiply-add units: 16 exponentials per cycle leave an SM idle for half of attention's time
+__device__ __forceinline__ pair_t pair_add(pair_t x, pair_t y)
+{
+    pair_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+// 2^x of finite x <= 127 on the multiply-add units: 16 exponentials per cycle leave an SM idle for half of attention's time
 // (heads of 128).  x = n + f with n whole and f in [-1/2, 1/2]: 2^f by a polynomial fitted to the least relative error (7.5e-5 of degree 3 for
 // bf16 weights, 2.6e-6 of degree 4 for f16 ones), n added to its exponent.  Below 2^-126 the result stays there.
 template <typename T>
-__device__ __forceinline__ void exp2_pair(float &x, float &y)
+__device__ __forceinline__ float exp2_soft(float x)
 {
     constexpr bool kFour = std::is_same<T, __half>::value;
-    const float c0 = kFour ? 0.9999992847442627f : 0.9999280571937561f, c1 = kFour ? 0.6931217908859253f : 0.6932609677314758f;
-    const float c2 = kFour ? 0.240247443318367f : 0.2426111251115799f, c3 = kFour ? 0.05591785907745361f : 0.0551716685295105f, c4 = 0.009570102207362652f;
     x = fmaxf(x, -126.f);
-    y = fmaxf(y, -126.f);
-    const float magic = 12582912.f;                      // 1.5 * 2^23: the sum's last bits are the rounded value
-    float rx, ry;
-    if constexpr (kFour)
-        asm("{\n\t.reg .b64 v, r, f, p, m, c;\n\t"
-            "mov.b64 v, {%0, %1};\n\tmov.b64 m, {%4, %4};\n\tadd.rn.f32x2 r, v, m;\n\tmov.b64 {%2, %3}, r;\n\t"
-            "sub.rn.f32x2 f, r, m;\n\tsub.rn.f32x2 f, v, f;\n\t"
-            "mov.b64 p, {%9, %9};\n\tmov.b64 c, {%8, %8};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 {%0, %1}, p;\n\t}"
-            : "+f"(x), "+f"(y), "=&f"(rx), "=&f"(ry) : "f"(magic), "f"(c0), "f"(c1), "f"(c2), "f"(c3), "f"(c4));
-    else
-        asm("{\n\t.reg .b64 v, r, f, p, m, c;\n\t"
-            "mov.b64 v, {%0, %1};\n\tmov.b64 m, {%4, %4};\n\tadd.rn.f32x2 r, v, m;\n\tmov.b64 {%2, %3}, r;\n\t"
-            "sub.rn.f32x2 f, r, m;\n\tsub.rn.f32x2 f, v, f;\n\t"
-            "mov.b64 p, {%8, %8};\n\tmov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 {%0, %1}, p;\n\t}"
-            : "+f"(x), "+f"(y), "=&f"(rx), "=&f"(ry) : "f"(magic), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-    x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(rx) << 23));
-    y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ry) << 23));
+    const float r = x + 12582912.f, f = x - (r - 12582912.f);            // 1.5 * 2^23: the sum's last bits are the rounded value
+    const float p = kFour ? fmaf(fmaf(fmaf(fmaf(0.009570102207362652f, f, 0.05591785907745361f), f, 0.240247443318367f), f, 0.6931217908859253f), f, 0.9999992847442627f)
+                          : fmaf(fmaf(fmaf(0.0551716685295105f, f, 0.2426111251115799f), f, 0.6932609677314758f), f, 0.9999280571937561f);
+    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
 }
-// 16 TMEM lanes as accumulators of products lie in registers: thread 4 r + c holds of each 8 columns 2 c and 2 c + 1 of the lanes r (y[4 n], y[4 n + 1])
-// and r + 8 (y[4 n + 2], y[4 n + 3]).  128 columns, with one wait.
-__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, float (&y)[64])
+// 64 columns of this lane's row; wait_row before they are used.
+__device__ __forceinline__ void tmem_ld_row(uint32_t addr, float (&y)[64])
 {
 #pragma unroll
     for (int c = 0; c < 64; c += 32)
-        asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
                      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                      : "=f"(y[c + 0]), "=f"(y[c + 1]), "=f"(y[c + 2]), "=f"(y[c + 3]), "=f"(y[c + 4]), "=f"(y[c + 5]), "=f"(y[c + 6]), "=f"(y[c + 7]),
                        "=f"(y[c + 8]), "=f"(y[c + 9]), "=f"(y[c + 10]), "=f"(y[c + 11]), "=f"(y[c + 12]), "=f"(y[c + 13]), "=f"(y[c + 14]), "=f"(y[c + 15]),
                        "=f"(y[c + 16]), "=f"(y[c + 17]), "=f"(y[c + 18]), "=f"(y[c + 19]), "=f"(y[c + 20]), "=f"(y[c + 21]), "=f"(y[c + 22]), "=f"(y[c + 23]),
                        "=f"(y[c + 24]), "=f"(y[c + 25]), "=f"(y[c + 26]), "=f"(y[c + 27]), "=f"(y[c + 28]), "=f"(y[c + 29]), "=f"(y[c + 30]), "=f"(y[c + 31])
-                     : "r"(addr + c * 2) : "memory");
+                     : "r"(addr + c) : "memory");
+}
+__device__ __forceinline__ void wait_row(float (&y)[64])
+{
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int c = 0; c < 64; c++) asm volatile("" : "+f"(y[c]));      // nothing that uses them moves in front of the wait
 }
-// The same of 32 columns, each row scaled.
-__device__ __forceinline__ void tmem_scale_rows(uint32_t addr, float low, float high)
+__device__ __forceinline__ float row_max(const float (&y)[64])
 {
-    float y[16];
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]), "=f"(y[4]), "=f"(y[5]), "=f"(y[6]), "=f"(y[7]), "=f"(y[8]), "=f"(y[9]), "=f"(y[10]), "=f"(y[11]),
-                   "=f"(y[12]), "=f"(y[13]), "=f"(y[14]), "=f"(y[15])
-                 : "r"(addr) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    float t[4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        asm volatile("" : "+f"(y[i]));
-        y[i] *= i & 2 ? high : low;
-    }
-    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                 ::"r"(addr), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]), "f"(y[8]), "f"(y[9]), "f"(y[10]), "f"(y[11]),
-                   "f"(y[12]), "f"(y[13]), "f"(y[14]), "f"(y[15]) : "memory");
+    for (int i = 0; i < 4; i++) t[i] = max3(y[i], y[4 + i], y[8 + i]);
+#pragma unroll
+    for (int e = 12; e < 60; e += 8)
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = max3(t[i], y[e + i], y[e + 4 + i]);
+    return max3(max3(t[0], t[1], y[60]), max3(t[2], t[3], y[61]), max3(y[62], y[63], y[63]));
 }
-// 32 columns of pairs: thread 4 r + c holds column 4 n + c of the lanes r (v[2 n]) and r + 8 (v[2 n + 1]).
-__device__ __forceinline__ void tmem_st_rows(uint32_t addr, const uint32_t (&v)[16])
-{
-    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-                   "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
-// All 256 threads of a tile's warps: whether any of them says so.
+// All 128 threads of a tile's warps: whether any of them says so.
 __device__ __forceinline__ bool any_of_tile(uint32_t tile, bool mine)
 {
     uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(any) : "r"((uint32_t)mine), "r"(tile + 1) : "memory");
     return any != 0;
 }
@@ -250,14 +221,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         mbar_init(&sh.q_empty, 3);                                        // the issuer, both tiles' warps
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_half[i], 8);
-            mbar_init(&sh.p_full[i], 8);
+            mbar_init(&sh.p_half[i], 4);
+            mbar_init(&sh.p_full[i], 4);
             mbar_init(&sh.o_full[i], 1);
         }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 17) tmem_alloc(&sh.tmem, 512);
+    if (warp == 9) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -268,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     {
         Way way;
         way.begin(a, blockIdx.x, gridDim.x, 1, reinterpret_cast<unsigned long long *>(s_q));
-        if (lane == 0 && (warp == 16 || warp == 18)) sh.way[warp == 18] = way;
+        if (lane == 0 && (warp == 8 || warp == 10)) sh.way[warp == 10] = way;
     }
     for (uint32_t i = tid; i < (kPrefillRows - rows) * PARTS * 8; i += kThreads) {            // the others are zero for good
         const uint32_t part = i / ((kPrefillRows - rows) * 8), at = i - part * (kPrefillRows - rows) * 8;
@@ -290,7 +261,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     };
     auto wait_all = [&](unsigned long long *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-    if (warp == 16) {
+    // Registers where they are needed: 256 * 216 + 128 * 72 = 384 * 168.
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
         const uint32_t shift = a.page_shift, page_keys = 1u << shift, box = min(page_keys, kKeys), boxes = kKeys / box, gone = a.pages << shift;
         uint32_t slot = 0, round = 0, block = 0;
         int armed = 0;
@@ -341,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (slot-- == 0) { slot = S - 1; round--; }
                 for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.full[slot], round & 1u); w++) { }
             }
-    } else if (warp == 18) {
+    } else if (warp == 10) {
         uint32_t unit = 0;
         bool ok = true, more = true;
         for (; more; unit++) {
@@ -374,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         }
         if (!ok && lane == 0 && unit > 0)                // given up: the copy in flight lands before the CTA exits
             for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.q_full, (unit - 1) & 1u); w++) { }
-    } else if (warp == 17) {
+    } else if (warp == 9) {
         // All lanes run along, one issues; nothing in here needs them together.
         const bool leader = elect_one();
         const uint32_t q16 = smem_u32(s_q) >> 4, ring16 = smem_u32(ring) >> 4;
@@ -463,16 +437,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             }
             if (!ok) break;
         }
+    }
     } else {
-        const uint32_t tile = warp >> 3, quad = warp & 3u, half = warp >> 2 & 1u, d = a.d;
-        // softmax: rows r and r + 8 of 16, four lanes each
-        const uint32_t row16 = tile * kTile + quad * 32 + half * 16 + lane / 4, pair = lane & 3u, lanes16 = (quad * 32u + half * 16u) << 16;
-        const uint32_t s_at = tmem + tile * 128 + lanes16, o16_at = tmem + 256 + tile * D + lanes16;
-        // results: a row of 32 and half of its columns
-        const uint32_t r_tile = quad * 32 + lane, row = tile * kTile + r_tile, o_at = tmem + 256 + tile * D + half * (D / 2) + ((quad * 32u) << 16);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const uint32_t tile = warp >> 2, quad = warp & 3u, r_tile = quad * 32 + lane, row = tile * kTile + r_tile, d = a.d;
+        const uint32_t lanes = (quad * 32u) << 16, s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * D + lanes;
         const float scale = a.scale_log2;
         const uint32_t token = row / slice, head = row - token * slice, first_token = tile * kTile / slice;     // of this row, of the tile's first
-        const uint32_t token16[2] = {row16 / slice, (row16 + 8) / slice};
         uint32_t slot = 0, round = 0, block = 0;         // of the ring, as the producer counts
         uint32_t s_seen = 0, o_seen = 0;
         // Where a wait runs out the tile's warps run on without waiting, and leave together at the next unit.
@@ -484,9 +455,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             const uint32_t begin = g.begin, end = g.end, stop = tile_end(g, tile, last_token[tile]), pairs = g.tokens * g.heads;
             const int first_pos = g.pos0 + (int)first_token, len = g.len;
             const int last_pos = g.pos0 + (int)min(last_token[tile], g.tokens - 1), window = (int)a.window;
-            const int pos[2] = {row16 < pairs ? g.pos0 + (int)token16[0] : -1, row16 + 8 < pairs ? g.pos0 + (int)token16[1] : -1};
+            const int pos = row < pairs ? g.pos0 + (int)token : -1;
             const bool holes = sh.holes[unit & 1u] != 0;
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+            float m = -INFINITY, l = 0.f;
             for (uint32_t kb = begin; kb < end; kb++, block++) {
                 if (++slot == S) { slot = 0; round++; }
                 const uint32_t v_slot = slot, v_round = round;
@@ -495,202 +466,163 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 wait(&sh.s_full[tile], s_seen & 1u);
                 s_seen++;
                 tc_fence_after();
-                float s[64];
-                tmem_ld_rows(s_at, s);
                 const int key0 = (int)(kb * kKeys);
                 const bool every = !holes && key0 + (int)kKeys <= len;
-                bool plain = every && key0 + (int)kKeys - 1 <= first_pos && !(window && key0 <= last_pos - window);      // nothing is masked
-                if (!plain) {
-                    uint32_t there[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
-                    if (!every) {
-                        // For sight of `there`, and to write into the values.  Not the keys' barrier: their stage is free by now and may have been
-                        // filled again, two phases on, where this parity would wait for a third.  The values' stage is free behind this tile's product only.
-                        wait(&sh.full[v_slot], v_round & 1u);
+                const bool plain = every && key0 + (int)kKeys - 1 <= first_pos && !(window && key0 <= last_pos - window);      // nothing is masked
+                uint32_t there[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                if (!every) {
+                    // For sight of `there`, and to write into the values.  Not the keys' barrier: their stage is free by now and may have been
+                    // filled again, two phases on, where this parity would wait for a third.  The values' stage is free behind this tile's product only.
+                    wait(&sh.full[v_slot], v_round & 1u);
 #pragma unroll
-                        for (int w = 0; w < 4; w++) there[w] = sh.there[block & 7u][w];
-                        // values that nobody sees, whatever the page holds there, become zeros
-                        uint8_t *v = ring + v_slot * kStage;
-                        for (uint32_t i = half * 128 + r_tile; i < kKeys * PARTS * 8; i += 256) {
-                            const uint32_t key = i / 8 % kKeys, w = key / 32, word = w == 0 ? there[0] : w == 1 ? there[1] : w == 2 ? there[2] : there[3];
-                            if (!(word >> (key % 32) & 1u)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    for (int w = 0; w < 4; w++) there[w] = sh.there[block & 7u][w];
+                    // values that nobody sees, whatever the page holds there, become zeros
+                    uint8_t *v = ring + v_slot * kStage;
+                    for (uint32_t i = r_tile; i < kKeys * PARTS * 8; i += 128) {
+                        const uint32_t key = i / 8 % kKeys, w = key / 32, word = w == 0 ? there[0] : w == 1 ? there[1] : w == 2 ? there[2] : there[3];
+                        if (!(word >> (key % 32) & 1u)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    any_of_tile(tile, false);            // all of them have, before the first weights are signalled
+                }
+                // 64 keys: what the row does not see
+                auto mask = [&](float (&s)[64], int c) {
+                    if (plain) return;
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int w = 0; w < 2; w++) {
+                        const uint32_t seen = there[2 * c + w] & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 64 * c + 32 * w);
 #pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const uint32_t seen = (there[w] & bits(window ? pos[h] - window + 1 : 0, pos[h] + 1, key0 + 32 * w)) >> (2 * pair);
-#pragma unroll
-                            for (int n = 0; n < 4; n++)
-#pragma unroll
-                                for (int e = 0; e < 2; e++) {
-                                    float &x = s[4 * (4 * w + n) + 2 * h + e];
-                                    x = seen >> (8 * n + e) & 1u ? x : -INFINITY;
-                                }
-                        }
+                        for (int e = 0; e < 32; e++) s[32 * w + e] = seen >> e & 1u ? s[32 * w + e] : -INFINITY;
+                    }
                     __syncwarp();
-                }
-                float top[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float t0 = max3(s[2 * h], s[2 * h + 1], s[4 + 2 * h]), t1 = max3(s[5 + 2 * h], s[8 + 2 * h], s[9 + 2 * h]);
-#pragma unroll
-                    for (int n = 3; n < 15; n += 2) {
-                        t0 = max3(t0, s[4 * n + 2 * h], s[4 * n + 1 + 2 * h]);
-                        t1 = max3(t1, s[4 * n + 4 + 2 * h], s[4 * n + 5 + 2 * h]);
-                    }
-                    t0 = max3(t0, s[60 + 2 * h], s[61 + 2 * h]);
-                    top[h] = max3(t0, t1, t1);
-                }
-#pragma unroll
-                for (int o = 1; o < 4; o *= 2)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float other = __shfl_xor_sync(0xffffffffu, top[h], o);
-                        top[h] = max3(top[h], other, other);
-                    }
-                top[0] *= scale;
-                top[1] *= scale;
-                plain = plain && __all_sync(0xffffffffu, fmaxf(fabsf(top[0]), fabsf(top[1])) <= FLT_MAX && top[0] == top[0] && top[1] == top[1]);     // and all rows are finite
-                // also where m is still -inf
-                const bool up[2] = {!(top[0] <= m[0] + 8.f) && top[0] > -INFINITY, !(top[1] <= m[1] + 8.f) && top[1] > -INFINITY};
-                if (__any_sync(0xffffffffu, up[0] || up[1])) {
-                    float keep[2];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        keep[h] = up[h] ? exp2_fast(m[h] - top[h]) : 1.f;
-                        l[h] *= keep[h];
-                        m[h] = up[h] ? top[h] : m[h];
-                    }
-                    if (kb != begin) {
+                };
+                float s[64], t[64];
+                tmem_ld_row(s_at, s);
+                tmem_ld_row(s_at + 64, t);
+                wait_row(s);
+                wait_row(t);
+                mask(s, 0);
+                mask(t, 1);
+                const float first = row_max(s), second = row_max(t), top = max3(first, second, second) * scale;
+                // Nothing to do where the maximum stays at or below the old one + 8 (finite behind the first block); -inf and NaN come here, too.
+                bool exact = !plain;
+                if (__any_sync(0xffffffffu, !(top <= m + 8.f && top >= -FLT_MAX))) {
+                    const bool up = !(top <= m + 8.f) && top > -INFINITY;              // also where m is still -inf
+                    const float keep = up ? exp2_fast(m - top) : 1.f;
+                    l *= keep;
+                    m = up ? top : m;
+                    exact = __any_sync(0xffffffffu, exact || !(fabsf(top) <= FLT_MAX));
+                    if (kb != begin && __any_sync(0xffffffffu, up)) {
 #pragma unroll 1
-                        for (uint32_t c = 0; c < D; c += 32) tmem_scale_rows(o16_at + c, keep[0], keep[1]);
+                        for (uint32_t c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + c, o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st16(o_at + c, o);
+                        }
                     }
                 }
-                const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-                if (!every) any_of_tile(tile, false);    // all values that become zeros have
-                auto weights = [&](int c, bool soft) {   // 64 keys: exponentials, sums, P
-                    uint32_t p[16];
-                    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+                const pair_t scales = pair_of(scale, scale);
+                const float base = m == -INFINITY ? 0.f : -m;
+                const pair_t bases = pair_of(base, base);
+                pair_t sum[2] = {0, 0};
+                auto weights = [&](const float (&s)[64], int c, bool soft) {       // 64 keys: exponentials, sums, P
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int h = e & 1;
-                        float x = s[32 * c + 2 * e], y = s[32 * c + 2 * e + 1];
-                        scaled_pair(x, y, scale, -base[h]);
-                        if (soft && e % 8 < kSoft) {
-                            exp2_pair<T>(x, y);
-                        } else {
-                            x = exp2_fast(x);
-                            y = exp2_fast(y);
+                    for (int i = 0; i < 64; i += 32) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            float x, y;
+                            parts_of(pair_fma(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), scales, bases), x, y);
+                            x = soft && e % 8 < kSoft ? exp2_soft<T>(x) : exp2_fast(x);
+                            y = soft && e % 8 < kSoft ? exp2_soft<T>(y) : exp2_fast(y);
+                            sum[e & 1] = pair_add(sum[e & 1], pair_of(x, y));
+                            p[e] = pack<T>(x, y);
                         }
-                        add_pair(sum[h][0], sum[h][1], x, y);
-                        p[e] = pack<T>(x, y);
+                        tmem_st16(s_at + 32 * c + i / 2, p);
                     }
-                    tmem_st_rows(s_at + 32 * c, p);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(c ? &sh.p_full[tile] : &sh.p_half[tile]);
-                    l[0] += sum[0][0] + sum[0][1];
-                    l[1] += sum[1][0] + sum[1][1];
                 };
-                if (plain) {
-                    weights(0, true);
-                    weights(1, true);
+                if (!exact) {
+                    weights(s, 0, true);
+                    weights(t, 1, true);
                 } else {
-                    weights(0, false);
-                    weights(1, false);
+                    weights(s, 0, false);
+                    weights(t, 1, false);
                 }
+                float x, y;
+                parts_of(pair_add(sum[0], sum[1]), x, y);
+                l += x + y;
             }
             // this tile's scores are done with the queries (its warps have met in this unit)
-            if (half == 0 && r_tile == 0) mbar_arrive(&sh.q_empty);
-#pragma unroll
-            for (int o = 1; o < 4; o *= 2)
-#pragma unroll
-                for (int h = 0; h < 2; h++) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
-            if (pair == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    sh.sum[tile][0][row16 - tile * kTile + 8 * h] = l[h];
-                    sh.sum[tile][1][row16 - tile * kTile + 8 * h] = m[h];
-                }
-            }
+            if (r_tile == 0) mbar_arrive(&sh.q_empty);
             if (stop > begin) {
                 wait(&sh.o_full[tile], o_seen & 1u);
                 o_seen++;
                 tc_fence_after();
             }
-            any_of_tile(tile, false);
-            const float row_l = sh.sum[tile][0][r_tile], row_m = sh.sum[tile][1][r_tile];
             if (tile * kTile < pairs) {
                 const bool alone = g.first && g.last;
-                const uint32_t c0 = half * (D / 2);
-                T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d + c0;
+                T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d;
                 float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kPrefillRows * (d + 2);
-                const float inv = row_l == 0.f ? 0.f : 1.f / row_l;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
                 bool bad = false;
 #pragma unroll 1
-                for (uint32_t c = 0; c < D / 2; c += 16) {
-                    uint32_t b[16];
+                for (uint32_t c = 0; c < D; c += 32) {
+                    float o[32];
                     if (stop > begin) {
-                        tmem_ld16(o_at + c, b);
+                        tmem_ld32(o_at + c, o);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) b[e] = 0u;
+                        for (int e = 0; e < 32; e++) o[e] = 0.f;
                     }
                     if (row < pairs) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 8) {
-                            if (c0 + c + e >= d) break;
-                            float o[8];
+                        for (int e = 0; e < 32; e += 8) {
+                            if (c + e >= d) break;
 #pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                o[i] = __uint_as_float(b[e + i]);
-                                bad |= !(fabsf(o[i]) <= FLT_MAX);
-                            }
+                            for (int i = 0; i < 8; i++) bad |= !(fabsf(o[e + i]) <= FLT_MAX);
                             if (alone) {
-                                *reinterpret_cast<uint4 *>(out + c + e) =
-                                    make_uint4(pack<T>(o[0] * inv, o[1] * inv), pack<T>(o[2] * inv, o[3] * inv), pack<T>(o[4] * inv, o[5] * inv), pack<T>(o[6] * inv, o[7] * inv));
+                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pack<T>(o[e] * inv, o[e + 1] * inv), pack<T>(o[e + 2] * inv, o[e + 3] * inv),
+                                                                                    pack<T>(o[e + 4] * inv, o[e + 5] * inv), pack<T>(o[e + 6] * inv, o[e + 7] * inv));
                             } else {
-                                *reinterpret_cast<float4 *>(part + row * d + c0 + c + e) = make_float4(o[0], o[1], o[2], o[3]);
-                                *reinterpret_cast<float4 *>(part + row * d + c0 + c + e + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                                *reinterpret_cast<float4 *>(part + row * d + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                                *reinterpret_cast<float4 *>(part + row * d + c + e + 4) = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
                             }
                         }
                     }
                     __syncwarp();                        // the next columns are read by the whole warp
                 }
-                if (!alone && half == 0 && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(row_m, row_l);
-                // a row that either thread finds spoilt is computed again by the first one's warp, behind both threads' stores
-                if (any_of_tile(tile, bad)) {
-                    sh.sum[tile][half][r_tile] = bad ? 1.f : 0.f;
-                    any_of_tile(tile, false);
-                    const bool redo = half == 0 && (sh.sum[tile][0][r_tile] != 0.f || sh.sum[tile][1][r_tile] != 0.f);
-                    for (uint32_t left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
-                        const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
-                        float rm, rl, acc[D / 32];
-                        row_again<T, D>(a, g, r, stop, rm, rl, acc);
-                        const uint32_t tok = r / g.heads, hd = r - tok * g.heads;
+                if (!alone && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(m, l);
+                for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
+                    const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
+                    float rm, rl, acc[D / 32];
+                    row_again<T, D>(a, g, r, stop, rm, rl, acc);
+                    const uint32_t tok = r / g.heads, hd = r - tok * g.heads;
+                    __syncwarp();                        // behind the row's own stores
 #pragma unroll
-                        for (int i = 0; i < D / 32; i++) {
-                            const uint32_t c = lane + 32 * i;
-                            if (c >= d) continue;
-                            if (alone) static_cast<T *>(a.out)[(size_t)(g.row0 + tok) * a.out_pitch + (size_t)(g.head0 + hd) * d + c] = rounded<T>(rl == 0.f ? 0.f : acc[i] / rl);
-                            else       part[r * d + c] = acc[i];
-                        }
-                        if (!alone && lane == 0) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * r) = make_float2(rm, rl);
+                    for (int i = 0; i < D / 32; i++) {
+                        const uint32_t c = lane + 32 * i;
+                        if (c >= d) continue;
+                        if (alone) static_cast<T *>(a.out)[(size_t)(g.row0 + tok) * a.out_pitch + (size_t)(g.head0 + hd) * d + c] = rounded<T>(rl == 0.f ? 0.f : acc[i] / rl);
+                        else       part[r * d + c] = acc[i];
                     }
+                    if (!alone && lane == 0) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * r) = make_float2(rm, rl);
+                    __syncwarp();
                 }
                 if (!alone && tid == 0) name_part(a, blockIdx.x, g);
             }
-            any_of_tile(tile, false);                    // sums read, before the next unit's; O read by all warps, before it is written again
             tc_fence_before();
             __syncwarp();
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 17) {
+    if (warp == 9) {
         __syncwarp();
         tc_fence_after();
         tmem_free(tmem, 512);

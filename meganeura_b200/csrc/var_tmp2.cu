@@ -1,0 +1,677 @@
+// Attention of many new tokens per sequence (portions of prompts, long drafts) over a paged cache of f16 or bf16, on tcgen05.
+//
+// A unit is 256 pairs of token and query head of one key / value head, two tiles of 128 rows that share the keys and values of a block
+// of 128.  Per block and tile S = Q K^T and O += P V are four to eight products of K = 16 each way; the tensor cores need 512 cycles for either (heads of 128),
+// and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a row per thread: S from TMEM, running maximum and sum in f32, P back into TMEM over S (as the
+//                   16-bit left operand of the second product), results out of TMEM.  Two warps per row need a barrier per block (280 cycles, 671 us for
+//                   4 x 2048 tokens); four lanes per row read TMEM at half the rate (500 cycles of a block, 653 us).
+//   warp 8          keys and values: TMA boxes of a page's tokens (128 at most) by 64 elements, a lane each, into a ring of stages that hold
+//                   128 keys or 128 values.
+//   warp 9          issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
+//                   S(j + 1) done knows that O(j) is.  O(j) begins when the weights of the first 64 keys are there.
+//   warp 10         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
+// Sums are kept relative to a maximum that may be 2^8 too low: only where a row's maximum grows by more is O scaled.  Weights are
+// rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.
+// TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
+#include <cfloat>
+#include <cstdint>
+
+#include "mgq_paged.cuh"
+
+namespace mgq {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kSoft = 2;                                 // of eight pairs of exponentials, those that go to the multiply-add units
+constexpr int kExtra = 4;                                // blocks of keys that starting and ending a unit take as long as
+constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
+constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
+template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return D / 64 * kHalf; }
+template <int D> __host__ __device__ constexpr int stages() { return D == 64 ? 8 : 5; }
+
+__device__ unsigned int g_prefill_error;
+
+using Way = Walk<kPrefillRows, kKeys, kExtra>;
+struct __align__(16) Shared {
+    unsigned long long full[8], empty[8], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2];
+    Way way[2];                                          // of the producers of keys and of queries
+    Segment kv_seg, next, seg[2];                        // of the producer of keys; of that of queries; of everybody else, two units in turn, no tokens behind the last
+    int more;
+    uint32_t there[8][4];                                // keys of a block that exist, for the last eight blocks
+    uint32_t holes[2];                                   // whether the unit's keys have pages that do not exist
+    uint32_t tmem;
+    volatile int failed;
+};
+template <int D> constexpr size_t smem_bytes() { return (size_t)(2 + stages<D>()) * stage_bytes<D>() + sizeof(Shared); }
+static_assert(smem_bytes<128>() <= 227 * 1024 && smem_bytes<64>() <= 227 * 1024, "shared memory of an SM");
+
+template <typename T> __device__ __forceinline__ uint32_t pack(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack<__half>(float x, float y)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float x, float y)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The largest; NaN if one is NaN.
+__device__ __forceinline__ float max3(float x, float y, float z)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+// Two f32 side by side, for instructions that take two.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair_of(float x, float y)
+{
+    pair_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void parts_of(pair_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ pair_t pair_fma(pair_t x, pair_t y, pair_t z)
+{
+    pair_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ pair_t pair_add(pair_t x, pair_t y)
+{
+    pair_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+// 2^x of finite x <= 127 on the multiply-add units: 16 exponentials per cycle leave an SM idle for half of attention's time
+// (heads of 128).  x = n + f with n whole and f in [-1/2, 1/2]: 2^f by a polynomial fitted to the least relative error (7.5e-5 of degree 3 for
+// bf16 weights, 2.6e-6 of degree 4 for f16 ones), n added to its exponent.  Below 2^-126 the result stays there.
+template <typename T>
+__device__ __forceinline__ float exp2_soft(float x)
+{
+    constexpr bool kFour = std::is_same<T, __half>::value;
+    x = fmaxf(x, -126.f);
+    const float r = x + 12582912.f, f = x - (r - 12582912.f);            // 1.5 * 2^23: the sum's last bits are the rounded value
+    const float p = kFour ? fmaf(fmaf(fmaf(fmaf(0.009570102207362652f, f, 0.05591785907745361f), f, 0.240247443318367f), f, 0.6931217908859253f), f, 0.9999992847442627f)
+                          : fmaf(fmaf(fmaf(0.0551716685295105f, f, 0.2426111251115799f), f, 0.6932609677314758f), f, 0.9999280571937561f);
+    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
+}
+// 64 columns of this lane's row; wait_row before they are used.
+__device__ __forceinline__ void tmem_ld_row(uint32_t addr, float (&y)[64])
+{
+#pragma unroll
+    for (int c = 0; c < 64; c += 32)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                     "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                     "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                     : "=f"(y[c + 0]), "=f"(y[c + 1]), "=f"(y[c + 2]), "=f"(y[c + 3]), "=f"(y[c + 4]), "=f"(y[c + 5]), "=f"(y[c + 6]), "=f"(y[c + 7]),
+                       "=f"(y[c + 8]), "=f"(y[c + 9]), "=f"(y[c + 10]), "=f"(y[c + 11]), "=f"(y[c + 12]), "=f"(y[c + 13]), "=f"(y[c + 14]), "=f"(y[c + 15]),
+                       "=f"(y[c + 16]), "=f"(y[c + 17]), "=f"(y[c + 18]), "=f"(y[c + 19]), "=f"(y[c + 20]), "=f"(y[c + 21]), "=f"(y[c + 22]), "=f"(y[c + 23]),
+                       "=f"(y[c + 24]), "=f"(y[c + 25]), "=f"(y[c + 26]), "=f"(y[c + 27]), "=f"(y[c + 28]), "=f"(y[c + 29]), "=f"(y[c + 30]), "=f"(y[c + 31])
+                     : "r"(addr + c) : "memory");
+}
+__device__ __forceinline__ void wait_row(float (&y)[64])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < 64; c++) asm volatile("" : "+f"(y[c]));      // nothing that uses them moves in front of the wait
+}
+__device__ __forceinline__ float row_max(const float (&y)[64])
+{
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) t[i] = max3(y[i], y[4 + i], y[8 + i]);
+#pragma unroll
+    for (int e = 12; e < 60; e += 8)
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = max3(t[i], y[e + i], y[e + 4 + i]);
+    return max3(max3(t[0], t[1], y[60]), max3(t[2], t[3], y[61]), max3(y[62], y[63], y[63]));
+}
+// All 128 threads of a tile's warps: whether any of them says so.
+__device__ __forceinline__ bool any_of_tile(uint32_t tile, bool mine)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)mine), "r"(tile + 1) : "memory");
+    return any != 0;
+}
+// Bits lo .. hi - 1 of the 32 that begin at `base`.
+__device__ __forceinline__ uint32_t bits(int lo, int hi, int base)
+{
+    lo = max(lo - base, 0);
+    hi = min(hi - base, 32);
+    return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - hi + lo)) << lo;
+}
+
+// Key blocks of one tile of a segment: [g.begin, what is returned).  last_token: that of the tile's last row, were all tokens there.
+__device__ __forceinline__ uint32_t tile_end(const Segment &g, uint32_t tile, uint32_t last_token)
+{
+    if (tile * kTile >= g.tokens * g.heads) return g.begin;
+    const int last = min(g.pos0 + (int)min(last_token, g.tokens - 1), g.len - 1);
+    return last < 0 ? g.begin : max(g.begin, min(g.end, (uint32_t)last / kKeys + 1));
+}
+
+// One row of a segment again, on the CUDA cores and without what it does not see: where a value that only other rows see is infinite or NaN, its
+// product with a weight of 0 has spoilt the row.  A whole warp; lane i has columns i, i + 32, ...
+template <typename T, int D>
+__device__ __noinline__ void row_again(const AttendArgs &a, const Segment &g, uint32_t r, uint32_t end, float &m, float &l, float (&acc)[D / 32])
+{
+    const uint32_t lane = threadIdx.x & 31u, token = r / g.heads, head = g.head0 + r - token * g.heads;
+    const int pos = g.pos0 + (int)token;
+    float q[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        const uint32_t c = lane + 32 * i;
+        q[i] = c < a.d ? to_f32(static_cast<const T *>(a.q)[(size_t)(g.row0 + token) * a.q_pitch + (size_t)head * a.d + c]) * a.scale_log2 : 0.f;
+        acc[i] = 0.f;
+    }
+    m = -INFINITY;
+    l = 0.f;
+    const int stop = min(min((int)(end * kKeys), pos + 1), g.len);
+    for (int key = (int)(g.begin * kKeys); key < stop; key++) {
+        if (a.window && key <= pos - (int)a.window) continue;
+        const uint32_t page = g.table[(uint32_t)key >> a.page_shift];
+        if (page >= a.pages) continue;
+        const size_t at = ((((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * a.d;
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+            if (lane + 32 * i < a.d) x = fmaf(q[i], to_f32(static_cast<const T *>(a.k)[at + lane + 32 * i]), x);
+        x = warp_sum(x);
+        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - base), p = exp2_fast(x - base);
+        l = l * keep + p;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+            if (lane + 32 * i < a.d) acc[i] = acc[i] * keep + (p != 0.f ? p * to_f32(static_cast<const T *>(a.v)[at + lane + 32 * i]) : 0.f);
+    }
+}
+
+template <typename T, int D>                             // D: head size rounded up to 64 or 128
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ CacheMaps maps, const __grid_constant__ CUtensorMap q_map, const AttendArgs a)
+{
+    constexpr int S = stages<D>(), PARTS = D / 64;
+    constexpr uint32_t kStage = stage_bytes<D>();
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+    constexpr uint32_t kInstrS = (1u << 4) | kType | (kKeys >> 3 << 17) | (kTile >> 4 << 24);
+    constexpr uint32_t kInstrO = (1u << 4) | kType | (1u << 16) | ((uint32_t)D >> 3 << 17) | (kTile >> 4 << 24);
+    extern __shared__ __align__(1024) uint8_t smem_raw[];                 // swizzled tiles lie on multiples of 1024
+    uint8_t *s_q = smem_raw, *ring = s_q + 2 * kStage;
+    Shared &sh = *reinterpret_cast<Shared *>(ring + S * kStage);
+    if (smem_u32(smem_raw) % 1024 != 0) {                                 // cannot be with the alignment above
+        if (threadIdx.x == 0) atomicExch(&g_prefill_error, 1u);
+        return;
+    }
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
+
+    if (tid == 0) {
+        for (int s = 0; s < S; s++) {
+            mbar_init(&sh.full[s], 1);
+            mbar_init(&sh.empty[s], 1);
+        }
+        mbar_init(&sh.q_full, 1);
+        mbar_init(&sh.q_empty, 3);                                        // the issuer, both tiles' warps
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_half[i], 4);
+            mbar_init(&sh.p_full[i], 4);
+            mbar_init(&sh.o_full[i], 1);
+        }
+        sh.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) tmem_alloc(&sh.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t slice = min(a.group, kPrefillRows), rows = kPrefillRows / slice * slice;       // heads of a unit, rows that TMA fills
+    {
+        Way way;
+        way.begin(a, blockIdx.x, gridDim.x, 1, reinterpret_cast<unsigned long long *>(s_q));
+        if (lane == 0 && (warp == 8 || warp == 10)) sh.way[warp == 10] = way;
+    }
+    for (uint32_t i = tid; i < (kPrefillRows - rows) * PARTS * 8; i += kThreads) {            // the others are zero for good
+        const uint32_t part = i / ((kPrefillRows - rows) * 8), at = i - part * (kPrefillRows - rows) * 8;
+        *reinterpret_cast<uint4 *>(s_q + part * 2 * kHalf + rows * 128 + at * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (tid == 0) clear_parts(a, blockIdx.x);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    // the tokens of the tiles' last rows
+    const uint32_t last_token[2] = {(kTile - 1) / slice, (2 * kTile - 1) / slice};
+    // Each lane by itself: false where the limit ran out, or another role has given up.
+    auto lane_wait = [&](unsigned long long *bar, uint32_t parity) {
+        return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, &sh.failed, &g_prefill_error);
+    };
+    auto wait = [&](unsigned long long *bar, uint32_t parity) {
+        const bool done = lane_wait(bar, parity);
+        __syncwarp();
+        return done;
+    };
+    auto wait_all = [&](unsigned long long *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+    // Registers where they are needed: 256 * 216 + 128 * 72 = 384 * 168.
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else           asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (warp == 8) {
+        const uint32_t shift = a.page_shift, page_keys = 1u << shift, box = min(page_keys, kKeys), boxes = kKeys / box, gone = a.pages << shift;
+        uint32_t slot = 0, round = 0, block = 0;
+        int armed = 0;
+        bool ok = true;
+        while (ok) {
+            int more_units = 0;
+            if (lane == 0) more_units = sh.way[0].next(a, sh.kv_seg);
+            __syncwarp();
+            if (!__shfl_sync(0xffffffffu, more_units, 0)) break;
+            const Segment &g = sh.kv_seg;
+            const int len = g.len, kv = (int)g.kv;
+            const uint32_t *table = g.table;
+            const uint32_t kb_end = g.end;
+            for (uint32_t kb = g.begin; ok && kb < kb_end; kb++, block++) {
+                // lane = box of the block + boxes * group of 64 elements
+                const uint32_t b = lane % boxes, part = lane / boxes, key = kb * kKeys + b * box;
+                uint32_t y = gone, have = 0;
+                if ((int)key < len) {
+                    const uint32_t page = table[key >> shift];
+                    if (page < a.pages) {
+                        y = (page << shift) + (key & (page_keys - 1));
+                        have = min(box, (uint32_t)len - key);
+                    }
+                }
+                uint32_t there[4];
+#pragma unroll
+                for (int w = 0; w < 4; w++) there[w] = __reduce_or_sync(0xffffffffu, bits(b * box, b * box + have, 32 * w));
+#pragma unroll
+                for (int what = 0; what < 2 && ok; what++) {
+                    if (!(ok = wait_all(&sh.empty[slot], (round & 1u) ^ 1u))) break;
+                    if (lane == 0) {
+                        if (what == 0)
+                            for (int w = 0; w < 4; w++) sh.there[block & 7u][w] = there[w];
+                        mbar_arrive_expect_tx(&sh.full[slot], kStage);
+                    }
+                    __syncwarp();
+                    if (part < PARTS)
+                        tma_load_3d(smem_u32(ring) + slot * kStage + part * kHalf + b * box * 128, what ? &maps.v : &maps.k, (int)part * 64, kv, (int)y, &sh.full[slot]);
+                    __syncwarp();
+                    armed++;
+                    if (++slot == S) { slot = 0; round++; }
+                }
+            }
+        }
+        // given up: the copies in flight land before the CTA exits
+        if (!ok && lane == 0)
+            for (int i = 0; i < min(armed, S); i++) {
+                if (slot-- == 0) { slot = S - 1; round--; }
+                for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.full[slot], round & 1u); w++) { }
+            }
+    } else if (warp == 10) {
+        uint32_t unit = 0;
+        bool ok = true, more = true;
+        for (; more; unit++) {
+            if (lane == 0) {
+                sh.next.tokens = 0;
+                sh.more = sh.way[1].next(a, sh.next);
+            }
+            __syncwarp();
+            more = sh.more != 0;
+            bool holes = false;
+            if (more && sh.next.end > sh.next.begin) {
+                const uint32_t first = sh.next.begin * kKeys >> a.page_shift, last = (min(sh.next.end * kKeys, (uint32_t)sh.next.len) - 1) >> a.page_shift;
+                for (uint32_t j = first + lane; j <= last; j += 32) holes |= sh.next.table[j] >= a.pages;
+            }
+            holes = __any_sync(0xffffffffu, holes);
+            if (!(ok = wait_all(&sh.q_empty, (unit & 1u) ^ 1u))) break;
+            if (lane == 0) {
+                Segment &g = sh.seg[unit & 1u];
+                g = sh.next;
+                if (!more) g.tokens = 0;
+                sh.holes[unit & 1u] = holes;
+                if (more && g.end > g.begin) {
+                    mbar_arrive_expect_tx(&sh.q_full, PARTS * rows * 128);
+                    for (int c = 0; c < PARTS; c++) tma_load_3d(smem_u32(s_q) + c * 2 * kHalf, &q_map, c * 64, (int)g.head0, (int)g.row0, &sh.q_full);
+                } else {
+                    mbar_arrive(&sh.q_full);
+                }
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0 && unit > 0)                // given up: the copy in flight lands before the CTA exits
+            for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.q_full, (unit - 1) & 1u); w++) { }
+    } else if (warp == 9) {
+        // All lanes run along, one issues; nothing in here needs them together.
+        const bool leader = elect_one();
+        const uint32_t q16 = smem_u32(s_q) >> 4, ring16 = smem_u32(ring) >> 4;
+        uint32_t slot = 0, round = 0, p_seen = 0;                         // p_seen: parities of the two tiles in bits 0 and 1
+        bool ok = true;
+        auto advance = [&]() {
+            if (++slot == S) { slot = 0; round++; }
+        };
+        auto scores = [&](uint32_t tile, uint32_t at) {
+            if (leader) {
+                const uint32_t q = q16 + tile * (kHalf / 16), k = ring16 + at * (kStage / 16);
+                umma_step<false>(tmem + tile * 128, q, k, kInstrS);
+#pragma unroll
+                for (uint32_t i = 1; i < D / 16; i++) umma_step<true>(tmem + tile * 128, q + i / 4 * (2 * kHalf / 16) + i % 4 * 2, k + i / 4 * (kHalf / 16) + i % 4 * 2, kInstrS);
+                umma_commit(&sh.s_full[tile]);
+            }
+        };
+        // 64 keys, 16 per product
+        auto values = [&](uint32_t tile, uint32_t at, uint32_t part, bool first) {
+            if (leader) {
+                const uint32_t v = ring16 + at * (kStage / 16), o = tmem + 256 + tile * D, p = tmem + tile * 128;
+#pragma unroll
+                for (uint32_t i = 0; i < kKeys / 32; i++) {
+                    const uint32_t step = part * 4 + i;
+                    umma_f16_ts_mn(o, p + step * 8, v + step * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0 || part > 0);
+                }
+            }
+        };
+        for (uint32_t unit = 0;; unit++) {
+            if (!(ok = lane_wait(&sh.q_full, unit & 1u))) break;
+            const Segment &g = sh.seg[unit & 1u];
+            if (g.tokens == 0) break;
+            const uint32_t begin = g.begin, end = g.end, stop[2] = {tile_end(g, 0, last_token[0]), tile_end(g, 1, last_token[1])};
+            if (end <= begin) {
+                if (leader) mbar_arrive(&sh.q_empty);
+                continue;
+            }
+            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+            tc_fence_after();
+#pragma unroll
+            for (uint32_t tile = 0; tile < 2; tile++)
+                if (stop[tile] > begin) scores(tile, slot);
+            if (leader) {
+                umma_commit(&sh.empty[slot]);
+                if (begin + 1 == end) umma_commit(&sh.q_empty);
+            }
+            advance();
+            for (uint32_t kb = begin; ok && kb < end; kb++) {
+                const uint32_t v_slot = slot;
+                if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+                tc_fence_after();
+                advance();
+                const bool more = kb + 1 < end;
+                bool waited = false;
+#pragma unroll
+                for (uint32_t tile = 0; tile < 2; tile++) {
+                    if (stop[tile] > kb) {
+                        if (!(ok = lane_wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
+                        tc_fence_after();
+                        values(tile, v_slot, 0, kb == begin);
+                        if (!(ok = lane_wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
+                        p_seen ^= 1u << tile;
+                        tc_fence_after();
+                        values(tile, v_slot, 1, false);
+                        if (kb + 1 == stop[tile] && leader) umma_commit(&sh.o_full[tile]);
+                    }
+                    if (stop[tile] > kb + 1) {
+                        if (!waited) {
+                            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+                            tc_fence_after();
+                            waited = true;
+                        }
+                        scores(tile, slot);
+                    }
+                }
+                if (!ok) break;
+                if (leader) umma_commit(&sh.empty[v_slot]);
+                if (more) {
+                    if (!waited && !(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+                    if (leader) {
+                        umma_commit(&sh.empty[slot]);
+                        if (kb + 2 == end) umma_commit(&sh.q_empty);      // no more scores of this unit
+                    }
+                    advance();
+                }
+            }
+            if (!ok) break;
+        }
+    } else if (warp < 8) {
+        const uint32_t tile = warp >> 2, quad = warp & 3u, r_tile = quad * 32 + lane, row = tile * kTile + r_tile, d = a.d;
+        const uint32_t lanes = (quad * 32u) << 16, s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * D + lanes;
+        const float scale = a.scale_log2;
+        const uint32_t token = row / slice, head = row - token * slice, first_token = tile * kTile / slice;     // of this row, of the tile's first
+        uint32_t slot = 0, round = 0, block = 0;         // of the ring, as the producer counts
+        uint32_t s_seen = 0, o_seen = 0;
+        // Where a wait runs out the tile's warps run on without waiting, and leave together at the next unit.
+        for (uint32_t unit = 0;; unit++) {
+            const bool there_is = wait(&sh.q_full, unit & 1u);
+            const Segment &g = sh.seg[unit & 1u];
+            if (any_of_tile(tile, !there_is)) break;
+            if (g.tokens == 0) break;
+            const uint32_t begin = g.begin, end = g.end, stop = tile_end(g, tile, last_token[tile]), pairs = g.tokens * g.heads;
+            const int first_pos = g.pos0 + (int)first_token, len = g.len;
+            const int last_pos = g.pos0 + (int)min(last_token[tile], g.tokens - 1), window = (int)a.window;
+            const int pos = row < pairs ? g.pos0 + (int)token : -1;
+            const bool holes = sh.holes[unit & 1u] != 0;
+            float m = -INFINITY, l = 0.f;
+            for (uint32_t kb = begin; kb < end; kb++, block++) {
+                if (++slot == S) { slot = 0; round++; }
+                const uint32_t v_slot = slot, v_round = round;
+                if (++slot == S) { slot = 0; round++; }
+                if (kb >= stop) continue;
+                wait(&sh.s_full[tile], s_seen & 1u);
+                s_seen++;
+                tc_fence_after();
+                const int key0 = (int)(kb * kKeys);
+                const bool every = !holes && key0 + (int)kKeys <= len;
+                const bool plain = every && key0 + (int)kKeys - 1 <= first_pos && !(window && key0 <= last_pos - window);      // nothing is masked
+                uint32_t there[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                if (!every) {
+                    // For sight of `there`, and to write into the values.  Not the keys' barrier: their stage is free by now and may have been
+                    // filled again, two phases on, where this parity would wait for a third.  The values' stage is free behind this tile's product only.
+                    wait(&sh.full[v_slot], v_round & 1u);
+#pragma unroll
+                    for (int w = 0; w < 4; w++) there[w] = sh.there[block & 7u][w];
+                    // values that nobody sees, whatever the page holds there, become zeros
+                    uint8_t *v = ring + v_slot * kStage;
+                    for (uint32_t i = r_tile; i < kKeys * PARTS * 8; i += 128) {
+                        const uint32_t key = i / 8 % kKeys, w = key / 32, word = w == 0 ? there[0] : w == 1 ? there[1] : w == 2 ? there[2] : there[3];
+                        if (!(word >> (key % 32) & 1u)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    any_of_tile(tile, false);            // all of them have, before the first weights are signalled
+                }
+                // 64 keys: what the row does not see
+                auto mask = [&](float (&s)[64], int c) {
+                    if (plain) return;
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        const uint32_t seen = there[2 * c + w] & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 64 * c + 32 * w);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) s[32 * w + e] = seen >> e & 1u ? s[32 * w + e] : -INFINITY;
+                    }
+                    __syncwarp();
+                };
+                float s[64], t[64];
+                tmem_ld_row(s_at, s);
+                tmem_ld_row(s_at + 64, t);
+                wait_row(s);
+                wait_row(t);
+                mask(s, 0);
+                mask(t, 1);
+                const float first = row_max(s), second = row_max(t), top = max3(first, second, second) * scale;
+                // Nothing to do where the maximum stays at or below the old one + 8 (finite behind the first block); -inf and NaN come here, too.
+                bool exact = !plain;
+                if (__any_sync(0xffffffffu, !(top <= m + 8.f && top >= -FLT_MAX))) {
+                    const bool up = !(top <= m + 8.f) && top > -INFINITY;              // also where m is still -inf
+                    const float keep = up ? exp2_fast(m - top) : 1.f;
+                    l *= keep;
+                    m = up ? top : m;
+                    exact = __any_sync(0xffffffffu, exact || !(fabsf(top) <= FLT_MAX));
+                    if (kb != begin && __any_sync(0xffffffffu, up)) {
+#pragma unroll 1
+                        for (uint32_t c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + c, o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st16(o_at + c, o);
+                        }
+                    }
+                }
+                const pair_t scales = pair_of(scale, scale);
+                const float base = m == -INFINITY ? 0.f : -m;
+                const pair_t bases = pair_of(base, base);
+                pair_t sum[2] = {0, 0};
+                auto weights = [&](const float (&s)[64], int c, bool soft) {       // 64 keys: exponentials, sums, P
+#pragma unroll
+                    for (int i = 0; i < 64; i += 32) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            float x, y;
+                            parts_of(pair_fma(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), scales, bases), x, y);
+                            x = soft && e % 8 < kSoft ? exp2_soft<T>(x) : exp2_fast(x);
+                            y = soft && e % 8 < kSoft ? exp2_soft<T>(y) : exp2_fast(y);
+                            sum[e & 1] = pair_add(sum[e & 1], pair_of(x, y));
+                            p[e] = pack<T>(x, y);
+                        }
+                        tmem_st16(s_at + 32 * c + i / 2, p);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c ? &sh.p_full[tile] : &sh.p_half[tile]);
+                };
+                    weights(s, 0, false);
+                    weights(t, 1, false);
+                float x, y;
+                parts_of(pair_add(sum[0], sum[1]), x, y);
+                l += x + y;
+            }
+            // this tile's scores are done with the queries (its warps have met in this unit)
+            if (r_tile == 0) mbar_arrive(&sh.q_empty);
+            if (stop > begin) {
+                wait(&sh.o_full[tile], o_seen & 1u);
+                o_seen++;
+                tc_fence_after();
+            }
+            if (tile * kTile < pairs) {
+                const bool alone = g.first && g.last;
+                T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d;
+                float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kPrefillRows * (d + 2);
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                bool bad = false;
+#pragma unroll 1
+                for (uint32_t c = 0; c < D; c += 32) {
+                    float o[32];
+                    if (stop > begin) {
+                        tmem_ld32(o_at + c, o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    }
+                    if (row < pairs) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            if (c + e >= d) break;
+#pragma unroll
+                            for (int i = 0; i < 8; i++) bad |= !(fabsf(o[e + i]) <= FLT_MAX);
+                            if (alone) {
+                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pack<T>(o[e] * inv, o[e + 1] * inv), pack<T>(o[e + 2] * inv, o[e + 3] * inv),
+                                                                                    pack<T>(o[e + 4] * inv, o[e + 5] * inv), pack<T>(o[e + 6] * inv, o[e + 7] * inv));
+                            } else {
+                                *reinterpret_cast<float4 *>(part + row * d + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                                *reinterpret_cast<float4 *>(part + row * d + c + e + 4) = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+                            }
+                        }
+                    }
+                    __syncwarp();                        // the next columns are read by the whole warp
+                }
+                if (!alone && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(m, l);
+                for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
+                    const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
+                    float rm, rl, acc[D / 32];
+                    row_again<T, D>(a, g, r, stop, rm, rl, acc);
+                    const uint32_t tok = r / g.heads, hd = r - tok * g.heads;
+                    __syncwarp();                        // behind the row's own stores
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) {
+                        const uint32_t c = lane + 32 * i;
+                        if (c >= d) continue;
+                        if (alone) static_cast<T *>(a.out)[(size_t)(g.row0 + tok) * a.out_pitch + (size_t)(g.head0 + hd) * d + c] = rounded<T>(rl == 0.f ? 0.f : acc[i] / rl);
+                        else       part[r * d + c] = acc[i];
+                    }
+                    if (!alone && lane == 0) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * r) = make_float2(rm, rl);
+                    __syncwarp();
+                }
+                if (!alone && tid == 0) name_part(a, blockIdx.x, g);
+            }
+            tc_fence_before();
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+template <typename T, int D>
+int launch_sized(const AttendArgs &a, const CacheMaps &maps, const CUtensorMap &q_map, cudaStream_t stream)
+{
+    auto *kernel = prefill_kernel<T, D>;
+    if (int rc = allow_smem(kernel, smem_bytes<D>())) return rc;
+    if (int rc = launch(kernel, dim3(kPrefillCtas), dim3(kThreads), smem_bytes<D>(), stream, maps, q_map, a)) return rc;
+    return launch(merge_kernel<T, (int)kPrefillRows>, dim3(kPrefillCtas, 16), dim3(kMergeThreads), 0, stream, a, kPrefillCtas);
+}
+
+// {head_dim, heads, rows} of the queries, for boxes of 64 elements by the heads of a key / value head by the tokens of a unit: as they lie in
+// shared memory then, the pairs of token and head are the rows.
+int encode_queries(CUtensorMap &map, int dtype, const AttendArgs &a)
+{
+    EncodeTiledFn encode = nullptr;
+    if (int rc = encode_fn(encode)) return rc;
+    const cuuint64_t dims[3] = {a.d, (cuuint64_t)a.kv_heads * a.group, a.rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.d * 2, (cuuint64_t)a.q_pitch * 2};
+    const cuuint32_t box[3] = {64, a.group, kPrefillRows / a.group}, elem[3] = {1, 1, 1};
+    const CUresult cr = encode(&map, dtype == MGQ_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(a.q), dims, strides, box,
+                               elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? MGQ_OK : fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+}
+
+}  // namespace
+
+bool prefill_takes(const AttendArgs &a, int dtype)
+{
+    auto on = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    // scores are masked and compared before they are scaled: a scale of 0 would make -inf NaN, a negative one turn the order around
+    return decode_takes(a, dtype) && a.d <= 128 && a.group <= kPrefillRows && a.scale_log2 >= 1e-30f && on(a.q) && on(a.out) && a.q_pitch % 8 == 0 && a.out_pitch % 8 == 0;
+}
+
+int launch_prefill(const AttendArgs &a, int dtype, cudaStream_t stream)
+{
+    CacheMaps maps;
+    if (int rc = encode_caches(maps, dtype, a, min(1u << a.page_shift, kKeys))) return rc;
+    CUtensorMap q_map;
+    if (int rc = encode_queries(q_map, dtype, a)) return rc;
+    if (dtype == MGQ_FMT_F16) return a.d <= 64 ? launch_sized<__half, 64>(a, maps, q_map, stream) : launch_sized<__half, 128>(a, maps, q_map, stream);
+    return a.d <= 64 ? launch_sized<__nv_bfloat16, 64>(a, maps, q_map, stream) : launch_sized<__nv_bfloat16, 128>(a, maps, q_map, stream);
+}
+
+int prefill_status()
+{
+    unsigned int err = 0;
+    MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_prefill_error, sizeof err));
+    if (!err) return MGQ_OK;
+    const unsigned int zero = 0;
+    MGQ_CUDA(cudaMemcpyToSymbol(g_prefill_error, &zero, sizeof zero));
+    return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the paged attention of many tokens ran out");
+}
+
+}  // namespace mgq
