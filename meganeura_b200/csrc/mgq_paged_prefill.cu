@@ -386,6 +386,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (leader) mbar_arrive(&sh.q_empty);
                 continue;
             }
+            // A wait takes the warp 100 cycles and more even where all is there already, so each stands where products are under way: for the next keys
+            // behind the first half of tile 0's values, for the next values behind that of tile 1's.
             if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
             tc_fence_after();
 #pragma unroll
@@ -396,43 +398,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (begin + 1 == end) umma_commit(&sh.q_empty);
             }
             advance();
-            for (uint32_t kb = begin; ok && kb < end; kb++) {
+            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+            for (uint32_t kb = begin; kb < end; kb++) {
                 const uint32_t v_slot = slot;
-                if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
-                tc_fence_after();
                 advance();
+                const uint32_t k_slot = slot, k_round = round;
                 const bool more = kb + 1 < end;
-                bool waited = false;
+                if (more) advance();                     // to the next values
 #pragma unroll
                 for (uint32_t tile = 0; tile < 2; tile++) {
-                    if (stop[tile] > kb) {
+                    const bool values_now = stop[tile] > kb;
+                    if (values_now) {
                         if (!(ok = lane_wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
                         tc_fence_after();
                         values(tile, v_slot, 0, kb == begin);
+                    }
+                    if (more && !(ok = lane_wait(&sh.full[tile ? slot : k_slot], (tile ? round : k_round) & 1u))) break;
+                    if (values_now) {
                         if (!(ok = lane_wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
                         p_seen ^= 1u << tile;
                         tc_fence_after();
                         values(tile, v_slot, 1, false);
                         if (kb + 1 == stop[tile] && leader) umma_commit(&sh.o_full[tile]);
                     }
-                    if (stop[tile] > kb + 1) {
-                        if (!waited) {
-                            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
-                            tc_fence_after();
-                            waited = true;
-                        }
-                        scores(tile, slot);
-                    }
+                    if (tile == 1 && leader) umma_commit(&sh.empty[v_slot]);
+                    if (stop[tile] > kb + 1) scores(tile, k_slot);
                 }
                 if (!ok) break;
-                if (leader) umma_commit(&sh.empty[v_slot]);
-                if (more) {
-                    if (!waited && !(ok = lane_wait(&sh.full[slot], round & 1u))) break;
-                    if (leader) {
-                        umma_commit(&sh.empty[slot]);
-                        if (kb + 2 == end) umma_commit(&sh.q_empty);      // no more scores of this unit
-                    }
-                    advance();
+                if (more && leader) {
+                    umma_commit(&sh.empty[k_slot]);
+                    if (kb + 2 == end) umma_commit(&sh.q_empty);          // no more scores of this unit
                 }
             }
             if (!ok) break;
