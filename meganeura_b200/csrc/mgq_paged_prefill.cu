@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     if (tid == 0) {
         for (int s = 0; s < S; s++) {
             mbar_init(&sh.full[s], 1);
-            mbar_init(&sh.empty[s], 1);
+            mbar_init(&sh.empty[s], 2);                                   // either tile's warps
         }
         mbar_init(&sh.q_full, 1);
         mbar_init(&sh.q_empty, 3);                                        // the issuer, both tiles' warps
@@ -387,16 +387,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 continue;
             }
             // A wait takes the warp 100 cycles and more even where all is there already, so each stands where products are under way: for the next keys
-            // behind the first half of tile 0's values, for the next values behind that of tile 1's.
+            // behind the first half of tile 0's values, for the next values behind that of tile 1's.  A commit takes 200: the stages are given back by the
+            // softmax warps, which learn from the scores' commits that their products are done.
             if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
             tc_fence_after();
 #pragma unroll
             for (uint32_t tile = 0; tile < 2; tile++)
                 if (stop[tile] > begin) scores(tile, slot);
-            if (leader) {
-                umma_commit(&sh.empty[slot]);
-                if (begin + 1 == end) umma_commit(&sh.q_empty);
-            }
+            if (begin + 1 == end && leader) umma_commit(&sh.q_empty);
             advance();
             if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
             for (uint32_t kb = begin; kb < end; kb++) {
@@ -421,14 +419,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                         values(tile, v_slot, 1, false);
                         if (kb + 1 == stop[tile] && leader) umma_commit(&sh.o_full[tile]);
                     }
-                    if (tile == 1 && leader) umma_commit(&sh.empty[v_slot]);
                     if (stop[tile] > kb + 1) scores(tile, k_slot);
                 }
                 if (!ok) break;
-                if (more && leader) {
-                    umma_commit(&sh.empty[k_slot]);
-                    if (kb + 2 == end) umma_commit(&sh.q_empty);          // no more scores of this unit
-                }
+                if (kb + 2 == end && leader) umma_commit(&sh.q_empty);    // no more scores of this unit
             }
             if (!ok) break;
         }
@@ -453,14 +447,38 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             const int pos = row < pairs ? g.pos0 + (int)token : -1;
             const bool holes = sh.holes[unit & 1u] != 0;
             float m = -INFINITY, l = 0.f;
+            uint32_t v_before = 0;
+            bool finished = stop <= begin;               // the last product is done, its values' stage given back
+            auto finish = [&]() {
+                if (finished) return;
+                finished = true;
+                wait(&sh.o_full[tile], o_seen & 1u);
+                o_seen++;
+                tc_fence_after();
+                if (r_tile == 0) mbar_arrive(&sh.empty[v_before]);
+            };
             for (uint32_t kb = begin; kb < end; kb++, block++) {
+                const uint32_t k_slot = slot, k_round = round;
                 if (++slot == S) { slot = 0; round++; }
                 const uint32_t v_slot = slot, v_round = round;
                 if (++slot == S) { slot = 0; round++; }
-                if (kb >= stop) continue;
+                if (kb >= stop) {
+                    finish();
+                    // nothing for this tile: it gives the stages back as soon as they are filled, not before
+                    wait(&sh.full[k_slot], k_round & 1u);
+                    if (r_tile == 0) mbar_arrive(&sh.empty[k_slot]);
+                    wait(&sh.full[v_slot], v_round & 1u);
+                    if (r_tile == 0) mbar_arrive(&sh.empty[v_slot]);
+                    continue;
+                }
                 wait(&sh.s_full[tile], s_seen & 1u);
                 s_seen++;
                 tc_fence_after();
+                if (r_tile == 0) {                       // these scores are done, and the product before them
+                    mbar_arrive(&sh.empty[k_slot]);
+                    if (kb != begin) mbar_arrive(&sh.empty[v_before]);
+                }
+                v_before = v_slot;
                 const int key0 = (int)(kb * kKeys);
                 const bool every = !holes && key0 + (int)kKeys <= len;
                 const bool plain = every && key0 + (int)kKeys - 1 <= first_pos && !(window && key0 <= last_pos - window);      // nothing is masked
@@ -555,11 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             }
             // this tile's scores are done with the queries (its warps have met in this unit)
             if (r_tile == 0) mbar_arrive(&sh.q_empty);
-            if (stop > begin) {
-                wait(&sh.o_full[tile], o_seen & 1u);
-                o_seen++;
-                tc_fence_after();
-            }
+            finish();
             if (tile * kTile < pairs) {
                 const bool alone = g.first && g.last;
                 T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d;
