@@ -206,58 +206,74 @@ __device__ __forceinline__ void name_part(const AttendArgs &a, uint32_t cta, con
 
 // Joins the parts of the unit that CTA blockIdx.x of an attention kernel began and did not end: with M the largest of the parts' maxima
 // o = sum 2^(m - M) o_part / sum 2^(m - M) l_part.  The parts are those of the CTAs that follow, up to the one that ends the
-// unit, added in this order.  Grid: (CTAs, anything): the rows are shared out over y, a warp takes a row.  Round trips to L2 bound it: states first,
-// then a row's maxima and weights by all lanes, then its sums, several parts in flight.
-constexpr int kMergeThreads = 128, kMergeWarps = kMergeThreads / 32, kMaxCtas = 148 * 3;
-template <typename T, int ROWS>
+// unit, added in this order.  Grid: (CTAs, anything): the rows are shared out over y, a warp takes a row.  Round trips to L2 bound it: a warp finds the
+// unit's end with one, then takes eight parts with each, maxima, weights and sums together.
+constexpr int kMergeThreads = 128, kMergeWarps = kMergeThreads / 32;
+template <typename T, int ROWS, int COLS>                // COLS: columns of a lane
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a, uint32_t ctas)
 {
-    __shared__ float s_weight[kMergeWarps][kMaxCtas];
-    __shared__ uint32_t s_end;
-    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, c0 = blockIdx.x;
+    constexpr int kBatch = COLS > 4 ? 4 : 8;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, c0 = blockIdx.x;
     pdl_launch_dependents();
     pdl_wait();
     const PartHead h = a.heads[2 * c0 + 1];
     if (h.state != kOpens) return;
-    if (t == 0) s_end = ctas - 1;
-    __syncthreads();
-    for (uint32_t c = c0 + 1 + t; c < ctas; c += kMergeThreads)
-        if (a.heads[2 * c].state == kCloses) {
-            atomicMin(&s_end, c);
+    uint32_t parts = 1;
+    for (;; parts += 32) {
+        const uint32_t c = c0 + parts + lane, last = __ballot_sync(0xffffffffu, c + 1 >= ctas || a.heads[2 * c].state == kCloses);
+        if (last) {
+            parts += __ffs(last);
             break;
         }
-    __syncthreads();
-    const uint32_t parts = s_end - c0 + 1, d = a.d;
+    }
+    const uint32_t d = a.d;
     const size_t size = (size_t)ROWS * (d + 2);
-    const float *first = a.parts + (2 * (size_t)c0 + 1) * size, *rest = a.parts + 2 * (size_t)c0 * size;     // part i > 0 at rest + 2 i size
-    auto part = [&](uint32_t i) { return i == 0 ? first : rest + 2 * i * size; };
     for (uint32_t r = blockIdx.y * kMergeWarps + warp; r < h.tokens * h.heads; r += gridDim.y * kMergeWarps) {
-        float top = -INFINITY;
-        for (uint32_t i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[ROWS * d + 2 * r]);
-        top = warp_max(top);
-        float l = 0.f;
-        for (uint32_t i = lane; i < parts; i += 32) {
-            const float m = part(i)[ROWS * d + 2 * r], mine = part(i)[ROWS * d + 2 * r + 1];
-            const float w = mine != 0.f ? exp2f(m - top) : 0.f;      // a NaN is a weight
-            s_weight[warp][i] = w;
-            l += w * mine;
+        float top = -INFINITY, l = 0.f, o[COLS];
+#pragma unroll
+        for (int i = 0; i < COLS; i++) o[i] = 0.f;
+        for (uint32_t p0 = 0; p0 < parts; p0 += kBatch) {
+            float2 ml[kBatch];
+            float v[kBatch][COLS];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                const uint32_t p = p0 + b;
+                const float *part = a.parts + (2 * (size_t)(c0 + p) + (p == 0 ? 1 : 0)) * size;
+                const bool live = p < parts;
+                ml[b] = live ? make_float2(part[ROWS * d + 2 * r], part[ROWS * d + 2 * r + 1]) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int i = 0; i < COLS; i++) v[b][i] = live && lane + 32 * i < d ? part[r * d + lane + 32 * i] : 0.f;
+            }
+            const float before = top;
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) top = fmaxf(top, ml[b].x);
+            const float keep = before > -INFINITY ? exp2f(before - top) : 1.f;
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < COLS; i++) o[i] *= keep;
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                const float w = ml[b].y != 0.f ? exp2f(ml[b].x - top) : 0.f;         // a NaN is a weight; a part without weight may hold anything
+                l += w * ml[b].y;
+#pragma unroll
+                for (int i = 0; i < COLS; i++) o[i] += w != 0.f ? w * v[b][i] : 0.f;
+            }
         }
-        l = warp_sum(l);
-        __syncwarp();
         const float scale = l == 0.f ? 0.f : 1.f / l;
         const uint32_t token = r / h.heads, head = r - token * h.heads;
         T *out = static_cast<T *>(a.out) + (size_t)(h.row0 + token) * a.out_pitch + (size_t)(h.head0 + head) * d;
-        for (uint32_t col = lane; col < d; col += 32) {
-            float o = 0.f;
-#pragma unroll 8
-            for (uint32_t i = 0; i < parts; i++) {
-                const float w = s_weight[warp][i], v = part(i)[r * d + col];
-                o += w != 0.f ? w * v : 0.f;                         // a part without weight may hold anything
-            }
-            out[col] = rounded<T>(o * scale);
-        }
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < COLS; i++)
+            if (lane + 32 * i < d) out[lane + 32 * i] = rounded<T>(o[i] * scale);
     }
+}
+// pairs: a bound of the rows of a unit that has parts.
+template <typename T, int ROWS>
+int launch_merge(const AttendArgs &a, uint32_t ctas, uint32_t pairs, cudaStream_t stream)
+{
+    const dim3 grid(ctas, (min(pairs, (uint32_t)ROWS) + kMergeWarps - 1) / kMergeWarps);
+    return a.d <= 128 ? launch(merge_kernel<T, ROWS, 4>, grid, dim3(kMergeThreads), 0, stream, a, ctas)
+                      : launch(merge_kernel<T, ROWS, 8>, grid, dim3(kMergeThreads), 0, stream, a, ctas);
 }
 
 // 16-bit types with heads of a multiple of 8 elements on 16-byte boundaries: few new tokens (mgq_paged_decode.cu).

@@ -10,15 +10,23 @@ constexpr int kThreads = 128, kWarps = 4;
 constexpr int kRows = 16, kKeys = 32;                    // pairs of token and head, keys of a block
 constexpr int kRowsPerWarp = kRows / kWarps;
 
+__device__ __forceinline__ void copy16(float *dst, const void *src, bool real)
+{
+    const uint32_t bytes = real ? 16 : 0;                // the rest is zero-filled
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
 // out[row, col] (+)= over a tile of 32 keys: a warp scores four rows with a key per lane, a thread sums one or two columns for all rows.
-template <typename T, int COLS>                          // COLS: columns per thread, heads of up to 128 * COLS
+// Four threads fetch a key and its value; with 16-byte rows in f32 (WIDE) asynchronously, a tile ahead.  Single tokens are bound by these loads,
+// portions by the multiply-adds' operands from shared memory.
+template <typename T, int COLS, bool WIDE>               // COLS: columns per thread, heads of up to 128 * COLS
 __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
 {
     extern __shared__ __align__(16) float s_mem[];
     __shared__ unsigned long long s_walk[40];
     __shared__ float s_p[kRows][kKeys], s_scale[kRows];
-    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, d = a.d, d4 = (d + 3) / 4 * 4, pitch = d4 + 4;
-    float *s_q = s_mem, *s_k = s_q + kRows * d4, *s_v = s_k + kKeys * pitch;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, d = a.d, d4 = (d + 3) / 4 * 4, pitch = d4 + 4, tile = 2 * kKeys * pitch;
+    float *s_q = s_mem, *s_tiles = s_q + kRows * d4;
     pdl_launch_dependents();
     pdl_wait();
     Walk<kRows, kKeys, 1> walk;
@@ -28,10 +36,32 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     Segment g;
     while (walk.next(a, g)) {
         const uint32_t pairs = g.tokens * g.heads;
+        auto fetch = [&](uint32_t kb) {
+            const uint32_t j = t / 4, key = kb * kKeys + j;
+            const uint32_t page = (int)key < g.len ? g.table[key >> a.page_shift] : 0xFFFFFFFFu;
+            const bool real = page < a.pages;
+            const size_t at = real ? ((((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * d : 0;
+            float *k = s_tiles + (WIDE && kb & 1u ? tile : 0) + j * pitch, *v = k + kKeys * pitch;
+            const T *k_src = static_cast<const T *>(a.k) + at, *v_src = static_cast<const T *>(a.v) + at;
+            if constexpr (WIDE) {
+                for (uint32_t c = t % 4 * 4; c < d; c += 16) {
+                    copy16(k + c, k_src + c, real);
+                    copy16(v + c, v_src + c, real);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            } else {
+                for (uint32_t c = t % 4; c < d4; c += 4) {
+                    k[c] = real && c < d ? to_f32(k_src[c]) : 0.f;
+                    v[c] = real && c < d ? to_f32(v_src[c]) : 0.f;
+                }
+            }
+        };
         __syncthreads();
-        for (uint32_t i = t; i < kRows * d4; i += kThreads) {
-            const uint32_t r = i / d4, c = i - r * d4, token = r / g.heads, head = r - token * g.heads;
-            s_q[i] = r < pairs && c < d ? to_f32(static_cast<const T *>(a.q)[(size_t)(g.row0 + token) * a.q_pitch + (g.head0 + head) * d + c]) : 0.f;
+        if (WIDE && g.begin < g.end) fetch(g.begin);
+        for (uint32_t r = warp; r < kRows; r += kWarps) {
+            const uint32_t token = r / g.heads, head = r - token * g.heads;
+            const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (r < pairs ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d;
+            for (uint32_t c = lane; c < d4; c += 32) s_q[r * d4 + c] = r < pairs && c < d ? to_f32(src[c]) : 0.f;
         }
         float m[kRowsPerWarp], l[kRowsPerWarp], acc[COLS][kRows];
         int pos[kRowsPerWarp];
@@ -48,22 +78,18 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
             for (int r = 0; r < kRows; r++) acc[c][r] = 0.f;
 
         for (uint32_t kb = g.begin; kb < g.end; kb++) {
-            __syncthreads();                             // the tile before has been used
-            for (uint32_t i = t; i < kKeys * d4; i += kThreads) {
-                const uint32_t j = i / d4, c = i - j * d4, key = kb * kKeys + j;
-                float kv = 0.f, vv = 0.f;
-                if ((int)key < g.len && c < d) {
-                    const uint32_t page = g.table[key >> a.page_shift];
-                    if (page < a.pages) {
-                        const size_t at = (((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads * d + (size_t)g.kv * d + c;
-                        kv = to_f32(static_cast<const T *>(a.k)[at]);
-                        vv = to_f32(static_cast<const T *>(a.v)[at]);
-                    }
+            if constexpr (WIDE) {
+                if (kb + 1 < g.end) {
+                    fetch(kb + 1);
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                } else {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
                 }
-                s_k[j * pitch + c] = kv;
-                s_v[j * pitch + c] = vv;
+            } else {
+                fetch(kb);
             }
             __syncthreads();
+            const float *s_k = s_tiles + (WIDE && kb & 1u ? tile : 0), *s_v = s_k + kKeys * pitch;
             const int key = (int)(kb * kKeys + lane);
             const bool there = key < g.len && g.table[(uint32_t)key >> a.page_shift] < a.pages;
             float s[kRowsPerWarp];
@@ -112,8 +138,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
                     }
                 }
             }
+            __syncthreads();                             // the tile has been used
         }
-        __syncthreads();
         const bool whole = g.first && g.last;
         if (whole) {
             if (lane == 0)
@@ -146,17 +172,20 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     }
 }
 
-constexpr uint32_t kCtas = 148 * 3;
+constexpr uint32_t kCtas = 148 * 2;                      // two tiles of 128 columns twice: two CTAs per SM
 
 template <typename T>
 int launch_attend(AttendArgs a, cudaStream_t stream)
 {
     const uint32_t d4 = (a.d + 3) / 4 * 4;
-    const size_t smem = ((size_t)kRows * d4 + 2 * kKeys * (d4 + 4)) * sizeof(float);
-    auto *kernel = a.d <= 128 ? attend_kernel<T, 1> : attend_kernel<T, 2>;
+    const bool wide = sizeof(T) == 4 && a.d % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
+    const size_t smem = ((size_t)kRows * d4 + (wide ? 2 : 1) * 2 * kKeys * (d4 + 4)) * sizeof(float);
+    auto *kernel = a.d <= 128 ? attend_kernel<T, 1, false> : attend_kernel<T, 2, false>;
+    if constexpr (sizeof(T) == 4)
+        if (wide) kernel = a.d <= 128 ? attend_kernel<T, 1, true> : attend_kernel<T, 2, true>;
     if (int rc = allow_smem(kernel, smem)) return rc;
     if (int rc = launch(kernel, dim3(kCtas), dim3(kThreads), smem, stream, a)) return rc;
-    return launch(merge_kernel<T, kRows>, dim3(kCtas, 4), dim3(kMergeThreads), 0, stream, a, kCtas);
+    return launch_merge<T, kRows>(a, kCtas, kRows, stream);
 }
 
 }  // namespace

@@ -469,22 +469,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 }
 
 template <typename T, int D, int MT>
-int launch_sized(const AttendArgs &a, const CacheMaps &maps, cudaStream_t stream)
+int launch_sized(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cudaStream_t stream)
 {
     constexpr uint32_t ctas = 148 * ctas_per_sm<D>();
     auto *kernel = decode_kernel<T, D, MT>;
     if (int rc = allow_smem(kernel, smem_bytes<D, MT>())) return rc;
     if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, MT>(), stream, maps, a)) return rc;
-    return launch(merge_kernel<T, 16 * MT>, dim3(ctas, 8), dim3(kMergeThreads), 0, stream, a, ctas);
+    return launch_merge<T, 16 * MT>(a, ctas, pairs, stream);
 }
 
 template <typename T>
 int launch_typed(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cudaStream_t stream)
 {
     const bool two = pairs > 16;
-    if (a.d <= 64) return two ? launch_sized<T, 64, 2>(a, maps, stream) : launch_sized<T, 64, 1>(a, maps, stream);
-    if (a.d <= 128) return two ? launch_sized<T, 128, 2>(a, maps, stream) : launch_sized<T, 128, 1>(a, maps, stream);
-    return launch_sized<T, 256, 1>(a, maps, stream);
+    if (a.d <= 64) return two ? launch_sized<T, 64, 2>(a, maps, pairs, stream) : launch_sized<T, 64, 1>(a, maps, pairs, stream);
+    if (a.d <= 128) return two ? launch_sized<T, 128, 2>(a, maps, pairs, stream) : launch_sized<T, 128, 1>(a, maps, pairs, stream);
+    return launch_sized<T, 256, 1>(a, maps, pairs, stream);
 }
 
 }  // namespace

@@ -644,7 +644,7 @@ int launch_sized(const AttendArgs &a, const CacheMaps &maps, const CUtensorMap &
     auto *kernel = prefill_kernel<T, D>;
     if (int rc = allow_smem(kernel, smem_bytes<D>())) return rc;
     if (int rc = launch(kernel, dim3(kPrefillCtas), dim3(kThreads), smem_bytes<D>(), stream, maps, q_map, a)) return rc;
-    return launch(merge_kernel<T, (int)kPrefillRows>, dim3(kPrefillCtas, 16), dim3(kMergeThreads), 0, stream, a, kPrefillCtas);
+    return launch_merge<T, (int)kPrefillRows>(a, kPrefillCtas, kPrefillRows, stream);
 }
 
 // {head_dim, heads, rows} of the queries, for boxes of 64 elements by the heads of a key / value head by the tokens of a unit: as they lie in

@@ -2,8 +2,8 @@
 // of drafted tokens against the target's probabilities with given random numbers (mgq_verify_drafts).
 //
 // Both stream rows of a vocabulary (150000 f32, 0.6 MB) and are bound by HBM when there are many rows, by latency when there are few.
-// A row is shared out over a cluster of up to eight CTAs whose sums meet through distributed shared memory, so that its
-// values are read once and stay in registers between the passes.
+// A row is shared out over a cluster of up to sixteen CTAs whose sums meet through distributed shared memory, so that its
+// values are read once and stay in registers between the passes: 20 of a thread's 40 registers, three CTAs per SM.
 #include <cfloat>
 #include <cstdint>
 
@@ -13,7 +13,7 @@ namespace mgq {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kHold = 10;                                // groups of four values a thread keeps: 8 CTAs hold a row of 163840
+constexpr int kHold = 5;                                 // groups of four values a thread keeps: 16 CTAs hold a row of 163840
 constexpr uint32_t kGroup = 4 * kThreads, kSlice = kHold * kGroup;
 
 template <typename T>
@@ -51,69 +51,79 @@ __device__ __forceinline__ void read4(const float *row, uint32_t c, uint32_t end
 // the largest is +inf, those that are share the row.  Rows without a finite or +inf logit are all zero.
 // The values of a CTA's slice stay in registers; a vocabulary beyond 8 slices is read again for each pass (HELD false).
 template <bool WIDE, bool HELD>
-__global__ void __launch_bounds__(kThreads, 2) probs_kernel(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t vocab)
+__global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t vocab)
 {
-    __shared__ float s_max[kWarps], s_sum[kWarps];
-    __shared__ uint32_t s_at[kWarps];
-    __shared__ float x_max, x_sum;
+    __shared__ float s_part[kWarps], x_max, x_sum;
     __shared__ uint32_t x_at;
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, part = blockIdx.y, parts = gridDim.y;
     const uint32_t each = ((vocab + parts - 1) / parts + 3) / 4 * 4, begin = min(part * each, vocab), end = min(begin + each, vocab);
+    if (t == 0) x_at = 0xFFFFFFFFu;
     pdl_launch_dependents();
     pdl_wait();
     const float *row = logits + (size_t)blockIdx.x * pitch;
     float *dst = out + (size_t)blockIdx.x * out_pitch;
-    const float temp = temperature ? temperature[blockIdx.x] : 1.f;
-    const bool greedy = !(temp > 0.f);
 
-    float v[kHold][4];
-    float m = -INFINITY;
-    uint32_t at = 0xFFFFFFFFu;
-    auto largest = [&](float x, uint32_t i) {
-        if (x > m || (x == m && i < at && x > -INFINITY)) { m = x; at = i; }
-    };
+    float v[HELD ? kHold : 1][4];
+    float m = -INFINITY;                                 // fmaxf passes over NaN
     if (HELD) {
 #pragma unroll
         for (int k = 0; k < kHold; k++) read4<WIDE>(row, begin + k * kGroup + 4 * t, end, -INFINITY, v[k]);
+    }
+    const float temp = temperature ? temperature[blockIdx.x] : 1.f;
+    if (HELD) {
 #pragma unroll
-        for (int k = 0; k < kHold; k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) largest(v[k][e], begin + k * kGroup + 4 * t + e);
+        for (int k = 0; k < kHold; k++) m = fmaxf(m, fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3])));
     } else {
         for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
             read4<WIDE>(row, c, end, -INFINITY, v[0]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) largest(v[0][e], c + e);
+            m = fmaxf(m, fmaxf(fmaxf(v[0][0], v[0][1]), fmaxf(v[0][2], v[0][3])));
         }
     }
-    auto merge = [&](float om, uint32_t oat) {
-        if (om > m || (om == m && oat < at)) { m = om; at = oat; }
-    };
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) merge(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
-    if (lane == 0) { s_max[warp] = m; s_at[warp] = at; }
+    m = warp_max(m);
+    if (lane == 0) s_part[warp] = m;
     __syncthreads();
-    for (int w = 0; w < kWarps; w++) merge(s_max[w], s_at[w]);
+    m = warp_max(s_part[lane % kWarps]);
     if (parts > 1) {
-        if (t == 0) { x_max = m; x_at = at; }
+        if (t == 0) x_max = m;
         cluster_sync();
-        for (uint32_t p = 0; p < parts; p++) merge(cluster_read(&x_max, p), cluster_read(&x_at, p));
+        m = warp_max(cluster_read(&x_max, lane % parts));
     }
 
-    const float inv = greedy ? 0.f : 1.f / temp;
+    const float inv = temp > 0.f ? 1.f / temp : 0.f;
+    uint32_t at = 0xFFFFFFFFu;                           // the greedy choice: of the largest, the lowest
+    if (!(temp > 0.f)) {                                 // uniform over the cluster
+        auto look = [&](uint32_t c, const float (&x)[4]) {
+#pragma unroll
+            for (int e = 3; e >= 0; e--)
+                if (x[e] == m && m > -INFINITY && c + e < at) at = c + e;
+        };
+        if (HELD) {
+#pragma unroll
+            for (int k = kHold - 1; k >= 0; k--) look(begin + k * kGroup + 4 * t, v[k]);
+        } else {
+            for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
+                read4<WIDE>(row, c, end, -INFINITY, v[0]);
+                look(c, v[0]);
+            }
+        }
+        if (at != 0xFFFFFFFFu) atomicMin(&x_at, at);
+        if (parts > 1) cluster_sync();
+        else           __syncthreads();
+        at = x_at;
+        for (uint32_t p = 0; parts > 1 && p < parts; p++) at = min(at, cluster_read(&x_at, p));
+    }
     auto weight = [&](float x, uint32_t i) {
-        if (greedy) return x == m && i == at ? 1.f : 0.f;          // an index behind the slice's end is another CTA's
+        if (!(temp > 0.f)) return x == m && i == at ? 1.f : 0.f;          // an index behind the slice's end is another CTA's
         return x == m ? (m > -INFINITY ? 1.f : 0.f) : x < m ? expf((x - m) * inv) : 0.f;
     };
     float sum = 0.f;
     if (HELD) {
 #pragma unroll
-        for (int k = 0; k < kHold; k++)
+        for (int k = 0; k < kHold; k++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[k][e] = weight(v[k][e], begin + k * kGroup + 4 * t + e);
-                sum += v[k][e];
-            }
+            for (int e = 0; e < 4; e++) v[k][e] = weight(v[k][e], begin + k * kGroup + 4 * t + e);
+            sum += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
+        }
     } else {
         for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
             read4<WIDE>(row, c, end, -INFINITY, v[0]);
@@ -122,15 +132,14 @@ __global__ void __launch_bounds__(kThreads, 2) probs_kernel(const float *logits,
         }
     }
     sum = warp_sum(sum);
-    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();                                     // the maxima have been read
+    if (lane == 0) s_part[warp] = sum;
     __syncthreads();
-    sum = 0.f;
-    for (int w = 0; w < kWarps; w++) sum += s_sum[w];
+    sum = warp_sum(lane < kWarps ? s_part[lane] : 0.f);
     if (parts > 1) {
         if (t == 0) x_sum = sum;
         cluster_sync();
-        sum = 0.f;
-        for (uint32_t p = 0; p < parts; p++) sum += cluster_read(&x_sum, p);
+        sum = warp_sum(lane < parts ? cluster_read(&x_sum, lane) : 0.f);
     }
     const float scale = sum > 0.f ? 1.f / sum : 0.f;
     auto store = [&](uint32_t c, const float (&p)[4]) {
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
             }
         };
         double sum = 0.0;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t c = w0 + 4 * lane; c < w1; c += 128) {
             double w[4];
             weights(c, w);
@@ -328,11 +337,18 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
 
 bool aligned16(const void *p, uint32_t pitch) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % 4 == 0; }
 
-// CTAs per row: few rows are spread over more of them.
-uint32_t row_parts(uint32_t rows, uint32_t vocab)
+// CTAs per row: as many as it takes to hold one, and more for few rows.
+uint32_t probs_parts(uint32_t rows, uint32_t vocab)
 {
     uint32_t parts = 1;
-    while (parts < 8 && (vocab > parts * kSlice || (rows * parts * 2 <= 296 && vocab > parts * kGroup))) parts *= 2;
+    while (parts < 16 && (vocab > parts * kSlice || (rows * parts * 2 <= 148 && vocab > parts * kGroup))) parts *= 2;
+    return parts;
+}
+// The rows of all sequences at once on the SMs: two CTAs each.
+uint32_t verify_parts(uint32_t sequences, uint32_t vocab)
+{
+    uint32_t parts = 1;
+    while (parts < 8 && sequences * parts * 2 <= 296 && vocab > parts * kGroup) parts *= 2;
     return parts;
 }
 
@@ -340,9 +356,10 @@ uint32_t row_parts(uint32_t rows, uint32_t vocab)
 
 int launch_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream)
 {
-    const uint32_t parts = row_parts(rows, vocab);
+    const uint32_t parts = probs_parts(rows, vocab);
     const bool wide = vocab % 4 == 0 && aligned16(logits, pitch) && aligned16(out, out_pitch), held = vocab <= parts * kSlice;
     auto *kernel = wide ? (held ? probs_kernel<true, true> : probs_kernel<true, false>) : (held ? probs_kernel<false, true> : probs_kernel<false, false>);
+    if (parts > 8) MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return launch_clustered(kernel, dim3(rows, parts), dim3(kThreads), parts, 0, static_cast<cudaStream_t>(stream), logits, pitch, temperature, out, out_pitch, vocab);
 }
 
@@ -351,7 +368,7 @@ int launch_verify_drafts(const float *target, uint32_t target_pitch, const float
                          uint32_t vocab, void *stream)
 {
     const VerifyArgs a{target, draft, tokens, starts, accept, sample, accepted, next, out, target_pitch, draft_pitch, rows, vocab};
-    const uint32_t parts = row_parts(sequences, vocab);
+    const uint32_t parts = verify_parts(sequences, vocab);
     const bool wide = vocab % 4 == 0 && aligned16(target, target_pitch) && (!draft || aligned16(draft, draft_pitch));
     return launch_clustered(wide ? verify_kernel<true> : verify_kernel<false>, dim3(sequences, parts), dim3(kThreads), parts, 0, static_cast<cudaStream_t>(stream), a);
 }
