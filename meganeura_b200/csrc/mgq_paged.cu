@@ -13,7 +13,7 @@ namespace mgq {
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
-constexpr uint32_t kPerThread = MGQ_PAGED_MAX_SEQUENCES / kPlanThreads;
+constexpr uint32_t kPerThread = MGQ_PAGED_MAX_SEQUENCES / kPlanThreads;         // a block has at least a thread per four sequences
 
 // Exclusive sums over the block in thread order; `total` is everybody's sum.
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long &total, unsigned long long *s_warp)
@@ -27,7 +27,7 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
     }
     if (lane == 31) s_warp[warp] = sum;
     __syncthreads();
-    unsigned long long w = s_warp[lane];                 // 32 warps
+    unsigned long long w = lane < blockDim.x / 32 ? s_warp[lane] : 0ull;
     const unsigned long long own = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -56,12 +56,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
 {
     extern __shared__ uint32_t s_plan[];
     __shared__ unsigned long long s_warp[kPlanWarps];
+    __shared__ uint32_t s_given;
     uint32_t *s_start = s_plan, *s_before = s_start + a.sequences + 1, *s_held = s_before + a.sequences, *s_got = s_held + a.sequences;
-    const uint32_t t = threadIdx.x, lane = t & 31u, part = blockIdx.y, parts = gridDim.y, warp = part * kPlanWarps + (t >> 5);
+    const uint32_t t = threadIdx.x, lane = t & 31u, part = blockIdx.y, parts = gridDim.y, threads = blockDim.x, warp = part * (threads / 32) + (t >> 5);
+    if (t == 0) s_given = 0;
     pdl_launch_dependents();
     pdl_wait();
 
-    const uint32_t count = min(*a.free_count, a.pages), each = (a.sequences + kPlanThreads - 1) / kPlanThreads, s0 = t * each;
+    const uint32_t count = min(*a.free_count, a.pages), each = (a.sequences + threads - 1) / threads, s0 = t * each;
     uint32_t cached[kPerThread], fresh[kPerThread], held[kPerThread];
     unsigned long long sum = 0, total;
 #pragma unroll
@@ -90,7 +92,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
     }
     const uint32_t last_row = (uint32_t)min(total, (unsigned long long)a.rows);
     unsigned long long before = block_scan(wanted, total, s_warp);
-    uint32_t pages_given = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kPerThread; i++) {
         const bool served = !narrow[i] && (need[i] == 0 || before + need[i] <= count);
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
             s_before[s] = (uint32_t)before;
             s_held[s] = held[i];
             s_got[s] = served ? need[i] : 0xFFFFFFFFu;
-            if (served) pages_given += need[i];
+            if (served && need[i]) atomicMax(&s_given, (uint32_t)before + need[i]);         // those that are served come first
             if (part == 0) {
                 a.starts[s] = s_start[s];
                 a.lengths[s] = served ? cached[i] + fresh[i] : cached[i];
@@ -108,25 +109,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
         before += need[i];
     }
     if (t == 0) s_start[a.sequences] = last_row;
-    unsigned long long given;
-    block_scan(pages_given, given, s_warp);
     if (parts > 1) cluster_sync();                       // every CTA has read held and free_count
     else           __syncthreads();
     if (part == 0) {
         if (t == 0) {
             a.starts[a.sequences] = last_row;
-            *a.free_count = count - (uint32_t)given;
+            *a.free_count = count - s_given;
             *a.lacking = (uint32_t)min(total > count ? total - count : 0ull, 0xFFFFFFFFull);
         }
-        for (uint32_t s = t; s < a.sequences; s += kPlanThreads)
+        for (uint32_t s = t; s < a.sequences; s += threads)
             if (s_got[s] != 0xFFFFFFFFu) a.held[s] = s_held[s] + s_got[s];
     }
-    for (uint32_t s = warp; s < a.sequences; s += parts * kPlanWarps) {
+    for (uint32_t s = warp; s < a.sequences; s += parts * (threads / 32)) {
         const uint32_t got = s_got[s] == 0xFFFFFFFFu ? 0u : s_got[s];
         for (uint32_t i = lane; i < got; i += 32)
             a.table[(size_t)s * a.table_width + s_held[s] + i] = a.free_pages[count - 1 - (s_before[s] + i)];
     }
-    for (uint32_t r = part * kPlanThreads + t; r < a.rows; r += parts * kPlanThreads) {
+    for (uint32_t r = part * threads + t; r < a.rows; r += parts * threads) {
         uint32_t slot = MGQ_NO_SLOT, position = 0;
         if (r < last_row) {
             uint32_t lo = 0, hi = a.sequences;           // the last sequence that starts at or before r, empty ones passed over
@@ -155,7 +154,8 @@ __global__ void __launch_bounds__(kPlanThreads) trim_kernel(const uint32_t *leng
     extern __shared__ uint32_t s_plan[];
     __shared__ unsigned long long s_warp[kPlanWarps];
     uint32_t *s_before = s_plan, *s_keep = s_before + sequences, *s_gone = s_keep + sequences;
-    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, each = (sequences + kPlanThreads - 1) / kPlanThreads, s0 = t * each;
+    const uint32_t t = threadIdx.x, lane = t & 31u, part = blockIdx.y, parts = gridDim.y, threads = blockDim.x, warp = part * (threads / 32) + (t >> 5);
+    const uint32_t each = (sequences + threads - 1) / threads, s0 = t * each;
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t count = min(*free_count, pages);
@@ -180,13 +180,16 @@ __global__ void __launch_bounds__(kPlanThreads) trim_kernel(const uint32_t *leng
         const uint32_t s = s0 + i;
         if (i < each && s < sequences) {
             s_before[s] = (uint32_t)before;
-            if (gone[i]) held[s] = s_keep[s];
         }
         before += gone[i];
     }
-    __syncthreads();
-    if (t == 0) *free_count = (uint32_t)min(count + total, (unsigned long long)pages);
-    for (uint32_t s = warp; s < sequences; s += kPlanWarps) {
+    if (parts > 1) cluster_sync();                       // every CTA has read held and free_count
+    else           __syncthreads();
+    if (part == 0)
+        for (uint32_t s = t; s < sequences; s += threads)
+            if (s_gone[s]) held[s] = s_keep[s];
+    if (part == 0 && t == 0) *free_count = (uint32_t)min(count + total, (unsigned long long)pages);
+    for (uint32_t s = warp; s < sequences; s += parts * (threads / 32)) {
         uint32_t *row = table + (size_t)s * table_width + s_keep[s];
         for (uint32_t i = lane; i < s_gone[s]; i += 32) {
             const unsigned long long place = count + total - 1 - (s_before[s] + i);
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(kPlanThreads) trim_kernel(const uint32_t *leng
 // ---------------------------------------------------------------- keys and values into the cache
 // A CTA takes a row at a time.  Its angles (position * theta^(-2i/d), product and reduction to one turn in 64 bits: at position 100000
 // an f32 product is off by up to 0.004) are computed once for all heads, then a thread rotates four pairs of a head per step.
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 256, kBatch = 4;
 
 struct AppendArgs {
     const void *q, *k, *v;
@@ -242,7 +245,7 @@ __device__ __forceinline__ void write_values(T *p, const float (&f)[N])
 }
 
 template <typename S, typename T, int N>      // source, cache; N values at a time
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a)
+__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(const AppendArgs a)
 {
     __shared__ float2 s_turn[MGQ_PAGED_MAX_HEAD / 2];
     const uint32_t t = threadIdx.x, half = a.d / 2, steps = half / N;
@@ -252,41 +255,64 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     for (uint32_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const uint32_t slot = a.slots[r];
         const bool stored = slot < a.cache_rows;
-        if (a.rotate && t < half) {
-            const double angle = (double)a.positions[r] * frequency, turn = 6.283185307179586476925286766559;
-            float2 w;
-            sincosf((float)fma(-rint(angle * (1.0 / turn)), turn, angle), &w.y, &w.x);
-            s_turn[t] = w;
-        }
-        __syncthreads();
-        const uint32_t q_items = a.q ? a.q_heads * steps : 0, k_items = a.kv_heads * steps, items = q_items + (stored ? 3 * k_items : 0);
-        for (uint32_t i = t; i < items; i += kAppendThreads) {
-            const uint32_t j = i < q_items ? i : i - q_items;
-            float lo[N], hi[N];
-            if (j < k_items || i < q_items) {            // a head's pairs (p, p + half)
-                const uint32_t head = j / steps, p = (j - head * steps) * N;
-                const S *src = i < q_items ? static_cast<const S *>(a.q) + (size_t)r * a.q_pitch : static_cast<const S *>(a.k) + (size_t)r * a.k_pitch;
-                T *dst = i < q_items ? static_cast<T *>(a.q_out) + (size_t)r * a.q_heads * a.d : static_cast<T *>(a.k_cache) + (size_t)slot * a.kv_heads * a.d;
-                read_values(src + head * a.d + p, lo);
-                read_values(src + head * a.d + p + half, hi);
-                if (a.rotate) {
+        const uint32_t q_items = a.q ? a.q_heads * steps : 0, k_items = a.kv_heads * steps, items = q_items + (stored ? 2 * k_items : 0);
+        // item: N pairs (p, p + half) of a head of q or k, 2 N values of v
+        for (uint32_t i0 = 0; i0 < items || i0 == 0; i0 += kBatch * kAppendThreads) {
+            float lo[kBatch][N], hi[kBatch][N];
 #pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const float2 w = s_turn[p + e];
-                        const float x = lo[e] * w.x - hi[e] * w.y;
-                        hi[e] = lo[e] * w.y + hi[e] * w.x;
-                        lo[e] = x;
-                    }
+            for (int b = 0; b < kBatch; b++) {           // all of a batch's loads first, for the first batch in front of the angles
+                const uint32_t i = i0 + b * kAppendThreads + t;
+                if (i >= items) continue;
+                const S *src;
+                uint32_t far = half;
+                if (i < q_items + k_items) {
+                    const bool is_q = i < q_items;
+                    const uint32_t j = is_q ? i : i - q_items, head = j / steps, p = (j - head * steps) * N;
+                    src = (is_q ? static_cast<const S *>(a.q) + (size_t)r * a.q_pitch : static_cast<const S *>(a.k) + (size_t)r * a.k_pitch) + head * a.d + p;
+                } else {
+                    src = static_cast<const S *>(a.v) + (size_t)r * a.v_pitch + (i - q_items - k_items) * 2 * N;
+                    far = N;
                 }
-                write_values(dst + head * a.d + p, lo);
-                write_values(dst + head * a.d + p + half, hi);
-            } else {
-                const uint32_t e = (j - k_items) * N;
-                read_values(static_cast<const S *>(a.v) + (size_t)r * a.v_pitch + e, lo);
-                write_values(static_cast<T *>(a.v_cache) + (size_t)slot * a.kv_heads * a.d + e, lo);
+                read_values(src, lo[b]);
+                read_values(src + far, hi[b]);
+            }
+            if (i0 == 0 && a.rotate) {
+                if (t < half) {
+                    const double angle = (double)a.positions[r] * frequency, turn = 6.283185307179586476925286766559;
+                    float2 w;
+                    sincosf((float)fma(-rint(angle * (1.0 / turn)), turn, angle), &w.y, &w.x);
+                    s_turn[t] = w;
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                const uint32_t i = i0 + b * kAppendThreads + t;
+                if (i >= items) continue;
+                T *dst;
+                uint32_t far = half;
+                if (i < q_items + k_items) {
+                    const bool is_q = i < q_items;
+                    const uint32_t j = is_q ? i : i - q_items, head = j / steps, p = (j - head * steps) * N;
+                    dst = (is_q ? static_cast<T *>(a.q_out) + (size_t)r * a.q_heads * a.d : static_cast<T *>(a.k_cache) + (size_t)slot * a.kv_heads * a.d) + head * a.d + p;
+                    if (a.rotate) {
+#pragma unroll
+                        for (int e = 0; e < N; e++) {
+                            const float2 w = s_turn[p + e];
+                            const float x = lo[b][e] * w.x - hi[b][e] * w.y;
+                            hi[b][e] = lo[b][e] * w.y + hi[b][e] * w.x;
+                            lo[b][e] = x;
+                        }
+                    }
+                } else {
+                    dst = static_cast<T *>(a.v_cache) + (size_t)slot * a.kv_heads * a.d + (i - q_items - k_items) * 2 * N;
+                    far = N;
+                }
+                write_values(dst, lo[b]);
+                write_values(dst + far, hi[b]);
             }
         }
-        __syncthreads();
+        if (a.rotate) __syncthreads();                   // the angles have been used
     }
 }
 
@@ -299,6 +325,9 @@ int launch_append_typed(const AppendArgs &a, bool wide, cudaStream_t stream)
 
 }  // namespace
 
+// Barriers of few threads are quick: 256 where that is a thread per sequence and a few rows each.
+static uint32_t plan_threads(uint32_t sequences, uint32_t rows) { return sequences <= 256 && rows <= 1024 ? 256 : kPlanThreads; }
+
 int launch_paged_plan(const uint32_t *cached, const uint32_t *fresh, uint32_t sequences, uint32_t page_size, uint32_t *table, uint32_t table_width, uint32_t *held,
                       const uint32_t *free_pages, uint32_t pages, uint32_t *free_count, uint32_t rows, uint32_t *starts, uint32_t *lengths, uint32_t *positions,
                       uint32_t *slots, uint32_t *lacking, void *stream)
@@ -307,9 +336,9 @@ int launch_paged_plan(const uint32_t *cached, const uint32_t *fresh, uint32_t se
                      slots, lacking};
     const size_t smem = (4 * (size_t)sequences + 1) * 4;
     if (int rc = allow_smem(plan_kernel, smem)) return rc;
-    // one CTA while its threads have few rows and pages each, a cluster of eight beyond
-    const uint32_t parts = rows <= 2 * kPlanThreads && sequences <= kPlanThreads / 2 ? 1 : 8;
-    return launch_clustered(plan_kernel, dim3(1, parts), dim3(kPlanThreads), parts, smem, static_cast<cudaStream_t>(stream), a);
+    // one CTA while its threads have few rows and its warps few sequences each, a cluster of eight beyond
+    const uint32_t threads = plan_threads(sequences, rows), parts = rows <= 2 * threads && sequences <= 2 * threads / 32 ? 1 : 8;
+    return launch_clustered(plan_kernel, dim3(1, parts), dim3(threads), parts, smem, static_cast<cudaStream_t>(stream), a);
 }
 
 int launch_paged_trim(const uint32_t *lengths, uint32_t sequences, uint32_t page_size, uint32_t *table, uint32_t table_width, uint32_t *held, uint32_t *free_pages,
@@ -317,8 +346,9 @@ int launch_paged_trim(const uint32_t *lengths, uint32_t sequences, uint32_t page
 {
     const size_t smem = 3 * (size_t)sequences * 4;
     if (int rc = allow_smem(trim_kernel, smem)) return rc;
-    return launch(trim_kernel, dim3(1), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), lengths, sequences, page_size, page_shift(page_size), table, table_width,
-                  held, free_pages, pages, free_count);
+    const uint32_t threads = plan_threads(sequences, 0), parts = sequences <= 2 * threads / 32 ? 1 : 8;
+    return launch_clustered(trim_kernel, dim3(1, parts), dim3(threads), parts, smem, static_cast<cudaStream_t>(stream), lengths, sequences, page_size, page_shift(page_size),
+                            table, table_width, held, free_pages, pages, free_count);
 }
 
 int launch_paged_append(const void *q, const void *k, const void *v, int src_dtype, const uint32_t *positions, const uint32_t *slots, void *q_out, void *k_cache,

@@ -2,8 +2,7 @@
 // of drafted tokens against the target's probabilities with given random numbers (mgq_verify_drafts).
 //
 // Both stream rows of a vocabulary (150000 f32, 0.6 MB) and are bound by HBM when there are many rows, by latency when there are few.
-// A row is shared out over a cluster of up to sixteen CTAs whose sums meet through distributed shared memory, so that its
-// values are read once and stay in registers between the passes: 20 of a thread's 40 registers, three CTAs per SM.
+// A row is shared out over a cluster of up to eight CTAs whose sums meet through distributed shared memory.
 #include <cfloat>
 #include <cstdint>
 
@@ -13,7 +12,7 @@ namespace mgq {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kHold = 5;                                 // groups of four values a thread keeps: 16 CTAs hold a row of 163840
+constexpr int kHold = 4;                                 // groups of four values that a thread reads at once
 constexpr uint32_t kGroup = 4 * kThreads, kSlice = kHold * kGroup;
 
 template <typename T>
@@ -32,28 +31,30 @@ __device__ __forceinline__ T cluster_read(const T *p, uint32_t rank)
     }
 }
 
-// Four values of a row from column c on; `fill` behind its end.
-template <bool WIDE>
+// Four values of a row from column c on; `fill` behind its end.  LAST: they are not read again.
+template <bool WIDE, bool LAST>
 __device__ __forceinline__ void read4(const float *row, uint32_t c, uint32_t end, float fill, float (&v)[4])
 {
     if (WIDE) {
         float4 q = make_float4(fill, fill, fill, fill);
-        if (c < end) q = __ldcs(reinterpret_cast<const float4 *>(row + c));
+        if (c < end) q = LAST ? __ldcs(reinterpret_cast<const float4 *>(row + c)) : *reinterpret_cast<const float4 *>(row + c);
         v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = c + e < end ? __ldcs(row + c + e) : fill;
+        for (int e = 0; e < 4; e++) v[e] = c + e < end ? row[c + e] : fill;
     }
 }
 
 // ---------------------------------------------------------------- probabilities
 // p_i = exp((l_i - m) / t) / sum; t <= 0 (or NaN): 1 for the lowest index among the largest logits.  NaN logits count as -inf; where
 // the largest is +inf, those that are share the row.  Rows without a finite or +inf logit are all zero.
-// The values of a CTA's slice stay in registers; a vocabulary beyond 8 slices is read again for each pass (HELD false).
+// A slice of up to 8192 values stays in registers (HELD): few rows over many CTAs, or small vocabularies.  Longer ones are read once for maximum and
+// sum, running together as in attention, and again for the result, which finds them in L2 (the rows in flight take 90 of its
+// 126 MB).  Keeping 320 rows of 151936 in the registers of clusters of 8 or 16 CTAs took 170 and 210 us: their loads come in bursts between barriers.
 template <bool WIDE, bool HELD>
 __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t vocab)
 {
-    __shared__ float s_part[kWarps], x_max, x_sum;
+    __shared__ float s_part[2][kWarps], x_max, x_sum;
     __shared__ uint32_t x_at;
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, part = blockIdx.y, parts = gridDim.y;
     const uint32_t each = ((vocab + parts - 1) / parts + 3) / 4 * 4, begin = min(part * each, vocab), end = min(begin + each, vocab);
@@ -62,104 +63,97 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
     pdl_wait();
     const float *row = logits + (size_t)blockIdx.x * pitch;
     float *dst = out + (size_t)blockIdx.x * out_pitch;
-
-    float v[HELD ? kHold : 1][4];
-    float m = -INFINITY;                                 // fmaxf passes over NaN
-    if (HELD) {
+    float v[kHold][4];
+    auto fetch = [&](uint32_t c0) {
 #pragma unroll
-        for (int k = 0; k < kHold; k++) read4<WIDE>(row, begin + k * kGroup + 4 * t, end, -INFINITY, v[k]);
-    }
-    const float temp = temperature ? temperature[blockIdx.x] : 1.f;
-    if (HELD) {
+        for (int k = 0; k < kHold; k++) read4<WIDE, HELD>(row, c0 + k * kGroup + 4 * t, end, -INFINITY, v[k]);
+    };
+    auto largest = [&]() {                               // fmaxf passes over NaN
+        float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kHold; k++) m = fmaxf(m, fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3])));
-    } else {
-        for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
-            read4<WIDE>(row, c, end, -INFINITY, v[0]);
-            m = fmaxf(m, fmaxf(fmaxf(v[0][0], v[0][1]), fmaxf(v[0][2], v[0][3])));
+        return m;
+    };
+    fetch(begin);
+    const float temp = temperature ? temperature[blockIdx.x] : 1.f;
+    const bool greedy = !(temp > 0.f);
+    const float inv = greedy ? 0.f : 1.f / temp;
+    auto weight = [&](float x, float m) { return x == m ? (m > -INFINITY ? 1.f : 0.f) : x < m ? expf((x - m) * inv) : 0.f; };
+    auto weights = [&](float m) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kHold; k++) sum += (weight(v[k][0], m) + weight(v[k][1], m)) + (weight(v[k][2], m) + weight(v[k][3], m));
+        return sum;
+    };
+
+    float m = largest(), sum = 0.f;
+    if (!HELD) {
+        // a thread's sum is relative to its own maximum
+        if (!greedy) sum = weights(m);
+        for (uint32_t c0 = begin + kSlice; c0 < end; c0 += kSlice) {
+            fetch(c0);
+            const float top = fmaxf(m, largest());
+            if (!greedy) sum = sum * weight(m, top) + weights(top);
+            m = top;
         }
     }
+    const float mine = m;
     m = warp_max(m);
-    if (lane == 0) s_part[warp] = m;
+    if (lane == 0) s_part[0][warp] = m;
     __syncthreads();
-    m = warp_max(s_part[lane % kWarps]);
+    m = warp_max(s_part[0][lane % kWarps]);
     if (parts > 1) {
         if (t == 0) x_max = m;
         cluster_sync();
         m = warp_max(cluster_read(&x_max, lane % parts));
     }
 
-    const float inv = temp > 0.f ? 1.f / temp : 0.f;
     uint32_t at = 0xFFFFFFFFu;                           // the greedy choice: of the largest, the lowest
-    if (!(temp > 0.f)) {                                 // uniform over the cluster
-        auto look = [&](uint32_t c, const float (&x)[4]) {
+    if (greedy) {                                        // uniform over the cluster
+        for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
+            if (!HELD) fetch(c0);
 #pragma unroll
-            for (int e = 3; e >= 0; e--)
-                if (x[e] == m && m > -INFINITY && c + e < at) at = c + e;
-        };
-        if (HELD) {
+            for (int k = kHold - 1; k >= 0; k--)
 #pragma unroll
-            for (int k = kHold - 1; k >= 0; k--) look(begin + k * kGroup + 4 * t, v[k]);
-        } else {
-            for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
-                read4<WIDE>(row, c, end, -INFINITY, v[0]);
-                look(c, v[0]);
-            }
+                for (int e = 3; e >= 0; e--) {
+                    const uint32_t c = c0 + k * kGroup + 4 * t + e;
+                    if (v[k][e] == m && m > -INFINITY && c < at) at = c;
+                }
         }
         if (at != 0xFFFFFFFFu) atomicMin(&x_at, at);
         if (parts > 1) cluster_sync();
         else           __syncthreads();
         at = x_at;
         for (uint32_t p = 0; parts > 1 && p < parts; p++) at = min(at, cluster_read(&x_at, p));
-    }
-    auto weight = [&](float x, uint32_t i) {
-        if (!(temp > 0.f)) return x == m && i == at ? 1.f : 0.f;          // an index behind the slice's end is another CTA's
-        return x == m ? (m > -INFINITY ? 1.f : 0.f) : x < m ? expf((x - m) * inv) : 0.f;
-    };
-    float sum = 0.f;
-    if (HELD) {
-#pragma unroll
-        for (int k = 0; k < kHold; k++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[k][e] = weight(v[k][e], begin + k * kGroup + 4 * t + e);
-            sum += (v[k][0] + v[k][1]) + (v[k][2] + v[k][3]);
-        }
+        sum = at != 0xFFFFFFFFu ? 1.f : 0.f;
     } else {
-        for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
-            read4<WIDE>(row, c, end, -INFINITY, v[0]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += weight(v[0][e], c + e);
+        sum = HELD ? weights(m) : sum * weight(mine, m);
+        sum = warp_sum(sum);
+        if (lane == 0) s_part[1][warp] = sum;
+        __syncthreads();
+        sum = warp_sum(lane < kWarps ? s_part[1][lane] : 0.f);
+        if (parts > 1) {
+            if (t == 0) x_sum = sum;
+            cluster_sync();
+            sum = warp_sum(lane < parts ? cluster_read(&x_sum, lane) : 0.f);
         }
-    }
-    sum = warp_sum(sum);
-    __syncthreads();                                     // the maxima have been read
-    if (lane == 0) s_part[warp] = sum;
-    __syncthreads();
-    sum = warp_sum(lane < kWarps ? s_part[lane] : 0.f);
-    if (parts > 1) {
-        if (t == 0) x_sum = sum;
-        cluster_sync();
-        sum = warp_sum(lane < parts ? cluster_read(&x_sum, lane) : 0.f);
     }
     const float scale = sum > 0.f ? 1.f / sum : 0.f;
-    auto store = [&](uint32_t c, const float (&p)[4]) {
-        if (WIDE) {
-            if (c < end) __stcs(reinterpret_cast<float4 *>(dst + c), make_float4(p[0] * scale, p[1] * scale, p[2] * scale, p[3] * scale));
-        } else {
+    for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
+        if (!HELD) fetch(c0);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (c + e < end) __stcs(dst + c + e, p[e] * scale);
-        }
-    };
-    if (HELD) {
+        for (int k = 0; k < kHold; k++) {
+            const uint32_t c = c0 + k * kGroup + 4 * t;
+            float p[4];
 #pragma unroll
-        for (int k = 0; k < kHold; k++) store(begin + k * kGroup + 4 * t, v[k]);
-    } else {
-        for (uint32_t c = begin + 4 * t; c < end; c += kGroup) {
-            read4<WIDE>(row, c, end, -INFINITY, v[0]);
+            for (int e = 0; e < 4; e++) p[e] = greedy ? (c + e == at ? 1.f : 0.f) : weight(v[k][e], m) * scale;
+            if (WIDE) {
+                if (c < end) __stcs(reinterpret_cast<float4 *>(dst + c), make_float4(p[0], p[1], p[2], p[3]));
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[0][e] = weight(v[0][e], c + e);
-            store(c, v[0]);
+                for (int e = 0; e < 4; e++)
+                    if (c + e < end) __stcs(dst + c + e, p[e]);
+            }
         }
     }
     if (parts > 1) cluster_sync();                       // nobody leaves while its sums are being read
@@ -169,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
 // Draft i of a sequence (fed as row start + i) is kept while u q(d) < p(d), with p and q from row start + i - 1: the products of
 // two f32 are exact in 64 bits.  At the first draft that is not kept the next token is drawn from max(p - q, 0), behind the last
 // one from p: the lowest index whose running sum exceeds u times the whole.  Running sums are in 64 bits, because with 150000
-// entries an f32 sum is wrong by more than many an entry: per thread and group of four, then warps in order, then CTAs in order.
+// entries an f32 sum is wrong by more than many an entry: per thread and group of four, then warps in order, then CTAs in order.  The warp's
+// piece that holds the pick is cut again among all warps: one warp going through it alone, 19 dependent loads one after another, took 23 of 42 us.
 struct VerifyArgs {
     const float *target, *draft;
     const uint32_t *tokens, *starts;
@@ -180,13 +175,14 @@ struct VerifyArgs {
 
 __device__ __forceinline__ double mass(float p) { return p > 0.f && p <= FLT_MAX ? (double)p : 0.0; }
 
+constexpr uint32_t kChunks = 64;                         // of a warp's piece, in the search
 template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
 {
     __shared__ double s_sum[kWarps];
     __shared__ double x_sum;
     __shared__ uint32_t s_kept, s_warp;
-    __shared__ double s_x;
+    __shared__ double s_x, s_chunk[kChunks];
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, seq = blockIdx.x, part = blockIdx.y, parts = gridDim.y;
     pdl_launch_dependents();
     pdl_wait();
@@ -229,10 +225,10 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
     // first the rest that the draft leaves over; where that is nothing, the target's own row
     for (int pass = all ? 1 : 0; pass < 2; pass++) {
         const bool rest = pass == 0;
-        auto weights = [&](uint32_t c, double (&w)[4]) {
+        auto weights = [&](uint32_t c, uint32_t w1, double (&w)[4]) {
             float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
-            read4<WIDE>(p, c, w1, 0.f, x);
-            if (rest && q) read4<WIDE>(q, c, w1, 0.f, y);
+            read4<WIDE, false>(p, c, w1, 0.f, x);
+            if (rest && q) read4<WIDE, false>(q, c, w1, 0.f, y);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 w[e] = mass(x[e]);
@@ -243,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
 #pragma unroll 8
         for (uint32_t c = w0 + 4 * lane; c < w1; c += 128) {
             double w[4];
-            weights(c, w);
+            weights(c, w1, w);
             sum += (w[0] + w[1]) + (w[2] + w[3]);
         }
 #pragma unroll
@@ -294,12 +290,35 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
             s_x = left;
         }
         __syncthreads();
-        if (warp != s_warp) return;
+        // chunks of 128 columns or a multiple, 64 at most
+        const uint32_t p0 = min(begin + s_warp * piece, end), p1 = min(p0 + piece, end), step = (piece / 128 + kChunks - 1) / kChunks * 128, chunks = (p1 - p0 + step - 1) / step;
+        for (uint32_t i = warp; i < chunks; i += kWarps) {
+            const uint32_t c1 = min(p0 + (i + 1) * step, p1);
+            double own = 0.0;
+            for (uint32_t c = p0 + i * step + 4 * lane; c < c1; c += 128) {
+                double w[4];
+                weights(c, c1, w);
+                own += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+            if (lane == 0) s_chunk[i] = own;
+        }
+        __syncthreads();
+        if (warp != 0) return;
         double left = s_x;
+        uint32_t chosen = 0;
+        for (uint32_t i = 0; i < chunks; i++)
+            if (s_chunk[i] > 0.0) chosen = i;
+        for (uint32_t i = 0; i < chunks; i++) {
+            if (s_chunk[i] > 0.0 && left < s_chunk[i]) { chosen = i; break; }
+            if (i < chosen) left -= s_chunk[i];
+        }
+        const uint32_t c_end = min(p0 + (chosen + 1) * step, p1);
         uint32_t token = MGQ_NO_TOKEN, highest = MGQ_NO_TOKEN;
-        for (uint32_t c0 = w0; c0 < w1 && token == MGQ_NO_TOKEN; c0 += 128) {
+        for (uint32_t c0 = p0 + chosen * step; c0 < c_end && token == MGQ_NO_TOKEN; c0 += 128) {
             double w[4];
-            weights(c0 + 4 * lane, w);                   // zeros behind the piece
+            weights(c0 + 4 * lane, c_end, w);            // zeros behind the chunk
             const double own = (w[0] + w[1]) + (w[2] + w[3]);
             double upto = own;
 #pragma unroll
@@ -337,11 +356,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
 
 bool aligned16(const void *p, uint32_t pitch) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % 4 == 0; }
 
-// CTAs per row: as many as it takes to hold one, and more for few rows.
+// CTAs per row: four where there are many, more for few, so that all SMs take part.
 uint32_t probs_parts(uint32_t rows, uint32_t vocab)
 {
     uint32_t parts = 1;
-    while (parts < 16 && (vocab > parts * kSlice || (rows * parts * 2 <= 148 && vocab > parts * kGroup))) parts *= 2;
+    while (parts < 8 && vocab > parts * kGroup && (parts < 4 ? vocab > parts * kSlice || rows * parts < 296 : rows * parts < 296)) parts *= 2;
     return parts;
 }
 // The rows of all sequences at once on the SMs: two CTAs each.
@@ -359,7 +378,6 @@ int launch_token_probs(const float *logits, uint32_t pitch, const float *tempera
     const uint32_t parts = probs_parts(rows, vocab);
     const bool wide = vocab % 4 == 0 && aligned16(logits, pitch) && aligned16(out, out_pitch), held = vocab <= parts * kSlice;
     auto *kernel = wide ? (held ? probs_kernel<true, true> : probs_kernel<true, false>) : (held ? probs_kernel<false, true> : probs_kernel<false, false>);
-    if (parts > 8) MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return launch_clustered(kernel, dim3(rows, parts), dim3(kThreads), parts, 0, static_cast<cudaStream_t>(stream), logits, pitch, temperature, out, out_pitch, vocab);
 }
 
