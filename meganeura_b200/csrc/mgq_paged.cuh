@@ -279,7 +279,7 @@ int launch_merge(const AttendArgs &a, uint32_t ctas, uint32_t pairs, cudaStream_
 // 16-bit types with heads of a multiple of 8 elements on 16-byte boundaries: few new tokens (mgq_paged_decode.cu).
 bool decode_takes(const AttendArgs &a, int dtype);
 uint32_t decode_ctas(uint32_t head_dim);
-constexpr int kDecodeRows = 32;
+constexpr int kDecodeRows = 16;
 int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream);      // pairs: a bound of a sequence's tokens * heads per key / value head
 
 // The same types with heads of up to 128, everything on 16-byte boundaries: many new tokens (mgq_paged_prefill.cu).

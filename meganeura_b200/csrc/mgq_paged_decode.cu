@@ -481,7 +481,7 @@ int launch_sized(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cud
 template <typename T>
 int launch_typed(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cudaStream_t stream)
 {
-    const bool two = pairs > 16;
+    const bool two = false && pairs > 16;
     if (a.d <= 64) return two ? launch_sized<T, 64, 2>(a, maps, pairs, stream) : launch_sized<T, 64, 1>(a, maps, pairs, stream);
     if (a.d <= 128) return two ? launch_sized<T, 128, 2>(a, maps, pairs, stream) : launch_sized<T, 128, 1>(a, maps, pairs, stream);
     return launch_sized<T, 256, 1>(a, maps, pairs, stream);
