@@ -209,11 +209,11 @@ __device__ __forceinline__ void name_part(const AttendArgs &a, uint32_t cta, con
 // unit, added in this order.  Grid: (CTAs, anything): the rows are shared out over y, a warp takes a row.  Round trips to L2 bound it: a warp finds the
 // unit's end with one, then takes eight parts with each, maxima, weights and sums together.
 constexpr int kMergeThreads = 128, kMergeWarps = kMergeThreads / 32;
-template <typename T, int ROWS, int COLS>                // COLS: columns of a lane
+template <typename T, int ROWS, int COLS, int BATCH, bool WIDE>      // COLS: columns of a lane; four side by side (WIDE) or one in 32
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a, uint32_t ctas)
 {
-    constexpr int kBatch = COLS > 4 ? 4 : 8;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, c0 = blockIdx.x;
+    auto column = [&](int i) { return WIDE ? 4 * lane + 128 * (i / 4) + i % 4 : lane + 32 * i; };
     pdl_launch_dependents();
     pdl_wait();
     const PartHead h = a.heads[2 * c0 + 1];
@@ -232,27 +232,35 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a
         float top = -INFINITY, l = 0.f, o[COLS];
 #pragma unroll
         for (int i = 0; i < COLS; i++) o[i] = 0.f;
-        for (uint32_t p0 = 0; p0 < parts; p0 += kBatch) {
-            float2 ml[kBatch];
-            float v[kBatch][COLS];
+        for (uint32_t p0 = 0; p0 < parts; p0 += BATCH) {
+            float2 ml[BATCH];
+            float v[BATCH][COLS];
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) {
+            for (int b = 0; b < BATCH; b++) {
                 const uint32_t p = p0 + b;
                 const float *part = a.parts + (2 * (size_t)(c0 + p) + (p == 0 ? 1 : 0)) * size;
                 const bool live = p < parts;
-                ml[b] = live ? make_float2(part[ROWS * d + 2 * r], part[ROWS * d + 2 * r + 1]) : make_float2(-INFINITY, 0.f);
+                ml[b] = live ? *reinterpret_cast<const float2 *>(part + ROWS * d + 2 * r) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int i = 0; i < COLS; i++) v[b][i] = live && lane + 32 * i < d ? part[r * d + lane + 32 * i] : 0.f;
+                for (int i = 0; i < COLS; i += WIDE ? 4 : 1) {
+                    const bool in = live && column(i) < d;
+                    if constexpr (WIDE) {
+                        const float4 q = in ? *reinterpret_cast<const float4 *>(part + r * d + column(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        v[b][i] = q.x; v[b][i + 1] = q.y; v[b][i + 2] = q.z; v[b][i + 3] = q.w;
+                    } else {
+                        v[b][i] = in ? part[r * d + column(i)] : 0.f;
+                    }
+                }
             }
             const float before = top;
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) top = fmaxf(top, ml[b].x);
+            for (int b = 0; b < BATCH; b++) top = fmaxf(top, ml[b].x);
             const float keep = before > -INFINITY ? exp2f(before - top) : 1.f;
             l *= keep;
 #pragma unroll
             for (int i = 0; i < COLS; i++) o[i] *= keep;
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) {
+            for (int b = 0; b < BATCH; b++) {
                 const float w = ml[b].y != 0.f ? exp2f(ml[b].x - top) : 0.f;         // a NaN is a weight; a part without weight may hold anything
                 l += w * ml[b].y;
 #pragma unroll
@@ -264,22 +272,25 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttendArgs a
         T *out = static_cast<T *>(a.out) + (size_t)(h.row0 + token) * a.out_pitch + (size_t)(h.head0 + head) * d;
 #pragma unroll
         for (int i = 0; i < COLS; i++)
-            if (lane + 32 * i < d) out[lane + 32 * i] = rounded<T>(o[i] * scale);
+            if (column(i) < d) out[column(i)] = rounded<T>(o[i] * scale);
     }
 }
-// pairs: a bound of the rows of a unit that has parts.
+// pairs: a bound of the rows of a unit that has parts.  Units of few rows may have many parts: eight at a time; of 256 rows a handful, and registers for
+// more warps count.
 template <typename T, int ROWS>
 int launch_merge(const AttendArgs &a, uint32_t ctas, uint32_t pairs, cudaStream_t stream)
 {
+    constexpr int kBatch = ROWS > 64 ? 2 : 8;
     const dim3 grid(ctas, (min(pairs, (uint32_t)ROWS) + kMergeWarps - 1) / kMergeWarps);
-    return a.d <= 128 ? launch(merge_kernel<T, ROWS, 4>, grid, dim3(kMergeThreads), 0, stream, a, ctas)
-                      : launch(merge_kernel<T, ROWS, 8>, grid, dim3(kMergeThreads), 0, stream, a, ctas);
+    auto *kernel = a.d % 4 == 0 ? (a.d <= 128 ? merge_kernel<T, ROWS, 4, kBatch, true> : merge_kernel<T, ROWS, 8, kBatch / 2, true>)
+                                : (a.d <= 128 ? merge_kernel<T, ROWS, 4, kBatch, false> : merge_kernel<T, ROWS, 8, kBatch / 2, false>);
+    return launch(kernel, grid, dim3(kMergeThreads), 0, stream, a, ctas);
 }
 
 // 16-bit types with heads of a multiple of 8 elements on 16-byte boundaries: few new tokens (mgq_paged_decode.cu).
 bool decode_takes(const AttendArgs &a, int dtype);
 uint32_t decode_ctas(uint32_t head_dim);
-constexpr int kDecodeRows = 16;
+constexpr int kDecodeRows = 16, kDecodePairs = 32;         // of a unit; of a sequence that is not yet many tokens'
 int launch_decode(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream);      // pairs: a bound of a sequence's tokens * heads per key / value head
 
 // The same types with heads of up to 128, everything on 16-byte boundaries: many new tokens (mgq_paged_prefill.cu).

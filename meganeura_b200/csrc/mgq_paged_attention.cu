@@ -220,11 +220,11 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
     const uint32_t pairs = (uint32_t)min((unsigned long long)max_fresh * a.group, 0xFFFFFFFFull);
     if (decode_takes(a, dtype)) {
         room(decode_ctas(head_dim));
-        if (pairs <= kDecodeRows || !prefill_takes(a, dtype)) return launch_decode(a, dtype, pairs, s);
+        if (pairs <= kDecodePairs || !prefill_takes(a, dtype)) return launch_decode(a, dtype, pairs, s);
         // both kinds of sequences may be there
-        a.rows_to = kDecodeRows;
-        if (int rc = launch_decode(a, dtype, kDecodeRows, s)) return rc;
-        a.rows_from = kDecodeRows + 1;
+        a.rows_to = kDecodePairs;
+        if (int rc = launch_decode(a, dtype, kDecodePairs, s)) return rc;
+        a.rows_from = kDecodePairs + 1;
         a.rows_to = 0xFFFFFFFFu;
         a.heads = reinterpret_cast<PartHead *>(a.parts + (size_t)decode_ctas(head_dim) * 2 * kDecodeRows * (head_dim + 2));
         a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);

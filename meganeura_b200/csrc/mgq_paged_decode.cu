@@ -1,11 +1,13 @@
 // Attention of few new tokens per sequence (single tokens, drafted ones) over a paged cache of f16 or bf16: reads every key and value
 // once, so HBM bounds it, and all that matters is that loads never pause.
 //
-// A unit's pairs of token and head (16 or 32: heads of one key / value head share its keys) are the rows of m16n8k16 products.  The
+// A unit's pairs of token and head (16: heads of one key / value head share its keys) are the rows of m16n8k16 products.  The
 // four warps of a CTA split the keys: each takes 16 of a block of 64, has a ring of its own for their keys and values, filled by
 // TMA boxes of 16 keys by 64 elements that run across the borders of units, and an online softmax of its own; nothing in the loop waits for another warp.  At a
 // unit's end the four sums are joined in shared memory.  Scores, maxima and sums are f32; a weight enters its product as the sum of two 16-bit values (the
 // tensor cores have time for both), so only the result is rounded.
+// More pairs than 16 are units of their own that find the keys in L2: 32 sequences of up to 20 pairs (323 MB) take 69 us, with two blocks of rows per warp
+// 103 us, on tcgen05 115 us; of 32 pairs each 118 and 107 us, four sequences of 32 pairs 29 and 40 us.  From 33 pairs on they are mgq_paged_prefill.cu's.
 // With 16-byte cp.async instead of boxes a step took 627 instructions and 64 single tokens of the Qwen3-8B shape 242 us.
 #include <cstdint>
 
@@ -16,6 +18,7 @@ namespace mgq {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kBlock = 64, kStep = 16;      // keys of a block, of a warp's step
+constexpr int kRows = 16;                                               // pairs of token and head
 constexpr int kChunk = 16, kPitch = kChunk + 2;                         // columns joined at a time
 constexpr int kStages = 3;
 constexpr uint32_t kTile = kStep * 128;                                 // 16 keys by 64 elements, as one swizzled box lies in shared memory
@@ -23,9 +26,7 @@ constexpr uint32_t kTile = kStep * 128;                                 // 16 ke
 // Stages of 16 keys and values fill the SM's shared memory, three per warp.
 template <int D> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 3 : D == 128 ? 2 : 1; }
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return 2 * D / 64 * kTile; }
-// Queries (two blocks of rows do not fit into the registers) and, behind a unit's last key, the warps' sums.
-template <int D, int MT> __host__ __device__ constexpr uint32_t rows_bytes() { return MT == 2 ? 32 * (D * 2 + 16) > kWarps * 32 * kPitch * 4 ? 32 * (D * 2 + 16) : kWarps * 32 * kPitch * 4 : kWarps * 16 * kPitch * 4; }
-template <int D, int MT> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * kStages * stage_bytes<D>() + rows_bytes<D, MT>(); }
+template <int D> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * kStages * stage_bytes<D>() + kWarps * kRows * kPitch * 4; }
 
 __device__ unsigned int g_decode_error;
 
@@ -80,25 +81,24 @@ __device__ __forceinline__ bool not_finite8(const uint4 &v)
     return bad;
 }
 
-template <typename T, int D, int MT>                     // D: head size rounded up to 64, 128 or 256; MT: blocks of 16 rows
+template <typename T, int D>                             // D: head size rounded up to 64, 128 or 256
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const __grid_constant__ CacheMaps maps, const AttendArgs a)
 {
-    constexpr int ROWS = 16 * MT, NT = D / 8, KT = D / 16, PARTS = D / 64, QB = D * 2 + 16;
+    constexpr int NT = D / 8, KT = D / 16, PARTS = D / 64;
     constexpr uint32_t kStage = stage_bytes<D>();
-    using Way = Walk<ROWS, kBlock, 1>;
+    using Way = Walk<kRows, kBlock, 1>;
     extern __shared__ uint8_t s_raw[];
     __shared__ unsigned long long s_walk[40];
     __shared__ __align__(8) unsigned long long s_full[kWarps][kStages];
     __shared__ Way s_way[kWarps];
     __shared__ Segment s_seg[kWarps][8];
     __shared__ uint32_t s_there[kWarps][kStages];
-    __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+    __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
     __shared__ volatile int s_failed;
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = __shfl_sync(0xffffffffu, t >> 5, 0), d = a.d;
     uint8_t *s_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t ring = smem_u32(s_mem) + warp * (kStages * kStage);
-    uint8_t *s_rows = s_mem + (size_t)kWarps * kStages * kStage;
-    float *s_join = reinterpret_cast<float *>(s_rows);
+    float *s_join = reinterpret_cast<float *>(s_mem + (size_t)kWarps * kStages * kStage);
     if (t == 0) {
         for (int i = 0; i < kWarps * kStages; i++) mbar_init(&s_full[i / kStages][i % kStages], 1);
         s_failed = 0;
@@ -197,42 +197,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
         const Segment g = s_seg[warp][c_seg & 7u];
         c_seg++;
         const uint32_t pairs = g.tokens * g.heads;
-        uint32_t q[MT == 1 ? KT : 1][4];
-        int pos[MT][2];
+        uint32_t q[KT][4];
+        int pos[2];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int half = 0; half < 2; half++) {
+            const uint32_t r = half * 8 + row, token = r / g.heads, head = r - token * g.heads;
+            const bool live = r < pairs;
+            pos[half] = live ? g.pos0 + (int)token : -1;
+            const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d + 2 * quad;
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const uint32_t r = mt * 16 + half * 8 + row, token = r / g.heads, head = r - token * g.heads;
-                const bool live = r < pairs;
-                pos[mt][half] = live ? g.pos0 + (int)token : -1;
-                const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d + 2 * quad;
-                if constexpr (MT == 1) {
+            for (int k = 0; k < KT; k++)
 #pragma unroll
-                    for (int k = 0; k < KT; k++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            q[k][half + 2 * j] = live && k * 16 + j * 8 + 2 * quad < d ? *reinterpret_cast<const uint32_t *>(src + k * 16 + j * 8) : 0u;
-                }
-            }
-        if constexpr (MT == 2) {
-            for (uint32_t i = t; i < ROWS * D / 2; i += kThreads) {
-                const uint32_t r = i / (D / 2), c = i % (D / 2) * 2, token = r / g.heads, head = r - token * g.heads;
-                uint32_t x = 0;
-                if (r < pairs && c < d) x = *reinterpret_cast<const uint32_t *>(static_cast<const T *>(a.q) + (size_t)(g.row0 + token) * a.q_pitch + (size_t)(g.head0 + head) * d + c);
-                *reinterpret_cast<uint32_t *>(s_rows + r * QB + c * 2) = x;
-            }
-            __syncthreads();
+                for (int j = 0; j < 2; j++)
+                    q[k][half + 2 * j] = live && k * 16 + j * 8 + 2 * quad < d ? *reinterpret_cast<const uint32_t *>(src + k * 16 + j * 8) : 0u;
         }
-        const uint32_t qaddr = smem_u32(s_rows) + (lane & 15u) * QB + (lane >> 4) * 16;
-        float o[MT][NT][4], m[MT][2], l[MT][2];
+        float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.f;
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
-        }
+        for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
         const uint32_t blocks = max(g.end, g.begin + 1) - g.begin;
         const int last_pos = g.pos0 + (int)g.tokens - 1;
         for (uint32_t b = 0; b < blocks; b++) {
@@ -254,71 +235,57 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // before the stage is filled again
                 __syncwarp();
             }
-            float s[MT][2][4];
+            float s[2][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int n = 0; n < 2; n++) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
+            for (int n = 0; n < 2; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
             for (int k = 0; k < KT; k++) {
                 uint32_t kf[4];
                 ldmatrix4(kf, kbase + k / 4 * kTile + kpiece[k % 4]);
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    uint32_t qf[4];
-                    if constexpr (MT == 1) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) qf[i] = q[k][i];
-                    } else {
-                        ldmatrix4(qf, qaddr + mt * 16 * QB + k * 32);
-                    }
-                    mma<T>(s[mt][0], qf, kf[0], kf[1]);
-                    mma<T>(s[mt][1], qf, kf[2], kf[3]);
-                }
+                mma<T>(s[0], q[k], kf[0], kf[1]);
+                mma<T>(s[1], q[k], kf[2], kf[3]);
             }
             const bool whole = there == 0xFFFFu && key0 + kStep - 1 <= g.pos0 && (!a.window || key0 > last_pos - (int)a.window);
             bool hidden = false;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int half = 0; half < 2; half++) {
+                float top = m[half];
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    float top = m[mt][half];
+                for (int n = 0; n < 2; n++)
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float x = s[mt][n][2 * half + e] * a.scale_log2;
-                            if (!whole) {
-                                const int key = key0 + n * 8 + 2 * (int)quad + e, p = pos[mt][half];
-                                const bool seen = key <= p && (there >> (n * 8 + 2 * quad + e) & 1u) && (!a.window || key > p - (int)a.window);
-                                hidden |= !seen;
-                                x = seen ? x : -INFINITY;
-                            }
-                            s[mt][n][2 * half + e] = x;
-                            top = fmaxf(top, x);
+                    for (int e = 0; e < 2; e++) {
+                        float x = s[n][2 * half + e] * a.scale_log2;
+                        if (!whole) {
+                            const int key = key0 + n * 8 + 2 * (int)quad + e, p = pos[half];
+                            const bool seen = key <= p && (there >> (n * 8 + 2 * quad + e) & 1u) && (!a.window || key > p - (int)a.window);
+                            hidden |= !seen;
+                            x = seen ? x : -INFINITY;
                         }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float base = top == -INFINITY ? 0.f : top;
-                    if (__any_sync(0xffffffffu, top > m[mt][half])) {
-                        const float keep = exp2_fast(m[mt][half] - base);
-                        l[mt][half] *= keep;
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            o[mt][n][2 * half] *= keep;
-                            o[mt][n][2 * half + 1] *= keep;
-                        }
-                        m[mt][half] = top;
+                        s[n][2 * half + e] = x;
+                        top = fmaxf(top, x);
                     }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float base = top == -INFINITY ? 0.f : top;
+                if (__any_sync(0xffffffffu, top > m[half])) {
+                    const float keep = exp2_fast(m[half] - base);
+                    l[half] *= keep;
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float p = exp2_fast(s[mt][n][2 * half + e] - base);
-                            s[mt][n][2 * half + e] = p;
-                            l[mt][half] += p;
-                        }
+                    for (int n = 0; n < NT; n++) {
+                        o[n][2 * half] *= keep;
+                        o[n][2 * half + 1] *= keep;
+                    }
+                    m[half] = top;
                 }
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float p = exp2_fast(s[n][2 * half + e] - base);
+                        s[n][2 * half + e] = p;
+                        l[half] += p;
+                    }
+            }
             // where some row does not see a value that another one sees and that is infinite or NaN, its product with a weight of 0 must not be formed
             if (!whole && __any_sync(0xffffffffu, hidden)) {
                 bool bad = false;
@@ -331,47 +298,38 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll 1
                     for (uint32_t j = 0; j < kStep; j++) {
-                        float p[MT][2];
+                        float p[2];
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                            for (int half = 0; half < 2; half++) {
-                                const float even = j < 8 ? s[mt][0][2 * half] : s[mt][1][2 * half], oddv = j < 8 ? s[mt][0][2 * half + 1] : s[mt][1][2 * half + 1];
-                                p[mt][half] = __shfl_sync(0xffffffffu, j & 1u ? oddv : even, (lane & ~3u) | (j & 7u) >> 1);
-                            }
+                        for (int half = 0; half < 2; half++) {
+                            const float even = j < 8 ? s[0][2 * half] : s[1][2 * half], oddv = j < 8 ? s[0][2 * half + 1] : s[1][2 * half + 1];
+                            p[half] = __shfl_sync(0xffffffffu, j & 1u ? oddv : even, (lane & ~3u) | (j & 7u) >> 1);
+                        }
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             uint32_t w;
                             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vbase + n / 8 * kTile + j * 128 + (((n % 8) ^ (j & 7u)) << 4) + quad * 4) : "memory");
                             const T *v = reinterpret_cast<const T *>(&w);
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++)
+                            for (int half = 0; half < 2; half++)
 #pragma unroll
-                                for (int half = 0; half < 2; half++)
-#pragma unroll
-                                    for (int e = 0; e < 2; e++)
-                                        o[mt][n][2 * half + e] += p[mt][half] != 0.f ? p[mt][half] * to_f32(v[e]) : 0.f;
+                                for (int e = 0; e < 2; e++)
+                                    o[n][2 * half + e] += p[half] != 0.f ? p[half] * to_f32(v[e]) : 0.f;
                         }
                     }
                     continue;
                 }
             }
-            uint32_t high[MT][4], low[MT][4];
+            uint32_t high[4], low[4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) split_pair<T>(s[mt][i >> 1][2 * (i & 1)], s[mt][i >> 1][2 * (i & 1) + 1], high[mt][i], low[mt][i]);
+            for (int i = 0; i < 4; i++) split_pair<T>(s[i >> 1][2 * (i & 1)], s[i >> 1][2 * (i & 1) + 1], high[i], low[i]);
 #pragma unroll
             for (int n = 0; n < NT; n += 2) {
                 uint32_t vf[4];
                 ldmatrix4_t(vf, vbase + n / 8 * kTile + vpiece[n / 2 % 4]);
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    mma<T>(o[mt][n], high[mt], vf[0], vf[1]);
-                    mma<T>(o[mt][n + 1], high[mt], vf[2], vf[3]);
-                    mma<T>(o[mt][n], low[mt], vf[0], vf[1]);
-                    mma<T>(o[mt][n + 1], low[mt], vf[2], vf[3]);
-                }
+                mma<T>(o[n], high, vf[0], vf[1]);
+                mma<T>(o[n + 1], high, vf[2], vf[3]);
+                mma<T>(o[n], low, vf[0], vf[1]);
+                mma<T>(o[n + 1], low, vf[2], vf[3]);
             }
         }
 
@@ -379,32 +337,28 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 
         // ---- the four warps' sums
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float sum = l[mt][half];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (quad == 0) {
-                    s_m[warp][mt * 16 + half * 8 + row] = m[mt][half];
-                    s_l[warp][mt * 16 + half * 8 + row] = sum;
-                }
+        for (int half = 0; half < 2; half++) {
+            float sum = l[half];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (quad == 0) {
+                s_m[warp][half * 8 + row] = m[half];
+                s_l[warp][half * 8 + row] = sum;
             }
+        }
         __syncthreads();
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int half = 0; half < 2; half++) {
+            const uint32_t r = half * 8 + row;
+            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+            const float mine = s_l[warp][r] != 0.f ? exp2_fast(m[half] - top) : 0.f;
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const uint32_t r = mt * 16 + half * 8 + row;
-                const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                const float mine = s_l[warp][r] != 0.f ? exp2_fast(m[mt][half] - top) : 0.f;
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) o[mt][n][2 * half + e] = mine != 0.f ? o[mt][n][2 * half + e] * mine : 0.f;
-            }
+                for (int e = 0; e < 2; e++) o[n][2 * half + e] = mine != 0.f ? o[n][2 * half + e] * mine : 0.f;
+        }
         const bool alone = g.first && g.last;
-        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * ROWS * (d + 2);
+        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kRows * (d + 2);
         // the sums of a row's weights, needed where it is finished or stored
         auto total = [&](uint32_t r, float &top) {
             top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
@@ -417,13 +371,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
         for (int c = 0; c < D / kChunk; c++) {
             if (c * kChunk >= (int)d) break;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int half = 0; half < 2; half++)
-                        *reinterpret_cast<float2 *>(s_join + (warp * ROWS + mt * 16 + half * 8 + row) * kPitch + n * 8 + 2 * quad) =
-                            make_float2(o[mt][2 * c + n][2 * half], o[mt][2 * c + n][2 * half + 1]);
+                for (int half = 0; half < 2; half++)
+                    *reinterpret_cast<float2 *>(s_join + (warp * kRows + half * 8 + row) * kPitch + n * 8 + 2 * quad) =
+                        make_float2(o[2 * c + n][2 * half], o[2 * c + n][2 * half + 1]);
             __syncthreads();
             for (uint32_t i = t; i < pairs * (kChunk / 2); i += kThreads) {
                 const uint32_t r = i / (kChunk / 2), col = i % (kChunk / 2) * 2;
@@ -431,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 float x = 0.f, y = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) {
-                    const float2 v = *reinterpret_cast<const float2 *>(s_join + (w * ROWS + r) * kPitch + col);
+                    const float2 v = *reinterpret_cast<const float2 *>(s_join + (w * kRows + r) * kPitch + col);
                     x += v.x;
                     y += v.y;
                 }
@@ -452,8 +404,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             if (t < pairs) {
                 float top;
                 const float sum = total(t, top);
-                part[ROWS * d + 2 * t] = top;
-                part[ROWS * d + 2 * t + 1] = sum;
+                part[kRows * d + 2 * t] = top;
+                part[kRows * d + 2 * t + 1] = sum;
             }
             if (t == 0) name_part(a, blockIdx.x, g);
             __syncthreads();                             // before the next unit's maxima
@@ -468,23 +420,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
         }
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D>
 int launch_sized(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cudaStream_t stream)
 {
     constexpr uint32_t ctas = 148 * ctas_per_sm<D>();
-    auto *kernel = decode_kernel<T, D, MT>;
-    if (int rc = allow_smem(kernel, smem_bytes<D, MT>())) return rc;
-    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, MT>(), stream, maps, a)) return rc;
-    return launch_merge<T, 16 * MT>(a, ctas, pairs, stream);
+    auto *kernel = decode_kernel<T, D>;
+    if (int rc = allow_smem(kernel, smem_bytes<D>())) return rc;
+    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D>(), stream, maps, a)) return rc;
+    return launch_merge<T, kRows>(a, ctas, pairs, stream);
 }
 
 template <typename T>
 int launch_typed(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cudaStream_t stream)
 {
-    const bool two = false && pairs > 16;
-    if (a.d <= 64) return two ? launch_sized<T, 64, 2>(a, maps, pairs, stream) : launch_sized<T, 64, 1>(a, maps, pairs, stream);
-    if (a.d <= 128) return two ? launch_sized<T, 128, 2>(a, maps, pairs, stream) : launch_sized<T, 128, 1>(a, maps, pairs, stream);
-    return launch_sized<T, 256, 1>(a, maps, pairs, stream);
+    if (a.d <= 64) return launch_sized<T, 64>(a, maps, pairs, stream);
+    if (a.d <= 128) return launch_sized<T, 128>(a, maps, pairs, stream);
+    return launch_sized<T, 256>(a, maps, pairs, stream);
 }
 
 }  // namespace

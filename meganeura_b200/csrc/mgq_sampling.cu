@@ -31,6 +31,13 @@ __device__ __forceinline__ T cluster_read(const T *p, uint32_t rank)
     }
 }
 
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Four values of a row from column c on; `fill` behind its end.  LAST: they are not read again.
 template <bool WIDE, bool LAST>
 __device__ __forceinline__ void read4(const float *row, uint32_t c, uint32_t end, float fill, float (&v)[4])
@@ -64,11 +71,15 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
     const float *row = logits + (size_t)blockIdx.x * pitch;
     float *dst = out + (size_t)blockIdx.x * out_pitch;
     float v[kHold][4];
-    auto fetch = [&](uint32_t c0) {
+    auto fetch = [&](uint32_t c0) {                      // NaN becomes -inf
 #pragma unroll
-        for (int k = 0; k < kHold; k++) read4<WIDE, HELD>(row, c0 + k * kGroup + 4 * t, end, -INFINITY, v[k]);
+        for (int k = 0; k < kHold; k++) {
+            read4<WIDE, HELD>(row, c0 + k * kGroup + 4 * t, end, -INFINITY, v[k]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[k][e] = fmaxf(v[k][e], -INFINITY);
+        }
     };
-    auto largest = [&]() {                               // fmaxf passes over NaN
+    auto largest = [&]() {
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kHold; k++) m = fmaxf(m, fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3])));
@@ -77,23 +88,25 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
     fetch(begin);
     const float temp = temperature ? temperature[blockIdx.x] : 1.f;
     const bool greedy = !(temp > 0.f);
-    const float inv = greedy ? 0.f : 1.f / temp;
-    auto weight = [&](float x, float m) { return x == m ? (m > -INFINITY ? 1.f : 0.f) : x < m ? expf((x - m) * inv) : 0.f; };
-    auto weights = [&](float m) {
+    // exponents of 2; the difference first, which is exact near the maximum however large that is.  No finite difference becomes inf * 0.
+    const float inv = greedy ? 0.f : fminf(1.4426950408889634f / temp, FLT_MAX);
+    auto weights = [&](float m) {                        // their sum, relative to a finite maximum
         float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kHold; k++) sum += (weight(v[k][0], m) + weight(v[k][1], m)) + (weight(v[k][2], m) + weight(v[k][3], m));
+        for (int k = 0; k < kHold; k++)
+            sum += (exp2_fast((v[k][0] - m) * inv) + exp2_fast((v[k][1] - m) * inv)) + (exp2_fast((v[k][2] - m) * inv) + exp2_fast((v[k][3] - m) * inv));
         return sum;
     };
+    auto finite = [](float m) { return fabsf(m) <= FLT_MAX ? m : 0.f; };         // sums of rows without a finite maximum are not used
 
     float m = largest(), sum = 0.f;
     if (!HELD) {
         // a thread's sum is relative to its own maximum
-        if (!greedy) sum = weights(m);
+        if (!greedy) sum = weights(finite(m));
         for (uint32_t c0 = begin + kSlice; c0 < end; c0 += kSlice) {
             fetch(c0);
             const float top = fmaxf(m, largest());
-            if (!greedy) sum = sum * weight(m, top) + weights(top);
+            if (!greedy) sum = sum * exp2_fast((finite(m) - finite(top)) * inv) + weights(finite(top));
             m = top;
         }
     }
@@ -108,6 +121,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
         m = warp_max(cluster_read(&x_max, lane % parts));
     }
 
+    const bool odd = !(fabsf(m) <= FLT_MAX);             // nothing above -inf, or +inf
     uint32_t at = 0xFFFFFFFFu;                           // the greedy choice: of the largest, the lowest
     if (greedy) {                                        // uniform over the cluster
         for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
@@ -125,9 +139,19 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
         else           __syncthreads();
         at = x_at;
         for (uint32_t p = 0; parts > 1 && p < parts; p++) at = min(at, cluster_read(&x_at, p));
-        sum = at != 0xFFFFFFFFu ? 1.f : 0.f;
     } else {
-        sum = HELD ? weights(m) : sum * weight(mine, m);
+        if (odd) {                                       // how many are +inf
+            sum = 0.f;
+            for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
+                if (!HELD) fetch(c0);
+#pragma unroll
+                for (int k = 0; k < kHold; k++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum += v[k][e] == INFINITY ? 1.f : 0.f;
+            }
+        } else {
+            sum = HELD ? weights(m) : mine > -INFINITY ? sum * exp2_fast((mine - m) * inv) : 0.f;
+        }
         sum = warp_sum(sum);
         if (lane == 0) s_part[1][warp] = sum;
         __syncthreads();
@@ -139,14 +163,13 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
         }
     }
     const float scale = sum > 0.f ? 1.f / sum : 0.f;
-    for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
-        if (!HELD) fetch(c0);
+    auto store = [&](uint32_t c0, auto value) {
 #pragma unroll
         for (int k = 0; k < kHold; k++) {
             const uint32_t c = c0 + k * kGroup + 4 * t;
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = greedy ? (c + e == at ? 1.f : 0.f) : weight(v[k][e], m) * scale;
+            for (int e = 0; e < 4; e++) p[e] = value(v[k][e], c + e);
             if (WIDE) {
                 if (c < end) __stcs(reinterpret_cast<float4 *>(dst + c), make_float4(p[0], p[1], p[2], p[3]));
             } else {
@@ -155,6 +178,11 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
                     if (c + e < end) __stcs(dst + c + e, p[e]);
             }
         }
+    };
+    for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
+        if (!HELD && !greedy) fetch(c0);
+        if (greedy || odd) store(c0, [&](float x, uint32_t c) { return greedy ? (c == at ? 1.f : 0.f) : x == INFINITY ? scale : 0.f; });
+        else               store(c0, [&](float x, uint32_t) { return exp2f((x - m) * inv) * scale; });
     }
     if (parts > 1) cluster_sync();                       // nobody leaves while its sums are being read
 }
