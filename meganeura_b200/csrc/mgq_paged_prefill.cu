@@ -23,7 +23,6 @@ namespace mgq {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kSoft = 0;                                 // of eight pairs of exponentials, those that go to the multiply-add units
 constexpr int kExtra = 4;                                // blocks of keys that starting and ending a unit take as long as
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
@@ -90,19 +89,6 @@ __device__ __forceinline__ pair_t pair_add(pair_t x, pair_t y)
     pair_t v;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
     return v;
-}
-// 2^x of finite x <= 127 on the multiply-add units: 16 exponentials per cycle leave an SM idle for half of attention's time
-// (heads of 128).  x = n + f with n whole and f in [-1/2, 1/2]: 2^f by a polynomial fitted to the least relative error (7.5e-5 of degree 3 for
-// bf16 weights, 2.6e-6 of degree 4 for f16 ones), n added to its exponent.  Below 2^-126 the result stays there.
-template <typename T>
-__device__ __forceinline__ float exp2_soft(float x)
-{
-    constexpr bool kFour = std::is_same<T, __half>::value;
-    x = fmaxf(x, -126.f);
-    const float r = x + 12582912.f, f = x - (r - 12582912.f);            // 1.5 * 2^23: the sum's last bits are the rounded value
-    const float p = kFour ? fmaf(fmaf(fmaf(fmaf(0.009570102207362652f, f, 0.05591785907745361f), f, 0.240247443318367f), f, 0.6931217908859253f), f, 0.9999992847442627f)
-                          : fmaf(fmaf(fmaf(0.0551716685295105f, f, 0.2426111251115799f), f, 0.6932609677314758f), f, 0.9999280571937561f);
-    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
 }
 // 64 columns of this lane's row; wait_row before they are used.
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, float (&y)[64])
@@ -511,20 +497,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 };
                 float s[64], t[64];
                 tmem_ld_row(s_at, s);
-                tmem_ld_row(s_at + 64, t);
                 wait_row(s);
-                wait_row(t);
+                tmem_ld_row(s_at + 64, t);               // on its way while the first half's maximum is found
                 mask(s, 0);
+                const float first = row_max(s);
+                wait_row(t);
                 mask(t, 1);
-                const float first = row_max(s), second = row_max(t), top = max3(first, second, second) * scale;
+                const float second = row_max(t), top = max3(first, second, second) * scale;
                 // Nothing to do where the maximum stays at or below the old one + 8 (finite behind the first block); -inf and NaN come here, too.
-                bool exact = !plain;
                 if (__any_sync(0xffffffffu, !(top <= m + 8.f && top >= -FLT_MAX))) {
                     const bool up = !(top <= m + 8.f) && top > -INFINITY;              // also where m is still -inf
                     const float keep = up ? exp2_fast(m - top) : 1.f;
                     l *= keep;
                     m = up ? top : m;
-                    exact = __any_sync(0xffffffffu, exact || !(fabsf(top) <= FLT_MAX));
                     if (kb != begin && __any_sync(0xffffffffu, up)) {
 #pragma unroll 1
                         for (uint32_t c = 0; c < D; c += 16) {
@@ -540,33 +525,34 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 const float base = m == -INFINITY ? 0.f : -m;
                 const pair_t bases = pair_of(base, base);
                 pair_t sum[2] = {0, 0};
-                auto weights = [&](const float (&s)[64], int c, bool soft) {       // 64 keys: exponentials, sums, P
+                // A quarter of the keys: exponentials, sums, P.  The first half is signalled in front of the third quarter's stores, when its own are long
+                // done: waiting for them at once cost the row 100 cycles, and the products of the first half have time.
+                auto weights = [&](const float (&s)[64], int quarter, auto before_stores) {
+                    uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 32) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            float x, y;
-                            parts_of(pair_fma(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), scales, bases), x, y);
-                            x = soft && e % 8 < kSoft ? exp2_soft<T>(x) : exp2_fast(x);
-                            y = soft && e % 8 < kSoft ? exp2_soft<T>(y) : exp2_fast(y);
-                            sum[e & 1] = pair_add(sum[e & 1], pair_of(x, y));
-                            p[e] = pack<T>(x, y);
-                        }
-                        tmem_st16(s_at + 32 * c + i / 2, p);
+                    for (int e = 0; e < 16; e++) {
+                        const int i = quarter % 2 * 32 + 2 * e;
+                        float x, y;
+                        parts_of(pair_fma(pair_of(s[i], s[i + 1]), scales, bases), x, y);
+                        x = exp2_fast(x);
+                        y = exp2_fast(y);
+                        sum[e & 1] = pair_add(sum[e & 1], pair_of(x, y));
+                        p[e] = pack<T>(x, y);
                     }
+                    before_stores();
+                    tmem_st16(s_at + 16 * quarter, p);
+                };
+                auto signal = [&](unsigned long long *bar) {
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(c ? &sh.p_full[tile] : &sh.p_half[tile]);
+                    if (lane == 0) mbar_arrive(bar);
                 };
-                if (!exact) {
-                    weights(s, 0, true);
-                    weights(t, 1, true);
-                } else {
-                    weights(s, 0, false);
-                    weights(t, 1, false);
-                }
+                weights(s, 0, [] {});
+                weights(s, 1, [] {});
+                weights(t, 2, [&] { signal(&sh.p_half[tile]); });
+                weights(t, 3, [] {});
+                signal(&sh.p_full[tile]);
                 float x, y;
                 parts_of(pair_add(sum[0], sum[1]), x, y);
                 l += x + y;
