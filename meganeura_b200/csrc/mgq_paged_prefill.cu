@@ -23,7 +23,7 @@ namespace mgq {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kExtra = 4;                                // blocks of keys that starting and ending a unit take as long as
+constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return D / 64 * kHalf; }
@@ -120,6 +120,25 @@ __device__ __forceinline__ float row_max(const float (&y)[64])
 #pragma unroll
         for (int i = 0; i < 4; i++) t[i] = max3(t[i], y[e + i], y[e + 4 + i]);
     return max3(max3(t[0], t[1], y[60]), max3(t[2], t[3], y[61]), max3(y[62], y[63], y[63]));
+}
+// Every eight lanes transpose their eight pieces of 16 bytes: afterwards lane i of them holds piece i of all eight lanes.
+__device__ __forceinline__ void transpose8(uint32_t (&v)[8][4])
+{
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) {
+        const bool upper = lane & s;
+#pragma unroll
+        for (int a = 0; a < 8; a++) {
+            if (a & s) continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? v[a][i] : v[a + s][i], s);
+                if (upper) v[a][i] = got;
+                else       v[a + s][i] = got;
+            }
+        }
+    }
 }
 // All 128 threads of a tile's warps: whether any of them says so.
 __device__ __forceinline__ bool any_of_tile(uint32_t tile, bool mine)
@@ -428,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             if (any_of_tile(tile, !there_is)) break;
             if (g.tokens == 0) break;
             const uint32_t begin = g.begin, end = g.end, stop = tile_end(g, tile, last_token[tile]), pairs = g.tokens * g.heads;
+            if (stop <= begin && r_tile == 0) mbar_arrive(&sh.q_empty);           // behind the meeting of this tile's warps
             const int first_pos = g.pos0 + (int)first_token, len = g.len;
             const int last_pos = g.pos0 + (int)min(last_token[tile], g.tokens - 1), window = (int)a.window;
             const int pos = row < pairs ? g.pos0 + (int)token : -1;
@@ -460,7 +480,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 wait(&sh.s_full[tile], s_seen & 1u);
                 s_seen++;
                 tc_fence_after();
-                if (r_tile == 0) {                       // these scores are done, and the product before them
+                if (r_tile == 0) {                       // these scores are done, and the product before them; with the last ones the queries
+                    if (kb + 1 == stop) mbar_arrive(&sh.q_empty);
                     mbar_arrive(&sh.empty[k_slot]);
                     if (kb != begin) mbar_arrive(&sh.empty[v_before]);
                 }
@@ -557,14 +578,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 parts_of(pair_add(sum[0], sum[1]), x, y);
                 l += x + y;
             }
-            // this tile's scores are done with the queries (its warps have met in this unit)
-            if (r_tile == 0) mbar_arrive(&sh.q_empty);
             finish();
             if (tile * kTile < pairs) {
+                // 128 bytes of eight rows at a time, turned so that a store covers whole lines of few rows: a thread storing its own row piece by piece
+                // took 5000 cycles of a unit, 12000 where it is a part.
                 const bool alone = g.first && g.last;
-                T *out = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d;
+                const unsigned long long at = (unsigned long long)(g.row0 + token) * a.out_pitch + (unsigned long long)(g.head0 + head) * d;
                 float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kPrefillRows * (d + 2);
                 const float inv = l == 0.f ? 0.f : 1.f / l;
+                const uint32_t first_row = tile * kTile + quad * 32 + (lane & 24u), piece = lane & 7u;
                 bool bad = false;
 #pragma unroll 1
                 for (uint32_t c = 0; c < D; c += 32) {
@@ -575,23 +597,41 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
 #pragma unroll
                         for (int e = 0; e < 32; e++) o[e] = 0.f;
                     }
-                    if (row < pairs) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (c + e >= d) break;
+                    for (int e = 0; e < 32; e++) bad |= !(fabsf(o[e]) <= FLT_MAX);
+                    if (alone) {                         // 64 bytes of a row, two such steps make a line
+                        uint32_t v[8][4];
 #pragma unroll
-                            for (int i = 0; i < 8; i++) bad |= !(fabsf(o[e + i]) <= FLT_MAX);
-                            if (alone) {
-                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pack<T>(o[e] * inv, o[e + 1] * inv), pack<T>(o[e + 2] * inv, o[e + 3] * inv),
-                                                                                    pack<T>(o[e + 4] * inv, o[e + 5] * inv), pack<T>(o[e + 6] * inv, o[e + 7] * inv));
-                            } else {
-                                *reinterpret_cast<float4 *>(part + row * d + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                                *reinterpret_cast<float4 *>(part + row * d + c + e + 4) = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
-                            }
+                        for (int e = 0; e < 16; e++) v[e / 4][e % 4] = pack<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+                        tmem_ld32(o_at + min(c + 32, (uint32_t)D - 32), o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            if (stop <= begin) o[e] = 0.f;
+                            bad |= !(fabsf(o[e]) <= FLT_MAX);
                         }
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[4 + e / 4][e % 4] = pack<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+                        transpose8(v);
+#pragma unroll
+                        for (int r = 0; r < 8; r++) {
+                            const unsigned long long there = __shfl_sync(0xffffffffu, at, (lane & 24u) + r);
+                            if (first_row + r < pairs && c + 8 * piece < d)
+                                *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + there + c + 8 * piece) = make_uint4(v[r][0], v[r][1], v[r][2], v[r][3]);
+                        }
+                        c += 32;
+                    } else {
+                        uint32_t v[8][4];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e / 4][e % 4] = __float_as_uint(o[e]);
+                        transpose8(v);
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            if (first_row + r < pairs && c + 4 * piece < d)
+                                *reinterpret_cast<uint4 *>(part + (first_row + r) * d + c + 4 * piece) = make_uint4(v[r][0], v[r][1], v[r][2], v[r][3]);
                     }
                     __syncwarp();                        // the next columns are read by the whole warp
                 }
+                bad = bad && row < pairs;
                 if (!alone && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(m, l);
                 for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
                     const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
