@@ -7,8 +7,8 @@ namespace mgq {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4;
-constexpr int kRows = 16, kKeys = 32;                    // pairs of token and head, keys of a block
-constexpr int kRowsPerWarp = kRows / kWarps;
+constexpr int kKeys = 32;                                // of a block
+constexpr int kRows = 16, kFewRows = 4;                  // pairs of token and head of a unit
 
 __device__ __forceinline__ void copy16(float *dst, const void *src, bool real)
 {
@@ -16,20 +16,22 @@ __device__ __forceinline__ void copy16(float *dst, const void *src, bool real)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
-// out[row, col] (+)= over a tile of 32 keys: a warp scores four rows with a key per lane, a thread sums one or two columns for all rows.
+// out[row, col] (+)= over a tile of 32 keys: a warp scores a quarter of the rows with a key per lane, a thread sums one or two columns for all rows.
+// Single tokens of up to four heads per key / value head take four rows, a warp each: with sixteen a block of keys took 11 us instead of 2.
 // Four threads fetch a key and its value; with 16-byte rows in f32 (WIDE) asynchronously, a tile ahead.  Single tokens are bound by these loads,
 // portions by the multiply-adds' operands from shared memory.
-template <typename T, int COLS, bool WIDE>               // COLS: columns per thread, heads of up to 128 * COLS
+template <typename T, int ROWS, int COLS, bool WIDE>     // COLS: columns per thread, heads of up to 128 * COLS
 __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
 {
+    constexpr int kRowsPerWarp = ROWS / kWarps;
     extern __shared__ __align__(16) float s_mem[];
     __shared__ unsigned long long s_walk[40];
-    __shared__ float s_p[kRows][kKeys], s_scale[kRows];
+    __shared__ float s_p[ROWS][kKeys], s_scale[ROWS];
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, d = a.d, d4 = (d + 3) / 4 * 4, pitch = d4 + 4, tile = 2 * kKeys * pitch;
-    float *s_q = s_mem, *s_tiles = s_q + kRows * d4;
+    float *s_q = s_mem, *s_tiles = s_q + ROWS * d4;
     pdl_launch_dependents();
     pdl_wait();
-    Walk<kRows, kKeys, 1> walk;
+    Walk<ROWS, kKeys, 0> walk;
     walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 
@@ -58,12 +60,12 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
         };
         __syncthreads();
         if (WIDE && g.begin < g.end) fetch(g.begin);
-        for (uint32_t r = warp; r < kRows; r += kWarps) {
+        for (uint32_t r = warp; r < ROWS; r += kWarps) {
             const uint32_t token = r / g.heads, head = r - token * g.heads;
             const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (r < pairs ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d;
             for (uint32_t c = lane; c < d4; c += 32) s_q[r * d4 + c] = r < pairs && c < d ? to_f32(src[c]) : 0.f;
         }
-        float m[kRowsPerWarp], l[kRowsPerWarp], acc[COLS][kRows];
+        float m[kRowsPerWarp], l[kRowsPerWarp], acc[COLS][ROWS];
         int pos[kRowsPerWarp];
 #pragma unroll
         for (int i = 0; i < kRowsPerWarp; i++) {
@@ -75,7 +77,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
 #pragma unroll
         for (int c = 0; c < COLS; c++)
 #pragma unroll
-            for (int r = 0; r < kRows; r++) acc[c][r] = 0.f;
+            for (int r = 0; r < ROWS; r++) acc[c][r] = 0.f;
 
         for (uint32_t kb = g.begin; kb < g.end; kb++) {
             if constexpr (WIDE) {
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
 #pragma unroll
             for (int i = 0; i < kRowsPerWarp; i++) {
                 const bool seen = there && key <= pos[i] && (!a.window || key > pos[i] - (int)a.window);
-                hidden |= !seen;
+                hidden |= there && !seen && warp * kRowsPerWarp + i < pairs;        // keys that are not there are zeros
                 const float x = seen ? s[i] * a.scale_log2 : -INFINITY, top = fmaxf(m[i], warp_max(x));
                 // a row whose seen scores are all -inf has no weight, like one that sees nothing; NaN stays NaN
                 const float w = !seen ? 0.f : x != x ? x : top > -INFINITY ? exp2f(x - top) : 0.f, keep = top > -INFINITY ? exp2f(m[i] - top) : 1.f;
@@ -122,13 +124,13 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
                 const uint32_t col = t + c * kThreads;
                 if (col >= d) continue;
 #pragma unroll
-                for (int r = 0; r < kRows; r++) acc[c][r] *= s_scale[r];
+                for (int r = 0; r < ROWS; r++) acc[c][r] *= s_scale[r];
                 for (int j = 0; j < kKeys; j += 4) {
                     float v[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) v[e] = s_v[(j + e) * pitch + col];
 #pragma unroll
-                    for (int r = 0; r < kRows; r++) {
+                    for (int r = 0; r < ROWS; r++) {
                         const float4 p = *reinterpret_cast<const float4 *>(&s_p[r][j]);
                         if (masked) {                    // what a row does not see stays out, infinities and NaN too
                             acc[c][r] += (p.x != 0.f ? p.x * v[0] : 0.f) + (p.y != 0.f ? p.y * v[1] : 0.f) + (p.z != 0.f ? p.z * v[2] : 0.f) + (p.w != 0.f ? p.w * v[3] : 0.f);
@@ -147,13 +149,13 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
                 for (int i = 0; i < kRowsPerWarp; i++) s_scale[warp * kRowsPerWarp + i] = l[i] == 0.f ? 0.f : 1.f / l[i];
             __syncthreads();
         }
-        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kRows * (d + 2);
+        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * ROWS * (d + 2);
 #pragma unroll
         for (int c = 0; c < COLS; c++) {
             const uint32_t col = t + c * kThreads;
             if (col >= d) continue;
 #pragma unroll
-            for (uint32_t r = 0; r < kRows; r++) {
+            for (uint32_t r = 0; r < ROWS; r++) {
                 if (r >= pairs) break;
                 const uint32_t token = r / g.heads, head = r - token * g.heads;
                 if (whole) static_cast<T *>(a.out)[(size_t)(g.row0 + token) * a.out_pitch + (g.head0 + head) * d + col] = rounded<T>(acc[c][r] * s_scale[r]);
@@ -164,8 +166,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
             if (lane == 0)
 #pragma unroll
                 for (int i = 0; i < kRowsPerWarp; i++) {
-                    part[kRows * d + 2 * (warp * kRowsPerWarp + i)] = m[i];
-                    part[kRows * d + 2 * (warp * kRowsPerWarp + i) + 1] = l[i];
+                    part[ROWS * d + 2 * (warp * kRowsPerWarp + i)] = m[i];
+                    part[ROWS * d + 2 * (warp * kRowsPerWarp + i) + 1] = l[i];
                 }
             if (t == 0) name_part(a, blockIdx.x, g);
         }
@@ -174,18 +176,23 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
 
 constexpr uint32_t kCtas = 148 * 2;                      // two tiles of 128 columns twice: two CTAs per SM
 
-template <typename T>
-int launch_attend(AttendArgs a, cudaStream_t stream)
+template <typename T, int ROWS>
+int launch_rows(const AttendArgs &a, cudaStream_t stream)
 {
     const uint32_t d4 = (a.d + 3) / 4 * 4;
     const bool wide = sizeof(T) == 4 && a.d % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
-    const size_t smem = ((size_t)kRows * d4 + (wide ? 2 : 1) * 2 * kKeys * (d4 + 4)) * sizeof(float);
-    auto *kernel = a.d <= 128 ? attend_kernel<T, 1, false> : attend_kernel<T, 2, false>;
+    const size_t smem = ((size_t)ROWS * d4 + (wide ? 2 : 1) * 2 * kKeys * (d4 + 4)) * sizeof(float);
+    auto *kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, false> : attend_kernel<T, ROWS, 2, false>;
     if constexpr (sizeof(T) == 4)
-        if (wide) kernel = a.d <= 128 ? attend_kernel<T, 1, true> : attend_kernel<T, 2, true>;
+        if (wide) kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, true> : attend_kernel<T, ROWS, 2, true>;
     if (int rc = allow_smem(kernel, smem)) return rc;
     if (int rc = launch(kernel, dim3(kCtas), dim3(kThreads), smem, stream, a)) return rc;
-    return launch_merge<T, kRows>(a, kCtas, kRows, stream);
+    return launch_merge<T, ROWS>(a, kCtas, ROWS, stream);
+}
+template <typename T>
+int launch_attend(const AttendArgs &a, uint32_t pairs, cudaStream_t stream)
+{
+    return pairs <= kFewRows ? launch_rows<T, kFewRows>(a, stream) : launch_rows<T, kRows>(a, stream);
 }
 
 }  // namespace
@@ -232,9 +239,9 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
     }
     room(kCtas);
     switch (dtype) {
-        case MGQ_FMT_F32: return launch_attend<float>(a, s);
-        case MGQ_FMT_F16: return launch_attend<__half>(a, s);
-        default: return launch_attend<__nv_bfloat16>(a, s);
+        case MGQ_FMT_F32: return launch_attend<float>(a, pairs, s);
+        case MGQ_FMT_F16: return launch_attend<__half>(a, pairs, s);
+        default: return launch_attend<__nv_bfloat16>(a, pairs, s);
     }
 }
 
