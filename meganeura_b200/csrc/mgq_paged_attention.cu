@@ -94,17 +94,21 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
             const float *s_k = s_tiles + (WIDE && kb & 1u ? tile : 0), *s_v = s_k + kKeys * pitch;
             const int key = (int)(kb * kKeys + lane);
             const bool there = key < g.len && g.table[(uint32_t)key >> a.page_shift] < a.pages;
-            float s[kRowsPerWarp];
+            float s[kRowsPerWarp], s2[kRowsPerWarp];     // two chains of multiply-adds per row
 #pragma unroll
-            for (int i = 0; i < kRowsPerWarp; i++) s[i] = 0.f;
+            for (int i = 0; i < kRowsPerWarp; i++) s[i] = s2[i] = 0.f;
+#pragma unroll 4
             for (uint32_t c = 0; c < d4; c += 4) {
                 const float4 kv = *reinterpret_cast<const float4 *>(s_k + lane * pitch + c);
 #pragma unroll
                 for (int i = 0; i < kRowsPerWarp; i++) {
                     const float4 qv = *reinterpret_cast<const float4 *>(s_q + (warp * kRowsPerWarp + i) * d4 + c);
-                    s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[i]))));
+                    s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, s[i]));
+                    s2[i] = fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s2[i]));
                 }
             }
+#pragma unroll
+            for (int i = 0; i < kRowsPerWarp; i++) s[i] += s2[i];
             bool hidden = false;                         // some pair of this tile is masked
 #pragma unroll
             for (int i = 0; i < kRowsPerWarp; i++) {
@@ -125,6 +129,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
                 if (col >= d) continue;
 #pragma unroll
                 for (int r = 0; r < ROWS; r++) acc[c][r] *= s_scale[r];
+#pragma unroll 2
                 for (int j = 0; j < kKeys; j += 4) {
                     float v[4];
 #pragma unroll
@@ -174,25 +179,35 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     }
 }
 
-constexpr uint32_t kCtas = 148 * 2;                      // two tiles of 128 columns twice: two CTAs per SM
+bool wide_rows(const AttendArgs &a, int dtype)
+{
+    return dtype == MGQ_FMT_F32 && a.d % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
+}
+size_t smem_bytes(uint32_t rows, uint32_t d, bool wide)
+{
+    const uint32_t d4 = (d + 3) / 4 * 4;
+    return ((size_t)rows * d4 + (wide ? 2 : 1) * 2 * kKeys * (d4 + 4)) * sizeof(float);
+}
+// As many CTAs as their shared memory lets an SM hold, four at most (registers); a form with fewer keys in flight than another one must not need a larger workspace.
+uint32_t plain_ctas(uint32_t rows, uint32_t d) { return 148 * min(4u, (uint32_t)(224 * 1024 / (smem_bytes(rows, d, true) + 3584))); }
 
 template <typename T, int ROWS>
-int launch_rows(const AttendArgs &a, cudaStream_t stream)
+int launch_rows(const AttendArgs &a, int dtype, cudaStream_t stream)
 {
-    const uint32_t d4 = (a.d + 3) / 4 * 4;
-    const bool wide = sizeof(T) == 4 && a.d % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
-    const size_t smem = ((size_t)ROWS * d4 + (wide ? 2 : 1) * 2 * kKeys * (d4 + 4)) * sizeof(float);
+    const bool wide = wide_rows(a, dtype);
+    const uint32_t ctas = plain_ctas(ROWS, a.d);
+    const size_t smem = smem_bytes(ROWS, a.d, wide);
     auto *kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, false> : attend_kernel<T, ROWS, 2, false>;
     if constexpr (sizeof(T) == 4)
         if (wide) kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, true> : attend_kernel<T, ROWS, 2, true>;
     if (int rc = allow_smem(kernel, smem)) return rc;
-    if (int rc = launch(kernel, dim3(kCtas), dim3(kThreads), smem, stream, a)) return rc;
-    return launch_merge<T, ROWS>(a, kCtas, ROWS, stream);
+    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem, stream, a)) return rc;
+    return launch_merge<T, ROWS>(a, ctas, ROWS, stream);
 }
 template <typename T>
-int launch_attend(const AttendArgs &a, uint32_t pairs, cudaStream_t stream)
+int launch_attend(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t stream)
 {
-    return pairs <= kFewRows ? launch_rows<T, kFewRows>(a, stream) : launch_rows<T, kRows>(a, stream);
+    return pairs <= kFewRows ? launch_rows<T, kFewRows>(a, dtype, stream) : launch_rows<T, kRows>(a, dtype, stream);
 }
 
 }  // namespace
@@ -202,7 +217,7 @@ size_t paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t hea
 {
     (void)heads; (void)kv_heads; (void)max_fresh;
     auto bytes = [&](uint32_t ctas, size_t rows) { return ctas * 2 * (sizeof(PartHead) + rows * (head_dim + 2) * sizeof(float)); };
-    const size_t plain = bytes(kCtas, kRows);
+    const size_t plain = max(bytes(plain_ctas(kRows, head_dim), kRows), bytes(plain_ctas(kFewRows, head_dim), kFewRows));
     return dtype == MGQ_FMT_F32 ? plain : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
 }
 
@@ -237,11 +252,11 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
         a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);
         return launch_prefill(a, dtype, s);
     }
-    room(kCtas);
+    room(plain_ctas(pairs <= kFewRows ? kFewRows : kRows, head_dim));
     switch (dtype) {
-        case MGQ_FMT_F32: return launch_attend<float>(a, pairs, s);
-        case MGQ_FMT_F16: return launch_attend<__half>(a, pairs, s);
-        default: return launch_attend<__nv_bfloat16>(a, pairs, s);
+        case MGQ_FMT_F32: return launch_attend<float>(a, dtype, pairs, s);
+        case MGQ_FMT_F16: return launch_attend<__half>(a, dtype, pairs, s);
+        default: return launch_attend<__nv_bfloat16>(a, dtype, pairs, s);
     }
 }
 
