@@ -179,6 +179,180 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     }
 }
 
+// ---------------------------------------------------------------- many new tokens in f32
+// 64 pairs of token and head against 64 keys at a time, as two register-tiled products: a thread has four rows and four keys of the scores (eight
+// 16-byte loads from shared memory for 64 multiply-adds), then the same rows and eight columns of the sums (twenty for 128), so the multiply-add units bound it.
+// Sixteen lanes share a row's maximum and sum by shuffles.  Keys are fetched while values are used and the other way around.
+constexpr int kTileThreads = 256, kTileRows = 64, kTileKeys = 64, kTilePitch = kTileKeys + 4;
+constexpr uint32_t kTileCtas = 148;
+size_t tile_smem(uint32_t d) { return ((size_t)(kTileRows + 2 * kTileKeys) * (d + 4) + kTileRows * kTilePitch) * sizeof(float); }
+
+template <int COLS>                                      // groups of four columns of a thread: heads of up to 64 * COLS
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const AttendArgs a)
+{
+    extern __shared__ __align__(16) float s_mem[];
+    __shared__ unsigned long long s_walk[40];
+    const uint32_t t = threadIdx.x, d = a.d, pitch = d + 4, tr = t / 16, tc = t % 16;
+    float *s_q = s_mem, *s_k = s_q + kTileRows * pitch, *s_v = s_k + kTileKeys * pitch, *s_p = s_v + kTileKeys * pitch;
+    pdl_launch_dependents();
+    pdl_wait();
+    Walk<kTileRows, kTileKeys, 1> walk;
+    walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
+    if (t == 0) clear_parts(a, blockIdx.x);
+
+    Segment g;
+    while (walk.next(a, g)) {
+        const uint32_t pairs = g.tokens * g.heads;
+        // four threads fetch a key or a value; those that are not there are zeros
+        auto fetch = [&](uint32_t kb, const void *from, float *to) {
+            const uint32_t j = t / 4, key = kb * kTileKeys + j;
+            const uint32_t page = (int)key < g.len ? g.table[key >> a.page_shift] : 0xFFFFFFFFu;
+            const bool real = page < a.pages;
+            const float *src = static_cast<const float *>(from) + (real ? ((((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * d : 0);
+            for (uint32_t c = t % 4 * 4; c < d; c += 16) copy16(to + j * pitch + c, src + c, real);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        __syncthreads();                                 // the unit before is done with shared memory
+        if (g.begin < g.end) {
+            fetch(g.begin, a.k, s_k);
+            fetch(g.begin, a.v, s_v);
+        }
+        for (uint32_t r = t / 32; r < kTileRows; r += kTileThreads / 32) {
+            const uint32_t token = r / g.heads, head = r - token * g.heads;
+            const float *src = static_cast<const float *>(a.q) + (size_t)(g.row0 + (r < pairs ? token : 0)) * a.q_pitch + (size_t)(g.head0 + head) * d;
+            for (uint32_t c = t % 32; c < d; c += 32) s_q[r * pitch + c] = r < pairs ? src[c] * a.scale_log2 : 0.f;
+        }
+        float m[4], l[4], o[4][COLS][4];
+        int pos[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t r = tr * 4 + i;
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+            pos[i] = r < pairs ? g.pos0 + (int)(r / g.heads) : -1;
+#pragma unroll
+            for (int c = 0; c < COLS; c++) o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.f;
+        }
+        const int last_pos = g.pos0 + (int)g.tokens - 1;
+        for (uint32_t kb = g.begin; kb < g.end; kb++) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");           // the keys; the values may be on their way
+            __syncthreads();
+            float s[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll 2
+            for (uint32_t c = 0; c < d; c += 4) {
+                float4 q[4], k[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[i] = *reinterpret_cast<const float4 *>(s_q + (tr * 4 + i) * pitch + c);
+#pragma unroll
+                for (int j = 0; j < 4; j++) k[j] = *reinterpret_cast<const float4 *>(s_k + (tc + 16 * j) * pitch + c);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] = fmaf(q[i].x, k[j].x, fmaf(q[i].y, k[j].y, fmaf(q[i].z, k[j].z, fmaf(q[i].w, k[j].w, s[i][j]))));
+            }
+            __syncthreads();                             // the keys have been used
+            if (kb + 1 < g.end) fetch(kb + 1, a.k, s_k);
+            else                asm volatile("cp.async.commit_group;" ::: "memory");
+            const int key0 = (int)(kb * kTileKeys);
+            bool hidden = false;
+            // everything is there and seen: the last key by the first token, the first one by the last
+            bool there[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int key = key0 + (int)tc + 16 * j;
+                there[j] = key < g.len && g.table[(uint32_t)key >> a.page_shift] < a.pages;
+            }
+            if (!__syncthreads_and(there[0] && there[1] && there[2] && there[3] && key0 + kTileKeys - 1 <= g.pos0 && (!a.window || key0 > last_pos - (int)a.window))) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int key = key0 + (int)tc + 16 * j;
+                        const bool seen = there[j] && key <= pos[i] && (!a.window || key > pos[i] - (int)a.window);
+                        hidden |= there[j] && !seen && tr * 4 + i < pairs;
+                        s[i][j] = seen ? s[i][j] : -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float top = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+#pragma unroll
+                for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                top = fmaxf(m[i], top);
+                const float base = top == -INFINITY ? 0.f : top, keep = exp2f(m[i] - base);
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] = exp2f(s[i][j] - base);     // 0 where nothing is seen, NaN stays
+                    sum += s[i][j];
+                    s_p[(tr * 4 + i) * kTilePitch + tc + 16 * j] = s[i][j];
+                }
+                l[i] = l[i] * keep + sum;                // of this lane; the sixteen are added at the end
+                m[i] = top;
+#pragma unroll
+                for (int c = 0; c < COLS; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[i][c][e] *= keep;
+            }
+            asm volatile("cp.async.wait_group 1;" ::: "memory");           // the values; the next keys may be on their way
+            const bool masked = __syncthreads_or(hidden);
+            auto sums = [&](auto product) {
+#pragma unroll 2
+                for (int j = 0; j < kTileKeys; j += 4) {
+                    float4 p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[i] = *reinterpret_cast<const float4 *>(s_p + (tr * 4 + i) * kTilePitch + j);
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) {
+                        const uint32_t col = tc * 4 + 64 * c;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float4 v = col < d ? *reinterpret_cast<const float4 *>(s_v + (j + e) * pitch + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const float w = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+                                product(o[i][c][0], w, v.x);
+                                product(o[i][c][1], w, v.y);
+                                product(o[i][c][2], w, v.z);
+                                product(o[i][c][3], w, v.w);
+                            }
+                        }
+                    }
+                }
+            };
+            // what a row does not see stays out, infinities and NaN too
+            if (masked) sums([](float &x, float w, float v) { x += w != 0.f ? w * v : 0.f; });
+            else        sums([](float &x, float w, float v) { x = fmaf(w, v, x); });
+            __syncthreads();                             // the values have been used
+            if (kb + 1 < g.end) fetch(kb + 1, a.v, s_v);
+            else                asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        const bool whole = g.first && g.last;
+        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kTileRows * (d + 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t r = tr * 4 + i, token = r / g.heads, head = r - token * g.heads;
+            float sum = l[i];
+#pragma unroll
+            for (int x = 1; x < 16; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (r < pairs) {
+                const float scale = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+                float *dst = whole ? static_cast<float *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d : part + r * d;
+#pragma unroll
+                for (int c = 0; c < COLS; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (tc * 4 + 64 * c < d) dst[tc * 4 + 64 * c + e] = o[i][c][e] * scale;
+                if (!whole && tc == 0) *reinterpret_cast<float2 *>(part + kTileRows * d + 2 * r) = make_float2(m[i], sum);
+            }
+        }
+        if (!whole && t == 0) name_part(a, blockIdx.x, g);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 bool wide_rows(const AttendArgs &a, int dtype)
 {
     return dtype == MGQ_FMT_F32 && a.d % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
@@ -209,6 +383,13 @@ int launch_attend(const AttendArgs &a, int dtype, uint32_t pairs, cudaStream_t s
 {
     return pairs <= kFewRows ? launch_rows<T, kFewRows>(a, dtype, stream) : launch_rows<T, kRows>(a, dtype, stream);
 }
+int launch_tile(const AttendArgs &a, cudaStream_t stream)
+{
+    auto *kernel = a.d <= 64 ? attend_tile_kernel<1> : attend_tile_kernel<2>;
+    if (int rc = allow_smem(kernel, tile_smem(a.d))) return rc;
+    if (int rc = launch(kernel, dim3(kTileCtas), dim3(kTileThreads), tile_smem(a.d), stream, a)) return rc;
+    return launch_merge<float, kTileRows>(a, kTileCtas, kTileRows, stream);
+}
 
 }  // namespace
 
@@ -218,7 +399,7 @@ size_t paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t hea
     (void)heads; (void)kv_heads; (void)max_fresh;
     auto bytes = [&](uint32_t ctas, size_t rows) { return ctas * 2 * (sizeof(PartHead) + rows * (head_dim + 2) * sizeof(float)); };
     const size_t plain = max(bytes(plain_ctas(kRows, head_dim), kRows), bytes(plain_ctas(kFewRows, head_dim), kFewRows));
-    return dtype == MGQ_FMT_F32 ? plain : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
+    return dtype == MGQ_FMT_F32 ? plain + bytes(kTileCtas, head_dim <= 128 ? kTileRows : 0) : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
 }
 
 int launch_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
@@ -252,7 +433,17 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
         a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);
         return launch_prefill(a, dtype, s);
     }
-    room(plain_ctas(pairs <= kFewRows ? kFewRows : kRows, head_dim));
+    const uint32_t few = pairs <= kFewRows ? kFewRows : kRows, ctas = plain_ctas(few, head_dim);
+    room(ctas);
+    if (pairs > kRows && head_dim <= 128 && wide_rows(a, dtype)) {
+        a.rows_to = kRows;
+        if (int rc = launch_attend<float>(a, dtype, kRows, s)) return rc;
+        a.rows_from = kRows + 1;
+        a.rows_to = 0xFFFFFFFFu;
+        a.heads = reinterpret_cast<PartHead *>(a.parts + (size_t)ctas * 2 * few * (head_dim + 2));
+        a.parts = reinterpret_cast<float *>(a.heads + 2 * kTileCtas);
+        return launch_tile(a, s);
+    }
     switch (dtype) {
         case MGQ_FMT_F32: return launch_attend<float>(a, dtype, pairs, s);
         case MGQ_FMT_F16: return launch_attend<__half>(a, dtype, pairs, s);

@@ -271,7 +271,8 @@ def test_attention_of_long_sequences_is_split_and_joined():
         check_attention(dtype, q, k, v, table, starts, lengths, run(q, k, v, table, starts, lengths, max(fresh)), d ** -0.5)
 
 
-@pytest.mark.parametrize("dtype,heads,kv_heads,d,window", [("bf16", 8, 2, 128, 0), ("f16", 6, 3, 64, 0), ("bf16", 8, 2, 80, 700), ("f16", 3, 1, 64, 100)])
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,window", [("bf16", 8, 2, 128, 0), ("f16", 6, 3, 64, 0), ("bf16", 8, 2, 80, 700), ("f16", 3, 1, 64, 100),
+                                                                 ("f32", 4, 1, 128, 0), ("f32", 3, 3, 52, 300)])
 def test_attention_of_long_portions(dtype, heads, kv_heads, d, window):
     """Enough work for several units per CTA and many blocks of keys per unit.  The oracle takes a sample of the rows."""
     rng = np.random.default_rng(17)
