@@ -272,12 +272,14 @@ int mgq_argmax(const float *logits, uint32_t n, void *workspace, uint32_t *out_t
  * mgq_paged_append: rows of k and v into the cache rows slots[r] (MGQ_NO_SLOT: not written), with theta > 0 k rotated by positions[r]
  *   (half-split pairs, angle = position * theta^(-2i/head_dim) in 64 bits), and rows of q likewise into q_out [rows, q_heads * head_dim]
  *   (q may be NULL: keys and values only).  Sources are f32 or of the cache's type; their rows are `pitch` elements apart.  Values
- *   are rounded to nearest.  Slots must differ from one another, else which row stays is open.
+ *   are rounded to nearest.  Slots must differ from one another, else what the cache row holds is open.
  * mgq_paged_attention: each new token's query heads over the tokens of its sequence up to itself, with window > 0 over the last
  *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  What a row does not
  *   see has no part in it, whatever it holds; a row that sees nothing is zero; rows behind the last sequence are left as they are.  max_fresh: no sequence has more
- *   new tokens in this step (it chooses kernels; more are not computed).  head_dim at most 256.  `workspace`: mgq_paged_attention_workspace(...) bytes for
+ *   new tokens in this step (it chooses kernels; where it does not hold the call takes longer).  A row whose seen scores are all -inf is zero, too.  head_dim at most 256.  `workspace`: mgq_paged_attention_workspace(...) bytes for
  *   the same arguments, 16-byte aligned, in any state; calls that may run at the same time (two streams, two graphs) need one each.
+ * Calls that change one pool or table must be ordered on one stream, outputs must not overlap inputs (q_out may be q).  Waits inside the kernels are bounded; one that
+ * ran out shows in mgq_device_status.
  * All need table_width * page_size below 2^30, the number of rows below 2^31, and at most MGQ_PAGED_MAX_SEQUENCES sequences. */
 #define MGQ_NO_SLOT  0xFFFFFFFFu
 #define MGQ_NO_PAGE  0xFFFFFFFFu
@@ -298,7 +300,7 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
                         uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
 
 /* mgq_token_probs: out[r, :] = softmax(logits[r, :] / temperature[r]); a temperature that is not above 0 gives 1 to the lowest index among the
- *   largest logits (temperature NULL: 1 everywhere).  NaN logits count as -inf; a row of them alone is zero.  Where the largest is +inf those that are share the row.
+ *   largest logits (temperature NULL: 1 everywhere).  out may be logits.  NaN logits count as -inf; a row of them alone is zero.  Where the largest is +inf those that are share the row.
  * mgq_verify_drafts: speculative sampling.  Sequence s fed its last token and then its drafts: rows [starts[s], starts[s + 1]), tokens[r] the
  *   token of row r.  target[r, :] are the target's probabilities behind row r, draft[r, :] those that tokens[r + 1] was drawn from (the
  *   last row of a sequence is not read), or draft NULL where drafts were chosen outright.  Draft by draft, tokens[r + 1] is kept while

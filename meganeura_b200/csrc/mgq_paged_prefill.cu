@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     }
                     __syncwarp();                        // the next columns are read by the whole warp
                 }
-                bad = bad && row < pairs;
+                bad = bad && row < pairs && l == l;      // a NaN among the seen scores makes all of the row NaN, as it should be
                 if (!alone && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(m, l);
                 for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
                     const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;

@@ -285,6 +285,42 @@ def test_attention_of_long_portions(dtype, heads, kv_heads, d, window):
             check_attention(dtype, q[r:r + 1], k, v, table[s:s + 1], [0, 1], [n], got[r:r + 1], d ** -0.5, window)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-35])
+def test_attention_with_any_scale(dtype, scale):
+    rng = np.random.default_rng(21)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, 8, 2, 64, 16, [100, 30], [1, 80])
+    check_attention(dtype, q, k, v, table, starts, lengths, run(q, k, v, table, starts, lengths, 80, scale=scale), scale)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d", [("bf16", 300, 1, 64), ("f32", 130, 1, 32), ("f16", 256, 2, 128)])
+def test_attention_of_very_many_heads_per_key_head(dtype, heads, kv_heads, d):
+    rng = np.random.default_rng(22)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 16, [70, 0], [1, 3])
+    check_attention(dtype, q, k, v, table, starts, lengths, run(q, k, v, table, starts, lengths, 3), d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 6, 200])
+def test_attention_hands_nan_on_to_the_rows_that_see_it(dtype, fresh):
+    """NaN in a query makes its row NaN; in a key all heads and rows that see it; neither reaches another row."""
+    import torch
+    rng = np.random.default_rng(23)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, 4, 2, 128, 16, [90, 50], [fresh, fresh])
+    clean = run(q, k, v, table, starts, lengths, fresh)
+    q[fresh // 2, 1] = float("nan")
+    got = run(q, k, v, table, starts, lengths, fresh)
+    assert torch.isnan(got[fresh // 2, 1]).all()
+    got[fresh // 2, 1] = clean[fresh // 2, 1]
+    assert torch.equal(got, clean)
+    q[fresh // 2, 1] = 0.5
+    clean = run(q, k, v, table, starts, lengths, fresh)
+    k[table[0, 2], 3, 0, 5] = float("nan")
+    got = run(q, k, v, table, starts, lengths, fresh)
+    assert torch.isnan(got[:fresh, :2]).all()                      # the heads of the first key head
+    assert torch.equal(got[:fresh, 2:], clean[:fresh, 2:]) and torch.equal(got[fresh:], clean[fresh:])
+
+
 def test_attention_with_many_sequences():
     rng = np.random.default_rng(9)
     cached, fresh = rng.integers(0, 40, 4096), rng.integers(0, 3, 4096)
@@ -326,6 +362,15 @@ def test_token_probs(rows, vocab, pad):
     assert off[at] <= bound[at], (at, host(got)[at], want[at])
     assert (out[:, vocab:] == 5.0).all()
     assert torch.equal(ops.token_probs(logits), ops.token_probs(logits, torch.ones(rows, device="cuda")))
+
+
+def test_token_probs_in_place():
+    import torch
+    from meganeura_b200 import ops
+    for rows, vocab in ((3, 999), (2, 5000), (5, 40000)):
+        x = torch.randn(rows, vocab, device="cuda")
+        want = ops.token_probs(x)
+        assert torch.equal(ops.token_probs(x, out=x), want) and x.data_ptr() == ops.token_probs(x, out=x).data_ptr()
 
 
 def test_token_probs_of_rows_with_infinities_nan_and_ties():
