@@ -201,11 +201,13 @@ struct VerifyArgs {
     uint32_t target_pitch, draft_pitch, rows, vocab;
 };
 
-__device__ __forceinline__ double mass(float p) { return p > 0.f && p <= FLT_MAX ? (double)p : 0.0; }
+// What counts of an entry: negative ones, infinities and NaN are nothing.  Positive floats are in order as integers, negative ones behind them all.
+__device__ __forceinline__ float mass(float p) { return __float_as_uint(p) <= 0x7F7FFFFFu ? p : 0.f; }
 
 constexpr uint32_t kChunks = 64;                         // of a warp's piece, in the search
+constexpr int kBatch = 4;                                // groups of four entries of either row that a thread reads at once
 template <bool WIDE>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs a)
 {
     __shared__ double s_sum[kWarps];
     __shared__ double x_sum;
@@ -253,22 +255,35 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a)
     // first the rest that the draft leaves over; where that is nothing, the target's own row
     for (int pass = all ? 1 : 0; pass < 2; pass++) {
         const bool rest = pass == 0;
-        auto weights = [&](uint32_t c, uint32_t w1, double (&w)[4]) {
-            float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
-            read4<WIDE, false>(p, c, w1, 0.f, x);
-            if (rest && q) read4<WIDE, false>(q, c, w1, 0.f, y);
+        auto read = [&](uint32_t c, uint32_t c1, float (&x)[4], float (&y)[4]) {
+            read4<WIDE, false>(p, c, c1, 0.f, x);
+            if (rest && q) read4<WIDE, false>(q, c, c1, 0.f, y);
+        };
+        // x - min(x, y) in 64 bits is exact, and 0 where y is larger
+        auto weigh = [&](uint32_t c, const float (&x)[4], const float (&y)[4], double (&w)[4]) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                w[e] = mass(x[e]);
-                if (rest) w[e] = q ? fmax(w[e] - mass(y[e]), 0.0) : c + e == taboo ? 0.0 : w[e];
+                const float some = mass(x[e]);
+                w[e] = (double)some;
+                if (rest) w[e] = q ? w[e] - (double)fminf(some, mass(y[e])) : c + e == taboo ? 0.0 : w[e];
             }
         };
+        auto weights = [&](uint32_t c, uint32_t c1, double (&w)[4]) {
+            float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
+            read(c, c1, x, y);
+            weigh(c, x, y, w);
+        };
         double sum = 0.0;
-#pragma unroll 8
-        for (uint32_t c = w0 + 4 * lane; c < w1; c += 128) {
-            double w[4];
-            weights(c, w1, w);
-            sum += (w[0] + w[1]) + (w[2] + w[3]);
+        for (uint32_t c0 = w0 + 4 * lane; c0 < w1; c0 += 128 * kBatch) {
+            float x[kBatch][4], y[kBatch][4] = {};
+#pragma unroll
+            for (int k = 0; k < kBatch; k++) read(c0 + 128 * k, w1, x[k], y[k]);
+#pragma unroll
+            for (int k = 0; k < kBatch; k++) {
+                double w[4];
+                weigh(c0 + 128 * k, x[k], y[k], w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+            }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
