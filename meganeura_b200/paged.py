@@ -59,12 +59,16 @@ def _pitch(name: str, t, device: int, inner: int) -> int:
         return inner
     if t.get_device() != device:
         raise ValueError(f"{name} must be on cuda:{device}, not {t.device}")
-    run = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size > 1 and stride != run:
-            raise ValueError(f"the rows of {name} must be contiguous")
-        run *= size
-    pitch = t.stride(0) if t.shape[0] > 1 else inner
+    shape, strides = t.shape, t.stride()
+    if shape[0] > 1 and strides[-1] == 1 and (len(shape) == 2 or len(shape) == 3 and strides[1] == shape[2]):       # what a slice of wider rows has
+        pitch = strides[0]
+    else:
+        run = 1
+        for size, stride in zip(reversed(shape[1:]), reversed(strides[1:])):
+            if size > 1 and stride != run:
+                raise ValueError(f"the rows of {name} must be contiguous")
+            run *= size
+        pitch = strides[0] if shape[0] > 1 else inner
     if not inner <= pitch < 1 << 32:
         raise ValueError(f"the rows of {name} are {pitch} elements apart")
     return pitch
