@@ -79,7 +79,7 @@ int mgq_paged_append(const void *q, const void *k, const void *v, int src_dtype,
 size_t mgq_paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh, int dtype)
 {
     if (!known(dtype) || heads == 0 || max_fresh == 0 || check_heads("paged_attention_workspace", heads, kv_heads, head_dim)) return 0;
-    return paged_attention_workspace(heads, kv_heads, head_dim, max_fresh, dtype);
+    return paged_attention_workspace(head_dim, dtype);
 }
 
 int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,

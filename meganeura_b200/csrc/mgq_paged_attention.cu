@@ -393,10 +393,9 @@ int launch_tile(const AttendArgs &a, cudaStream_t stream)
 
 }  // namespace
 
-// Parts of the kernel that serves these arguments (the largest of them where the alignment decides).
-size_t paged_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh, int dtype)
+// Parts of the kernels that may serve a call: alignment and lengths decide which.
+size_t paged_attention_workspace(uint32_t head_dim, int dtype)
 {
-    (void)heads; (void)kv_heads; (void)max_fresh;
     auto bytes = [&](uint32_t ctas, size_t rows) { return ctas * 2 * (sizeof(PartHead) + rows * (head_dim + 2) * sizeof(float)); };
     const size_t plain = max(bytes(plain_ctas(kRows, head_dim), kRows), bytes(plain_ctas(kFewRows, head_dim), kFewRows));
     return dtype == MGQ_FMT_F32 ? plain + bytes(kTileCtas, head_dim <= 128 ? kTileRows : 0) : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
