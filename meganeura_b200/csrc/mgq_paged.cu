@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
     extern __shared__ uint32_t s_plan[];
     __shared__ unsigned long long s_warp[kPlanWarps];
     __shared__ uint32_t s_given;
-    uint32_t *s_start = s_plan, *s_before = s_start + a.sequences + 1, *s_held = s_before + a.sequences, *s_got = s_held + a.sequences;
+    uint32_t *s_start = s_plan, *s_before = s_start + a.sequences + 1, *s_held = s_before + a.sequences, *s_got = s_held + a.sequences, *s_cached = s_got + a.sequences;
     const uint32_t t = threadIdx.x, lane = t & 31u, part = blockIdx.y, parts = gridDim.y, threads = blockDim.x, warp = part * (threads / 32) + (t >> 5);
     if (t == 0) s_given = 0;
     pdl_launch_dependents();
@@ -99,17 +99,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
         if (i < each && s < a.sequences) {
             s_before[s] = (uint32_t)before;
             s_held[s] = held[i];
+            s_cached[s] = cached[i];
             s_got[s] = served ? need[i] : 0xFFFFFFFFu;
             if (served && need[i]) atomicMax(&s_given, (uint32_t)before + need[i]);         // those that are served come first
-            if (part == 0) {
-                a.starts[s] = s_start[s];
-                a.lengths[s] = served ? cached[i] + fresh[i] : cached[i];
-            }
+            if (part == 0) a.starts[s] = s_start[s];
         }
         before += need[i];
     }
     if (t == 0) s_start[a.sequences] = last_row;
-    if (parts > 1) cluster_sync();                       // every CTA has read held and free_count
+    if (parts > 1) cluster_sync();                       // every CTA has read cached (which may be lengths), held and free_count
     else           __syncthreads();
     if (part == 0) {
         if (t == 0) {
@@ -117,8 +115,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
             *a.free_count = count - s_given;
             *a.lacking = (uint32_t)min(total > count ? total - count : 0ull, 0xFFFFFFFFull);
         }
-        for (uint32_t s = t; s < a.sequences; s += threads)
-            if (s_got[s] != 0xFFFFFFFFu) a.held[s] = s_held[s] + s_got[s];
+        for (uint32_t s = t; s < a.sequences; s += threads) {
+            const bool served = s_got[s] != 0xFFFFFFFFu;
+            if (served) a.held[s] = s_held[s] + s_got[s];
+            a.lengths[s] = s_cached[s] + (served ? s_start[s + 1] - s_start[s] : 0u);
+        }
     }
     for (uint32_t s = warp; s < a.sequences; s += parts * (threads / 32)) {
         const uint32_t got = s_got[s] == 0xFFFFFFFFu ? 0u : s_got[s];
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
                 if (s_start[mid] <= r) lo = mid;
                 else                   hi = mid;
             }
-            position = a.cached[lo] + r - s_start[lo];
+            position = s_cached[lo] + r - s_start[lo];
             const uint32_t j = position >> a.page_shift;
             if (s_got[lo] != 0xFFFFFFFFu) {
                 const uint32_t page = j < s_held[lo] ? a.table[(size_t)lo * a.table_width + j] : a.free_pages[count - 1 - (s_before[lo] + j - s_held[lo])];
@@ -334,7 +335,7 @@ int launch_paged_plan(const uint32_t *cached, const uint32_t *fresh, uint32_t se
 {
     const PlanArgs a{cached, fresh, sequences, page_size, page_shift(page_size), table, table_width, held, free_count, free_pages, pages, rows, starts, lengths, positions,
                      slots, lacking};
-    const size_t smem = (4 * (size_t)sequences + 1) * 4;
+    const size_t smem = (5 * (size_t)sequences + 1) * 4;
     if (int rc = allow_smem(plan_kernel, smem)) return rc;
     // one CTA while its threads have few rows and its warps few sequences each, a cluster of eight beyond
     const uint32_t threads = plan_threads(sequences, rows), parts = rows <= 2 * threads && sequences <= 2 * threads / 32 ? 1 : 8;

@@ -72,6 +72,8 @@ int mgq_paged_append(const void *q, const void *k, const void *v, int src_dtype,
     if (!(theta >= 0.f) || theta > 1e30f) return fail(MGQ_ERR_SHAPE, "paged_append: theta %g", (double)theta);
     const uintptr_t src = element(src_dtype), dst = element(cache_dtype);
     if (odd(q, src) || odd(k, src) || odd(v, src) || odd(q_out, dst) || odd(k_cache, dst) || odd(v_cache, dst)) return fail(MGQ_ERR_ALIGN, "paged_append: misaligned pointer");
+    if (q && q == q_out && (src_dtype != cache_dtype || (rows > 1 && q_pitch != q_heads * head_dim)))
+        return fail(MGQ_ERR_SHAPE, "paged_append: queries rotated in place must be of the cache's type and dense");
     return launch_paged_append(q, k, v, src_dtype, positions, slots, q_out, k_cache, v_cache, cache_dtype, rows, q_heads, kv_heads, head_dim, q_pitch, k_pitch, v_pitch,
                                (unsigned long long)pages * page_size, theta, stream);
 }

@@ -47,6 +47,10 @@ def verify(**change):
     return _lib.lib.mgq_verify_drafts(*a.values(), None)
 
 
+def test_append_in_place_needs_dense_queries_of_the_caches_type():
+    assert append(q_pitch=600) == SHAPE and append(dtype=1) == SHAPE and append(src=0, dtype=4) == SHAPE
+
+
 @pytest.mark.parametrize("call,change,status", [
     *[(plan, {name: None}, NULL) for name in ("cached", "fresh", "table", "held", "free", "count", "starts", "lengths", "positions", "slots", "lacking")],
     (plan, dict(page_size=12), SHAPE), (plan, dict(page_size=4), SHAPE), (plan, dict(page_size=2048), SHAPE), (plan, dict(pages=0), SHAPE),

@@ -74,6 +74,25 @@ def test_plan_when_pages_run_out_rows_run_out_or_a_row_of_the_table_is_too_narro
     check_plan([2, 8], [5, 1], table, held, free, count, 8, 6)
 
 
+@pytest.mark.parametrize("sequences", [3, 300, 2000])
+def test_plan_of_a_step_whose_lengths_are_the_next_steps_cached_tokens(sequences):
+    from meganeura_b200 import ops
+    rng, page, rows, steps = np.random.default_rng(sequences), 8, 3 * sequences, 4
+    cached, pages, width = rng.integers(0, 20, sequences), 5 * sequences, 6
+    table, held, free, count = pool(rng, cached, page, pages, width)
+    step = ops.PagedStep.empty(sequences, rows)
+    step.lengths.copy_(words(cached))
+    d = [words(x) for x in (table, held, free, [count])]
+    for _ in range(steps):                             # every one in the tensors of the one before
+        fresh = rng.integers(0, 4, sequences)
+        starts, lengths, positions, slots, lacking, table, held, count = PO.plan(cached, fresh, table, held, free, count, page, rows)
+        ops.paged_plan(step.lengths, words(fresh), *d, page, rows, step=step)
+        for name, want in (("starts", starts), ("lengths", lengths), ("positions", positions), ("slots", slots), ("lacking", [lacking])):
+            assert np.array_equal(host(getattr(step, name)), np.asarray(want)), name
+        assert np.array_equal(host(d[0]), table) and np.array_equal(host(d[1]), held) and host(d[3])[0] == count
+        cached = lengths
+
+
 # ---------------------------------------------------------------------------------------------- keys and values into the cache
 
 @pytest.mark.parametrize("src,dtype", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
@@ -112,6 +131,17 @@ def test_append(src, dtype, rows, heads, kv_heads, d, page, theta, layout):
         near(flat[torch.from_numpy(slots[~lost]).cuda()], want[~lost], size[~lost])
         rest = np.setdiff1d(np.arange(pages * page), slots)
         assert (flat[torch.from_numpy(rest).cuda()] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_rotates_queries_in_place(dtype):
+    import torch
+    from meganeura_b200 import ops
+    q, k = (torch.randn(700, h, 64, device="cuda").to(torch_type(dtype)) for h in (6, 2))
+    caches = [torch.zeros(90, 8, 2, 64, dtype=torch_type(dtype), device="cuda") for _ in range(2)]
+    at = words(np.arange(700))
+    want = ops.paged_append(q, k, k, at, at, *caches, theta=1e4)
+    assert ops.paged_append(q, k, k, at, at, *caches, theta=1e4, q_out=q) is q and torch.equal(q, want)
 
 
 def test_append_keeps_infinities_and_nan_as_a_cast_does():
