@@ -298,6 +298,13 @@ bool prefill_takes(const AttendArgs &a, int dtype);
 constexpr uint32_t kPrefillCtas = 148, kPrefillRows = 256;
 int launch_prefill(const AttendArgs &a, int dtype, cudaStream_t stream);
 
+// f32 with heads of up to 128, a multiple of 4, on 16-byte boundaries: up to eight pairs of a sequence per key / value head (mgq_paged_few.cu).
+bool few_takes(const AttendArgs &a, int dtype);
+constexpr uint32_t kFewPairs = 8;
+uint32_t few_ctas(uint32_t rows);                          // rows of a unit: 1, 4 or 8
+size_t few_part_floats(uint32_t rows, uint32_t d);
+int launch_few(const AttendArgs &a, uint32_t rows, cudaStream_t stream);
+
 // {head_dim, kv_heads, pages * page_size} of a cache, for boxes of 64 elements by `tokens` tokens of one head in the 128-byte swizzle.  What
 // lies outside the cache reads as zero.
 struct CacheMaps {

@@ -373,7 +373,11 @@ int launch_rows(const AttendArgs &a, int dtype, cudaStream_t stream)
     const size_t smem = smem_bytes(ROWS, a.d, wide);
     auto *kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, false> : attend_kernel<T, ROWS, 2, false>;
     if constexpr (sizeof(T) == 4)
-        if (wide) kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, true> : attend_kernel<T, ROWS, 2, true>;
+        if (wide) {
+            kernel = attend_kernel<T, ROWS, 2, true>;
+            if constexpr (ROWS > kFewRows)               // few rows of small heads are mgq_paged_few.cu's
+                if (a.d <= 128) kernel = attend_kernel<T, ROWS, 1, true>;
+        }
     if (int rc = allow_smem(kernel, smem)) return rc;
     if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem, stream, a)) return rc;
     return launch_merge<T, ROWS>(a, ctas, ROWS, stream);
@@ -398,7 +402,9 @@ size_t paged_attention_workspace(uint32_t head_dim, int dtype)
 {
     auto bytes = [&](uint32_t ctas, size_t rows) { return ctas * 2 * (sizeof(PartHead) + rows * (head_dim + 2) * sizeof(float)); };
     const size_t plain = max(bytes(plain_ctas(kRows, head_dim), kRows), bytes(plain_ctas(kFewRows, head_dim), kFewRows));
-    return dtype == MGQ_FMT_F32 ? plain + bytes(kTileCtas, head_dim <= 128 ? kTileRows : 0) : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
+    size_t few = 0;
+    for (uint32_t rows : {1u, 4u, 8u}) few = max(few, few_ctas(rows) * 2 * (sizeof(PartHead) + few_part_floats(rows, head_dim) * sizeof(float)));
+    return dtype == MGQ_FMT_F32 ? max(plain, few + bytes(kTileCtas, head_dim <= 128 ? kTileRows : 0)) : max(plain, bytes(decode_ctas(head_dim), kDecodeRows) + bytes(kPrefillCtas, head_dim <= 128 ? kPrefillRows : 0));
 }
 
 int launch_paged_attention(const void *q, const void *k_cache, const void *v_cache, int dtype, const uint32_t *table, const uint32_t *starts, const uint32_t *lengths,
@@ -432,17 +438,20 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
         a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);
         return launch_prefill(a, dtype, s);
     }
-    const uint32_t few = pairs <= kFewRows ? kFewRows : kRows, ctas = plain_ctas(few, head_dim);
-    room(ctas);
-    if (pairs > kRows && head_dim <= 128 && wide_rows(a, dtype)) {
-        a.rows_to = kRows;
-        if (int rc = launch_attend<float>(a, dtype, kRows, s)) return rc;
-        a.rows_from = kRows + 1;
+    if (few_takes(a, dtype) && (pairs <= kFewPairs || pairs > kRows)) {
+        const uint32_t rows = pairs == 1 ? 1 : min(pairs, max(a.group, kFewPairs / 2)) <= 4 ? 4 : 8;
+        room(few_ctas(rows));
+        if (pairs <= kFewPairs) return launch_few(a, rows, s);
+        // both kinds of sequences may be there
+        a.rows_to = kFewPairs;
+        if (int rc = launch_few(a, rows, s)) return rc;
+        a.rows_from = kFewPairs + 1;
         a.rows_to = 0xFFFFFFFFu;
-        a.heads = reinterpret_cast<PartHead *>(a.parts + (size_t)ctas * 2 * few * (head_dim + 2));
+        a.heads = reinterpret_cast<PartHead *>(a.parts + few_ctas(rows) * 2 * few_part_floats(rows, head_dim));
         a.parts = reinterpret_cast<float *>(a.heads + 2 * kTileCtas);
         return launch_tile(a, s);
     }
+    room(plain_ctas(pairs <= kFewRows ? kFewRows : kRows, head_dim));
     switch (dtype) {
         case MGQ_FMT_F32: return launch_attend<float>(a, dtype, pairs, s);
         case MGQ_FMT_F16: return launch_attend<__half>(a, dtype, pairs, s);
