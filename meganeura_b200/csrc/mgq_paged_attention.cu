@@ -17,8 +17,7 @@ __device__ __forceinline__ void copy16(float *dst, const void *src, bool real)
 }
 
 // out[row, col] (+)= over a tile of 32 keys: a warp scores a quarter of the rows with a key per lane, a thread sums one or two columns for all rows.
-// Single tokens of up to four heads per key / value head take four rows, a warp each: with sixteen a block of keys took 11 us instead of 2.
-// Four threads fetch a key and its value; with 16-byte rows in f32 (WIDE) asynchronously, a tile ahead.  Single tokens are bound by these loads,
+// Up to four pairs take four rows, a warp each: with sixteen a block of keys took 11 us instead of 2.  Four threads fetch a key and its value; with 16-byte rows in f32 (WIDE) asynchronously, a tile ahead.  Single tokens are bound by these loads,
 // portions by the multiply-adds' operands from shared memory.
 template <typename T, int ROWS, int COLS, bool WIDE>     // COLS: columns per thread, heads of up to 128 * COLS
 __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
@@ -439,7 +438,8 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
         return launch_prefill(a, dtype, s);
     }
     if (few_takes(a, dtype) && (pairs <= kFewPairs || pairs > kRows)) {
-        const uint32_t rows = pairs == 1 ? 1 : min(pairs, max(a.group, kFewPairs / 2)) <= 4 ? 4 : 8;
+        // eight rows rather than two units of four: 32 sequences of two tokens of four heads took 195 and 255 us
+        const uint32_t rows = pairs == 1 ? 1 : pairs <= 4 ? 4 : 8;
         room(few_ctas(rows));
         if (pairs <= kFewPairs) return launch_few(a, rows, s);
         // both kinds of sequences may be there

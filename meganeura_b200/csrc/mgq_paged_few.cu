@@ -3,7 +3,9 @@
 // Every key and value is read once and HBM bounds it, so the loads go straight to registers, a step ahead, and no warp waits for another one until a unit
 // ends.  L lanes share a key, each with every L-th 16 bytes of it and of its value: a score takes log2(L) shuffles, and a lane's sums are those of its own
 // columns.  The 32 / L groups of a warp see different keys and have maxima, weights and sums of their own, joined at the unit's end.  A warp's eight keys of a
-// block of 32 lie in one page.  Queries are read from shared memory, a line for all groups.
+// block of 32 lie in one page.  Sums are relative to a maximum that may be 2^8 too low: with a maximum that is followed at once, some row of some group had a
+// new one in half of the steps (287 us against 239 for 32 single tokens over 1.06 GB).  Queries are read from shared memory, a line for all groups.
+#include <cfloat>
 #include <cstdint>
 
 #include "mgq_paged.cuh"
@@ -16,8 +18,15 @@ constexpr uint32_t kMaxHead = 128;
 
 // Rows of a part in the workspace: four at least, so that parts begin on 16 bytes.
 __host__ __device__ constexpr int stored(int rows) { return rows < 4 ? 4 : rows; }
-// CTAs of an SM, as their registers allow.
-__host__ __device__ constexpr int ctas_per_sm(int rows) { return rows == 1 ? 4 : 3; }
+// CTAs of an SM, as their registers allow (eight rows in four: 274 us for 195).
+__host__ __device__ constexpr int ctas_per_sm(int rows) { return rows == 8 ? 3 : 4; }
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <int R, int L, int C>                           // rows of a unit, lanes of a key, 16-byte pieces of a lane: heads of up to 4 * L * C
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const AttendArgs a)
@@ -46,7 +55,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const Att
         int pos[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            m[r] = -INFINITY;
+            m[r] = -FLT_MAX;                             // differences stay numbers; a score of -inf has no weight
             l[r] = 0.f;
             pos[r] = (uint32_t)r < pairs ? g.pos0 + (int)(r / g.heads) : -1;
 #pragma unroll
@@ -90,31 +99,34 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const Att
             for (int x = 1; x < L; x *= 2)
 #pragma unroll
                 for (int r = 0; r < R; r++) s[r] += __shfl_xor_sync(0xffffffffu, s[r], x);
-            bool hidden = false, grows = false;
-            float top[R];
-            bool seen[R];
+            const int key0 = first_key(i);
+            bool masked = false;                         // some row does not see a key that is there
+            if (!(key0 + (int)G <= last && key0 + (int)G - 1 <= g.pos0 && __all_sync(0xffffffffu, there[at]) && !(a.window && key0 <= last - 1 - (int)a.window))) {
+                bool hidden = false;
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                seen[r] = there[at] && key <= pos[r] && (!a.window || key > pos[r] - (int)a.window);
-                hidden |= there[at] && !seen[r] && (uint32_t)r < pairs;          // keys that are not there are zeros
-                top[r] = seen[r] ? fmaxf(m[r], s[r]) : m[r];
-                grows |= top[r] > m[r];
+                for (int r = 0; r < R; r++) {
+                    const bool seen = there[at] && key <= pos[r] && (!a.window || key > pos[r] - (int)a.window);
+                    hidden |= there[at] && !seen && (uint32_t)r < pairs;
+                    s[r] = seen ? s[r] : -INFINITY;
+                }
+                masked = __any_sync(0xffffffffu, hidden);
             }
+            bool grows = false;
+#pragma unroll
+            for (int r = 0; r < R; r++) grows |= s[r] > m[r] + 8.f;
             if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const float keep = top[r] > -INFINITY ? exp2f(m[r] - top[r]) : 1.f;
+                    const float top = s[r] > m[r] + 8.f ? s[r] : m[r], keep = exp2_fast(m[r] - top);
                     l[r] *= keep;
-                    m[r] = top[r];
+                    m[r] = top;
 #pragma unroll
                     for (int e = 0; e < 4 * C; e++) o[r][e] *= keep;
                 }
             }
-            const bool masked = __any_sync(0xffffffffu, hidden);
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                // a row whose seen scores are all -inf has no weight, like one that sees nothing; NaN stays NaN
-                const float w = !seen[r] ? 0.f : s[r] != s[r] ? s[r] : m[r] > -INFINITY ? exp2f(s[r] - m[r]) : 0.f;
+                const float w = exp2_fast(s[r] - m[r]);
                 l[r] += w;
                 if (masked && w == 0.f) continue;        // what a row does not see stays out, infinities and NaN too
 #pragma unroll
@@ -194,10 +206,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const Att
     }
 }
 
-template <int R, int L>
+// Lanes per key for heads of up to 64 and up to 128.
+template <int R, int SMALL, int LARGE>
 int launch_sized(const AttendArgs &a, cudaStream_t stream)
 {
-    auto *kernel = a.d <= 64 ? few_kernel<R, L, 16 / L> : few_kernel<R, L, 32 / L>;
+    auto *kernel = a.d <= 64 ? few_kernel<R, SMALL, 16 / SMALL> : few_kernel<R, LARGE, 32 / LARGE>;
     const uint32_t ctas = few_ctas(R);
     if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), 0, stream, a)) return rc;
     return launch_merge<float, stored(R)>(a, ctas, R, stream);
@@ -212,10 +225,12 @@ bool few_takes(const AttendArgs &a, int dtype)
 }
 size_t few_part_floats(uint32_t rows, uint32_t d) { return (size_t)stored((int)rows) * (d + 2); }
 uint32_t few_ctas(uint32_t rows) { return 148u * ctas_per_sm((int)rows); }
-// rows: of a unit, 1, 4 or 8.  Eight rows have sixteen lanes per key, because the sums of eight lanes would not fit the registers.
+// rows: of a unit, 1, 4 or 8.  More lanes per key hold fewer sums each, so that an SM holds more warps, but take more shuffles: 32 single tokens of four
+// heads of 128 per key / value head took 239 us with eight lanes (three CTAs per SM) and 221 with sixteen (four), of three heads of 64 53 and 75.  One row takes
+// eight: 64 single tokens of 12 heads of 80 (2 GB) 381 us.
 int launch_few(const AttendArgs &a, uint32_t rows, cudaStream_t stream)
 {
-    return rows == 1 ? launch_sized<1, 8>(a, stream) : rows == 4 ? launch_sized<4, 8>(a, stream) : launch_sized<8, 16>(a, stream);
+    return rows == 1 ? launch_sized<1, 8, 8>(a, stream) : rows == 4 ? launch_sized<4, 8, 16>(a, stream) : launch_sized<8, 8, 16>(a, stream);
 }
 
 }  // namespace mgq
