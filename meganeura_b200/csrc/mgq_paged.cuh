@@ -298,9 +298,11 @@ bool prefill_takes(const AttendArgs &a, int dtype);
 constexpr uint32_t kPrefillCtas = 148, kPrefillRows = 256;
 int launch_prefill(const AttendArgs &a, int dtype, cudaStream_t stream);
 
-// f32 with heads of up to 128, a multiple of 4, on 16-byte boundaries: up to eight pairs of a sequence per key / value head (mgq_paged_few.cu).
+// f32 with heads of up to 128, a multiple of 4, on 16-byte boundaries: up to 24 pairs of a sequence per key / value head (mgq_paged_few.cu); from 25 on the
+// tiles of 64 rows.  16 sequences of four heads of 128: 16 pairs 199 and 310 us, 24 pairs 290 and 310, 28 pairs 364 and 310; of one head of 80: 16
+// pairs 292 and 378, 24 pairs 431 and 391.
 bool few_takes(const AttendArgs &a, int dtype);
-constexpr uint32_t kFewPairs = 8;
+constexpr uint32_t kFewPairs = 24;
 uint32_t few_ctas(uint32_t rows);                          // rows of a unit: 1, 4 or 8
 size_t few_part_floats(uint32_t rows, uint32_t d);
 int launch_few(const AttendArgs &a, uint32_t rows, cudaStream_t stream);

@@ -17,8 +17,8 @@ __device__ __forceinline__ void copy16(float *dst, const void *src, bool real)
 }
 
 // out[row, col] (+)= over a tile of 32 keys: a warp scores a quarter of the rows with a key per lane, a thread sums one or two columns for all rows.
-// Up to four pairs take four rows, a warp each: with sixteen a block of keys took 11 us instead of 2.  Four threads fetch a key and its value; with 16-byte rows in f32 (WIDE) asynchronously, a tile ahead.  Single tokens are bound by these loads,
-// portions by the multiply-adds' operands from shared memory.
+// Up to four pairs take four rows, a warp each: with sixteen a block of keys took 11 us instead of 2.  Four threads fetch a key and its value; with 16-byte
+// rows in f32 (WIDE) asynchronously, a tile ahead.  Few rows are bound by these loads, many by the multiply-adds' operands from shared memory.
 template <typename T, int ROWS, int COLS, bool WIDE>     // COLS: columns per thread, heads of up to 128 * COLS
 __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
 {
@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Atte
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
+// f32 with heads over 128 (smaller ones of this kind are other kernels').
 bool wide_rows(const AttendArgs &a, int dtype)
 {
     return dtype == MGQ_FMT_F32 && a.d % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
@@ -372,11 +373,7 @@ int launch_rows(const AttendArgs &a, int dtype, cudaStream_t stream)
     const size_t smem = smem_bytes(ROWS, a.d, wide);
     auto *kernel = a.d <= 128 ? attend_kernel<T, ROWS, 1, false> : attend_kernel<T, ROWS, 2, false>;
     if constexpr (sizeof(T) == 4)
-        if (wide) {
-            kernel = attend_kernel<T, ROWS, 2, true>;
-            if constexpr (ROWS > kFewRows)               // few rows of small heads are mgq_paged_few.cu's
-                if (a.d <= 128) kernel = attend_kernel<T, ROWS, 1, true>;
-        }
+        if (wide) kernel = attend_kernel<T, ROWS, 2, true>;      // smaller heads are mgq_paged_few.cu's and the tiles'
     if (int rc = allow_smem(kernel, smem)) return rc;
     if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem, stream, a)) return rc;
     return launch_merge<T, ROWS>(a, ctas, ROWS, stream);
@@ -437,9 +434,9 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
         a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);
         return launch_prefill(a, dtype, s);
     }
-    if (few_takes(a, dtype) && (pairs <= kFewPairs || pairs > kRows)) {
-        // eight rows rather than two units of four: 32 sequences of two tokens of four heads took 195 and 255 us
-        const uint32_t rows = pairs == 1 ? 1 : pairs <= 4 ? 4 : 8;
+    if (few_takes(a, dtype)) {
+        // of more than eight pairs units of eight; beside sequences of many tokens most others have one token
+        const uint32_t rows = pairs > kFewPairs ? (a.group <= 4 ? 4 : 8) : pairs == 1 ? 1 : pairs <= 4 ? 4 : 8;
         room(few_ctas(rows));
         if (pairs <= kFewPairs) return launch_few(a, rows, s);
         // both kinds of sequences may be there

@@ -1,10 +1,11 @@
-// Attention of up to eight pairs of token and head per key / value head over a paged cache of f32: single tokens, short drafts.
+// Attention of few new tokens per sequence over a paged cache of f32 (single tokens, drafts): units of up to eight pairs of token and head.
 //
-// Every key and value is read once and HBM bounds it, so the loads go straight to registers, a step ahead, and no warp waits for another one until a unit
-// ends.  L lanes share a key, each with every L-th 16 bytes of it and of its value: a score takes log2(L) shuffles, and a lane's sums are those of its own
-// columns.  The 32 / L groups of a warp see different keys and have maxima, weights and sums of their own, joined at the unit's end.  A warp's eight keys of a
-// block of 32 lie in one page.  Sums are relative to a maximum that may be 2^8 too low: with a maximum that is followed at once, some row of some group had a
-// new one in half of the steps (287 us against 239 for 32 single tokens over 1.06 GB).  Queries are read from shared memory, a line for all groups.
+// Up to four pairs read every key and value once and HBM bounds them, eight the multiply-adds.  The loads go straight to registers, a step ahead, and no
+// warp waits for another one until a unit ends.  L lanes share a key, each with every L-th 16 bytes of it and of its value: a score takes log2(L) shuffles,
+// and a lane's sums are those of its own columns.  The 32 / L groups of a warp see different keys and have maxima, weights and sums of their own, joined at the
+// unit's end.  A warp's eight keys of a block of 32 lie in one page.  Queries are read from shared memory, a line for all groups.
+// Sums are relative to a maximum that may be 2^8 too low: with a maximum that is followed at once, some row of some group had a new one in half of the
+// steps (287 us against 239 for 32 single tokens over 1.06 GB).
 #include <cfloat>
 #include <cstdint>
 
