@@ -426,6 +426,9 @@ int launch_sized(const AttendArgs &a, const CacheMaps &maps, uint32_t pairs, cud
     constexpr uint32_t ctas = 148 * ctas_per_sm<D>();
     auto *kernel = decode_kernel<T, D>;
     if (int rc = allow_smem(kernel, smem_bytes<D>())) return rc;
+    // left to itself the driver divides L1 and shared memory so that one CTA less fits for heads of 64: 128 single tokens of three such heads (0.4 GB)
+    // took 118 us instead of 88
+    MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D>(), stream, maps, a)) return rc;
     return launch_merge<T, kRows>(a, ctas, pairs, stream);
 }
@@ -457,9 +460,12 @@ int encode_caches(CacheMaps &maps, int dtype, const AttendArgs &a, uint32_t toke
     const cuuint64_t strides[2] = {(cuuint64_t)a.d * 2, (cuuint64_t)a.kv_heads * a.d * 2};
     const cuuint32_t box[3] = {64, 1, tokens}, elem[3] = {1, 1, 1};
     const CUtensorMapDataType type = dtype == MGQ_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    // a token's row of a head in whole pieces of 256 bytes, or what L2 fetches beyond it is another head's and may be gone by then: heads of 64 took 131 and
+    // 118 us (128 single tokens, 0.4 GB), of 80 318 and 243 (64 single tokens, 1 GB), with 128 bytes 118 and 274
+    const CUtensorMapL2promotion promotion = a.d % 128 == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
     for (int i = 0; i < 2; i++) {
         const CUresult cr = encode(i ? &maps.v : &maps.k, type, 3, const_cast<void *>(i ? a.v : a.k), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                   CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (cr != CUDA_SUCCESS) return fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
     }
     return MGQ_OK;
