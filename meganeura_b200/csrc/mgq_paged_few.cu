@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const Att
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, d = a.d, group = lane / L, part = lane % L;
     pdl_launch_dependents();
     pdl_wait();
-    Walk<R, kBlock, 1> walk;
+    Walk<R, kBlock, R == 1 ? 1 : 2> walk;                // a unit's end takes as long as two blocks (one row: one)
     walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 
