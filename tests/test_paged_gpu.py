@@ -394,6 +394,23 @@ def test_token_probs(rows, vocab, pad):
     assert torch.equal(ops.token_probs(logits), ops.token_probs(logits, torch.ones(rows, device="cuda")))
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,fresh", [
+    ("f32", 1, 1, 64, 1), ("f32", 4, 1, 128, 1), ("f32", 7, 1, 64, 1), ("f32", 4, 2, 80, 7), ("f32", 8, 1, 128, 3), ("f32", 2, 1, 64, 40), ("f32", 2, 1, 256, 1),
+    ("bf16", 4, 1, 128, 1), ("f16", 4, 1, 64, 5), ("bf16", 4, 1, 128, 60),
+])
+@pytest.mark.parametrize("slope", [1 / 64, 1.0, -1.0, 40.0])
+def test_attention_whose_scores_rise_or_fall_from_key_to_key(dtype, heads, kv_heads, d, fresh, slope):
+    import torch
+    rng = np.random.default_rng(d + fresh)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 16, [333, 90], [fresh, fresh])
+    q[..., 0], q[..., 1:] = 4.0, q[..., 1:] / 64                   # scores: slope * position, and a little of the rest
+    flat = k.flatten(0, 1)
+    for s, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        flat[torch.from_numpy(table[s]).cuda()[at // 16] * 16 + at % 16, :, 0] = (slope / 4 * at.float()).to(k.dtype)[:, None]
+    check_attention(dtype, q, k, v, table, starts, lengths, run(q, k, v, table, starts, lengths, fresh, scale=1.0), 1.0)
+
+
 def test_token_probs_in_place():
     import torch
     from meganeura_b200 import ops
