@@ -274,13 +274,15 @@ int mgq_argmax(const float *logits, uint32_t n, void *workspace, uint32_t *out_t
  *   (q may be NULL: keys and values only).  Sources are f32 or of the cache's type; their rows are `pitch` elements apart.  Values
  *   are rounded to nearest.  Slots must differ from one another, else what the cache row holds is open.
  * mgq_paged_attention: each new token's query heads over the tokens of its sequence up to itself, with window > 0 over the last
- *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  What a row does not
- *   see has no part in it, whatever it holds; a row that sees nothing, or only scores of -inf, is zero, one that sees an infinite
- *   value infinite or NaN; rows behind the last sequence are left as they are.  max_fresh: no sequence has more new tokens in this step (it chooses kernels; where it does not hold the call takes longer).  head_dim at
- *   most 256.  `workspace`: mgq_paged_attention_workspace(...) bytes for the same arguments, 16-byte aligned, in any state; calls that may run
- *   at the same time (two streams, two graphs) need one each.
- * Calls that change one pool or table must be ordered on one stream.  Outputs must not overlap inputs, except that lengths may be cached (the lengths of the step before) and
- * q_out may be q where that is dense and of the cache's type.  Waits inside the kernels are bounded; one that ran out shows in mgq_device_status.
+ *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  What a
+ *   row does not see has no part in it, whatever it holds; a row that sees nothing, or only scores of -inf, is zero, one that sees an
+ *   infinite value infinite or NaN; rows behind the last sequence are left as they are.  max_fresh: no sequence has more new tokens in
+ *   this step (it chooses kernels; where it does not hold the call takes longer).  head_dim at most 256.  `workspace`:
+ *   mgq_paged_attention_workspace(...) bytes for the same arguments, 16-byte aligned, in any state; calls that may run at the same time
+ *   (two streams, two graphs) need one each.
+ * Calls that change one pool or table must be ordered on one stream.  Outputs must not overlap inputs, except that lengths may be cached
+ * (the lengths of the step before) and q_out may be q where that is dense and of the cache's type.  Waits inside the kernels are bounded;
+ * one that ran out shows in mgq_device_status.
  * All need table_width * page_size below 2^30, the number of rows below 2^31, and at most MGQ_PAGED_MAX_SEQUENCES sequences. */
 #define MGQ_NO_SLOT  0xFFFFFFFFu
 #define MGQ_NO_PAGE  0xFFFFFFFFu
@@ -301,15 +303,16 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
                         uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
 
 /* mgq_token_probs: out[r, :] = softmax(logits[r, :] / temperature[r]); a temperature that is not above 0 gives 1 to the lowest index among the
- *   largest logits (temperature NULL: 1 everywhere).  out may be logits.  NaN logits count as -inf; a row of them alone is zero.  Where the largest is +inf those that are share the row.
+ *   largest logits (temperature NULL: 1 everywhere).  out may be logits.  NaN logits count as -inf; a row of them alone is zero.  Where the
+ *   largest is +inf those that are share the row.
  * mgq_verify_drafts: speculative sampling.  Sequence s fed its last token and then its drafts: rows [starts[s], starts[s + 1]), tokens[r] the
  *   token of row r.  target[r, :] are the target's probabilities behind row r, draft[r, :] those that tokens[r + 1] was drawn from (the
  *   last row of a sequence is not read), or draft NULL where drafts were chosen outright.  Draft by draft, tokens[r + 1] is kept while
  *   accept[r] * draft[r, it] < target[r, it] (draft NULL: accept[r] < target[r, it]); accepted[s] counts them.  Then next[s] is drawn: behind a draft
  *   that is not kept from max(target - draft, 0) (draft NULL: from target without it; where nothing is left from target), behind the
  *   last one from target: the lowest index at which the running sum exceeds sample[s] times the whole.  out[r] has the kept tokens, then next,
- *   then MGQ_NO_TOKEN.  Sums are in 64 bits; entries that are negative, infinite or NaN count as 0; rows need not sum to 1.  next is MGQ_NO_TOKEN where target has no mass, and
- *   for a sequence without rows.  A sequence of one row has no drafts: its next token is sampled.
+ *   then MGQ_NO_TOKEN.  Sums are in 64 bits; entries that are negative, infinite or NaN count as 0; rows need not sum to 1.  next is
+ *   MGQ_NO_TOKEN where target has no mass, and for a sequence without rows.  A sequence of one row has no drafts: its next token is sampled.
  * Rows are `pitch` elements apart; all values f32.  Outputs of mgq_verify_drafts must not overlap its inputs. */
 int mgq_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream);
 int mgq_verify_drafts(const float *target, uint32_t target_pitch, const float *draft, uint32_t draft_pitch, const uint32_t *tokens, const uint32_t *starts,

@@ -201,8 +201,9 @@ __global__ void __launch_bounds__(kPlanThreads) trim_kernel(const uint32_t *leng
 }
 
 // ---------------------------------------------------------------- keys and values into the cache
-// A CTA takes a row at a time, four CTAs per SM (4096 rows of the Qwen3-8B shape, 151 MB: 26.7 us, with three 31.3).  Its angles (position * theta^(-2i/d), product and reduction to one turn in 64 bits: at position 100000
-// an f32 product is off by up to 0.004) are computed once for all heads, then a thread rotates four pairs of a head per step.
+// A CTA takes a row at a time, four CTAs per SM (4096 rows of the Qwen3-8B shape, 151 MB: 26.7 us, with three 31.3).  Its angles (position *
+// theta^(-2i/d), product and reduction to one turn in 64 bits: at position 100000 an f32 product is off by up to 0.004) are computed once for
+// all heads, then a thread rotates four pairs of a head per step.
 constexpr int kAppendThreads = 256, kBatch = 4;
 
 struct AppendArgs {

@@ -1,8 +1,9 @@
 // Attention of many new tokens per sequence (portions of prompts, long drafts) over a paged cache of f16 or bf16, on tcgen05.
 //
 // A unit is 256 pairs of token and query head of one key / value head, two tiles of 128 rows that share the keys and values of a block
-// of 128.  Per block and tile S = Q K^T and O += P V are four to eight products of K = 16 each way; the tensor cores need 512 cycles for either (heads of 128),
-// and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.
+// of 128.  Per block and tile S = Q K^T and O += P V are four to eight products of K = 16 each way; the tensor cores need 512 cycles for either (heads
+// of 128; a product of 128 x 128 x 16 takes 64), and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.  A tile's chain
+// takes 3200 per block (4 x 2048 tokens behind up to 6144: 575 us, 1107 TFLOP/s in a burst).
 //   warps 0-3, 4-7  softmax of tile 0 and 1, a row per thread: S from TMEM, running maximum and sum in f32, P back into TMEM over S (as the
 //                   16-bit left operand of the second product), results out of TMEM.  Two warps per row need a barrier per block (280 cycles, 671 us for
 //                   4 x 2048 tokens); four lanes per row read TMEM at half the rate (500 cycles of a block, 653 us).
