@@ -101,12 +101,13 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
 
     float m = largest(), sum = 0.f;
     if (!HELD) {
-        // a thread's sum is relative to its own maximum
+        // a thread's sum is relative to its own maximum, and nothing while that is -inf: the factor would be 2^(the next maximum's size), which can be
+        // infinite, and 0 * inf a NaN
         if (!greedy) sum = weights(finite(m));
         for (uint32_t c0 = begin + kSlice; c0 < end; c0 += kSlice) {
             fetch(c0);
             const float top = fmaxf(m, largest());
-            if (!greedy) sum = sum * exp2_fast((finite(m) - finite(top)) * inv) + weights(finite(top));
+            if (!greedy) sum = (m > -INFINITY ? sum * exp2_fast((m - finite(top)) * inv) : 0.f) + weights(finite(top));
             m = top;
         }
     }

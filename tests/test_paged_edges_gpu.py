@@ -1,0 +1,65 @@
+"""The operators over a paged cache and from logits to tokens, at values and lengths where their kernels' arithmetic or order could go wrong."""
+import math
+
+import numpy as np
+import pytest
+
+from oracle import paged_oracle as PO
+from paged_util import host
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- probabilities
+
+def check_probs(logits, temperature):
+    import torch
+    from meganeura_b200 import ops
+    t = np.asarray(temperature, np.float32)
+    got = host(ops.token_probs(torch.from_numpy(logits).cuda(), torch.from_numpy(t).cuda()))
+    want = PO.probs(logits, t)
+    assert np.isfinite(got).all()
+    # the exponent (x - m) / t is off by 2^-22 of its size, which is at most 104 where a weight is not below f32's range; the exponential 2^-22, the
+    # sum 2^-18.  Below f32's normal range a weight is a multiple of 2^-149: expf's two units there, and half a unit of the product with 1 / sum
+    clean = np.where(np.isnan(logits), -np.inf, logits).astype(np.float64)
+    top = clean.max(1, keepdims=True)
+    with np.errstate(invalid="ignore"):
+        spread = np.nan_to_num(np.minimum(104.0, (top - clean) / np.maximum(t, 1e-30)[:, None]), nan=0.0)
+    off, bound = np.abs(got - want), want * (2.0 ** -22 * (spread + 1) + 2.0 ** -18) + 2.5 * 2.0 ** -149
+    at = np.unravel_index((off - bound).argmax(), off.shape)
+    assert off[at] <= bound[at], (at, got[at], want[at])
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 151936), (3, 70001), (80, 40000), (2, 300004), (4, 32768), (3, 5001)])
+@pytest.mark.parametrize("kept", ["late", "top", "prefix", "alternating"])
+def test_token_probs_of_masked_rows(rows, vocab, kept):
+    """-inf (or NaN) in all but a few columns, as masks of a grammar, top-k or padding of the vocabulary leave them, with small and large temperatures."""
+    rng = np.random.default_rng(vocab)
+    logits = np.full((rows, vocab), -np.inf, np.float32)
+    if kept != "prefix":
+        logits[1::2] = np.nan
+    for r in range(rows):
+        n = min(300, vocab // 4)
+        cols = {"late": np.arange(vocab - n, vocab), "top": rng.choice(vocab, 50, replace=False), "prefix": np.arange(n), "alternating": np.arange(r % 2, vocab, 2)}[kept]
+        logits[r, cols] = rng.standard_normal(len(cols)) * 3 - [1, 10, 26, 100, 200, 300][r % 6]
+    for t in (0.05, 0.3, 1.0, 4.0):
+        check_probs(logits, [t] * rows)
+    check_probs(logits, rng.choice([0.0, 0.1, 2.0], rows))
+
+
+@pytest.mark.parametrize("vocab", [151936, 70001])
+def test_token_probs_of_long_rows_with_infinities_and_ties(vocab):
+    rng = np.random.default_rng(vocab)
+    logits = (rng.standard_normal((9, vocab)) * 3 - 50).astype(np.float32)
+    logits[0] = -np.inf                                            # nothing is left
+    logits[1] = np.nan
+    logits[2, [vocab - 1, vocab // 2, 70]] = np.inf                # these share the row
+    logits[3, :vocab // 3], logits[3, vocab - 5] = -np.inf, np.inf
+    logits[4, [vocab - 2, vocab // 2 + 1, vocab // 4]] = 9.0       # the largest, in several CTAs' shares
+    logits[5, :] = -3e38                                           # the type's lowest values as a mask
+    logits[5, vocab // 2:vocab // 2 + 40] = -70.0
+    logits[6, :] = np.finfo(np.float32).min
+    logits[7, ::2] = np.nan
+    logits[8, :vocab - 1] = -np.inf
+    for t in (1.0, 0.1, 0.0):
+        check_probs(logits, [t] * 9)
