@@ -303,8 +303,8 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
                         uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
 
 /* mgq_token_probs: out[r, :] = softmax(logits[r, :] / temperature[r]); a temperature that is not above 0 gives 1 to the lowest index among the
- *   largest logits (temperature NULL: 1 everywhere).  out may be logits.  NaN logits count as -inf; a row of them alone is zero.  Where the
- *   largest is +inf those that are share the row.
+ *   largest logits (temperature NULL: 1 everywhere), one of +inf the same to every logit above -inf.  out may be logits.  NaN logits count as -inf; a row of
+ *   them alone is zero.  Where the largest is +inf those that are share the row.
  * mgq_verify_drafts: speculative sampling.  Sequence s fed its last token and then its drafts: rows [starts[s], starts[s + 1]), tokens[r] the
  *   token of row r.  target[r, :] are the target's probabilities behind row r, draft[r, :] those that tokens[r + 1] was drawn from (the
  *   last row of a sequence is not read), or draft NULL where drafts were chosen outright.  Draft by draft, tokens[r + 1] is kept while

@@ -88,13 +88,16 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
     fetch(begin);
     const float temp = temperature ? temperature[blockIdx.x] : 1.f;
     const bool greedy = !(temp > 0.f);
-    // exponents of 2; the difference first, which is exact near the maximum however large that is.  No finite difference becomes inf * 0.
-    const float inv = greedy ? 0.f : fminf(1.4426950408889634f / temp, FLT_MAX);
+    // exponents of 2; the difference first, which is exact near the maximum however large that is, and half of it, which no two finite numbers make
+    // infinite.  The factor is neither infinite, so that no difference of 0 becomes NaN, nor 0 (a temperature of +inf: the smallest number, with which all
+    // finite differences weigh 2^-1e-6 at least), so that -inf stays -inf.
+    const float inv = greedy ? 0.f : fmaxf(fminf(2.8853900817779268f / temp, FLT_MAX), 1.4e-45f);
+    auto exponent = [&](float x, float m) { return fmaf(x, 0.5f, -0.5f * m) * inv; };
     auto weights = [&](float m) {                        // their sum, relative to a finite maximum
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < kHold; k++)
-            sum += (exp2_fast((v[k][0] - m) * inv) + exp2_fast((v[k][1] - m) * inv)) + (exp2_fast((v[k][2] - m) * inv) + exp2_fast((v[k][3] - m) * inv));
+            sum += (exp2_fast(exponent(v[k][0], m)) + exp2_fast(exponent(v[k][1], m))) + (exp2_fast(exponent(v[k][2], m)) + exp2_fast(exponent(v[k][3], m)));
         return sum;
     };
     auto finite = [](float m) { return fabsf(m) <= FLT_MAX ? m : 0.f; };         // sums of rows without a finite maximum are not used
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
         for (uint32_t c0 = begin + kSlice; c0 < end; c0 += kSlice) {
             fetch(c0);
             const float top = fmaxf(m, largest());
-            if (!greedy) sum = (m > -INFINITY ? sum * exp2_fast((m - finite(top)) * inv) : 0.f) + weights(finite(top));
+            if (!greedy) sum = (m > -INFINITY ? sum * exp2_fast(exponent(m, finite(top))) : 0.f) + weights(finite(top));
             m = top;
         }
     }
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
                     for (int e = 0; e < 4; e++) sum += v[k][e] == INFINITY ? 1.f : 0.f;
             }
         } else {
-            sum = HELD ? weights(m) : mine > -INFINITY ? sum * exp2_fast((mine - m) * inv) : 0.f;
+            sum = HELD ? weights(m) : mine > -INFINITY ? sum * exp2_fast(exponent(mine, m)) : 0.f;
         }
         sum = warp_sum(sum);
         if (lane == 0) s_part[1][warp] = sum;
@@ -183,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
     for (uint32_t c0 = begin; c0 < end; c0 += kSlice) {
         if (!HELD && !greedy) fetch(c0);
         if (greedy || odd) store(c0, [&](float x, uint32_t c) { return greedy ? (c == at ? 1.f : 0.f) : x == INFINITY ? scale : 0.f; });
-        else               store(c0, [&](float x, uint32_t) { return exp2f((x - m) * inv) * scale; });
+        else               store(c0, [&](float x, uint32_t) { return exp2f(exponent(x, m)) * scale; });
     }
     if (parts > 1) cluster_sync();                       // nobody leaves while its sums are being read
 }

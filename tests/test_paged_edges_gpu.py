@@ -63,3 +63,28 @@ def test_token_probs_of_long_rows_with_infinities_and_ties(vocab):
     logits[8, :vocab - 1] = -np.inf
     for t in (1.0, 0.1, 0.0):
         check_probs(logits, [t] * 9)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 151936), (3, 70001), (4, 32768), (3, 5001), (2, 7), (80, 40000)])
+def test_token_probs_at_an_infinite_temperature_and_of_values_at_the_range_s_ends(rows, vocab):
+    import torch
+    from meganeura_b200 import ops
+    rng = np.random.default_rng(vocab)
+    big = np.finfo(np.float32).max
+    for masked in (False, True):
+        logits = (rng.standard_normal((rows, vocab)) * 20).astype(np.float32)
+        logits[1, ::2] = -big                                      # a finite mask is a number like any other
+        logits[0, -1] = big
+        if masked:
+            logits[:, 1::3] = -np.inf
+            logits[1, 4::7] = np.nan
+        seen = np.where(np.isnan(logits), -np.inf, logits) > -np.inf
+        got = host(ops.token_probs(torch.from_numpy(logits).cuda(), torch.full((rows,), math.inf, device="cuda")))
+        want = seen / seen.sum(1, keepdims=True)
+        # a difference of at most 2^129 times 2^-149 is an exponent of 2^-20 at most, in the weight and in the sum; the sum adds 2^-18
+        assert (np.abs(got - want) <= want * (2.0 ** -19 + 2.0 ** -18)).all()
+        # the largest differences there are: 2 * 3.4e38 / 1e38 = 6.8
+        t = np.full(rows, 1e38, np.float32)
+        got = host(ops.token_probs(torch.from_numpy(logits).cuda(), torch.from_numpy(t).cuda()))
+        want = PO.probs(logits, t)
+        assert (np.abs(got - want) <= want * (2.0 ** -22 * 8 + 2.0 ** -18)).all()
