@@ -283,8 +283,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             const Segment &g = sh.kv_seg;
             const int len = g.len, kv = (int)g.kv;
             const uint32_t *table = g.table;
-            const uint32_t kb_end = g.end;
-            for (uint32_t kb = g.begin; ok && kb < kb_end; kb++, block++) {
+            const uint32_t kb_begin = g.begin, kb_end = g.end;
+            __syncwarp();                                // all lanes have read: behind a unit without blocks lane 0 writes the next one at once
+            for (uint32_t kb = kb_begin; ok && kb < kb_end; kb++, block++) {
                 // lane = box of the block + boxes * group of 64 elements
                 const uint32_t b = lane % boxes, part = lane / boxes, key = kb * kKeys + b * box;
                 uint32_t y = gone, have = 0;

@@ -88,3 +88,33 @@ def test_token_probs_at_an_infinite_temperature_and_of_values_at_the_range_s_end
         got = host(ops.token_probs(torch.from_numpy(logits).cuda(), torch.from_numpy(t).cuda()))
         want = PO.probs(logits, t)
         assert (np.abs(got - want) <= want * (2.0 ** -22 * 8 + 2.0 ** -18)).all()
+
+
+# ---------------------------------------------------------------------------------------------- attention: units in every order
+
+def attend(q, k, v, table, starts, lengths, most, **kw):
+    from meganeura_b200 import ops
+    from paged_util import words
+    out = ops.paged_attention(q, k, v, words(table), words(starts), words(lengths), most, **kw)
+    ops.device_status()                                            # no wait inside the kernels ran out
+    return out
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64)])
+def test_attention_of_many_tokens_whose_units_often_have_no_keys(dtype, d):
+    """Sequences without tokens in the cache (lengths of 0, pages that nobody has) between others, one behind another and at both ends."""
+    import torch
+    rng = np.random.default_rng(d)
+    fresh = np.tile([40, 90, 33, 200, 64], 120)
+    empty = np.array([(s // 5) % 3 != 1 or s % 5 == 2 for s in range(len(fresh))])
+    from paged_util import attention_inputs, check_attention
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, 4, 2, d, 16, np.where(empty, 0, rng.integers(0, 300, len(fresh))), fresh)
+    lengths = np.where(empty, 0, lengths)
+    first = attend(q, k, v, table, starts, lengths, 200)
+    for s in np.flatnonzero(empty):
+        assert (first[int(starts[s]):int(starts[s + 1])] == 0).all()
+    for s in np.flatnonzero(~empty)[::9]:
+        rows = slice(int(starts[s]), int(starts[s + 1]))
+        check_attention(dtype, q[rows], k, v, table[s:s + 1], [0, fresh[s]], [lengths[s]], first[rows], d ** -0.5)
+    for _ in range(5):
+        assert torch.equal(attend(q, k, v, table, starts, lengths, 200), first)
