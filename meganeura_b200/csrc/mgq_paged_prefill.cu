@@ -356,83 +356,82 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         if (!ok && lane == 0 && unit > 0)                // given up: the copy in flight lands before the CTA exits
             for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&sh.q_full, (unit - 1) & 1u); w++) { }
     } else if (warp == 9) {
-        // All lanes run along, one issues; nothing in here needs them together.
-        const bool leader = elect_one();
-        const uint32_t q16 = smem_u32(s_q) >> 4, ring16 = smem_u32(ring) >> 4;
-        uint32_t slot = 0, round = 0, p_seen = 0;                         // p_seen: parities of the two tiles in bits 0 and 1
-        bool ok = true;
-        auto advance = [&]() {
-            if (++slot == S) { slot = 0; round++; }
-        };
-        auto scores = [&](uint32_t tile, uint32_t at) {
-            if (leader) {
+        // One lane alone: a lane that ran along without issuing could fall two phases of a barrier behind, since nothing here or in the other roles waits for it, and
+        // would then wait for a phase that is over.
+        if (elect_one()) {
+            const uint32_t q16 = smem_u32(s_q) >> 4, ring16 = smem_u32(ring) >> 4;
+            uint32_t slot = 0, round = 0, p_seen = 0;                         // p_seen: parities of the two tiles in bits 0 and 1
+            bool ok = true;
+            auto advance = [&]() {
+                if (++slot == S) { slot = 0; round++; }
+            };
+            auto scores = [&](uint32_t tile, uint32_t at) {
                 const uint32_t q = q16 + tile * (kHalf / 16), k = ring16 + at * (kStage / 16);
                 umma_step<false>(tmem + tile * 128, q, k, kInstrS);
 #pragma unroll
                 for (uint32_t i = 1; i < D / 16; i++) umma_step<true>(tmem + tile * 128, q + i / 4 * (2 * kHalf / 16) + i % 4 * 2, k + i / 4 * (kHalf / 16) + i % 4 * 2, kInstrS);
                 umma_commit(&sh.s_full[tile]);
-            }
-        };
-        // 64 keys, 16 per product
-        auto values = [&](uint32_t tile, uint32_t at, uint32_t part, bool first) {
-            if (leader) {
+            };
+            // 64 keys, 16 per product
+            auto values = [&](uint32_t tile, uint32_t at, uint32_t part, bool first) {
                 const uint32_t v = ring16 + at * (kStage / 16), o = tmem + 256 + tile * D, p = tmem + tile * 128;
 #pragma unroll
                 for (uint32_t i = 0; i < kKeys / 32; i++) {
                     const uint32_t step = part * 4 + i;
                     umma_f16_ts_mn(o, p + step * 8, v + step * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0 || part > 0);
                 }
-            }
-        };
-        for (uint32_t unit = 0;; unit++) {
-            if (!(ok = lane_wait(&sh.q_full, unit & 1u))) break;
-            const Segment &g = sh.seg[unit & 1u];
-            if (g.tokens == 0) break;
-            const uint32_t begin = g.begin, end = g.end, stop[2] = {tile_end(g, 0, last_token[0]), tile_end(g, 1, last_token[1])};
-            if (end <= begin) {
-                if (leader) mbar_arrive(&sh.q_empty);
-                continue;
-            }
-            // A wait takes the warp 100 cycles and more even where all is there already, so each stands where products are under way: for the next keys
-            // behind the first half of tile 0's values, for the next values behind that of tile 1's.  A commit takes 200: the stages are given back by the
-            // softmax warps, which learn from the scores' commits that their products are done.
-            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
-            tc_fence_after();
+            };
+            for (uint32_t unit = 0;; unit++) {
+                if (!(ok = lane_wait(&sh.q_full, unit & 1u))) break;
+                const Segment &g = sh.seg[unit & 1u];
+                if (g.tokens == 0) break;
+                const uint32_t begin = g.begin, end = g.end, stop[2] = {tile_end(g, 0, last_token[0]), tile_end(g, 1, last_token[1])};
+                if (end <= begin) {
+                    mbar_arrive(&sh.q_empty);
+                    continue;
+                }
+                // A wait takes the warp 100 cycles and more even where all is there already, so each stands where products are under way: for the next keys
+                // behind the first half of tile 0's values, for the next values behind that of tile 1's.  A commit takes 200: the stages are given back by the
+                // softmax warps, which learn from the scores' commits that their products are done.
+                if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+                tc_fence_after();
 #pragma unroll
-            for (uint32_t tile = 0; tile < 2; tile++)
-                if (stop[tile] > begin) scores(tile, slot);
-            if (begin + 1 == end && leader) umma_commit(&sh.q_empty);
-            advance();
-            if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
-            for (uint32_t kb = begin; kb < end; kb++) {
-                const uint32_t v_slot = slot;
+                for (uint32_t tile = 0; tile < 2; tile++)
+                    if (stop[tile] > begin) scores(tile, slot);
+                if (begin + 1 == end) umma_commit(&sh.q_empty);
                 advance();
-                const uint32_t k_slot = slot, k_round = round;
-                const bool more = kb + 1 < end;
-                if (more) advance();                     // to the next values
+                if (!(ok = lane_wait(&sh.full[slot], round & 1u))) break;
+                for (uint32_t kb = begin; kb < end; kb++) {
+                    const uint32_t v_slot = slot;
+                    advance();
+                    const uint32_t k_slot = slot, k_round = round;
+                    const bool more = kb + 1 < end;
+                    if (more) advance();                     // to the next values
 #pragma unroll
-                for (uint32_t tile = 0; tile < 2; tile++) {
-                    const bool values_now = stop[tile] > kb;
-                    if (values_now) {
-                        if (!(ok = lane_wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
-                        tc_fence_after();
-                        values(tile, v_slot, 0, kb == begin);
+                    for (uint32_t tile = 0; tile < 2; tile++) {
+                        const bool values_now = stop[tile] > kb;
+                        if (values_now) {
+                            if (!(ok = lane_wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
+                            tc_fence_after();
+                            values(tile, v_slot, 0, kb == begin);
+                        }
+                        if (more && !(ok = lane_wait(&sh.full[tile ? slot : k_slot], (tile ? round : k_round) & 1u))) break;
+                        if (values_now) {
+                            if (!(ok = lane_wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
+                            p_seen ^= 1u << tile;
+                            tc_fence_after();
+                            values(tile, v_slot, 1, false);
+                            if (kb + 1 == stop[tile]) umma_commit(&sh.o_full[tile]);
+                        }
+                        if (stop[tile] > kb + 1) scores(tile, k_slot);
                     }
-                    if (more && !(ok = lane_wait(&sh.full[tile ? slot : k_slot], (tile ? round : k_round) & 1u))) break;
-                    if (values_now) {
-                        if (!(ok = lane_wait(&sh.p_full[tile], p_seen >> tile & 1u))) break;
-                        p_seen ^= 1u << tile;
-                        tc_fence_after();
-                        values(tile, v_slot, 1, false);
-                        if (kb + 1 == stop[tile] && leader) umma_commit(&sh.o_full[tile]);
-                    }
-                    if (stop[tile] > kb + 1) scores(tile, k_slot);
+                    if (!ok) break;
+                    if (kb + 2 == end) umma_commit(&sh.q_empty);    // no more scores of this unit
                 }
                 if (!ok) break;
-                if (kb + 2 == end && leader) umma_commit(&sh.q_empty);    // no more scores of this unit
             }
-            if (!ok) break;
         }
+        __syncwarp();
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");

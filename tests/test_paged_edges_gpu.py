@@ -118,3 +118,20 @@ def test_attention_of_many_tokens_whose_units_often_have_no_keys(dtype, d):
         check_attention(dtype, q[rows], k, v, table[s:s + 1], [0, fresh[s]], [lengths[s]], first[rows], d ** -0.5)
     for _ in range(5):
         assert torch.equal(attend(q, k, v, table, starts, lengths, 200), first)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d", [("bf16", 8, 2, 128), ("f16", 3, 1, 64), ("bf16", 2, 2, 80)])
+def test_attention_of_very_many_short_units_of_many_tokens(dtype, heads, kv_heads, d):
+    """Units of one or two blocks of keys, some with one tile and some with two: every wait of the kernel's roles meets its next phase at once."""
+    import torch
+    from paged_util import attention_inputs, check_attention
+    rng = np.random.default_rng(heads)
+    fresh = rng.integers(33 * kv_heads // heads + 1, 70, 1500)
+    cached = rng.choice([0, 1, 60, 127, 128, 200], 1500)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 8, cached, fresh)
+    first = attend(q, k, v, table, starts, lengths, 70)
+    for s in range(0, 1500, 97):
+        rows = slice(int(starts[s]), int(starts[s + 1]))
+        check_attention(dtype, q[rows], k, v, table[s:s + 1], [0, fresh[s]], [lengths[s]], first[rows], d ** -0.5)
+    for _ in range(10):
+        assert torch.equal(attend(q, k, v, table, starts, lengths, 70), first)
