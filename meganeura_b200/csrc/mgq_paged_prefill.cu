@@ -471,11 +471,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 if (++slot == S) { slot = 0; round++; }
                 if (kb >= stop) {
                     finish();
-                    // nothing for this tile: it gives the stages back as soon as they are filled, not before
-                    wait(&sh.full[k_slot], k_round & 1u);
-                    if (r_tile == 0) mbar_arrive(&sh.empty[k_slot]);
-                    wait(&sh.full[v_slot], v_round & 1u);
-                    if (r_tile == 0) mbar_arrive(&sh.empty[v_slot]);
+                    // Nothing for this tile: it gives the stages back as soon as they are filled, not before.  Its first warp alone, lanes together: once the stage is
+                    // given back it may be filled again, and another warp that has not looked yet would wait for a phase that is over.
+                    if (quad == 0) {
+                        wait(&sh.full[k_slot], k_round & 1u);
+                        if (lane == 0) mbar_arrive(&sh.empty[k_slot]);
+                        wait(&sh.full[v_slot], v_round & 1u);
+                        if (lane == 0) mbar_arrive(&sh.empty[v_slot]);
+                    }
                     continue;
                 }
                 wait(&sh.s_full[tile], s_seen & 1u);

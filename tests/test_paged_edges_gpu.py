@@ -135,3 +135,22 @@ def test_attention_of_very_many_short_units_of_many_tokens(dtype, heads, kv_head
         check_attention(dtype, q[rows], k, v, table[s:s + 1], [0, fresh[s]], [lengths[s]], first[rows], d ** -0.5)
     for _ in range(10):
         assert torch.equal(attend(q, k, v, table, starts, lengths, 70), first)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,window", [("bf16", 8, 2, 128, 0), ("f16", 4, 4, 64, 0), ("f16", 8, 1, 64, 500)])
+def test_attention_of_units_whose_second_tile_has_nothing_to_do(dtype, heads, kv_heads, d, window):
+    """Up to 128 pairs over long sequences: the idle tile hands on the stages of every block, for many units one behind another and beside full ones."""
+    import torch
+    from paged_util import attention_inputs, check_attention
+    rng = np.random.default_rng(heads + d)
+    g = heads // kv_heads
+    fresh = np.array([128 // g, 33 // g + 1, 200, 100 // g, 128 // g + 1, 64 // g] * 10)
+    cached = rng.integers(1500, 4000, len(fresh))
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 32, cached, fresh)
+    first = attend(q, k, v, table, starts, lengths, 200, window=window)
+    for s in range(0, len(fresh), 7):
+        i = int(rng.integers(0, fresh[s]))
+        r = int(starts[s]) + i                                     # the row alone, as the last token of its sequence
+        check_attention(dtype, q[r:r + 1], k, v, table[s:s + 1], [0, 1], [cached[s] + i + 1], first[r:r + 1], d ** -0.5, window)
+    for _ in range(10):
+        assert torch.equal(attend(q, k, v, table, starts, lengths, 200, window=window), first)
