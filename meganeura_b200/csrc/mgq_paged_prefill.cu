@@ -25,6 +25,9 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
+// Exponents are score * scale - m in one rounding, m is rounded before, by up to 2^-24 of its size.  That is a factor which all weights of a row have in common, but
+// beyond some size it takes them out of their type's range (from 2^27 on infinite f16 weights, from 2^34 rows of zeros): such rows are computed again.
+constexpr float kHuge = 0x1p20f;
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return D / 64 * kHalf; }
@@ -165,39 +168,77 @@ __device__ __forceinline__ uint32_t tile_end(const Segment &g, uint32_t tile, ui
     return last < 0 ? g.begin : max(g.begin, min(g.end, (uint32_t)last / kKeys + 1));
 }
 
-// One row of a segment again, on the CUDA cores and without what it does not see: where a value that only other rows see is infinite or NaN, its
-// product with a weight of 0 has spoilt the row.  A whole warp; lane i has columns i, i + 32, ...
-template <typename T, int D>
-__device__ __noinline__ void row_again(const AttendArgs &a, const Segment &g, uint32_t r, uint32_t end, float &m, float &l, float (&acc)[D / 32])
+// 8 values of T as f32, from 16 bytes.
+template <typename T>
+__device__ __forceinline__ void read8(const T *p, float (&f)[8])
 {
-    const uint32_t lane = threadIdx.x & 31u, token = r / g.heads, head = g.head0 + r - token * g.heads;
-    const int pos = g.pos0 + (int)token;
-    float q[D / 32];
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    const T *e = reinterpret_cast<const T *>(&v);
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-        const uint32_t c = lane + 32 * i;
-        q[i] = c < a.d ? to_f32(static_cast<const T *>(a.q)[(size_t)(g.row0 + token) * a.q_pitch + (size_t)head * a.d + c]) * a.scale_log2 : 0.f;
-        acc[i] = 0.f;
+    for (int i = 0; i < 8; i++) f[i] = to_f32(e[i]);
+}
+// One row of a segment again, on the CUDA cores and without what it does not see: where a value that only other rows see is infinite or NaN, its
+// product with a weight of 0 has spoilt the row, and where scores are huge their weights have left the type's range.  A whole warp: eight lanes share a key, each with 8 of
+// 64 columns; the four groups have maxima and sums of their own, joined at the end, when all of them hold the row.
+template <typename T, int D>
+__device__ __noinline__ void row_again(const AttendArgs &a, const Segment &g, uint32_t r, uint32_t end, float &m, float &l, float (&acc)[D / 64][8])
+{
+    const uint32_t lane = threadIdx.x & 31u, token = r / g.heads, head = g.head0 + r - token * g.heads, column = lane % 8 * 8;
+    const int pos = g.pos0 + (int)token;
+    float q[D / 64][8];
+#pragma unroll
+    for (int c = 0; c < D / 64; c++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[c][e] = acc[c][e] = 0.f;
+        if (column + 64 * c < a.d) read8(static_cast<const T *>(a.q) + (size_t)(g.row0 + token) * a.q_pitch + (size_t)head * a.d + column + 64 * c, q[c]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[c][e] *= a.scale_log2;
     }
     m = -INFINITY;
     l = 0.f;
     const int stop = min(min((int)(end * kKeys), pos + 1), g.len);
-    for (int key = (int)(g.begin * kKeys); key < stop; key++) {
-        if (a.window && key <= pos - (int)a.window) continue;
-        const uint32_t page = g.table[(uint32_t)key >> a.page_shift];
-        if (page >= a.pages) continue;
-        const size_t at = ((((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * a.d;
-        float x = 0.f;
+#pragma unroll 2
+    for (int key0 = (int)(g.begin * kKeys); key0 < stop; key0 += 4) {
+        const int key = key0 + (int)(lane / 8);
+        const uint32_t page = key < stop && !(a.window && key <= pos - (int)a.window) ? g.table[(uint32_t)key >> a.page_shift] : 0xFFFFFFFFu;
+        const bool seen = page < a.pages;
+        const size_t at = seen ? ((((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * a.d + column : 0;
+        float x = 0.f, k[D / 64][8], v[D / 64][8];
 #pragma unroll
-        for (int i = 0; i < D / 32; i++)
-            if (lane + 32 * i < a.d) x = fmaf(q[i], to_f32(static_cast<const T *>(a.k)[at + lane + 32 * i]), x);
-        x = warp_sum(x);
+        for (int c = 0; c < D / 64; c++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) k[c][e] = v[c][e] = 0.f;
+            if (seen && column + 64 * c < a.d) {
+                read8(static_cast<const T *>(a.k) + at + 64 * c, k[c]);
+                read8(static_cast<const T *>(a.v) + at + 64 * c, v[c]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) x = fmaf(q[c][e], k[c][e], x);
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+        x = seen ? x : -INFINITY;
         const float top = fmaxf(m, x), base = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - base), p = exp2_fast(x - base);
         l = l * keep + p;
         m = top;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++)
-            if (lane + 32 * i < a.d) acc[i] = acc[i] * keep + (p != 0.f ? p * to_f32(static_cast<const T *>(a.v)[at + lane + 32 * i]) : 0.f);
+        for (int c = 0; c < D / 64; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[c][e] = fmaf(p, v[c][e], acc[c][e] * keep);
+    }
+#pragma unroll
+    for (int o = 8; o < 32; o *= 2) {
+        const float top = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o)), keep = l != 0.f ? exp2_fast(m - top) : 0.f;      // a NaN is a weight
+        m = top;
+        l *= keep;
+        l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+        for (int c = 0; c < D / 64; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float mine = keep != 0.f ? acc[c][e] * keep : 0.f;
+                acc[c][e] = mine + __shfl_xor_sync(0xffffffffu, mine, o);
+            }
     }
 }
 
@@ -454,6 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             const int pos = row < pairs ? g.pos0 + (int)token : -1;
             const bool holes = sh.holes[unit & 1u] != 0;
             float m = -INFINITY, l = 0.f;
+            bool huge = false;
             uint32_t v_before = 0;
             bool finished = stop <= begin;               // the last product is done, its values' stage given back
             auto finish = [&]() {
@@ -535,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     const float keep = up ? exp2_fast(m - top) : 1.f;
                     l *= keep;
                     m = up ? top : m;
+                    huge |= up && fabsf(top) > kHuge;
                     if (kb != begin && __any_sync(0xffffffffu, up)) {
 #pragma unroll 1
                         for (uint32_t c = 0; c < D; c += 16) {
@@ -635,20 +678,29 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     }
                     __syncwarp();                        // the next columns are read by the whole warp
                 }
-                bad = bad && row < pairs && l == l;      // a NaN among the seen scores makes all of the row NaN, as it should be
+                bad = row < pairs && (huge || (bad && l == l));          // a NaN among the seen scores makes all of the row NaN, as it should be
                 if (!alone && row < pairs) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * row) = make_float2(m, l);
                 for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
                     const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
-                    float rm, rl, acc[D / 32];
+                    float rm, rl, acc[D / 64][8];
                     row_again<T, D>(a, g, r, stop, rm, rl, acc);
                     const uint32_t tok = r / g.heads, hd = r - tok * g.heads;
                     __syncwarp();                        // behind the row's own stores
 #pragma unroll
-                    for (int i = 0; i < D / 32; i++) {
-                        const uint32_t c = lane + 32 * i;
-                        if (c >= d) continue;
-                        if (alone) static_cast<T *>(a.out)[(size_t)(g.row0 + tok) * a.out_pitch + (size_t)(g.head0 + hd) * d + c] = rounded<T>(rl == 0.f ? 0.f : acc[i] / rl);
-                        else       part[r * d + c] = acc[i];
+                    for (int c = 0; c < D / 64; c++) {
+                        const uint32_t column = lane * 8 + 64 * c;
+                        if (lane >= 8 || column >= d) continue;
+                        if (alone) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v[e] = rl == 0.f ? 0u : pack<T>(acc[c][2 * e] / rl, acc[c][2 * e + 1] / rl);
+                            *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + (size_t)(g.row0 + tok) * a.out_pitch + (size_t)(g.head0 + hd) * d + column) =
+                                make_uint4(v[0], v[1], v[2], v[3]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 4)
+                                *reinterpret_cast<float4 *>(part + r * d + column + e) = make_float4(acc[c][e], acc[c][e + 1], acc[c][e + 2], acc[c][e + 3]);
+                        }
                     }
                     if (!alone && lane == 0) *reinterpret_cast<float2 *>(part + kPrefillRows * d + 2 * r) = make_float2(rm, rl);
                     __syncwarp();

@@ -154,3 +154,83 @@ def test_attention_of_units_whose_second_tile_has_nothing_to_do(dtype, heads, kv
         check_attention(dtype, q[r:r + 1], k, v, table[s:s + 1], [0, 1], [cached[s] + i + 1], first[r:r + 1], d ** -0.5, window)
     for _ in range(10):
         assert torch.equal(attend(q, k, v, table, starts, lengths, 200, window=window), first)
+
+
+# ---------------------------------------------------------------------------------------------- attention: scores and weights at the range's ends
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,fresh", [
+    ("bf16", 8, 2, 128, 60), ("f16", 8, 2, 128, 60), ("f16", 3, 1, 64, 200), ("bf16", 4, 4, 80, 300), ("bf16", 8, 2, 128, 1), ("f16", 8, 2, 64, 5), ("f16", 4, 2, 256, 3),
+    ("f32", 4, 1, 128, 1), ("f32", 4, 2, 64, 5), ("f32", 8, 2, 128, 60), ("f32", 2, 1, 256, 7), ("bf16", 3, 1, 20, 9),
+])
+@pytest.mark.parametrize("scale", [0.0883883, 1.0, 37.0])
+def test_attention_with_scores_far_beyond_what_a_weight_distinguishes(dtype, heads, kv_heads, d, fresh, scale):
+    """Scores of 2^20 to 2^50, whole steps of 2^17 and more apart: a row is the mean of the values whose score is the largest that it sees."""
+    import torch
+    from paged_util import EPS, attention_inputs, words
+    rng = np.random.default_rng(d + fresh)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 16, [500, 90], [fresh, fresh])
+    a, b = (2.0 ** 13, 2.0 ** 8) if dtype == "f16" else (2.0 ** 22, 2.0 ** 20)
+    level = rng.integers(1, 100, k.shape[:3])
+    level[rng.random(level.shape) < 0.02] = 100                   # the same score more than once
+    q.zero_(), k.zero_()
+    q[..., 3] = a
+    for sign in (1.0, -1.0):                                       # the largest far above 0, and far below
+        k[..., 3] = torch.from_numpy(sign * b * level).to(k)
+        got = host(attend(q, k, v, table, starts, lengths, fresh, scale=scale))
+        values = host(v).astype(np.float64)
+        for s in range(2):
+            slots = table[s, np.arange(lengths[s]) // 16] * 16 + np.arange(lengths[s]) % 16
+            lv, vv = sign * level.reshape(-1, kv_heads)[slots], values.reshape(-1, kv_heads, d)[slots]
+            for i in {0, 1, fresh // 2, fresh - 1} & set(range(fresh)):
+                n = lengths[s] - fresh + i + 1
+                for h in range(heads):
+                    o = h * kv_heads // heads
+                    best = lv[:n, o] == lv[:n, o].max()
+                    want, size = vv[:n, o][best].mean(0), np.abs(vv[:n, o][best]).mean(0)
+                    # equal weights: half a step of the result, and f32 sums of at most 100 values.  Relative to a maximum that is itself rounded a weight of many
+                    # tokens is 2^(score - maximum) with an exponent other than 0, and then rounded to its type, while the sum has it unrounded: half a step more
+                    rounded = EPS[dtype] / 2 if dtype != "f32" and fresh * heads // kv_heads > 32 else 0.0
+                    assert (np.abs(got[int(starts[s]) + i, h] - want) <= EPS[dtype] / 2 * np.abs(want) + (rounded + 2.0 ** -17) * size + 2.0 ** -24).all(), (sign, s, i, h)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,fresh", [("bf16", 8, 2, 128, 60), ("f16", 3, 1, 64, 200), ("f16", 8, 2, 128, 1), ("f32", 4, 2, 64, 40), ("f32", 4, 2, 64, 1)])
+def test_attention_whose_first_keys_score_far_below_the_others(dtype, heads, kv_heads, d, fresh):
+    """Scores of about -2^30 for the first 300 keys: while only they have been seen the maximum is that low, and nothing of it may stay."""
+    from paged_util import EPS, attention_inputs
+    rng = np.random.default_rng(fresh)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 16, [900], [fresh])
+    a, b = (2.0 ** 13, 2.0 ** 14) if dtype == "f16" else (2.0 ** 16, 2.0 ** 16)
+    q[..., 3], k[..., 3] = a, 0.0
+    slots = table[0, np.arange(lengths[0]) // 16] * 16 + np.arange(lengths[0]) % 16
+    import torch
+    k.flatten(0, 1)[torch.from_numpy(slots[:300]).cuda(), :, 3] = -b
+    want, size, _ = PO.attention(host(q), host(k), host(v), table, starts, lengths, d ** -0.5)
+    got = host(attend(q, k, v, table, starts, lengths, fresh))
+    # half a step of the result and of a weight; scores of the others: 64 to 128 products, a few units each of 2^-24 * 60
+    assert (np.abs(got - want) <= EPS[dtype] / 2 * (np.abs(want) + size) + 2.0 ** -13 * size + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64), ("bf16", 80)])
+def test_attention_of_many_tokens_whose_rows_are_all_computed_again(dtype, d):
+    """An infinite value that every row sees, in one column: the others are as without it.  One that only the last token sees: nobody else changes."""
+    import torch
+    from paged_util import attention_inputs, check_attention
+    rng = np.random.default_rng(d)
+    q, k, v, table, starts, lengths = attention_inputs(rng, dtype, 8, 2, d, 32, [6000, 40], [130, 70])
+    clean = attend(q, k, v, table, starts, lengths, 130)
+    flat, at = v.flatten(0, 1), int(table[0, 0]) * 32 + 5
+    old = flat[at, 1, 7].clone()
+    flat[at, 1, 7] = math.inf
+    got = attend(q, k, v, table, starts, lengths, 130)
+    assert not torch.isfinite(got[:130, 4:, 7]).any()
+    got[:130, 4:, 7] = clean[:130, 4:, 7]
+    flat[at, 1, 7] = old
+    for i in (0, 64, 129):
+        check_attention(dtype, q[i:i + 1], k, v, table[:1], [0, 1], [6001 + i], got[i:i + 1], d ** -0.5)
+    assert torch.equal(got[130:], clean[130:])
+    at = int(table[0, 6129 // 32]) * 32 + 6129 % 32
+    flat[at, 0, 3] = math.nan
+    got = attend(q, k, v, table, starts, lengths, 130)
+    assert torch.isnan(got[129, :4, 3]).all()
+    for i in (0, 65, 128):
+        check_attention(dtype, q[i:i + 1], k, v, table[:1], [0, 1], [6001 + i], got[i:i + 1], d ** -0.5)
