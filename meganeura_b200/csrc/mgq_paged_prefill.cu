@@ -45,6 +45,7 @@ struct __align__(16) Shared {
     uint32_t holes[2];                                   // whether the unit's keys have pages that do not exist
     uint32_t tmem;
     volatile int failed;
+    volatile uint32_t again;                             // counts on while rows are computed again
 };
 template <int D> constexpr size_t smem_bytes() { return (size_t)(2 + stages<D>()) * stage_bytes<D>() + sizeof(Shared); }
 static_assert(smem_bytes<128>() <= 227 * 1024 && smem_bytes<64>() <= 227 * 1024, "shared memory of an SM");
@@ -160,6 +161,24 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int base)
     return hi <= lo ? 0u : (0xFFFFFFFFu >> (32 - hi + lo)) << lo;
 }
 
+// mbar_wait for roles that may wait for rows that are computed again: that takes as long as there are keys, and while `again` counts on nobody gives up.
+__device__ __forceinline__ bool wait_for(Shared &sh, unsigned long long *bar, uint32_t parity)
+{
+    uint32_t again = sh.again;
+    for (uint32_t i = 0; i < kWaitLimit; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (sh.failed) return false;
+        const uint32_t now = sh.again;
+        if (now != again) {
+            again = now;
+            i = 0;
+        }
+    }
+    sh.failed = 1;
+    atomicExch(&g_prefill_error, 1u);
+    return false;
+}
+
 // Key blocks of one tile of a segment: [g.begin, what is returned).  last_token: that of the tile's last row, were all tokens there.
 __device__ __forceinline__ uint32_t tile_end(const Segment &g, uint32_t tile, uint32_t last_token)
 {
@@ -168,63 +187,110 @@ __device__ __forceinline__ uint32_t tile_end(const Segment &g, uint32_t tile, ui
     return last < 0 ? g.begin : max(g.begin, min(g.end, (uint32_t)last / kKeys + 1));
 }
 
-// 8 values of T as f32, from 16 bytes.
+// 8 values of T as f32.
 template <typename T>
-__device__ __forceinline__ void read8(const T *p, float (&f)[8])
+__device__ __forceinline__ void unpack(const uint4 &v, float (&f)[8])
 {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
     const T *e = reinterpret_cast<const T *>(&v);
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = to_f32(e[i]);
 }
 // One row of a segment again, on the CUDA cores and without what it does not see: where a value that only other rows see is infinite or NaN, its
 // product with a weight of 0 has spoilt the row, and where scores are huge their weights have left the type's range.  A whole warp: eight lanes share a key, each with 8 of
-// 64 columns; the four groups have maxima and sums of their own, joined at the end, when all of them hold the row.
+// 64 columns, and the four groups of lanes have maxima and sums of their own, joined at the end, when all of them hold the row.  Loads' latency bounds it: eight keys at
+// a time, fetched while the eight before are used, their pages looked up another step ahead.
 template <typename T, int D>
-__device__ __noinline__ void row_again(const AttendArgs &a, const Segment &g, uint32_t r, uint32_t end, float &m, float &l, float (&acc)[D / 64][8])
+__device__ __noinline__ void row_again(const AttendArgs &a, Shared &sh, const Segment &g, uint32_t r, uint32_t end, float &m_out, float &l_out, float (&out)[D / 64][8])
 {
+    constexpr int C = D / 64, kStep = 8, N = kStep / 4;
     const uint32_t lane = threadIdx.x & 31u, token = r / g.heads, head = g.head0 + r - token * g.heads, column = lane % 8 * 8;
-    const int pos = g.pos0 + (int)token;
-    float q[D / 64][8];
+    const int pos = g.pos0 + (int)token, first = (int)(g.begin * kKeys), stop = min(min((int)(end * kKeys), pos + 1), g.len);
+    float q[C][8], acc[C][8], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int c = 0; c < D / 64; c++) {
+    for (int c = 0; c < C; c++) {
+        const bool in = column + 64 * c < a.d;
+        const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + token) * a.q_pitch + (size_t)head * a.d + column + 64 * c;
+        unpack<T>(in ? *reinterpret_cast<const uint4 *>(src) : make_uint4(0u, 0u, 0u, 0u), q[c]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) q[c][e] = acc[c][e] = 0.f;
-        if (column + 64 * c < a.d) read8(static_cast<const T *>(a.q) + (size_t)(g.row0 + token) * a.q_pitch + (size_t)head * a.d + column + 64 * c, q[c]);
-#pragma unroll
-        for (int e = 0; e < 8; e++) q[c][e] *= a.scale_log2;
-    }
-    m = -INFINITY;
-    l = 0.f;
-    const int stop = min(min((int)(end * kKeys), pos + 1), g.len);
-#pragma unroll 2
-    for (int key0 = (int)(g.begin * kKeys); key0 < stop; key0 += 4) {
-        const int key = key0 + (int)(lane / 8);
-        const uint32_t page = key < stop && !(a.window && key <= pos - (int)a.window) ? g.table[(uint32_t)key >> a.page_shift] : 0xFFFFFFFFu;
-        const bool seen = page < a.pages;
-        const size_t at = seen ? ((((size_t)page << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * a.d + column : 0;
-        float x = 0.f, k[D / 64][8], v[D / 64][8];
-#pragma unroll
-        for (int c = 0; c < D / 64; c++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) k[c][e] = v[c][e] = 0.f;
-            if (seen && column + 64 * c < a.d) {
-                read8(static_cast<const T *>(a.k) + at + 64 * c, k[c]);
-                read8(static_cast<const T *>(a.v) + at + 64 * c, v[c]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) x = fmaf(q[c][e], k[c][e], x);
+        for (int e = 0; e < 8; e++) {
+            q[c][e] *= a.scale_log2;
+            acc[c][e] = 0.f;
         }
+    }
+    uint4 k[N][C], v[N][C];
+    uint32_t page[N];
+    bool seen[N];
+    auto look_up = [&](int key0) {
 #pragma unroll
-        for (int o = 1; o < 8; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x = seen ? x : -INFINITY;
-        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - base), p = exp2_fast(x - base);
-        l = l * keep + p;
+        for (int n = 0; n < N; n++) {
+            const int key = key0 + 4 * n + (int)(lane / 8);
+            page[n] = key < stop && !(a.window && key <= pos - (int)a.window) ? g.table[(uint32_t)key >> a.page_shift] : 0xFFFFFFFFu;
+        }
+    };
+    auto fetch = [&](int key0) {
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int key = key0 + 4 * n + (int)(lane / 8);
+            seen[n] = page[n] < a.pages;
+            const size_t at = seen[n] ? ((((size_t)page[n] << a.page_shift) + (key & ((1u << a.page_shift) - 1))) * a.kv_heads + g.kv) * a.d + column : 0;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                k[n][c] = v[n][c] = make_uint4(0u, 0u, 0u, 0u);
+                if (seen[n] && column + 64 * c < a.d) {
+                    k[n][c] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k) + at + 64 * c);
+                    v[n][c] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.v) + at + 64 * c);
+                }
+            }
+        }
+    };
+    look_up(first);
+    fetch(first);
+    look_up(first + kStep);
+    for (int key0 = first; key0 < stop; key0 += kStep) {
+        if (lane == 0 && (key0 - first) % 1024 == 0) sh.again = sh.again + 1;     // other warps may do so at once: only that it changes counts
+        float x[N], w[N][C][8];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            x[n] = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                unpack<T>(k[n][c], w[n][c]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[n] = fmaf(q[c][e], w[n][c][e], x[n]);
+                unpack<T>(v[n][c], w[n][c]);
+            }
+        }
+        bool real[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) real[n] = seen[n];
+        fetch(key0 + kStep);
+        look_up(key0 + 2 * kStep);
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2)
+#pragma unroll
+            for (int n = 0; n < N; n++) x[n] += __shfl_xor_sync(0xffffffffu, x[n], o);
+        float top = m;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            x[n] = real[n] ? x[n] : -INFINITY;
+            top = fmaxf(top, x[n]);
+        }
+        const float base = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - base);
         m = top;
+        l *= keep;
 #pragma unroll
-        for (int c = 0; c < D / 64; c++)
+        for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) acc[c][e] = fmaf(p, v[c][e], acc[c][e] * keep);
+            for (int e = 0; e < 8; e++) acc[c][e] *= keep;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const float p = exp2_fast(x[n] - base);
+            l += p;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc[c][e] = fmaf(p, w[n][c][e], acc[c][e]);
+        }
     }
 #pragma unroll
     for (int o = 8; o < 32; o *= 2) {
@@ -233,13 +299,19 @@ __device__ __noinline__ void row_again(const AttendArgs &a, const Segment &g, ui
         l *= keep;
         l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-        for (int c = 0; c < D / 64; c++)
+        for (int c = 0; c < C; c++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float mine = keep != 0.f ? acc[c][e] * keep : 0.f;
                 acc[c][e] = mine + __shfl_xor_sync(0xffffffffu, mine, o);
             }
     }
+    m_out = m;
+    l_out = l;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) out[c][e] = acc[c][e];
 }
 
 template <typename T, int D>                             // D: head size rounded up to 64 or 128
@@ -273,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             mbar_init(&sh.o_full[i], 1);
         }
         sh.failed = 0;
+        sh.again = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) tmem_alloc(&sh.tmem, 512);
@@ -299,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const uint32_t last_token[2] = {(kTile - 1) / slice, (2 * kTile - 1) / slice};
     // Each lane by itself: false where the limit ran out, or another role has given up.
     auto lane_wait = [&](unsigned long long *bar, uint32_t parity) {
-        return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, &sh.failed, &g_prefill_error);
+        return mbar_try_wait(bar, parity) || wait_for(sh, bar, parity);
     };
     auto wait = [&](unsigned long long *bar, uint32_t parity) {
         const bool done = lane_wait(bar, parity);
@@ -683,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 for (uint32_t left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
                     const uint32_t r = tile * kTile + quad * 32 + __ffs(left) - 1;
                     float rm, rl, acc[D / 64][8];
-                    row_again<T, D>(a, g, r, stop, rm, rl, acc);
+                    row_again<T, D>(a, sh, g, r, stop, rm, rl, acc);
                     const uint32_t tok = r / g.heads, hd = r - tok * g.heads;
                     __syncwarp();                        // behind the row's own stores
 #pragma unroll

@@ -234,3 +234,21 @@ def test_attention_of_many_tokens_whose_rows_are_all_computed_again(dtype, d):
     assert torch.isnan(got[129, :4, 3]).all()
     for i in (0, 65, 128):
         check_attention(dtype, q[i:i + 1], k, v, table[:1], [0, 1], [6001 + i], got[i:i + 1], d ** -0.5)
+
+
+def test_attention_waits_for_rows_that_are_computed_again_however_many():
+    """A value that every row sees is infinite: all rows of every unit, one after another over 12000 keys, while the kernel's other roles wait."""
+    import torch
+    from paged_util import attention_inputs, check_attention
+    rng = np.random.default_rng(31)
+    q, k, v, table, starts, lengths = attention_inputs(rng, "bf16", 32, 8, 128, 64, [12000], [1200])
+    clean = attend(q, k, v, table, starts, lengths, 1200)
+    at = int(table[0, 1]) * 64 + 9
+    old = v.flatten(0, 1)[at, :, 77].clone()
+    v.flatten(0, 1)[at, :, 77] = -math.inf
+    got = attend(q, k, v, table, starts, lengths, 1200)            # asks for the waits that ran out
+    v.flatten(0, 1)[at, :, 77] = old
+    assert not torch.isfinite(got[..., 77]).any()
+    got[..., 77] = clean[..., 77]
+    for i in rng.integers(0, 1200, 12).tolist():
+        check_attention("bf16", q[i:i + 1], k, v, table, [0, 1], [12001 + i], got[i:i + 1], 128 ** -0.5)
