@@ -5,7 +5,8 @@
 // four warps of a CTA split the keys: each takes 16 of a block of 64, has a ring of its own for their keys and values, filled by
 // TMA boxes of 16 keys by 64 elements that run across the borders of units, and an online softmax of its own; nothing in the loop waits for another warp.  At a
 // unit's end the four sums are joined in shared memory.  Scores, maxima and sums are f32; a weight enters its product as the sum of two 16-bit values (the
-// tensor cores have time for both), so only the result is rounded.
+// tensor cores have time for both): 2^-18 of it is lost for bf16, 2^-22 for f16, whose weights are 2^15 times as large as they should be, sums too, so that
+// what both parts drop is below 2^-40 of the largest weight instead of 2^-25.  So the result is what is rounded.
 // More pairs than 16 are units of their own that find the keys in L2: 32 sequences of up to 20 pairs (323 MB) take 69 us, with two blocks of rows per warp
 // 103 us, on tcgen05 115 us; of 32 pairs each 118 and 107 us, four sequences of 32 pairs 29 and 40 us.  From 33 pairs on they are mgq_paged_prefill.cu's.
 // With 16-byte cp.async instead of boxes a step took 627 instructions and 64 single tokens of the Qwen3-8B shape 242 us.
@@ -88,6 +89,7 @@ template <typename T, int D>                             // D: head size rounded
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const __grid_constant__ CacheMaps maps, const AttendArgs a)
 {
     constexpr int NT = D / 8, KT = D / 16, PARTS = D / 64;
+    constexpr float kUp = std::is_same<T, __half>::value ? 32768.f : 1.f;       // weights and their sums
     constexpr uint32_t kStage = stage_bytes<D>();
     using Way = Walk<kRows, kBlock, kExtra>;
     extern __shared__ uint8_t s_raw[];
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 for (int n = 0; n < 2; n++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float p = exp2_fast(s[n][2 * half + e] - base);
+                        const float p = exp2_fast(s[n][2 * half + e] - base) * kUp;
                         s[n][2 * half + e] = p;
                         l[half] += p;
                     }
