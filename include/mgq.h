@@ -274,9 +274,10 @@ int mgq_argmax(const float *logits, uint32_t n, void *workspace, uint32_t *out_t
  *   (q may be NULL: keys and values only).  Sources are f32 or of the cache's type; their rows are `pitch` elements apart.  Values
  *   are rounded to nearest.  Slots must differ from one another, else what the cache row holds is open.
  * mgq_paged_attention: each new token's query heads over the tokens of its sequence up to itself, with window > 0 over the last
- *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  What a
- *   row does not see has no part in it, whatever it holds; a row that sees nothing, or only scores of -inf, is zero, one that sees an
- *   infinite value infinite or NaN; rows behind the last sequence are left as they are.  max_fresh: no sequence has more new tokens in
+ *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  In f16 and bf16 the
+ *   result is rounded once; where a sequence has more than 32 new tokens times heads per key / value head (head_dim up to 128), each weight is
+ *   rounded to the type as well before it meets its value.  What a row does not see has no part in it, whatever it holds; a row that sees
+ *   nothing, or only scores of -inf, is zero, one that sees an infinite value infinite or NaN (or without it, where its weight is below f32's range); rows behind the last sequence are left as they are.  max_fresh: no sequence has more new tokens in
  *   this step (it chooses kernels; where it does not hold the call takes longer).  head_dim at most 256.  `workspace`:
  *   mgq_paged_attention_workspace(...) bytes for the same arguments, 16-byte aligned, in any state; calls that may run at the same time
  *   (two streams, two graphs) need one each.

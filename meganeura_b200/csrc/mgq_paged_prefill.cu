@@ -12,8 +12,10 @@
 //   warp 9          issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
 //                   S(j + 1) done knows that O(j) is.  O(j) begins when the weights of the first 64 keys are there.
 //   warp 10         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
-// Sums are kept relative to a maximum that may be 2^8 too low: only where a row's maximum grows by more is O scaled.  Weights are
-// rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.
+// Sums are kept relative to a maximum that may be 2^8 too low, in f16 2^7: only where a row's maximum grows by more is O scaled.  Weights are
+// rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.  f16 weights are relative to 2^-8
+// of that maximum, so that they go up to 2^15, have all their bits down to 2^-22 of it and are not lost above 2^-33 (to 2^-25 in steps of 2^-36 it was 8 % slower
+// in f16, because the maximum may then grow by 2^4 only).
 // TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
 #include <cfloat>
 #include <cstdint>
@@ -28,6 +30,9 @@ constexpr int kExtra = 2;                                // blocks of keys that 
 // Exponents are score * scale - m in one rounding, m is rounded before, by up to 2^-24 of its size.  That is a factor which all weights of a row have in common, but
 // beyond some size it takes them out of their type's range (from 2^27 on infinite f16 weights, from 2^34 rows of zeros): such rows are computed again.
 constexpr float kHuge = 0x1p20f;
+// How far below a row's maximum m lies when it is set, and how far above m the maximum may grow, in powers of two.
+template <typename T> constexpr float kUnder = std::is_same<T, __half>::value ? 8.f : 0.f;
+template <typename T> constexpr float kRoom = std::is_same<T, __half>::value ? 15.f : 8.f;
 constexpr uint32_t kKeys = 128, kTile = 128;             // keys of a block, rows of a tile
 constexpr uint32_t kHalf = kKeys * 128;                  // 128 rows of 64 elements
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return D / 64 * kHalf; }
@@ -644,12 +649,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 wait_row(t);
                 mask(t, 1);
                 const float second = row_max(t), top = max3(first, second, second) * scale;
-                // Nothing to do where the maximum stays at or below the old one + 8 (finite behind the first block); -inf and NaN come here, too.
-                if (__any_sync(0xffffffffu, !(top <= m + 8.f && top >= -FLT_MAX))) {
-                    const bool up = !(top <= m + 8.f) && top > -INFINITY;              // also where m is still -inf
-                    const float keep = up ? exp2_fast(m - top) : 1.f;
+                // Nothing to do where the maximum stays at or below m + kRoom (finite behind the first block); -inf and NaN come here, too.
+                if (__any_sync(0xffffffffu, !(top <= m + kRoom<T> && top >= -FLT_MAX))) {
+                    const bool up = !(top <= m + kRoom<T>) && top > -INFINITY;              // also where m is still -inf
+                    const float under = up ? top - kUnder<T> : m, keep = up ? exp2_fast(m - under) : 1.f;
                     l *= keep;
-                    m = up ? top : m;
+                    m = under;
                     huge |= up && fabsf(top) > kHuge;
                     if (kb != begin && __any_sync(0xffffffffu, up)) {
 #pragma unroll 1

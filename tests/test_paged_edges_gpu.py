@@ -254,8 +254,8 @@ def test_attention_waits_for_rows_that_are_computed_again_however_many():
         check_attention("bf16", q[i:i + 1], k, v, table, [0, 1], [12001 + i], got[i:i + 1], 128 ** -0.5)
 
 
-@pytest.mark.parametrize("dtype,heads,kv_heads,d,fresh", [("f16", 8, 2, 128, 1), ("f16", 8, 2, 64, 5), ("f16", 4, 2, 256, 1), ("bf16", 8, 2, 128, 1), ("bf16", 8, 2, 128, 60),
-                                                          ("f32", 4, 2, 64, 1), ("f32", 4, 2, 64, 40)])
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,fresh", [("f16", 8, 2, 128, 1), ("f16", 8, 2, 64, 5), ("f16", 4, 2, 256, 1), ("f16", 8, 2, 128, 60), ("f16", 3, 1, 64, 200),
+                                                          ("bf16", 8, 2, 128, 1), ("bf16", 8, 2, 128, 60), ("f32", 4, 2, 64, 1), ("f32", 4, 2, 64, 40)])
 @pytest.mark.parametrize("score", [-10.0, -17.0, -20.0, -24.0])
 @pytest.mark.parametrize("place", ["first", "middle", "last"])
 def test_attention_keeps_small_weights_beside_one_that_dominates(dtype, heads, kv_heads, d, fresh, score, place):
@@ -280,10 +280,10 @@ def test_attention_keeps_small_weights_beside_one_that_dominates(dtype, heads, k
         for h in range(0, heads, 2):
             x = values[:n, h * kv_heads // heads]
             want = w @ x / w.sum()
-            # A weight is off by 2^-17 (the exponent's rounding and the exponential), of many tokens by half a step of its type; f16 keeps weights down to 2^-36
-            # (many tokens) or 2^-40 (few) of the largest.  A sum that holds the 1 first loses up to 2^-25 with each addition behind it: of up to 600 parts that are
-            # joined one by one, and in a part of a few dozen more, in numerator and denominator.  The result is rounded once, in f16 to a multiple of 2^-24 at least.
-            least = 0.0 if dtype != "f16" else 2.0 ** -36 if many else 2.0 ** -40
+            # A weight is off by 2^-17 (the exponent's rounding and the exponential), of many tokens by half a step of its type; f16 rounds it to a multiple of 2^-32
+            # (many tokens) or 2^-39 (few) of the largest.  A sum that holds the 1 first loses up to 2^-25 with each addition behind it: of up to 600 parts that
+            # are joined one by one, and in a part of a few dozen more, in numerator and denominator.  The result is rounded once, in f16 to a multiple of 2^-24.
+            least = 0.0 if dtype != "f16" else 2.0 ** -33 if many else 2.0 ** -40
             weight = 2.0 ** -17 + 2 * 640 * 2.0 ** -25 + (EPS[dtype] / 2 if many and dtype != "f32" else 0.0)
             bound = EPS[dtype] / 2 * want + weight * want + least * x.sum(0) / w.sum() + 2.0 ** -25
             off = np.abs(got[i, h] - want)
