@@ -8,6 +8,8 @@ namespace {
 bool known(int dtype) { return dtype == MGQ_FMT_F32 || dtype == MGQ_FMT_F16 || dtype == MGQ_FMT_BF16; }
 uintptr_t element(int dtype) { return dtype == MGQ_FMT_F32 ? 4 : 2; }
 bool odd(const void *p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+// Whether one of several words' or floats' arrays does not begin on 4 bytes.
+template <typename... P> bool odd_words(const P *...p) { return (odd(p, 4) || ...); }
 
 int check_pages(const char *what, uint32_t page_size, uint32_t pages)
 {
@@ -43,6 +45,7 @@ int mgq_paged_plan(const uint32_t *cached, const uint32_t *fresh, uint32_t seque
         return fail(MGQ_ERR_NULL, "paged_plan: null pointer");
     if (int rc = check_table("paged_plan", sequences, page_size, pages, table_width)) return rc;
     if (rows == 0 || rows >= (1u << 31)) return fail(MGQ_ERR_SHAPE, "paged_plan: %u rows", rows);
+    if (odd_words(cached, fresh, table, held, free_pages, free_count, starts, lengths, positions, slots, lacking)) return fail(MGQ_ERR_ALIGN, "paged_plan: misaligned pointer");
     return launch_paged_plan(cached, fresh, sequences, page_size, table, table_width, held, free_pages, pages, free_count, rows, starts, lengths, positions, slots, lacking,
                              stream);
 }
@@ -52,6 +55,7 @@ int mgq_paged_trim(const uint32_t *lengths, uint32_t sequences, uint32_t page_si
 {
     if (!lengths || !table || !held || !free_pages || !free_count) return fail(MGQ_ERR_NULL, "paged_trim: null pointer");
     if (int rc = check_table("paged_trim", sequences, page_size, pages, table_width)) return rc;
+    if (odd_words(lengths, table, held, free_pages, free_count)) return fail(MGQ_ERR_ALIGN, "paged_trim: misaligned pointer");
     return launch_paged_trim(lengths, sequences, page_size, table, table_width, held, free_pages, pages, free_count, stream);
 }
 
@@ -71,7 +75,8 @@ int mgq_paged_append(const void *q, const void *k, const void *v, int src_dtype,
         return fail(MGQ_ERR_SHAPE, "paged_append: rows of %u, %u and %u elements are shorter than their heads", q_pitch, k_pitch, v_pitch);
     if (!(theta >= 0.f) || theta > 1e30f) return fail(MGQ_ERR_SHAPE, "paged_append: theta %g", (double)theta);
     const uintptr_t src = element(src_dtype), dst = element(cache_dtype);
-    if (odd(q, src) || odd(k, src) || odd(v, src) || odd(q_out, dst) || odd(k_cache, dst) || odd(v_cache, dst)) return fail(MGQ_ERR_ALIGN, "paged_append: misaligned pointer");
+    if (odd(q, src) || odd(k, src) || odd(v, src) || odd(q_out, dst) || odd(k_cache, dst) || odd(v_cache, dst) || odd_words(positions, slots))
+        return fail(MGQ_ERR_ALIGN, "paged_append: misaligned pointer");
     if (q && q == q_out && (src_dtype != cache_dtype || (rows > 1 && q_pitch != q_heads * head_dim)))
         return fail(MGQ_ERR_SHAPE, "paged_append: queries rotated in place must be of the cache's type and dense");
     return launch_paged_append(q, k, v, src_dtype, positions, slots, q_out, k_cache, v_cache, cache_dtype, rows, q_heads, kv_heads, head_dim, q_pitch, k_pitch, v_pitch,
@@ -96,7 +101,7 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
     if (rows == 0 || rows >= (1u << 31) || max_fresh == 0) return fail(MGQ_ERR_SHAPE, "paged_attention: %u rows, at most %u of a sequence", rows, max_fresh);
     if (q_pitch < heads * head_dim || out_pitch < heads * head_dim) return fail(MGQ_ERR_SHAPE, "paged_attention: rows of %u and %u elements are shorter than %u heads of %u", q_pitch, out_pitch, heads, head_dim);
     const uintptr_t e = element(dtype);
-    if (odd(q, e) || odd(k_cache, e) || odd(v_cache, e) || odd(out, e) || odd(workspace, 16)) return fail(MGQ_ERR_ALIGN, "paged_attention: misaligned pointer");
+    if (odd(q, e) || odd(k_cache, e) || odd(v_cache, e) || odd(out, e) || odd(workspace, 16) || odd_words(table, starts, lengths)) return fail(MGQ_ERR_ALIGN, "paged_attention: misaligned pointer");
     return launch_paged_attention(q, k_cache, v_cache, dtype, table, starts, lengths, out, sequences, rows, max_fresh, heads, kv_heads, head_dim, page_size, pages,
                                   table_width, q_pitch, out_pitch, scale, window, workspace, stream);
 }
@@ -106,6 +111,7 @@ int mgq_token_probs(const float *logits, uint32_t pitch, const float *temperatur
     if (!logits || !out) return fail(MGQ_ERR_NULL, "token_probs: null pointer");
     if (rows == 0 || rows >= (1u << 31) || vocab == 0 || vocab >= (1u << 31)) return fail(MGQ_ERR_SHAPE, "token_probs: %u rows of %u", rows, vocab);
     if (pitch < vocab || out_pitch < vocab) return fail(MGQ_ERR_SHAPE, "token_probs: rows %u and %u apart are shorter than the vocabulary of %u", pitch, out_pitch, vocab);
+    if (odd_words(logits, temperature, out)) return fail(MGQ_ERR_ALIGN, "token_probs: misaligned pointer");
     return launch_token_probs(logits, pitch, temperature, out, out_pitch, rows, vocab, stream);
 }
 
@@ -118,6 +124,7 @@ int mgq_verify_drafts(const float *target, uint32_t target_pitch, const float *d
         return fail(MGQ_ERR_SHAPE, "verify_drafts: %u sequences, %u rows of %u", sequences, rows, vocab);
     if (target_pitch < vocab || (draft && draft_pitch < vocab))
         return fail(MGQ_ERR_SHAPE, "verify_drafts: rows %u and %u apart are shorter than the vocabulary of %u", target_pitch, draft_pitch, vocab);
+    if (odd_words(target, draft, tokens, starts, accept, sample, accepted, next, out)) return fail(MGQ_ERR_ALIGN, "verify_drafts: misaligned pointer");
     return launch_verify_drafts(target, target_pitch, draft, draft_pitch, tokens, starts, accept, sample, accepted, next, out, sequences, rows, vocab, stream);
 }
 
