@@ -159,6 +159,11 @@ def __getattr__(name: str):
     return globals()[name]
 
 
-__all__ = [*_PAGED, "Plan", "set_option", "device_status", "packed_bytes", "quantize", "dequantize", "shard_columns", "matmul", "matmul_host",
+def __dir__():
+    return sorted({*globals(), *_PAGED})
+
+
+# without _PAGED: `from ops import *` takes every name in here, and would import torch for them
+__all__ = ["Plan", "set_option", "device_status", "packed_bytes", "quantize", "dequantize", "shard_columns", "matmul", "matmul_host",
            "FMT_Q4", "FMT_Q8", "A_F32", "A_BF16"]
 _ = _lib
