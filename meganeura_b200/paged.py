@@ -17,7 +17,9 @@ NO_SLOT = NO_PAGE = NO_TOKEN = -1           # MGQ_NO_SLOT and its like as they r
 
 _FORMATS = {torch.float32: FMT_F32, torch.float16: FMT_F16, torch.bfloat16: FMT_BF16}
 _i32, _f32 = torch.int32, torch.float32
-_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# what torch.cuda.current_device and current_stream ask, without their checks (2 us of a call); a torch without CUDA has neither
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 class PagedStep(NamedTuple):

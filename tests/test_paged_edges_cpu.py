@@ -29,3 +29,13 @@ def test_all_of_ops_is_imported_without_torch_and_its_lazy_names_are_found():
           "from meganeura_b200 import ops\n"
           "assert callable(matmul) and 'paged_plan' in dir(ops)\n")
     child("from meganeura_b200 import ops\nassert callable(ops.verify_drafts) and ops.NO_SLOT == -1\n")
+
+
+def test_a_torch_without_cuda_imports_the_operators_and_they_refuse_its_tensors():
+    child("import torch\n"
+          "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+          "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+          "from meganeura_b200 import ops\n"
+          "try: ops.token_probs(torch.zeros(2, 8))\n"
+          "except ValueError: pass\n"
+          "else: raise SystemExit(1)\n")
