@@ -55,6 +55,13 @@ def _refuse(device: int, **wanted):
     raise AssertionError("nothing to refuse")
 
 
+def _words(**values):
+    """Refuses whole numbers that a 32-bit word of the C entries would cut."""
+    for name, value in values.items():
+        if not 0 <= value < 1 << 32:
+            raise ValueError(f"{name} {value} is not from 0 to 2^32 - 1")
+
+
 def _pitch(name: str, t, device: int, inner: int) -> int:
     """Elements from row to row of a tensor whose rows of `inner` elements are contiguous."""
     if t.is_contiguous() and t.get_device() == device:
@@ -104,6 +111,8 @@ def paged_plan(cached, fresh, table, held, free_pages, free_count, page_size: in
     """
     device, sequences, width = _table(table)
     each, one = (sequences,), (1,)
+    if not (0 <= page_size < 1 << 32 and 0 <= rows < 1 << 32):
+        _words(page_size=page_size, rows=rows)
     if not (_is(cached, _i32, device, each) and _is(fresh, _i32, device, each) and _is(held, _i32, device, each) and _is(free_count, _i32, device, one)
             and free_pages.dim() == 1 and _is(free_pages, _i32, device, free_pages.shape)):
         _refuse(device, cached=(cached, _i32, each), fresh=(fresh, _i32, each), held=(held, _i32, each), free_count=(free_count, _i32, one), free_pages=(free_pages, _i32, (None,)))
@@ -127,6 +136,8 @@ def paged_trim(lengths, table, held, free_pages, free_count, page_size: int, str
     """Returns the pages behind the first lengths[s] tokens of each sequence to the pool (mgq_paged_trim)."""
     device, sequences, width = _table(table)
     each, one = (sequences,), (1,)
+    if not 0 <= page_size < 1 << 32:
+        _words(page_size=page_size)
     if not (_is(lengths, _i32, device, each) and _is(held, _i32, device, each) and _is(free_count, _i32, device, one) and free_pages.dim() == 1
             and _is(free_pages, _i32, device, free_pages.shape)):
         _refuse(device, lengths=(lengths, _i32, each), held=(held, _i32, each), free_count=(free_count, _i32, one), free_pages=(free_pages, _i32, (None,)))
@@ -192,6 +203,9 @@ def paged_attention(q, k_cache, v_cache, table, starts, lengths, max_fresh: int,
         _refuse(device, table=(table, _i32, (None, None)), starts=(starts, _i32, (sequences + 1,)), lengths=(lengths, _i32, (sequences,)))
     if window < 0 or max_fresh < 1:
         raise ValueError(f"window {window} is negative or max_fresh {max_fresh} not positive")
+    if window >> 31:                                    # no sequence is that long
+        window = 0
+    most = min(max_fresh, 0xFFFFFFFF)
     q_pitch = _pitch("q", q, device, heads * d)
     if out is not None and (out.dtype is not dtype or out.shape != q.shape):
         raise ValueError("out must have the shape and the type of q")
@@ -199,9 +213,9 @@ def paged_attention(q, k_cache, v_cache, table, starts, lengths, max_fresh: int,
 
     def call(sp):
         o = torch.zeros((rows, heads, d), dtype=dtype, device=q.device) if out is None else out
-        room = torch.empty(_attention_workspace(heads, kv_heads, d, max_fresh, fmt), dtype=torch.uint8, device=q.device)
+        room = torch.empty(_attention_workspace(heads, kv_heads, d, most, fmt), dtype=torch.uint8, device=q.device)
         check(lib.mgq_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), fmt, table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), o.data_ptr(),
-                                      sequences, rows, max_fresh, heads, kv_heads, d, page_size, pages, width, q_pitch, _pitch("out", o, device, heads * d),
+                                      sequences, rows, most, heads, kv_heads, d, page_size, pages, width, q_pitch, _pitch("out", o, device, heads * d),
                                       d ** -0.5 if scale is None else scale, window, room.data_ptr(), sp))
         return o
     return _on(device, stream, call)

@@ -288,3 +288,23 @@ def test_attention_keeps_small_weights_beside_one_that_dominates(dtype, heads, k
             bound = EPS[dtype] / 2 * want + weight * want + least * x.sum(0) / w.sum() + 2.0 ** -25
             off = np.abs(got[i, h] - want)
             assert (off <= bound).all(), (i, h, (off / bound).max())
+
+
+# ---------------------------------------------------------------------------------------------- what the Python side hands on
+
+def test_whole_numbers_beyond_32_bits_are_refused_or_mean_what_they_say():
+    import torch
+    from meganeura_b200 import ops
+    from paged_util import attention_inputs, words
+    rng = np.random.default_rng(3)
+    w = words(np.zeros(2))
+    for page_size, rows in ((2 ** 32 + 16, 8), (-16, 8), (16, 2 ** 32 + 8)):
+        with pytest.raises(ValueError):
+            ops.paged_plan(w, w, words(np.zeros((2, 4))), w.clone(), words(np.zeros(8)), w[:1].clone(), page_size, rows)
+    with pytest.raises(ValueError):
+        ops.paged_trim(w, words(np.zeros((2, 4))), w.clone(), words(np.zeros(8)), w[:1].clone(), 2 ** 32 + 16)
+    q, k, v, table, starts, lengths = attention_inputs(rng, "bf16", 4, 2, 64, 16, [60, 9], [50, 1])
+    want = attend(q, k, v, table, starts, lengths, 50)
+    for window in (2 ** 31, 2 ** 32 + 5, 2 ** 63):
+        assert torch.equal(attend(q, k, v, table, starts, lengths, 50, window=window), want)
+    assert torch.equal(attend(q, k, v, table, starts, lengths, 2 ** 32 + 1), want)
