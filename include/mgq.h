@@ -312,7 +312,7 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
  *   accept[r] * draft[r, it] < target[r, it] (draft NULL: accept[r] < target[r, it]); accepted[s] counts them.  Then next[s] is drawn: behind a draft
  *   that is not kept from max(target - draft, 0) (draft NULL: from target without it; where nothing is left from target), behind the
  *   last one from target: the lowest index at which the running sum exceeds sample[s] times the whole.  out[r] has the kept tokens, then next,
- *   then MGQ_NO_TOKEN.  Sums are in 64 bits; entries that are negative, infinite or NaN count as 0; rows need not sum to 1.  next is
+ *   then MGQ_NO_TOKEN; rows behind the last sequence are left as they are.  Sums are in 64 bits; entries that are negative, infinite or NaN count as 0; rows need not sum to 1.  next is
  *   MGQ_NO_TOKEN where target has no mass, and for a sequence without rows.  A sequence of one row has no drafts: its next token is sampled.
  * Rows are `pitch` elements apart; all values f32.  Outputs of mgq_verify_drafts must not overlap its inputs. */
 int mgq_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream);

@@ -250,7 +250,8 @@ def verify_drafts(target, draft, tokens, starts, accept, sample, out=None, strea
 
     target, draft: [rows, vocab] float32 probabilities (draft None: chosen outright); tokens: [rows] int32, each sequence's last token and its drafts; starts:
     [sequences + 1] int32; accept: [rows], sample: [sequences] float32 in [0, 1).  Returns (accepted [sequences], next [sequences],
-    tokens [rows]: kept drafts, next, then NO_TOKEN), into the three tensors of `out` where given.
+    tokens [rows]: kept drafts, next, then NO_TOKEN), into the three tensors of `out` where given; rows behind the last sequence keep what they hold (NO_TOKEN
+    where out is None).
     """
     device, rows, vocab, t_pitch = _logits("target", target)
     sequences = starts.shape[0] - 1
@@ -266,7 +267,10 @@ def verify_drafts(target, draft, tokens, starts, accept, sample, out=None, strea
         _refuse(device, accepted=(out[0], _i32, each), next=(out[1], _i32, each), out=(out[2], _i32, row))
 
     def call(sp):
-        o = tuple(torch.empty(n, dtype=_i32, device=target.device) for n in (sequences, sequences, rows)) if out is None else tuple(out)
+        if out is None:
+            o = (*torch.empty((2, sequences), dtype=_i32, device=target.device), torch.full((rows,), NO_TOKEN, dtype=_i32, device=target.device))
+        else:
+            o = tuple(out)
         check(lib.mgq_verify_drafts(target.data_ptr(), t_pitch, None if draft is None else draft.data_ptr(), d_pitch, tokens.data_ptr(), starts.data_ptr(), accept.data_ptr(),
                                     sample.data_ptr(), o[0].data_ptr(), o[1].data_ptr(), o[2].data_ptr(), sequences, rows, vocab, sp))
         return o

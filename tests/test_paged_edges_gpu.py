@@ -308,3 +308,14 @@ def test_whole_numbers_beyond_32_bits_are_refused_or_mean_what_they_say():
     for window in (2 ** 31, 2 ** 32 + 5, 2 ** 63):
         assert torch.equal(attend(q, k, v, table, starts, lengths, 50, window=window), want)
     assert torch.equal(attend(q, k, v, table, starts, lengths, 2 ** 32 + 1), want)
+
+
+def test_verified_tokens_of_rows_behind_the_last_sequence_are_none():
+    import torch
+    from meganeura_b200 import ops
+    from paged_util import words
+    p = torch.softmax(torch.randn(40, 100, device="cuda"), 1)
+    for _ in range(3):
+        torch.full((4000,), 77, dtype=torch.int32, device="cuda")                      # what new tensors may hold
+        got = ops.verify_drafts(p, None, words(np.arange(40)), words([0, 3, 5]), torch.rand(40, device="cuda"), torch.rand(2, device="cuda"))
+        assert got[0].shape == got[1].shape == (2,) and got[2].shape == (40,) and (got[2][5:] == ops.NO_TOKEN).all()
