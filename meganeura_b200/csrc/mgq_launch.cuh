@@ -46,14 +46,21 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-// A float of the same shared variable in CTA `rank` of the cluster.
-__device__ __forceinline__ float cluster_load(const float *p, uint32_t rank)
+// A 4- or 8-byte value of the same shared variable in CTA `rank` of the cluster.
+template <typename T>
+__device__ __forceinline__ T cluster_load(const T *p, uint32_t rank)
 {
     uint32_t addr;
-    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+    if constexpr (sizeof(T) == 8) {
+        unsigned long long v;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+        return *reinterpret_cast<T *>(&v);
+    } else {
+        uint32_t v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+        return *reinterpret_cast<T *>(&v);
+    }
 }
 
 // Opts a kernel into more than 48 KB of shared memory, static part included (a no-op for the driver when repeated).
@@ -112,6 +119,14 @@ __device__ __forceinline__ void load8(const float *p, float (&f)[8])
 {
     const float4 a = *reinterpret_cast<const float4 *>(p), b = *(reinterpret_cast<const float4 *>(p) + 1);
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
+// 2^x in one instruction, 2^-22 off at most; results below f32's normal range are 0.
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 __device__ __forceinline__ float sigmoid_f(float z) { return 1.0f / (1.0f + expf(-z)); }

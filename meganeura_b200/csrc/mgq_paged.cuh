@@ -90,9 +90,8 @@ struct Walk {
         return c;
     }
 
-    // Every thread of the block: this CTA's piece.  `scratch`: 40 words of shared memory, free again when the call returns.  Pieces have
-    // at least `least` key blocks where there are that many.
-    __device__ __forceinline__ void begin(const AttendArgs &a, uint32_t cta, uint32_t ctas, uint32_t least, unsigned long long *scratch)
+    // Every thread of the block: this CTA's piece.  `scratch`: 40 words of shared memory, free again when the call returns.
+    __device__ __forceinline__ void begin(const AttendArgs &a, uint32_t cta, uint32_t ctas, unsigned long long *scratch)
     {
         slice = min(a.group, (uint32_t)ROWS);
         slices = (a.group + slice - 1) / slice;
@@ -118,7 +117,7 @@ struct Walk {
             if (w < warp) base += scratch[w];
             total += scratch[w];
         }
-        const unsigned long long pieces = min((unsigned long long)ctas, max(total / least, 1ull));
+        const unsigned long long pieces = min((unsigned long long)ctas, max(total, 1ull));
         const unsigned long long w0 = cta < pieces ? total * cta / pieces : total, w1 = cta < pieces ? total * (cta + 1) / pieces : total;
         if (w0 >= base && w0 < base + mine) {            // one thread at most
             unsigned long long rest = w0 - base, c = 0;

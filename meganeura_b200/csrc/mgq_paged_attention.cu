@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
     pdl_launch_dependents();
     pdl_wait();
     Walk<ROWS, kKeys, 0> walk;
-    walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
+    walk.begin(a, blockIdx.x, gridDim.x, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 
     Segment g;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Atte
     pdl_launch_dependents();
     pdl_wait();
     Walk<kTileRows, kTileKeys, 1> walk;
-    walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
+    walk.begin(a, blockIdx.x, gridDim.x, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 
     Segment g;

@@ -67,12 +67,6 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t &high, uin
         low = *reinterpret_cast<const uint32_t *>(&l);
     }
 }
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // Whether one of 8 values of T is infinite or NaN.
 template <typename T>
 __device__ __forceinline__ bool not_finite8(const uint4 &v)
@@ -113,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
     pdl_wait();
     {
         Way way;
-        way.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
+        way.begin(a, blockIdx.x, gridDim.x, s_walk);
         if (lane == 0) s_way[warp] = way;
     }
     if (t == 0) clear_parts(a, blockIdx.x);

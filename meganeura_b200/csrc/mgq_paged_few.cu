@@ -22,13 +22,6 @@ __host__ __device__ constexpr int stored(int rows) { return rows < 4 ? 4 : rows;
 // CTAs of an SM, as their registers allow (eight rows in four: 274 us for 195).
 __host__ __device__ constexpr int ctas_per_sm(int rows) { return rows == 8 ? 3 : 4; }
 
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <int R, int L, int C>                           // rows of a unit, lanes of a key, 16-byte pieces of a lane: heads of up to 4 * L * C
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const AttendArgs a)
 {
@@ -40,7 +33,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R)) few_kernel(const Att
     pdl_launch_dependents();
     pdl_wait();
     Walk<R, kBlock, R == 1 ? 1 : 2> walk;                // a unit's end takes as long as two blocks (one row: one)
-    walk.begin(a, blockIdx.x, gridDim.x, 1, s_walk);
+    walk.begin(a, blockIdx.x, gridDim.x, s_walk);
     if (t == 0) clear_parts(a, blockIdx.x);
 
     Segment g;

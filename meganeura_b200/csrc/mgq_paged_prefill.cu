@@ -3,7 +3,7 @@
 // A unit is 256 pairs of token and query head of one key / value head, two tiles of 128 rows that share the keys and values of a block
 // of 128.  Per block and tile S = Q K^T and O += P V are four to eight products of K = 16 each way; the tensor cores need 512 cycles for either (heads
 // of 128; a product of 128 x 128 x 16 takes 64), and the exponentials of a tile, 16 per cycle on the SM, 1024: two tiles in turn keep both busy.  A tile's chain
-// takes 3200 per block (4 x 2048 tokens behind up to 6144: 575 us, 1107 TFLOP/s in a burst).
+// takes 3200 per block (4 x 2048 tokens behind up to 6144, 549 GFLOP: 562 us and 977 TFLOP/s call after call, where the clock falls; 505 to 530 us for a few).
 //   warps 0-3, 4-7  softmax of tile 0 and 1, a row per thread: S from TMEM, running maximum and sum in f32, P back into TMEM over S (as the
 //                   16-bit left operand of the second product), results out of TMEM.  Two warps per row need a barrier per block (280 cycles, 671 us for
 //                   4 x 2048 tokens); four lanes per row read TMEM at half the rate (500 cycles of a block, 653 us).
@@ -12,10 +12,11 @@
 //   warp 9          issues S(j + 1) of a tile right behind O(j) of the same tile: products run in order, so P is read before S overwrites it, and whoever sees
 //                   S(j + 1) done knows that O(j) is.  O(j) begins when the weights of the first 64 keys are there.
 //   warp 10         finds the units, and loads their queries by TMA as soon as the last scores of the unit before are done.
-// Sums are kept relative to a maximum that may be 2^8 too low, in f16 2^7: only where a row's maximum grows by more is O scaled.  Weights are
-// rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.  f16 weights are relative to 2^-8
-// of that maximum, so that they go up to 2^15, have all their bits down to 2^-22 of it and are not lost above 2^-33 (to 2^-25 in steps of 2^-36 it was 8 % slower
-// in f16, because the maximum may then grow by 2^4 only).
+// Sums are kept relative to a maximum that may be 2^8 too low, in f16 2^7: only where a row's maximum grows by more is O scaled.
+// Weights are rounded to the values' type, as the tensor cores take both operands in one type; their sum is of the unrounded ones in f32.  In bf16 that leaves the
+// results of 4 x 2048 tokens 2.19e-3 (2-norm) off the exact ones, where rounding these alone leaves 1.65e-3; with what is dropped as a second operand it
+// was 1.65e-3, too, but 742 us.  f16 weights are relative to 2^-8 of the maximum, so that they go up to 2^15, have all their bits down to 2^-22 of it
+// and are not lost above 2^-33 (relative to 2^-11, with a maximum that may grow by 2^4 only, calls took 8 % longer).
 // TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
 #include <cfloat>
 #include <cstdint>
@@ -65,12 +66,6 @@ template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float x, flo
 {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // The largest; NaN if one is NaN.
 __device__ __forceinline__ float max3(float x, float y, float z)
@@ -363,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const uint32_t slice = min(a.group, kPrefillRows), rows = kPrefillRows / slice * slice;       // heads of a unit, rows that TMA fills
     {
         Way way;
-        way.begin(a, blockIdx.x, gridDim.x, 1, reinterpret_cast<unsigned long long *>(s_q));
+        way.begin(a, blockIdx.x, gridDim.x, reinterpret_cast<unsigned long long *>(s_q));
         if (lane == 0 && (warp == 8 || warp == 10)) sh.way[warp == 10] = way;
     }
     for (uint32_t i = tid; i < (kPrefillRows - rows) * PARTS * 8; i += kThreads) {            // the others are zero for good

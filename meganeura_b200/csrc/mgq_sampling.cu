@@ -15,29 +15,6 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kHold = 4;                                 // groups of four values that a thread reads at once
 constexpr uint32_t kGroup = 4 * kThreads, kSlice = kHold * kGroup;
 
-template <typename T>
-__device__ __forceinline__ T cluster_read(const T *p, uint32_t rank)
-{
-    uint32_t addr;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    if constexpr (sizeof(T) == 8) {
-        unsigned long long v;
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-        return *reinterpret_cast<T *>(&v);
-    } else {
-        uint32_t v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-        return *reinterpret_cast<T *>(&v);
-    }
-}
-
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Four values of a row from column c on; `fill` behind its end.  LAST: they are not read again.
 template <bool WIDE, bool LAST>
 __device__ __forceinline__ void read4(const float *row, uint32_t c, uint32_t end, float fill, float (&v)[4])
@@ -122,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
     if (parts > 1) {
         if (t == 0) x_max = m;
         cluster_sync();
-        m = warp_max(cluster_read(&x_max, lane % parts));
+        m = warp_max(cluster_load(&x_max, lane % parts));
     }
 
     const bool odd = !(fabsf(m) <= FLT_MAX);             // nothing above -inf, or +inf
@@ -142,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
         if (parts > 1) cluster_sync();
         else           __syncthreads();
         at = x_at;
-        for (uint32_t p = 0; parts > 1 && p < parts; p++) at = min(at, cluster_read(&x_at, p));
+        for (uint32_t p = 0; parts > 1 && p < parts; p++) at = min(at, cluster_load(&x_at, p));
     } else {
         if (odd) {                                       // how many are +inf
             sum = 0.f;
@@ -163,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 3) probs_kernel(const float *logits,
         if (parts > 1) {
             if (t == 0) x_sum = sum;
             cluster_sync();
-            sum = warp_sum(lane < parts ? cluster_read(&x_sum, lane) : 0.f);
+            sum = warp_sum(lane < parts ? cluster_load(&x_sum, lane) : 0.f);
         }
     }
     const float scale = sum > 0.f ? 1.f / sum : 0.f;
@@ -303,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs a)
         total = 0.0;
         double base = 0.0;
         for (uint32_t i = 0; i < 8; i++) {
-            tot[i] = i < parts ? (parts > 1 ? cluster_read(&x_sum, i) : whole) : 0.0;
+            tot[i] = i < parts ? (parts > 1 ? cluster_load(&x_sum, i) : whole) : 0.0;
             if (i == part) base = total;
             total += tot[i];
         }
