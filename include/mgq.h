@@ -274,17 +274,19 @@ int mgq_argmax(const float *logits, uint32_t n, void *workspace, uint32_t *out_t
  *   (q may be NULL: keys and values only).  Sources are f32 or of the cache's type; their rows are `pitch` elements apart.  Values
  *   are rounded to nearest.  Slots must differ from one another, else what the cache row holds is open.
  * mgq_paged_attention: each new token's query heads over the tokens of its sequence up to itself, with window > 0 over the last
- *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  In f16 and bf16 the
- *   result is rounded once; where a sequence has more than 32 new tokens times heads per key / value head (head_dim up to 128), each weight is
- *   rounded to the type as well before it meets its value.  What a row does not see has no part in it, whatever it holds; a row that sees
- *   nothing, or only scores of -inf, is zero, one that sees an infinite value infinite or NaN (or without it, where its weight is below f32's range); rows behind the last sequence are left as they are.  max_fresh: no sequence has more new tokens in
- *   this step (it chooses kernels; where it does not hold the call takes longer).  head_dim at most 256.  `workspace`:
- *   mgq_paged_attention_workspace(...) bytes for the same arguments, 16-byte aligned, in any state; calls that may run at the same time
- *   (two streams, two graphs) need one each.
+ *   `window` of these: out = softmax(scale q.k) v, f32 sums.  q, out and the caches have one type (MGQ_FMT_F32, _F16 or _BF16).  In f16 and
+ *   bf16 the result is rounded once; where a sequence has more than 32 new tokens times heads per key / value head (head_dim up to 128),
+ *   each weight is rounded to the type as well before it meets its value.  What a row does not see has no part in it, whatever it holds; a
+ *   row that sees nothing, or only scores of -inf, is zero, one that sees an infinite value infinite or NaN (or without it, where its
+ *   weight is below f32's range); rows behind the last sequence are left as they are.  Of a sequence that the plan did not serve the rows
+ *   mean nothing: they are taken for the last of its cached tokens.  max_fresh: no sequence has more new tokens in this step (it chooses
+ *   kernels; where it does not hold the call takes longer).  head_dim at most 256.  `workspace`: mgq_paged_attention_workspace(...) bytes
+ *   for the same arguments, 16-byte aligned, in any state; calls that may run at the same time (two streams, two graphs) need one each.
  * Calls that change one pool or table must be ordered on one stream.  Outputs must not overlap inputs, except that lengths may be cached
  * (the lengths of the step before) and q_out may be q where that is dense and of the cache's type.  Waits inside the kernels are bounded;
  * one that ran out shows in mgq_device_status.
- * All need table_width * page_size below 2^30, the number of rows below 2^31, and at most MGQ_PAGED_MAX_SEQUENCES sequences. */
+ * All need table_width * page_size below 2^30, the number of rows below 2^31, at most MGQ_PAGED_MAX_SEQUENCES sequences, and pointers that
+ * are multiples of what they point to (MGQ_ERR_ALIGN). */
 #define MGQ_NO_SLOT  0xFFFFFFFFu
 #define MGQ_NO_PAGE  0xFFFFFFFFu
 #define MGQ_NO_TOKEN 0xFFFFFFFFu
