@@ -305,6 +305,38 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
                         void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,
                         uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
 
+/* 8-bit integers with scales in f32: a value is code * scale, codes -127 to 127.
+ *
+ * mgq_quantize_rows: rows of x (f32, f16 or bf16, `pitch` elements apart) as codes[rows, k] and scales[rows]: with top = max |x| of a row, scale = top / 127
+ *   (0 where top < 2^-100) and code = x * (1 / scale) rounded to the nearest whole number, ties to even, every step in f32.  A row with an infinity or NaN has
+ *   codes of 0 and a scale that is not finite, so its values are NaN.  Weights [n, k] are quantized with it, too, a scale per channel.
+ * mgq_matmul_int8: out[m, n] = (sum over k of a[m, k] * w[n, k]) * a_scales[m] * w_scales[n] (+ addend[m, n]).  The sum is exact in 32 bits, so k is at most
+ *   MGQ_INT8_MAX_K (codes of -128 included), the rest f32, rounded once to `dtype`, the type of out and addend (f32, f16 or bf16), whose rows are
+ *   `pitch` elements apart.  k a multiple of 16, a and w dense and on 16 bytes.  out may be addend.
+ *
+ * Paged caches of such codes: k_cache, v_cache [pages][page_size][kv_heads][head_dim] with k_scales, v_scales [pages][page_size / block][kv_heads], a scale for `block`
+ * consecutive tokens of a page and a head (block a power of two from 16 to page_size, head_dim a multiple of 16, pages * page_size below 2^31, caches
+ * on 16 bytes).  Pages, tables, slots and steps are those of the paged operators above, whose words and limits hold here as well.
+ * mgq_paged_append_int8: as mgq_paged_append, for one block and head at a time: old = 0 if the block's first slot is among the rows, else its scale; scale =
+ *   max(old, scale of the new rows' largest); the new rows' codes, and where the scale grew those of the slots that are not written, code * (old / scale)
+ *   to the nearest.  So a block keeps what it holds until its first slot is written again.  Rows of one block stand one behind another, as the plan
+ *   writes them; a value that is not finite makes the block's scale so and its values NaN, until it starts anew.  q_dtype: the type of q_out, f16 or bf16;
+ *   sources are f32 or of that type.
+ * mgq_paged_attention_int8: as mgq_paged_attention with keys and values code * scale; q and out are f16 or bf16 (dtype).  The result is rounded once.  Scales are
+ *   not negative, and values of more than 2^96 may come out infinite.  `workspace`: mgq_paged_attention_int8_workspace(...) bytes, as there. */
+#define MGQ_INT8_MAX_K 131056
+int mgq_quantize_rows(const void *x, int dtype, uint32_t pitch, int8_t *codes, float *scales, uint32_t rows, uint32_t k, void *stream);
+int mgq_matmul_int8(const int8_t *a, const float *a_scales, const int8_t *w, const float *w_scales, const void *addend, void *out, int dtype, uint32_t m, uint32_t k,
+                    uint32_t n, uint32_t addend_pitch, uint32_t out_pitch, void *stream);
+int mgq_paged_append_int8(const void *q, const void *k, const void *v, int src_dtype, const uint32_t *positions, const uint32_t *slots, void *q_out, int q_dtype,
+                          int8_t *k_cache, int8_t *v_cache, float *k_scales, float *v_scales, uint32_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                          uint32_t q_pitch, uint32_t k_pitch, uint32_t v_pitch, uint32_t page_size, uint32_t pages, uint32_t block, float theta, void *stream);
+size_t mgq_paged_attention_int8_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh);
+int mgq_paged_attention_int8(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales, const float *v_scales, int dtype, const uint32_t *table,
+                             const uint32_t *starts, const uint32_t *lengths, void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads,
+                             uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, uint32_t block, uint32_t table_width, uint32_t q_pitch,
+                             uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
+
 /* mgq_token_probs: out[r, :] = softmax(logits[r, :] / temperature[r]); a temperature that is not above 0 gives 1 to the lowest index among the
  *   largest logits (temperature NULL: 1 everywhere), one of +inf the same to every logit above -inf.  out may be logits.  NaN logits count as -inf; a row of
  *   them alone is zero.  Where the largest is +inf those that are share the row.

@@ -77,6 +77,13 @@ SIGNATURES = {
     "mgq_cached_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp]),
     "mgq_argmax_workspace": (_sz, []),
     "mgq_argmax": (_int, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _vp]),
+    "mgq_quantize_rows": (_int, [_vp, _int, _u32, _vp, _vp, _u32, _u32, _vp]),
+    "mgq_matmul_int8": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _u32, _u32, _u32, _u32, _u32, _vp]),
+    "mgq_paged_append_int8": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, ctypes.c_float,
+                                     _vp]),
+    "mgq_paged_attention_int8_workspace": (_sz, [_u32, _u32, _u32, _u32]),
+    "mgq_paged_attention_int8": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, ctypes.c_float,
+                                        _u32, _vp, _vp]),
     "mgq_paged_plan": (_int, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mgq_paged_trim": (_int, [_vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _vp]),
     "mgq_paged_append": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, ctypes.c_float, _vp]),

@@ -1,0 +1,44 @@
+// What the kernels of 8-bit integers share: how a value becomes a code and a scale, and a product's arguments and end.
+#pragma once
+#include <cstdint>
+
+#include "mgq_launch.cuh"
+
+namespace mgq {
+
+// Rows and blocks whose largest magnitude is below are zeros: their scale's inverse would leave f32's range.
+constexpr float kLeast = 0x1p-100f;
+// From the largest magnitude's bit pattern.  Both divisions are rounded to nearest: the same scale and codes as the same formulas anywhere else.
+__device__ __forceinline__ float scale_of(uint32_t top) { return __uint_as_float(top) < kLeast ? 0.f : __uint_as_float(top) / 127.f; }
+__device__ __forceinline__ float inverse_of(float scale) { return scale > 0.f && scale < INFINITY ? 1.f / scale : 0.f; }
+// Four values, in units of their scale, to the nearest whole numbers; NaN is 0.  At most 127 * (1 + 3 * 2^-24) comes in, so nothing is cut off.
+__device__ __forceinline__ uint32_t codes_of(float x, float y, float z, float w)
+{
+    uint32_t v;
+    asm("{\n\t.reg .b32 h;\n\t"
+        "cvt.pack.sat.s8.s32.b32 h, %4, %3, 0;\n\t"
+        "cvt.pack.sat.s8.s32.b32 %0, %2, %1, h;\n\t}"
+        : "=r"(v) : "r"(__float2int_rn(x)), "r"(__float2int_rn(y)), "r"(__float2int_rn(z)), "r"(__float2int_rn(w)));
+    return v;
+}
+
+// out[m, n] = (sum over k of a[m, k] w[n, k]) a_scales[m] w_scales[n] (+ addend[m, n])
+struct ProductArgs {
+    const int8_t *a, *w;
+    const float *a_scales, *w_scales;
+    const void *addend;
+    void *out;
+    uint32_t m, k, n, addend_pitch, out_pitch;
+};
+template <typename T>
+__device__ __forceinline__ void finish(const ProductArgs &a, uint32_t m, uint32_t n, int sum, float a_scale, float w_scale)
+{
+    float y = (float)sum * a_scale * w_scale;
+    if (a.addend) y += to_f32(static_cast<const T *>(a.addend)[(size_t)m * a.addend_pitch + n]);
+    T *out = static_cast<T *>(a.out) + (size_t)m * a.out_pitch + n;
+    if constexpr (sizeof(T) == 4) *out = y;
+    else if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(y);
+    else *out = __float2bfloat16_rn(y);
+}
+
+}  // namespace mgq

@@ -32,6 +32,16 @@ int check_heads(const char *what, uint32_t heads, uint32_t kv_heads, uint32_t he
     if ((unsigned long long)heads * head_dim >= (1ull << 31)) return fail(MGQ_ERR_SHAPE, "%s: %u heads of %u", what, heads, head_dim);
     return MGQ_OK;
 }
+// A cache of codes: its blocks, its heads, and that TMA can address it.
+int check_codes(const char *what, uint32_t page_size, uint32_t pages, uint32_t block, uint32_t kv_heads, uint32_t head_dim, const void *k_cache, const void *v_cache)
+{
+    if (block < 16 || block > page_size || (block & (block - 1))) return fail(MGQ_ERR_SHAPE, "%s: blocks of %u tokens are not a power of two from 16 to the page size %u", what, block, page_size);
+    if ((unsigned long long)pages * page_size >= (1ull << 31)) return fail(MGQ_ERR_SHAPE, "%s: %u pages of %u tokens", what, pages, page_size);
+    if (head_dim % 16) return fail(MGQ_ERR_SHAPE, "%s: head_dim %u is not a multiple of 16", what, head_dim);
+    if ((unsigned long long)kv_heads * head_dim >= (1ull << 31)) return fail(MGQ_ERR_SHAPE, "%s: %u key / value heads of %u", what, kv_heads, head_dim);
+    if (odd(k_cache, 16) || odd(v_cache, 16)) return fail(MGQ_ERR_ALIGN, "%s: the caches must begin on 16 bytes", what);
+    return MGQ_OK;
+}
 
 }  // namespace
 
@@ -104,6 +114,77 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
     if (odd(q, e) || odd(k_cache, e) || odd(v_cache, e) || odd(out, e) || odd(workspace, 16) || odd_words(table, starts, lengths)) return fail(MGQ_ERR_ALIGN, "paged_attention: misaligned pointer");
     return launch_paged_attention(q, k_cache, v_cache, dtype, table, starts, lengths, out, sequences, rows, max_fresh, heads, kv_heads, head_dim, page_size, pages,
                                   table_width, q_pitch, out_pitch, scale, window, workspace, stream);
+}
+
+int mgq_paged_append_int8(const void *q, const void *k, const void *v, int src_dtype, const uint32_t *positions, const uint32_t *slots, void *q_out, int q_dtype,
+                          int8_t *k_cache, int8_t *v_cache, float *k_scales, float *v_scales, uint32_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                          uint32_t q_pitch, uint32_t k_pitch, uint32_t v_pitch, uint32_t page_size, uint32_t pages, uint32_t block, float theta, void *stream)
+{
+    if (!k || !v || !positions || !slots || !k_cache || !v_cache || !k_scales || !v_scales || (q && !q_out)) return fail(MGQ_ERR_NULL, "paged_append_int8: null pointer");
+    if ((q_dtype != MGQ_FMT_F16 && q_dtype != MGQ_FMT_BF16) || (src_dtype != MGQ_FMT_F32 && src_dtype != q_dtype))
+        return fail(MGQ_ERR_FORMAT, "paged_append_int8: sources of type %d, queries of type %d (f16, bf16; sources f32 or the queries' type)", src_dtype, q_dtype);
+    if (int rc = check_pages("paged_append_int8", page_size, pages)) return rc;
+    if (int rc = check_heads("paged_append_int8", q ? q_heads : kv_heads, kv_heads, head_dim)) return rc;
+    if (int rc = check_codes("paged_append_int8", page_size, pages, block, kv_heads, head_dim, k_cache, v_cache)) return rc;
+    if (q && q_heads == 0) return fail(MGQ_ERR_SHAPE, "paged_append_int8: no query heads");
+    if (rows == 0 || (unsigned long long)rows * 2 * kv_heads >= (1ull << 30)) return fail(MGQ_ERR_SHAPE, "paged_append_int8: %u rows of %u heads", rows, kv_heads);
+    if ((q && q_pitch < q_heads * head_dim) || k_pitch < kv_heads * head_dim || v_pitch < kv_heads * head_dim)
+        return fail(MGQ_ERR_SHAPE, "paged_append_int8: rows of %u, %u and %u elements are shorter than their heads", q_pitch, k_pitch, v_pitch);
+    if (!(theta >= 0.f) || theta > 1e30f) return fail(MGQ_ERR_SHAPE, "paged_append_int8: theta %g", (double)theta);
+    const uintptr_t src = element(src_dtype);
+    if (odd(q, src) || odd(k, src) || odd(v, src) || odd(q_out, 2) || odd_words(positions, slots, k_scales, v_scales)) return fail(MGQ_ERR_ALIGN, "paged_append_int8: misaligned pointer");
+    if (q && q == q_out && (src_dtype != q_dtype || (rows > 1 && q_pitch != q_heads * head_dim)))
+        return fail(MGQ_ERR_SHAPE, "paged_append_int8: queries rotated in place must be of the result's type and dense");
+    return launch_paged_append_int8(q, k, v, src_dtype, positions, slots, q_out, q_dtype, k_cache, v_cache, k_scales, v_scales, rows, q_heads, kv_heads, head_dim, q_pitch,
+                                    k_pitch, v_pitch, page_size, pages, block, theta, stream);
+}
+
+size_t mgq_paged_attention_int8_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_fresh)
+{
+    if (heads == 0 || max_fresh == 0 || head_dim % 16 || check_heads("paged_attention_int8_workspace", heads, kv_heads, head_dim)) return 0;
+    return paged_attention_int8_workspace(head_dim);
+}
+
+int mgq_paged_attention_int8(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales, const float *v_scales, int dtype, const uint32_t *table,
+                             const uint32_t *starts, const uint32_t *lengths, void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads,
+                             uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, uint32_t block, uint32_t table_width, uint32_t q_pitch,
+                             uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream)
+{
+    if (!q || !k_cache || !v_cache || !k_scales || !v_scales || !table || !starts || !lengths || !out || !workspace) return fail(MGQ_ERR_NULL, "paged_attention_int8: null pointer");
+    if (dtype != MGQ_FMT_F16 && dtype != MGQ_FMT_BF16) return fail(MGQ_ERR_FORMAT, "paged_attention_int8: queries of type %d (f16, bf16)", dtype);
+    if (int rc = check_table("paged_attention_int8", sequences, page_size, pages, table_width)) return rc;
+    if (int rc = check_heads("paged_attention_int8", heads, kv_heads, head_dim)) return rc;
+    if (int rc = check_codes("paged_attention_int8", page_size, pages, block, kv_heads, head_dim, k_cache, v_cache)) return rc;
+    if (heads == 0) return fail(MGQ_ERR_SHAPE, "paged_attention_int8: no query heads");
+    if (rows == 0 || rows >= (1u << 31) || max_fresh == 0) return fail(MGQ_ERR_SHAPE, "paged_attention_int8: %u rows, at most %u of a sequence", rows, max_fresh);
+    if (q_pitch < heads * head_dim || out_pitch < heads * head_dim)
+        return fail(MGQ_ERR_SHAPE, "paged_attention_int8: rows of %u and %u elements are shorter than %u heads of %u", q_pitch, out_pitch, heads, head_dim);
+    if (odd(q, 2) || odd(out, 2) || odd(workspace, 16) || odd_words(table, starts, lengths, k_scales, v_scales)) return fail(MGQ_ERR_ALIGN, "paged_attention_int8: misaligned pointer");
+    return launch_paged_attention_int8(q, k_cache, v_cache, k_scales, v_scales, dtype, table, starts, lengths, out, sequences, rows, max_fresh, heads, kv_heads, head_dim,
+                                       page_size, pages, block, table_width, q_pitch, out_pitch, scale, window, workspace, stream);
+}
+
+int mgq_quantize_rows(const void *x, int dtype, uint32_t pitch, int8_t *codes, float *scales, uint32_t rows, uint32_t k, void *stream)
+{
+    if (!x || !codes || !scales) return fail(MGQ_ERR_NULL, "quantize_rows: null pointer");
+    if (!known(dtype)) return fail(MGQ_ERR_FORMAT, "quantize_rows: type %d is not f32, f16 or bf16", dtype);
+    if (rows == 0 || rows >= (1u << 31) || k == 0 || k >= (1u << 31)) return fail(MGQ_ERR_SHAPE, "quantize_rows: %u rows of %u", rows, k);
+    if (pitch < k) return fail(MGQ_ERR_SHAPE, "quantize_rows: rows %u apart are shorter than %u", pitch, k);
+    if (odd(x, element(dtype)) || odd_words(scales)) return fail(MGQ_ERR_ALIGN, "quantize_rows: misaligned pointer");
+    return launch_quantize_rows(x, dtype, pitch, codes, scales, rows, k, stream);
+}
+
+int mgq_matmul_int8(const int8_t *a, const float *a_scales, const int8_t *w, const float *w_scales, const void *addend, void *out, int dtype, uint32_t m, uint32_t k,
+                    uint32_t n, uint32_t addend_pitch, uint32_t out_pitch, void *stream)
+{
+    if (!a || !a_scales || !w || !w_scales || !out) return fail(MGQ_ERR_NULL, "matmul_int8: null pointer");
+    if (!known(dtype)) return fail(MGQ_ERR_FORMAT, "matmul_int8: type %d is not f32, f16 or bf16", dtype);
+    if (m == 0 || m >= (1u << 31) || n == 0 || n >= (1u << 31)) return fail(MGQ_ERR_SHAPE, "matmul_int8: %u rows, %u columns", m, n);
+    if (k == 0 || k % 16 || k > MGQ_INT8_MAX_K) return fail(MGQ_ERR_SHAPE, "matmul_int8: k = %u is not a multiple of 16 up to %d", k, MGQ_INT8_MAX_K);
+    if (out_pitch < n || (addend && addend_pitch < n)) return fail(MGQ_ERR_SHAPE, "matmul_int8: rows %u and %u apart are shorter than %u", out_pitch, addend_pitch, n);
+    if (odd(a, 16) || odd(w, 16) || odd(out, element(dtype)) || odd(addend, element(dtype)) || odd_words(a_scales, w_scales))
+        return fail(MGQ_ERR_ALIGN, "matmul_int8: misaligned pointer (codes begin on 16 bytes)");
+    return launch_matmul_int8(a, a_scales, w, w_scales, addend, out, dtype, m, k, n, addend_pitch, out_pitch, stream);
 }
 
 int mgq_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream)

@@ -1,0 +1,608 @@
+// Attention of few new tokens per sequence (single tokens, drafted ones) over a paged cache of 8-bit codes: reads every code once, so HBM bounds it, and what
+// the codes need before they can be multiplied has to fit beside that.
+//
+// A unit's pairs of token and head (8 or 16: heads of one key / value head share its keys) are the columns of m16n8k16 products in f16 whose rows are 16 keys of a
+// head (scores) or 16 of its dimensions (results): codes are the left operand of both, eight pairs cost no more than they are, and the accumulators of eight
+// pairs of 128 are 32 registers.  The order of k inside a product, and of the results' rows, is free, so a lane takes 16 consecutive codes of a key with one
+// load.  A code becomes an f16 exactly: with 0x64 above its biased byte it reads 1024 + 128 + code.
+// Scores: q enters as f16, times a power of two that bf16 rows need to fit its range; a row's is undone in f32 with the block's scale.  Weights: times the
+// block's scale, as the sum of two f16, so that only the result is rounded.  They are relative to a maximum that may be 2^8 too low (kRoom), and to a power of
+// two of the blocks' scales (`e`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from the scores' layout to the right
+// operand's are transposed 8 x 8 at a time (movmatrix).
+// The four warps of a CTA split the keys: each takes 32 of a block of 128, has a ring of its own for their codes and scales, filled by TMA boxes of 16 keys
+// and 4-byte copies that run across the borders of units; nothing in the loop waits for another warp.  At a unit's end the four sums are joined in shared memory.
+#include <cstdint>
+
+#include "mgq_paged_int8.cuh"
+#include "mgq_tcgen05.cuh"
+
+namespace mgq {
+namespace {
+
+constexpr int kThreads = 128, kWarps = 4, kStep = 32, kBlock = kWarps * kStep;      // keys of a warp's step, of all four
+constexpr int kGroups = kStep / 16;                      // 16 keys lie in one page and one block
+constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
+constexpr float kRoom = 8.f;
+constexpr int kUp = 7;                                   // weights are 2^kUp times what they should be: 2^15 at most, and all of their bits down to 2^-21 of the largest
+
+template <int D> __host__ __device__ constexpr uint32_t row_bytes() { return D < 128 ? D : 128; }                  // of a box: 64 or 128, in the swizzle of that size
+template <int D> __host__ __device__ constexpr uint32_t box_bytes() { return 16 * row_bytes<D>(); }
+template <int D> __host__ __device__ constexpr uint32_t group_bytes() { return D / row_bytes<D>() * box_bytes<D>(); }
+template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return 2 * kGroups * group_bytes<D>(); }   // keys of all groups, then values
+template <int D, int NP> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 4 : D == 128 ? (NP == 1 ? 3 : 2) : 1; }
+template <int D> __host__ __device__ constexpr int stages() { return D == 64 ? 3 : D == 128 ? 2 : 3; }
+constexpr int kJoin = 4;                                 // blocks of 16 columns joined at a time
+constexpr uint32_t kJoinPitch = kJoin * 16 + 2;
+template <int D, int NP> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * stages<D>() * stage_bytes<D>() + kWarps * NP * 8 * kJoinPitch * 4; }
+
+__device__ unsigned int g_decode8_error;
+
+struct Maps {
+    CUtensorMap k, v;
+};
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+constexpr uint32_t kBias = 0x80808080u, kHigh = 0x64646464u;
+// Two f16 whose bytes are 0x64 and a biased code each, less 1024 + 128.
+__device__ __forceinline__ uint32_t unbiased(uint32_t v)
+{
+    const uint32_t off = 0x64806480u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&off));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_half(float x, float y)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 2^e for e from -126 to 127.
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <typename T, int D, int NP>                     // D: head size rounded up to 64, 128 or 256; NP: blocks of 8 pairs
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel(const __grid_constant__ Maps maps, const Attend8Args a, bool wide)
+{
+    constexpr int KT = D / 16, S = stages<D>(), PARTS = D / row_bytes<D>();
+    constexpr uint32_t kStage = stage_bytes<D>(), kRow = row_bytes<D>(), kBox = box_bytes<D>(), kGroup = group_bytes<D>();
+    constexpr uint32_t kPer = kRow / 4;                  // consecutive codes of a key that a lane takes for the scores
+    constexpr uint32_t kOwn = kRow / 8;                  // and of a value for the results
+    constexpr uint32_t kWords = kPer / 4;
+    using Way = Walk<8 * NP, kBlock, kExtra>;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ unsigned long long s_walk[40];
+    __shared__ __align__(8) unsigned long long s_full[kWarps][S];
+    __shared__ Way s_way[kWarps];
+    __shared__ Segment s_seg[kWarps][8];
+    __shared__ float s_scale[kWarps][S][kGroups][2];
+    __shared__ int s_have[kWarps][S][kGroups];
+    __shared__ float s_m[kWarps][8 * NP], s_l[kWarps][8 * NP];
+    __shared__ volatile int s_failed;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = __shfl_sync(0xffffffffu, t >> 5, 0), d = a.d;
+    uint8_t *s_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t ring = smem_u32(s_mem) + warp * (S * kStage);
+    float *s_join = reinterpret_cast<float *>(s_mem + (size_t)kWarps * S * kStage);
+    if (t == 0) {
+        for (int i = 0; i < kWarps * S; i++) mbar_init(&s_full[i / S][i % S], 4 * kGroups);      // a box and a scale of keys and of values each
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    {
+        Way way;
+        way.begin(a, blockIdx.x, gridDim.x, s_walk);
+        if (lane == 0) s_way[warp] = way;
+    }
+    if (t == 0) clear_parts(a, blockIdx.x);
+    __syncwarp();
+
+    // ---- the producer's side of a warp: one step of 32 keys at a time, a segment without keys is a step without loads.  Lane = group of 16 keys * 2 + (keys or
+    // values) brings its box and scale; it has looked up its page a step ahead.
+    uint32_t p_seg = 0, p_block = 0, p_end = 0, p_slot = 0;      // segments begun, its next and last block, ring slot
+    bool p_live = true;
+    const uint32_t *p_table = nullptr;
+    int p_len = 0, p_kv = 0;
+    uint32_t p_page = 0xFFFFFFFFu;
+    const uint32_t p_group = lane >> 1 & (kGroups - 1);
+    auto look_up = [&]() {
+        const uint32_t key = p_block * kBlock + warp * kStep + p_group * 16;
+        p_page = p_block < p_end && (int)key < p_len ? p_table[key >> a.page_shift] : 0xFFFFFFFFu;
+    };
+    auto produce = [&]() {
+        if (p_live && p_block >= p_end) {                // the next segment
+            if (lane == 0) {
+                Segment g;
+                const bool more = s_way[warp].next(a, g);
+                g.table = more ? g.table : nullptr;
+                s_seg[warp][p_seg & 7u] = g;
+            }
+            __syncwarp();
+            const Segment &g = s_seg[warp][p_seg & 7u];
+            p_live = g.table != nullptr;
+            if (p_live) {
+                p_seg++;
+                p_table = g.table;
+                p_len = g.end <= g.begin ? 0 : g.len;
+                p_kv = (int)g.kv;
+                p_block = g.begin;
+                p_end = max(g.end, g.begin + 1);
+                look_up();
+            }
+        }
+        if (p_live) {
+            if (lane < 2 * kGroups) {
+                const uint32_t key = p_block * kBlock + warp * kStep + p_group * 16, within = (1u << a.page_shift) - 1;
+                const bool values = lane & 1u, real = p_page < a.pages;         // also: in front of the sequence's end
+                unsigned long long *bar = &s_full[warp][p_slot];
+                const uint32_t scale = smem_u32(&s_scale[warp][p_slot][p_group][values]);
+                if (!values) s_have[warp][p_slot][p_group] = real ? min(16, p_len - (int)key) : 0;       // written before the arrivals that publish it
+                if (real) {
+                    const uint32_t slot = (p_page << a.page_shift) + (key & within), dst = ring + p_slot * kStage + (values * kGroups + p_group) * kGroup;
+                    const float *from = (values ? a.v_scales : a.k_scales) + (size_t)(slot >> a.block_shift) * a.kv_heads + p_kv;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale), "l"(from) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+                    mbar_arrive_expect_tx(bar, kGroup);
+#pragma unroll
+                    for (int c = 0; c < PARTS; c++) tma_load_3d(dst + c * kBox, values ? &maps.v : &maps.k, c * 128, p_kv, (int)slot, bar);
+                } else {
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale), "f"(0.f) : "memory");
+                    mbar_arrive(bar);
+                    mbar_arrive(bar);
+                }
+            }
+            __syncwarp();
+            p_block++;
+            look_up();
+            p_slot = p_slot == S - 1 ? 0 : p_slot + 1;
+        }
+    };
+#pragma unroll 1
+    for (int i = 0; i < S - 1; i++) produce();
+
+    // ---- the consumer's side
+    uint32_t c_seg = 0, slot = 0, parity = 0;
+    bool ok = true;
+    const uint32_t row = lane >> 2, quad = lane & 3u;
+    // byte `at` of row r of a box, as the swizzle of 64 or 128 bytes places its 16-byte pieces
+    auto place = [](uint32_t r, uint32_t at) { return r * kRow + (at ^ (kRow == 128 ? (r & 7u) << 4 : (r >> 1 & 3u) << 4)); };
+    while (c_seg < p_seg) {
+        const Segment g = s_seg[warp][c_seg & 7u];
+        c_seg++;
+        const uint32_t pairs = g.tokens * g.heads;
+        // queries of pair `row` of each block of 8: for part c of 128 dimensions those from c * 128 + quad * kPer on
+        uint32_t q[NP][KT][2];
+        float factor[NP][2];                             // of the pairs 2 quad and 2 quad + 1, whose scores this lane has
+        int pos[NP][2];
+#pragma unroll
+        for (int n = 0; n < NP; n++) {
+            const uint32_t r = n * 8 + row, token = r / g.heads, head = r - token * g.heads;
+            const bool live = r < pairs;
+            const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + (live ? head : 0)) * d;
+            float up = 1.f;
+            T v[PARTS][kPer];
+#pragma unroll
+            for (int c = 0; c < PARTS; c++)
+#pragma unroll
+                for (uint32_t e = 0; e < kPer; e += 8) {
+                    const uint32_t at = c * 128 + quad * kPer + e;              // d is a multiple of 16: all eight or none
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (live && at < d) {
+                        if (wide) {
+                            w = *reinterpret_cast<const uint4 *>(src + at);
+                        } else {
+                            uint16_t x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) x[i] = reinterpret_cast<const uint16_t *>(src)[at + i];
+                            w = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(&v[c][e]) = w;
+                }
+            if constexpr (!std::is_same<T, __half>::value) {
+                uint32_t top = 0;                        // exponents of bf16
+#pragma unroll
+                for (int c = 0; c < PARTS; c++)
+#pragma unroll
+                    for (uint32_t e = 0; e < kPer; e++) top = max(top, (uint32_t)__bfloat16_as_ushort(v[c][e]) & 0x7FFFu);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int exponent = min(max((int)(top >> 7) - 127 - 13, -100), 112);     // the largest becomes 2^13 to 2^14
+                up = power(-exponent);
+                const float f = power(exponent);
+                factor[n][0] = __shfl_sync(0xffffffffu, f, 8 * quad) * a.scale_log2;
+                factor[n][1] = __shfl_sync(0xffffffffu, f, 8 * quad + 4) * a.scale_log2;
+            } else {
+                factor[n][0] = factor[n][1] = a.scale_log2;
+            }
+#pragma unroll
+            for (int c = 0; c < PARTS; c++)
+#pragma unroll
+                for (uint32_t w = 0; w < kWords; w++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const T x = v[c][4 * w + 2 * h], y = v[c][4 * w + 2 * h + 1];
+                        q[n][c * kWords + w][h] = pack_half(to_f32(x) * up, to_f32(y) * up);
+                    }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t p = n * 8 + 2 * quad + e;
+                pos[n][e] = p < pairs ? g.pos0 + (int)(p / g.heads) : -1;
+            }
+        }
+        float o[NP][KT][4], m[NP][2], l[NP][2];
+        int e2 = -1000;                                  // results are relative to 2^e2, the blocks' scales below it
+#pragma unroll
+        for (int n = 0; n < NP; n++) {
+#pragma unroll
+            for (int j = 0; j < KT; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
+        const uint32_t blocks = max(g.end, g.begin + 1) - g.begin;
+        const int last_pos = g.pos0 + (int)g.tokens - 1;
+        for (uint32_t b = 0; b < blocks; b++) {
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode8_error)))) break;
+            const uint32_t base = ring + slot * kStage;
+            int have[kGroups];
+            float ks[kGroups], vs[kGroups];
+#pragma unroll
+            for (int i = 0; i < kGroups; i++) {
+                have[i] = s_have[warp][slot][i];
+                ks[i] = s_scale[warp][slot][i][0];
+                vs[i] = s_scale[warp][slot][i][1];
+            }
+            slot = slot == S - 1 ? 0 : slot + 1;
+            parity ^= slot == 0;
+            produce();
+            const int key0 = (int)((g.begin + b) * kBlock + warp * kStep);
+            if (have[0] + have[kGroups - 1] == 0 || key0 > last_pos) continue;
+            float s[kGroups][NP][4];
+#pragma unroll
+            for (int i = 0; i < kGroups; i++) {
+#pragma unroll
+                for (int n = 0; n < NP; n++) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < PARTS; c++) {
+                    const uint32_t k = base + i * kGroup + c * kBox;
+                    uint32_t w[2][kWords];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (uint32_t e = 0; e < kWords; e += 4) {
+                            const uint4 x = lds16(k + place(row + 8 * h, quad * kPer + 4 * e));
+                            w[h][e] = x.x ^ kBias; w[h][e + 1] = x.y ^ kBias; w[h][e + 2] = x.z ^ kBias; w[h][e + 3] = x.w ^ kBias;
+                        }
+#pragma unroll
+                    for (uint32_t e = 0; e < kWords; e++) {
+                        const uint32_t f[4] = {unbiased(__byte_perm(w[0][e], kHigh, 0x4140)), unbiased(__byte_perm(w[1][e], kHigh, 0x4140)),
+                                               unbiased(__byte_perm(w[0][e], kHigh, 0x4342)), unbiased(__byte_perm(w[1][e], kHigh, 0x4342))};
+#pragma unroll
+                        for (int n = 0; n < NP; n++) mma(s[i][n], f, q[n][c * kWords + e][0], q[n][c * kWords + e][1]);
+                    }
+                }
+            }
+            // keys `row` and `row` + 8 of a group by pairs 2 quad and 2 quad + 1
+            const bool whole = have[0] + have[kGroups - 1] == kStep && key0 + kStep - 1 <= g.pos0 && (!a.window || key0 > last_pos - (int)a.window);
+            bool up = false;
+#pragma unroll
+            for (int i = 0; i < kGroups; i++)
+#pragma unroll
+                for (int n = 0; n < NP; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float x = __fmul_rn(s[i][n][e], factor[n][e & 1] * ks[i]);
+                        if (!whole) {
+                            const int at = (int)row + e / 2 * 8, key = key0 + i * 16 + at, p = pos[n][e & 1];
+                            x = at < have[i] && key <= p && (!a.window || key > p - (int)a.window) ? x : -INFINITY;
+                        }
+                        s[i][n][e] = x;
+                        up |= x > m[n][e & 1] + kRoom;   // never where x is -inf or NaN
+                    }
+            if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                for (int n = 0; n < NP; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float top = m[n][e];
+#pragma unroll
+                        for (int i = 0; i < kGroups; i++) top = fmaxf(top, fmaxf(s[i][n][e], s[i][n][e + 2]));
+#pragma unroll
+                        for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        const float keep = top > m[n][e] ? exp2_fast(m[n][e] - top) : 1.f;
+                        m[n][e] = top;
+                        l[n][e] *= keep;
+#pragma unroll
+                        for (int j = 0; j < KT; j++) {
+                            o[n][j][e] *= keep;
+                            o[n][j][e + 2] *= keep;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < kGroups; i++) {
+                // the block's scale below 2^e2: from 2^-3 on where e2 follows it
+                const int exponent = (int)(__float_as_uint(vs[i]) >> 23 & 255u) - 126;              // vs < 2^exponent; 129 for one that is not finite
+                if (exponent > e2 && exponent < 129) {
+                    const int next = min(exponent + 2, 127);
+                    if (e2 > -1000) {
+                        const float keep = power(max(e2 - next, -126));
+#pragma unroll
+                        for (int n = 0; n < NP; n++)
+#pragma unroll
+                            for (int j = 0; j < KT; j++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[n][j][e] *= keep;
+                    }
+                    e2 = next;
+                }
+                const int shift = kUp - max(e2, -124);                       // vs * 2^shift in two steps, as 2^shift alone may be out of range
+                const float by = vs[i] * power(max(min(shift, 100), -126)) * power(max(shift - 100, 0));
+                uint32_t high[NP][2], low[NP][2];
+#pragma unroll
+                for (int n = 0; n < NP; n++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float x = s[i][n][2 * h + e], p = exp2_fast(__fsub_rn(x, m[n][e] == -INFINITY ? 0.f : m[n][e]));
+                            l[n][e] += p;
+                            w[e] = whole || x != -INFINITY ? p * by : 0.f;                           // no product where nothing is seen: the scale may be anything
+                        }
+                        const __half2 first = __floats2half2_rn(w[0], w[1]);
+                        high[n][h] = transpose(*reinterpret_cast<const uint32_t *>(&first));
+                        low[n][h] = transpose(pack_half(w[0] - __low2float(first), w[1] - __high2float(first)));
+                    }
+                // values of keys 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9, dimensions row * kOwn on: a product's rows are two of them each
+#pragma unroll
+                for (int c = 0; c < PARTS; c++) {
+                    const uint32_t v = base + (kGroups + i) * kGroup + c * kBox;
+                    uint32_t w[4][kOwn / 4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t at = v + place(2 * quad + (k & 1) + (k >> 1) * 8, row * kOwn);
+                        if constexpr (kOwn == 16) {
+                            const uint4 x = lds16(at);
+                            w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
+                        } else {
+                            const uint2 x = lds8(at);
+                            w[k][0] = x.x; w[k][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < kOwn / 4; e++) {
+                        // [a0 b0 a1 b1] and [a2 b2 a3 b3] of the keys a, b
+                        const uint32_t x0 = __byte_perm(w[0][e], w[1][e], 0x5140) ^ kBias, x1 = __byte_perm(w[0][e], w[1][e], 0x7362) ^ kBias;
+                        const uint32_t y0 = __byte_perm(w[2][e], w[3][e], 0x5140) ^ kBias, y1 = __byte_perm(w[2][e], w[3][e], 0x7362) ^ kBias;
+                        const uint32_t f[2][4] = {{unbiased(__byte_perm(x0, kHigh, 0x4140)), unbiased(__byte_perm(x0, kHigh, 0x4342)),
+                                                   unbiased(__byte_perm(y0, kHigh, 0x4140)), unbiased(__byte_perm(y0, kHigh, 0x4342))},
+                                                  {unbiased(__byte_perm(x1, kHigh, 0x4140)), unbiased(__byte_perm(x1, kHigh, 0x4342)),
+                                                   unbiased(__byte_perm(y1, kHigh, 0x4140)), unbiased(__byte_perm(y1, kHigh, 0x4342))}};
+#pragma unroll
+                        for (int n = 0; n < NP; n++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                float (&acc)[4] = o[n][c * (kOwn / 2) + 2 * e + j];
+                                mma(acc, f[j], high[n][0], high[n][1]);
+                                mma(acc, f[j], low[n][0], low[n][1]);
+                            }
+                    }
+                }
+            }
+        }
+
+        if (!ok) break;
+
+        // ---- the four warps' sums
+#pragma unroll
+        for (int n = 0; n < NP; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float sum = l[n][e];
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                if (row == 0) {
+                    s_m[warp][n * 8 + 2 * quad + e] = m[n][e];
+                    s_l[warp][n * 8 + 2 * quad + e] = sum;
+                }
+            }
+        __syncthreads();
+        auto total = [&](uint32_t r, float &top) {
+            top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) sum += s_l[w][r] != 0.f ? s_l[w][r] * exp2_fast(s_m[w][r] - top) : 0.f;
+            return sum;
+        };
+        const float scale2 = power(max(e2, -124)) * (1.f / (1 << kUp));
+#pragma unroll
+        for (int n = 0; n < NP; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t r = n * 8 + 2 * quad + e;
+                const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])), mine = s_l[warp][r] != 0.f ? exp2_fast(m[n][e] - top) : 0.f;
+#pragma unroll
+                for (int j = 0; j < KT; j++) {
+                    o[n][j][e] = mine != 0.f ? o[n][j][e] * mine * scale2 : 0.f;
+                    o[n][j][e + 2] = mine != 0.f ? o[n][j][e + 2] * mine * scale2 : 0.f;
+                }
+            }
+        const bool alone = g.first && g.last;
+        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * (8 * NP) * (d + 2);
+        // kJoin blocks of 16 results at a time: of every lane row's kOwn dimensions (of 128) those from c0 on
+        constexpr int kAt = kJoin < KT ? kJoin : KT, kSpan = 2 * kAt;          // dimensions of a lane row joined at a time
+#pragma unroll
+        for (int j0 = 0; j0 < KT; j0 += kAt) {
+#pragma unroll
+            for (int n = 0; n < NP; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float *dst = s_join + (warp * (8 * NP) + n * 8 + 2 * quad + e) * kJoinPitch + row * kSpan;
+#pragma unroll
+                    for (int j = 0; j < kAt; j++) *reinterpret_cast<float2 *>(dst + 2 * j) = make_float2(o[n][j0 + j][e], o[n][j0 + j][e + 2]);
+                }
+            __syncthreads();
+            for (uint32_t i = t; i < pairs * 8; i += kThreads) {
+                const uint32_t r = i / 8, at = i % 8;
+                const uint32_t per = kOwn / 2, column = j0 / per * 128 + at * kOwn + j0 % per * 2;
+                if (column >= d) continue;
+                float x[kSpan];
+#pragma unroll
+                for (int c = 0; c < kSpan; c += 2) {
+                    x[c] = x[c + 1] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; w++) {
+                        const float2 v = *reinterpret_cast<const float2 *>(s_join + (w * (8 * NP) + r) * kJoinPitch + at * kSpan + c);
+                        x[c] += v.x;
+                        x[c + 1] += v.y;
+                    }
+                }
+                if (alone) {
+                    float top;
+                    const float sum = total(r, top), inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const uint32_t token = r / g.heads, head = r - token * g.heads;
+                    T *dst = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d + column;
+                    T y[kSpan];
+#pragma unroll
+                    for (int c = 0; c < kSpan; c++) y[c] = rounded<T>(x[c] * inv);
+                    if (wide) {
+#pragma unroll
+                        for (int c = 0; c < kSpan; c += 8) *reinterpret_cast<uint4 *>(dst + c) = *reinterpret_cast<const uint4 *>(y + c);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kSpan; c++) dst[c] = y[c];
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kSpan; c += 2) *reinterpret_cast<float2 *>(part + r * d + column + c) = make_float2(x[c], x[c + 1]);
+                }
+            }
+            __syncthreads();
+        }
+        if (!alone) {
+            if (t < pairs) {
+                float top;
+                const float sum = total(t, top);
+                part[8 * NP * d + 2 * t] = top;
+                part[8 * NP * d + 2 * t + 1] = sum;
+            }
+            if (t == 0) name_part(a, blockIdx.x, g);
+            __syncthreads();                             // before the next unit's maxima
+        }
+    }
+    // given up: the copies in flight land before the CTA exits
+    if (!ok && lane == 0)
+        for (int i = 0; i < S - 1; i++) {
+            for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&s_full[warp][slot], parity); w++) { }
+            slot = slot == S - 1 ? 0 : slot + 1;
+            parity ^= slot == 0;
+        }
+}
+
+template <typename T, int D, int NP>
+int launch_sized(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pairs, cudaStream_t stream)
+{
+    constexpr uint32_t ctas = 148 * ctas_per_sm<D, NP>();
+    auto *kernel = decode8_kernel<T, D, NP>;
+    if (int rc = allow_smem(kernel, smem_bytes<D, NP>())) return rc;
+    MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, NP>(), stream, maps, a, wide)) return rc;
+    return launch_merge<T, 8 * NP>(a, ctas, pairs, stream);
+}
+
+template <typename T>
+int launch_typed(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pairs, cudaStream_t stream)
+{
+    if (a.d > 128) return launch_sized<T, 256, 1>(a, maps, wide, pairs, stream);
+    if (pairs <= 8) return a.d <= 64 ? launch_sized<T, 64, 1>(a, maps, wide, pairs, stream) : launch_sized<T, 128, 1>(a, maps, wide, pairs, stream);
+    return a.d <= 64 ? launch_sized<T, 64, 2>(a, maps, wide, pairs, stream) : launch_sized<T, 128, 2>(a, maps, wide, pairs, stream);
+}
+
+// {head_dim, kv_heads, pages * page_size} of a cache, for boxes of 64 or 128 codes by 16 tokens of one head, in the swizzle of that size.  What lies outside
+// reads as zero.
+int encode_codes(CUtensorMap &map, const void *base, const Attend8Args &a)
+{
+    EncodeTiledFn encode = nullptr;
+    if (int rc = encode_fn(encode)) return rc;
+    const cuuint64_t dims[3] = {a.d, a.kv_heads, (cuuint64_t)a.pages << a.page_shift};
+    const cuuint64_t strides[2] = {a.d, (cuuint64_t)a.kv_heads * a.d};
+    const cuuint32_t box[3] = {a.d <= 64 ? 64u : 128u, 1, 16}, elem[3] = {1, 1, 1};
+    const CUresult cr = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               a.d <= 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                               a.d % 128 == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? MGQ_OK : fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+}
+
+}  // namespace
+
+uint32_t decode8_ctas(uint32_t head_dim) { return 148 * (head_dim <= 64 ? ctas_per_sm<64, 1>() : head_dim <= 128 ? ctas_per_sm<128, 1>() : ctas_per_sm<256, 1>()); }
+
+int launch_decode8(const Attend8Args &a, int dtype, uint32_t pairs, cudaStream_t stream)
+{
+    Maps maps;
+    if (int rc = encode_codes(maps.k, a.k, a)) return rc;
+    if (int rc = encode_codes(maps.v, a.v, a)) return rc;
+    auto on = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool wide = on(a.q) && on(a.out) && a.q_pitch % 8 == 0 && a.out_pitch % 8 == 0;
+    return dtype == MGQ_FMT_F16 ? launch_typed<__half>(a, maps, wide, pairs, stream) : launch_typed<__nv_bfloat16>(a, maps, wide, pairs, stream);
+}
+
+int decode8_status()
+{
+    unsigned int err = 0;
+    MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_decode8_error, sizeof err));
+    if (!err) return MGQ_OK;
+    const unsigned int zero = 0;
+    MGQ_CUDA(cudaMemcpyToSymbol(g_decode8_error, &zero, sizeof zero));
+    return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the attention of few tokens over 8-bit codes ran out");
+}
+
+size_t paged_attention_int8_workspace(uint32_t head_dim)
+{
+    const uint32_t ctas = decode8_ctas(head_dim);
+    return ctas * 2 * (sizeof(PartHead) + (size_t)kDecode8Rows * (head_dim + 2) * sizeof(float));
+}
+
+int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales, const float *v_scales, int dtype, const uint32_t *table,
+                                const uint32_t *starts, const uint32_t *lengths, void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads,
+                                uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, uint32_t block, uint32_t table_width, uint32_t q_pitch,
+                                uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream)
+{
+    Attend8Args a{};
+    a.q = q; a.k = k_cache; a.v = v_cache; a.out = out;
+    a.k_scales = k_scales; a.v_scales = v_scales; a.block_shift = page_shift(block);
+    a.starts = starts; a.lengths = lengths; a.table = table;
+    a.sequences = sequences; a.rows = rows; a.kv_heads = kv_heads; a.group = heads / kv_heads; a.d = head_dim;
+    a.page_shift = page_shift(page_size); a.pages = pages; a.table_width = table_width;
+    a.window = window < (1u << 31) ? window : 0u;                      // no sequence is longer
+    a.q_pitch = q_pitch; a.out_pitch = out_pitch;
+    a.rows_from = 1; a.rows_to = 0xFFFFFFFFu;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const uint32_t pairs = (uint32_t)min((unsigned long long)max_fresh * a.group, 0xFFFFFFFFull);
+    a.heads = static_cast<PartHead *>(workspace);
+    a.parts = reinterpret_cast<float *>(a.heads + 2 * decode8_ctas(a.d));
+    return launch_decode8(a, dtype, pairs, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace mgq

@@ -839,7 +839,7 @@ int prefill_status()
 {
     unsigned int err = 0;
     MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_prefill_error, sizeof err));
-    if (!err) return MGQ_OK;
+    if (!err) return decode8_status();
     const unsigned int zero = 0;
     MGQ_CUDA(cudaMemcpyToSymbol(g_prefill_error, &zero, sizeof zero));
     return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the paged attention of many tokens ran out");

@@ -147,23 +147,28 @@ def matmul_host(fmt: int, a: np.ndarray, w_dev_ptr: int, k: int, n: int, addend:
     return out
 
 
-# Operators of many sequences over one paged cache and of their tokens (paged.py), which needs torch from the start.
+# Operators of many sequences over one paged cache and of their tokens (paged.py), and of 8-bit integers (int8.py), which need torch from the start.
 _PAGED = ("PagedStep", "paged_plan", "paged_trim", "paged_append", "paged_attention", "token_probs", "verify_drafts", "NO_SLOT", "NO_PAGE", "NO_TOKEN")
+_INT8 = ("quantize_rows", "matmul_int8", "paged_append_int8", "paged_attention_int8")
 
 
 def __getattr__(name: str):
-    if name not in _PAGED:
+    if name in _PAGED:
+        from . import paged
+        globals().update({n: getattr(paged, n) for n in _PAGED})
+    elif name in _INT8:
+        from . import int8
+        globals().update({n: getattr(int8, n) for n in _INT8})
+    else:
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
-    from . import paged
-    globals().update({n: getattr(paged, n) for n in _PAGED})
     return globals()[name]
 
 
 def __dir__():
-    return sorted({*globals(), *_PAGED})
+    return sorted({*globals(), *_PAGED, *_INT8})
 
 
-# without _PAGED: `from ops import *` takes every name in here, and would import torch for them
+# without _PAGED and _INT8: `from ops import *` takes every name in here, and would import torch for them
 __all__ = ["Plan", "set_option", "device_status", "packed_bytes", "quantize", "dequantize", "shard_columns", "matmul", "matmul_host",
            "FMT_Q4", "FMT_Q8", "A_F32", "A_BF16"]
 _ = _lib
