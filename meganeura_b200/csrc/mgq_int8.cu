@@ -114,12 +114,12 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs
 {
     __shared__ int s_sum[kWarps][16][8 * NT + 1];
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, row = lane >> 2, quad = lane & 3u;
-    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * NT, k = a.k;
+    const uint32_t n0 = blockIdx.x * 16, k = a.k;
     const uint32_t steps = (k + 63) / 64, from = steps * warp / kWarps, to = steps * (warp + 1) / kWarps;
     const int8_t *w0 = a.w + (size_t)min(n0 + row, a.n - 1) * k, *w1 = a.w + (size_t)min(n0 + row + 8, a.n - 1) * k;       // rows behind the last are not stored
     const int8_t *x[NT];
 #pragma unroll
-    for (int i = 0; i < NT; i++) x[i] = a.a + (size_t)min(m0 + i * 8 + row, a.m - 1) * k;
+    for (int i = 0; i < NT; i++) x[i] = a.a + (size_t)min(i * 8 + row, a.m - 1) * k;
     int c[NT][4] = {};
     uint4 w[kAhead][2];
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
@@ -163,11 +163,11 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs
     __syncthreads();
     for (uint32_t i = t; i < 16 * 8 * NT; i += kWarps * 32) {
         const uint32_t n = i % 16, m = i / 16;
-        if (n0 + n >= a.n || m0 + m >= a.m) continue;
+        if (n0 + n >= a.n || m >= a.m) continue;
         int sum = 0;
 #pragma unroll
         for (int v = 0; v < kWarps; v++) sum += s_sum[v][n][m];
-        finish<T>(a, m0 + m, n0 + n, sum, a.a_scales[m0 + m], a.w_scales[n0 + n]);
+        finish<T>(a, m, n0 + n, sum, a.a_scales[m], a.w_scales[n0 + n]);
     }
 }
 
@@ -175,8 +175,7 @@ template <typename T>
 int launch_few(const ProductArgs &a, cudaStream_t stream)
 {
     const uint32_t tiles = (a.n + 15) / 16;
-    return a.m <= 8 ? launch(few_rows_kernel<T, 1>, dim3(tiles, 1), dim3(kWarps * 32), 0, stream, a)
-                    : launch(few_rows_kernel<T, 2>, dim3(tiles, (a.m + 15) / 16), dim3(kWarps * 32), 0, stream, a);
+    return launch(a.m <= 8 ? few_rows_kernel<T, 1> : few_rows_kernel<T, 2>, dim3(tiles), dim3(kWarps * 32), 0, stream, a);
 }
 
 }  // namespace
@@ -196,6 +195,7 @@ int launch_matmul_int8(const int8_t *x, const float *x_scales, const int8_t *w, 
 {
     const ProductArgs a{x, w, x_scales, w_scales, addend, out, m, k, n, addend_pitch, out_pitch};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (m > kFewRows) return launch_product_tc(a, dtype, stream);
     switch (dtype) {
         case MGQ_FMT_F32: return launch_few<float>(a, s);
         case MGQ_FMT_F16: return launch_few<__half>(a, s);

@@ -41,4 +41,7 @@ __device__ __forceinline__ void finish(const ProductArgs &a, uint32_t m, uint32_
     else *out = __float2bfloat16_rn(y);
 }
 
+constexpr uint32_t kFewRows = 16;                          // of activations: mma.sync (mgq_int8.cu), beyond them tcgen05 (mgq_int8_tc.cu)
+int launch_product_tc(const ProductArgs &a, int dtype, void *stream);
+
 }  // namespace mgq

@@ -106,7 +106,8 @@ int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8
                                 const uint32_t *starts, const uint32_t *lengths, void *out, uint32_t sequences, uint32_t rows, uint32_t max_fresh, uint32_t heads,
                                 uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, uint32_t block, uint32_t table_width, uint32_t q_pitch,
                                 uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
-int decode8_status();
+int decode8_status();                 // mgq_paged_int8_decode.cu
+int int8_status();                    // mgq_int8_tc.cu
 int launch_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream);
 int launch_verify_drafts(const float *target, uint32_t target_pitch, const float *draft, uint32_t draft_pitch, const uint32_t *tokens, const uint32_t *starts,
                          const float *accept, const float *sample, uint32_t *accepted, uint32_t *next, uint32_t *out, uint32_t sequences, uint32_t rows,

@@ -14,9 +14,9 @@ namespace mgq {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 
-// cluster_y: CTAs along y that form a cluster.
+// CTAs that form a cluster.
 template <typename... Params, typename... Args>
-int launch_clustered(void (*kernel)(Params...), dim3 grid, dim3 block, uint32_t cluster_y, size_t smem, cudaStream_t stream, Args... args)
+int launch_clusters(void (*kernel)(Params...), dim3 grid, dim3 block, dim3 cluster, size_t smem, cudaStream_t stream, Args... args)
 {
     cudaLaunchConfig_t lc{};
     lc.gridDim = grid;
@@ -27,13 +27,19 @@ int launch_clustered(void (*kernel)(Params...), dim3 grid, dim3 block, uint32_t 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 1;
-    attr[1].val.clusterDim.y = cluster_y;
-    attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = cluster.z;
     lc.attrs = attr;
-    lc.numAttrs = cluster_y > 1 ? 2 : 1;
+    lc.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
     MGQ_CUDA(cudaLaunchKernelEx(&lc, kernel, static_cast<Params>(args)...));
     return MGQ_OK;
+}
+// cluster_y: CTAs along y that form a cluster.
+template <typename... Params, typename... Args>
+int launch_clustered(void (*kernel)(Params...), dim3 grid, dim3 block, uint32_t cluster_y, size_t smem, cudaStream_t stream, Args... args)
+{
+    return launch_clusters(kernel, grid, block, dim3(1, cluster_y), smem, stream, static_cast<Params>(args)...);
 }
 template <typename... Params, typename... Args>
 int launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args)

@@ -572,7 +572,7 @@ int decode8_status()
 {
     unsigned int err = 0;
     MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_decode8_error, sizeof err));
-    if (!err) return MGQ_OK;
+    if (!err) return int8_status();
     const unsigned int zero = 0;
     MGQ_CUDA(cudaMemcpyToSymbol(g_decode8_error, &zero, sizeof zero));
     return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the attention of few tokens over 8-bit codes ran out");
