@@ -91,11 +91,11 @@ int launch_quantize(const void *x, uint32_t pitch, int8_t *codes, float *scales,
 }
 
 // ---------------------------------------------------------------- few rows
-// HBM bound: the weights are read once.  m16n8k32 products of 16 weight rows (left) by 8 activation rows; the order of k inside a product is free as long
+// HBM bound: the weights are read once.  m16n8k32 products of 16 weight rows (left) by up to 8 activation rows; the order of k inside a product is free as long
 // as both operands have the same, so a lane loads 16 consecutive bytes of a row for two products, straight from global memory to registers.  The warps of a
 // CTA share out k and meet in shared memory; sums are whole numbers, so their order is free.  The first weights are brought into L2 before the wait for the
 // kernels in front, which may write activations and weights: a load before it could see old ones.
-constexpr int kWarps = 4, kAhead = 4;                    // steps of 64 k that a warp has under way
+constexpr int kAhead = 4;                                // steps of 64 k that a warp has under way
 
 __device__ __forceinline__ uint4 load_stream(const int8_t *p)
 {
@@ -109,25 +109,24 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int NT>                            // NT: blocks of 8 activation rows
-__global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs a)
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) few_rows_kernel(const ProductArgs a)
 {
-    __shared__ int s_sum[kWarps][16][8 * NT + 1];
+    __shared__ int s_sum[WARPS][16][kFewRows + 1];
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5, row = lane >> 2, quad = lane & 3u;
     const uint32_t n0 = blockIdx.x * 16, k = a.k;
-    const uint32_t steps = (k + 63) / 64, from = steps * warp / kWarps, to = steps * (warp + 1) / kWarps;
+    const uint32_t steps = (k + 63) / 64, from = steps * warp / WARPS, to = steps * (warp + 1) / WARPS;
     const int8_t *w0 = a.w + (size_t)min(n0 + row, a.n - 1) * k, *w1 = a.w + (size_t)min(n0 + row + 8, a.n - 1) * k;       // rows behind the last are not stored
-    const int8_t *x[NT];
-#pragma unroll
-    for (int i = 0; i < NT; i++) x[i] = a.a + (size_t)min(i * 8 + row, a.m - 1) * k;
-    int c[NT][4] = {};
-    uint4 w[kAhead][2];
+    const int8_t *x = a.a + (size_t)min(row, a.m - 1) * k;
+    int c[4] = {};
+    uint4 w[kAhead][2], b[kAhead];
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-    auto weights = [&](uint32_t s, int slot) {
+    auto fetch = [&](uint32_t s, int slot) {
         const uint32_t at = s * 64 + quad * 16;
         const bool in = s < to && at < k;
         w[slot][0] = in ? load_stream(w0 + at) : none;
         w[slot][1] = in ? load_stream(w1 + at) : none;
+        b[slot] = in ? *reinterpret_cast<const uint4 *>(x + at) : none;
     };
     if (quad == 0)
         for (uint32_t s = from & ~1u; s < min(from + kAhead, to); s += 2) {               // 128 bytes
@@ -137,45 +136,33 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs
     pdl_launch_dependents();
     pdl_wait();
 #pragma unroll
-    for (int i = 0; i < kAhead; i++) weights(from + i, i);
-    for (uint32_t s0 = from; s0 < to; s0 += kAhead) {
-        uint4 b[kAhead][NT];
+    for (int i = 0; i < kAhead; i++) fetch(from + i, i);
+    for (uint32_t s0 = from; s0 < to; s0 += kAhead)
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const uint32_t at = (s0 + i) * 64 + quad * 16;
-#pragma unroll
-            for (int j = 0; j < NT; j++) b[i][j] = s0 + i < to && at < k ? *reinterpret_cast<const uint4 *>(x[j] + at) : none;
+            mma_s8(c, w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, b[i].x, b[i].y);
+            mma_s8(c, w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, b[i].z, b[i].w);
+            fetch(s0 + kAhead + i, i);
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                mma_s8(c[j], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, b[i][j].x, b[i][j].y);
-                mma_s8(c[j], w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, b[i][j].z, b[i][j].w);
-            }
-            weights(s0 + kAhead + i, i);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s_sum[warp][row + e / 2 * 8][j * 8 + 2 * quad + e % 2] = c[j][e];
+    for (int e = 0; e < 4; e++) s_sum[warp][row + e / 2 * 8][2 * quad + e % 2] = c[e];
     __syncthreads();
-    for (uint32_t i = t; i < 16 * 8 * NT; i += kWarps * 32) {
+    for (uint32_t i = t; i < 16 * a.m; i += WARPS * 32) {
         const uint32_t n = i % 16, m = i / 16;
-        if (n0 + n >= a.n || m >= a.m) continue;
+        if (n0 + n >= a.n) continue;
         int sum = 0;
 #pragma unroll
-        for (int v = 0; v < kWarps; v++) sum += s_sum[v][n][m];
+        for (int v = 0; v < WARPS; v++) sum += s_sum[v][n][m];
         finish<T>(a, m, n0 + n, sum, a.a_scales[m], a.w_scales[n0 + n]);
     }
 }
 
+constexpr uint32_t kManyTiles = 740;
 template <typename T>
 int launch_few(const ProductArgs &a, cudaStream_t stream)
 {
     const uint32_t tiles = (a.n + 15) / 16;
-    return launch(a.m <= 8 ? few_rows_kernel<T, 1> : few_rows_kernel<T, 2>, dim3(tiles), dim3(kWarps * 32), 0, stream, a);
+    return tiles < kManyTiles ? launch(few_rows_kernel<T, 16>, dim3(tiles), dim3(512), 0, stream, a) : launch(few_rows_kernel<T, 4>, dim3(tiles), dim3(128), 0, stream, a);
 }
 
 }  // namespace

@@ -30,18 +30,19 @@ struct ProductArgs {
     void *out;
     uint32_t m, k, n, addend_pitch, out_pitch;
 };
+template <typename T> __device__ __forceinline__ T to_type(float y);
+template <> __device__ __forceinline__ float to_type<float>(float y) { return y; }
+template <> __device__ __forceinline__ __half to_type<__half>(float y) { return __float2half_rn(y); }
+template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(float y) { return __float2bfloat16_rn(y); }
 template <typename T>
 __device__ __forceinline__ void finish(const ProductArgs &a, uint32_t m, uint32_t n, int sum, float a_scale, float w_scale)
 {
     float y = (float)sum * a_scale * w_scale;
     if (a.addend) y += to_f32(static_cast<const T *>(a.addend)[(size_t)m * a.addend_pitch + n]);
-    T *out = static_cast<T *>(a.out) + (size_t)m * a.out_pitch + n;
-    if constexpr (sizeof(T) == 4) *out = y;
-    else if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(y);
-    else *out = __float2bfloat16_rn(y);
+    static_cast<T *>(a.out)[(size_t)m * a.out_pitch + n] = to_type<T>(y);
 }
 
-constexpr uint32_t kFewRows = 16;                          // of activations: mma.sync (mgq_int8.cu), beyond them tcgen05 (mgq_int8_tc.cu)
+constexpr uint32_t kFewRows = 8;                           // of activations: mma.sync (mgq_int8.cu), beyond them tcgen05 (mgq_int8_tc.cu)
 int launch_product_tc(const ProductArgs &a, int dtype, void *stream);
 
 }  // namespace mgq
