@@ -94,7 +94,7 @@ int launch_paged_attention(const void *q, const void *k_cache, const void *v_cac
                            uint32_t pages, uint32_t table_width, uint32_t q_pitch, uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
 int paged_status();                   // mgq_paged_decode.cu
 int prefill_status();                 // mgq_paged_prefill.cu
-// 8-bit integers (mgq_int8.cu) and caches of them (mgq_paged_int8.cu, mgq_paged_int8_decode.cu).
+// 8-bit integers (mgq_int8.cu) and caches of them (mgq_paged_int8*.cu).
 int launch_quantize_rows(const void *x, int dtype, uint32_t pitch, int8_t *codes, float *scales, uint32_t rows, uint32_t k, void *stream);
 int launch_matmul_int8(const int8_t *a, const float *a_scales, const int8_t *w, const float *w_scales, const void *addend, void *out, int dtype, uint32_t m, uint32_t k,
                        uint32_t n, uint32_t addend_pitch, uint32_t out_pitch, void *stream);
@@ -107,6 +107,7 @@ int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8
                                 uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, uint32_t block, uint32_t table_width, uint32_t q_pitch,
                                 uint32_t out_pitch, float scale, uint32_t window, void *workspace, void *stream);
 int decode8_status();                 // mgq_paged_int8_decode.cu
+int prefill8_status();                // mgq_paged_int8_prefill.cu
 int int8_status();                    // mgq_int8_tc.cu
 int launch_token_probs(const float *logits, uint32_t pitch, const float *temperature, float *out, uint32_t out_pitch, uint32_t rows, uint32_t vocab, void *stream);
 int launch_verify_drafts(const float *target, uint32_t target_pitch, const float *draft, uint32_t draft_pitch, const uint32_t *tokens, const uint32_t *starts,

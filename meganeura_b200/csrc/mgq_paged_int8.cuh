@@ -14,6 +14,11 @@ struct Attend8Args : AttendArgs {
 // Few new tokens per sequence (mgq_paged_int8_decode.cu).
 uint32_t decode8_ctas(uint32_t head_dim);
 constexpr uint32_t kDecode8Rows = 16;                      // of a unit, at most
+constexpr uint32_t kDecode8Pairs = 32;                     // of a sequence that is not yet many tokens'
 int launch_decode8(const Attend8Args &a, int dtype, uint32_t pairs, cudaStream_t stream);    // pairs: a bound of a sequence's tokens * heads per key / value head
+
+// Many new tokens: heads of up to 128, queries and results on 16 bytes (mgq_paged_int8_prefill.cu).
+bool prefill8_takes(const Attend8Args &a);
+int launch_prefill8(const Attend8Args &a, int dtype, cudaStream_t stream);
 
 }  // namespace mgq

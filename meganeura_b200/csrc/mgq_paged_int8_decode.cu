@@ -572,7 +572,7 @@ int decode8_status()
 {
     unsigned int err = 0;
     MGQ_CUDA(cudaMemcpyFromSymbol(&err, g_decode8_error, sizeof err));
-    if (!err) return int8_status();
+    if (!err) return prefill8_status();
     const unsigned int zero = 0;
     MGQ_CUDA(cudaMemcpyToSymbol(g_decode8_error, &zero, sizeof zero));
     return fail(MGQ_ERR_TIMEOUT, "a bounded wait inside the attention of few tokens over 8-bit codes ran out");
@@ -581,7 +581,8 @@ int decode8_status()
 size_t paged_attention_int8_workspace(uint32_t head_dim)
 {
     const uint32_t ctas = decode8_ctas(head_dim);
-    return ctas * 2 * (sizeof(PartHead) + (size_t)kDecode8Rows * (head_dim + 2) * sizeof(float));
+    const size_t many = head_dim <= 128 ? kPrefillCtas * 2 * (sizeof(PartHead) + (size_t)kPrefillRows * (head_dim + 2) * sizeof(float)) : 0;
+    return ctas * 2 * (sizeof(PartHead) + (size_t)kDecode8Rows * (head_dim + 2) * sizeof(float)) + many;
 }
 
 int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales, const float *v_scales, int dtype, const uint32_t *table,
@@ -602,7 +603,16 @@ int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8
     const uint32_t pairs = (uint32_t)min((unsigned long long)max_fresh * a.group, 0xFFFFFFFFull);
     a.heads = static_cast<PartHead *>(workspace);
     a.parts = reinterpret_cast<float *>(a.heads + 2 * decode8_ctas(a.d));
-    return launch_decode8(a, dtype, pairs, static_cast<cudaStream_t>(stream));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (pairs <= kDecode8Pairs || !prefill8_takes(a)) return launch_decode8(a, dtype, pairs, s);
+    // both kinds of sequences may be there
+    a.rows_to = kDecode8Pairs;
+    if (int rc = launch_decode8(a, dtype, kDecode8Pairs, s)) return rc;
+    a.rows_from = kDecode8Pairs + 1;
+    a.rows_to = 0xFFFFFFFFu;
+    a.heads = reinterpret_cast<PartHead *>(a.parts + (size_t)decode8_ctas(a.d) * 2 * kDecode8Rows * (a.d + 2));
+    a.parts = reinterpret_cast<float *>(a.heads + 2 * kPrefillCtas);
+    return launch_prefill8(a, dtype, s);
 }
 
 }  // namespace mgq
