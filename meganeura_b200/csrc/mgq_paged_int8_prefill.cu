@@ -40,9 +40,10 @@ __device__ unsigned int g_prefill8_error;
 using Way = Walk<kPrefillRows, kKeys, kExtra>;
 struct __align__(16) Shared {
     unsigned long long full[6], empty[6], code_full[4], code_empty[4], sc_full[2], sc_empty[2], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2];
-    float factor[2][kBatch][kGroups], weight[2][kBatch][kGroups];          // of a block's groups of 16 keys
+    alignas(16) float factor[2][kBatch][kGroups], weight[2][kBatch][kGroups];          // of a block's groups of 16 keys
     float drop[2][kBatch], power[2][kBatch];             // what O is multiplied by at a block, and 2^e
     uint32_t there[2][kBatch][4];                        // keys that exist
+    uint32_t odd[2][kBatch];                             // whether a scale is not finite
     Way way[3];                                          // of the producers of codes, queries, scales
     Segment kv_seg, sc_seg, next, seg[2];                // of those; of everybody else, two units in turn, no tokens behind the last
     int more;
@@ -290,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                         before = was;
                     }
                 }
+                const uint32_t odd = __ballot_sync(0xffffffffu, !(ks <= FLT_MAX && vs <= FLT_MAX));
                 if (!(ok = wait_all(&sh.sc_empty[b], (batch >> 1 & 1u) ^ 1u))) break;
                 if (kb < kb_end) {
                     const uint32_t i = lane / 8;
@@ -300,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                     if (group == 0) {
                         sh.drop[b][i] = before == -1000 || before == mine ? 1.f : power_of(max(before - mine, -126));
                         sh.power[b][i] = power_of(mine);
+                        sh.odd[b][i] = odd >> (8 * i) & 0xFFu;
                     }
                     reinterpret_cast<uint16_t *>(sh.there[b][i])[group] = (uint16_t)there;
                 }
@@ -498,6 +501,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 if (!plain)
 #pragma unroll
                     for (int w = 0; w < 4; w++) seen[w] = sees(w);
+                // Of two groups of 16 keys.  Where a scale is not finite, one that this row does not see must have no say.
+                const bool odd = !plain && sh.odd[sb][in_batch];
+                auto pair_for = [&](const float *p, int i, float otherwise) {
+                    float2 v = *reinterpret_cast<const float2 *>(p + 2 * i);
+                    if (odd && !(seen[i] & 0xFFFFu)) v.x = otherwise;
+                    if (odd && !(seen[i] >> 16)) v.y = otherwise;
+                    return v;
+                };
                 auto mask = [&](float (&s)[64], int c) {
                     if (plain) return;
 #pragma unroll
@@ -506,9 +517,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                         for (int e = 0; e < 32; e++) s[32 * w + e] = seen[2 * c + w] >> e & 1u ? s[32 * w + e] : -INFINITY;
                     __syncwarp();
                 };
-                // of 16 keys; one that this row does not see has no say, whatever its scales are
-                auto group_seen = [&](int i) { return plain || (seen[i / 2] >> (i % 2 * 16) & 0xFFFFu) != 0; };
-                auto factor_of = [&](int i) { return group_seen(i) ? factors[i] : 1.f; };
                 float s[64], t[64];
                 tmem_ld_row(s_at, s);
                 wait_row(s);
@@ -516,11 +524,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 mask(s, 0);
                 float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) top = max3(top, max16(s + 16 * i) * factor_of(i), max16(s + 16 * i + 16) * factor_of(i + 1));
+                for (int i = 0; i < 2; i++) {
+                    const float2 f = pair_for(factors, i, 1.f);
+                    top = max3(top, max16(s + 32 * i) * f.x, max16(s + 32 * i + 16) * f.y);
+                }
                 wait_row(t);
                 mask(t, 1);
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) top = max3(top, max16(t + 16 * i) * factor_of(4 + i), max16(t + 16 * i + 16) * factor_of(5 + i));
+                for (int i = 0; i < 2; i++) {
+                    const float2 f = pair_for(factors, 2 + i, 1.f);
+                    top = max3(top, max16(t + 32 * i) * f.x, max16(t + 32 * i + 16) * f.y);
+                }
                 // Nothing to do where the maximum stays at or below m + kRoom (finite behind the first block); -inf and NaN come here, too.
                 const bool calm = top <= m + kRoom && top >= -FLT_MAX && drop == 1.f;
                 if (__any_sync(0xffffffffu, !calm)) {
@@ -547,10 +561,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 // A quarter of the keys: exponentials, sums, P.  The first half is signalled in front of the third quarter's stores, when its own are long done.
                 auto weights = [&](auto rounds_first, const float (&s)[64], int quarter, auto before_stores) {
                     uint32_t p[16];
+                    const float2 both_f = pair_for(factors, quarter, 1.f), both_w = pair_for(by, quarter, 0.f);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const int group = 2 * quarter + i, at = quarter % 2 * 32 + 16 * i;
-                        const float f = factor_of(group), w = group_seen(group) ? by[group] : 0.f;
+                        const int at = quarter % 2 * 32 + 16 * i;
+                        const float f = i ? both_f.y : both_f.x, w = i ? both_w.y : both_w.x;
                         const pair_t f2 = pair_of(f, f), w2 = pair_of(w, w);
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
