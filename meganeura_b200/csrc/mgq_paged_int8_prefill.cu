@@ -18,7 +18,6 @@
 // TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
 #include <cfloat>
 #include <cstdint>
-#include <type_traits>
 
 #include "mgq_paged_int8.cuh"
 #include "mgq_paged_prefill.cuh"
@@ -558,24 +557,33 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 const float base = m == -INFINITY ? 0.f : -m;
                 const pair_t bases = pair_of(base, base);
                 pair_t sum[2] = {0, 0};
+                // Where scores are huge their products with the factors are rounded here, so that the maximum's weight is 1 however large m is; the sums below are then
+                // exact.  In the loop this would be twice its code, whose jumps cost a tenth of the time.
+                const bool scaled = __any_sync(0xffffffffu, huge);
+                if (__builtin_expect(scaled, 0)) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float2 f = pair_for(factors, i, 1.f), h = pair_for(factors, 2 + i, 1.f);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            s[32 * i + e] = __fmul_rn(s[32 * i + e], e < 16 ? f.x : f.y);
+                            t[32 * i + e] = __fmul_rn(t[32 * i + e], e < 16 ? h.x : h.y);
+                        }
+                    }
+                }
                 // A quarter of the keys: exponentials, sums, P.  The first half is signalled in front of the third quarter's stores, when its own are long done.
-                auto weights = [&](auto rounds_first, const float (&s)[64], int quarter, auto before_stores) {
+                auto weights = [&](const float (&s)[64], int quarter, auto before_stores) {
                     uint32_t p[16];
                     const float2 both_f = pair_for(factors, quarter, 1.f), both_w = pair_for(by, quarter, 0.f);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const int at = quarter % 2 * 32 + 16 * i;
-                        const float f = i ? both_f.y : both_f.x, w = i ? both_w.y : both_w.x;
+                        const float f = scaled ? 1.f : i ? both_f.y : both_f.x, w = i ? both_w.y : both_w.x;
                         const pair_t f2 = pair_of(f, f), w2 = pair_of(w, w);
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             float x, y;
-                            if constexpr (decltype(rounds_first)::value) {       // not as pairs: the assembler makes one rounding of a product and a sum of them
-                                x = __fadd_rn(__fmul_rn(s[at + 2 * e], f), base);
-                                y = __fadd_rn(__fmul_rn(s[at + 2 * e + 1], f), base);
-                            } else {
-                                parts_of(pair_fma(pair_of(s[at + 2 * e], s[at + 2 * e + 1]), f2, bases), x, y);
-                            }
+                            parts_of(pair_fma(pair_of(s[at + 2 * e], s[at + 2 * e + 1]), f2, bases), x, y);
                             x = exp2_fast(x);
                             y = exp2_fast(y);
                             const pair_t both = pair_of(x, y);
@@ -593,14 +601,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar);
                 };
-                auto all_weights = [&](auto rounds_first) {
-                    weights(rounds_first, s, 0, [] {});
-                    weights(rounds_first, s, 1, [] {});
-                    weights(rounds_first, t, 2, [&] { signal(&sh.p_half[tile]); });
-                    weights(rounds_first, t, 3, [] {});
-                };
-                if (__any_sync(0xffffffffu, huge)) all_weights(std::true_type());
-                else                               all_weights(std::false_type());
+                weights(s, 0, [] {});
+                weights(s, 1, [] {});
+                weights(t, 2, [&] { signal(&sh.p_half[tile]); });
+                weights(t, 3, [] {});
                 leave_batch();
                 signal(&sh.p_full[tile]);
                 float x, y;
