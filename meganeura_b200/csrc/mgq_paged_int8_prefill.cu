@@ -18,6 +18,7 @@
 // TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "mgq_paged_int8.cuh"
 #include "mgq_paged_prefill.cuh"
@@ -69,6 +70,24 @@ __device__ __forceinline__ float max16(const float *y)
 {
     const float a = max3(y[0], y[1], y[2]), b = max3(y[3], y[4], y[5]), c = max3(y[6], y[7], y[8]), d = max3(y[9], y[10], y[11]);
     return max3(max3(a, b, c), max3(d, y[12], y[13]), max3(y[14], y[15], y[15]));
+}
+// 32 columns of this lane's row; wait_quarter before they are used.
+__device__ __forceinline__ void tmem_ld_quarter(uint32_t addr, float (&y)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]), "=f"(y[4]), "=f"(y[5]), "=f"(y[6]), "=f"(y[7]),
+                   "=f"(y[8]), "=f"(y[9]), "=f"(y[10]), "=f"(y[11]), "=f"(y[12]), "=f"(y[13]), "=f"(y[14]), "=f"(y[15]),
+                   "=f"(y[16]), "=f"(y[17]), "=f"(y[18]), "=f"(y[19]), "=f"(y[20]), "=f"(y[21]), "=f"(y[22]), "=f"(y[23]),
+                   "=f"(y[24]), "=f"(y[25]), "=f"(y[26]), "=f"(y[27]), "=f"(y[28]), "=f"(y[29]), "=f"(y[30]), "=f"(y[31])
+                 : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void wait_quarter(float (&y)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < 32; c++) asm volatile("" : "+f"(y[c]));      // nothing that uses them moves in front of the wait
 }
 // Four codes as two pairs of f16 or bf16.  f16: 0x64 above a biased code reads 1024 + 128 + code.  bf16: 0x43 above seven bits reads 128 + them, and 128 or, with
 // the sign, 256 is taken off.
@@ -182,9 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
     };
     auto wait_all = [&](unsigned long long *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-    // Registers where they are needed: 256 * 208 + 256 * 48 = 512 * 128.
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 8) {
         const uint32_t shift = a.page_shift, page_keys = 1u << shift, box = min(page_keys, kKeys), boxes = kKeys / box, gone = a.pages << shift;
         uint32_t slot = 0, round = 0;
@@ -420,7 +437,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
         __syncwarp();
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t tile = warp >> 2, quad = warp & 3u, r_tile = quad * 32 + lane, row = tile * kTile + r_tile, d = a.d;
         const uint32_t lanes = (quad * 32u) << 16, s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * D + lanes;
         const uint32_t token = row / slice, head = row - token * slice, first_token = tile * kTile / slice;     // of this row, of the tile's first
@@ -492,48 +508,54 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 const float *factors = sh.factor[sb][in_batch], *by = sh.weight[sb][in_batch];
                 const float drop = sh.drop[sb][in_batch];
                 power = sh.power[sb][in_batch];
-                // 32 keys: those that the row sees
-                auto sees = [&](int w) {
-                    return sh.there[sb][in_batch][w] & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 32 * w);
+                auto signal = [&](unsigned long long *bar) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar);
                 };
-                uint32_t seen[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
-                if (!plain)
-#pragma unroll
-                    for (int w = 0; w < 4; w++) seen[w] = sees(w);
-                // Of two groups of 16 keys.  Where a scale is not finite, one that this row does not see must have no say.
+                // Both passes over the scores stand twice in the code: for blocks where something is masked (or huge), and for those where nothing is.  In one
+                // loop the first kind's instructions lie between the second's, and what runs on the SM at the same time no longer fits its instruction cache.
+                // Of 32 keys: those that the row sees, the factors or weights of their two groups, and scores without what it does not see.  Where a scale is not finite,
+                // one that this row does not see must have no say.
                 const bool odd = !plain && sh.odd[sb][in_batch];
-                auto pair_for = [&](const float *p, int i, float otherwise) {
+                auto sees = [&](int w) { return sh.there[sb][in_batch][w] & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 32 * w); };
+                auto pair_for = [&](auto simple, const float *p, int i, float otherwise) {
                     float2 v = *reinterpret_cast<const float2 *>(p + 2 * i);
-                    if (odd && !(seen[i] & 0xFFFFu)) v.x = otherwise;
-                    if (odd && !(seen[i] >> 16)) v.y = otherwise;
+                    if (!decltype(simple)::value && odd) {
+                        const uint32_t seen = sees(i);
+                        if (!(seen & 0xFFFFu)) v.x = otherwise;
+                        if (!(seen >> 16)) v.y = otherwise;
+                    }
                     return v;
                 };
-                auto mask = [&](float (&s)[64], int c) {
-                    if (plain) return;
+                auto mask = [&](auto simple, float (&s)[32], int w) {
+                    if (decltype(simple)::value || plain) return;
+                    const uint32_t seen = sees(w);
 #pragma unroll
-                    for (int w = 0; w < 2; w++)
-#pragma unroll
-                        for (int e = 0; e < 32; e++) s[32 * w + e] = seen[2 * c + w] >> e & 1u ? s[32 * w + e] : -INFINITY;
+                    for (int e = 0; e < 32; e++) s[e] = seen >> e & 1u ? s[e] : -INFINITY;
                     __syncwarp();
                 };
-                float s[64], t[64];
-                tmem_ld_row(s_at, s);
-                wait_row(s);
-                tmem_ld_row(s_at + 64, t);               // on its way while the first half's maximum is found
-                mask(s, 0);
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float2 f = pair_for(factors, i, 1.f);
-                    top = max3(top, max16(s + 32 * i) * f.x, max16(s + 32 * i + 16) * f.y);
-                }
-                wait_row(t);
-                mask(t, 1);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float2 f = pair_for(factors, 2 + i, 1.f);
-                    top = max3(top, max16(t + 32 * i) * f.x, max16(t + 32 * i + 16) * f.y);
-                }
+                float x[32], y[32], top = -INFINITY;
+                auto find_top = [&](auto simple) {
+                    auto largest = [&](float (&s)[32], int w) {
+                        mask(simple, s, w);
+                        const float2 f = pair_for(simple, factors, w, 1.f);
+                        top = max3(top, max16(s) * f.x, max16(s + 16) * f.y);
+                    };
+                    tmem_ld_quarter(s_at, x);
+#pragma unroll 1
+                    for (int h = 0; h < 2; h++) {
+                        wait_quarter(x);
+                        tmem_ld_quarter(s_at + 64 * h + 32, y);
+                        largest(x, 2 * h);
+                        wait_quarter(y);
+                        tmem_ld_quarter(s_at + (h ? 0 : 64), x);             // in the end the first ones again
+                        largest(y, 2 * h + 1);
+                    }
+                };
+                if (plain) find_top(std::true_type());
+                else       find_top(std::false_type());
                 // Nothing to do where the maximum stays at or below m + kRoom (finite behind the first block); -inf and NaN come here, too.
                 const bool calm = top <= m + kRoom && top >= -FLT_MAX && drop == 1.f;
                 if (__any_sync(0xffffffffu, !calm)) {
@@ -554,62 +576,55 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                         }
                     }
                 }
+                const bool scaled = __any_sync(0xffffffffu, huge);
                 const float base = m == -INFINITY ? 0.f : -m;
                 const pair_t bases = pair_of(base, base);
                 pair_t sum[2] = {0, 0};
-                // Where scores are huge their products with the factors are rounded here, so that the maximum's weight is 1 however large m is; the sums below are then
-                // exact.  In the loop this would be twice its code, whose jumps cost a tenth of the time.
-                const bool scaled = __any_sync(0xffffffffu, huge);
-                if (__builtin_expect(scaled, 0)) {
+                // A quarter of the keys: exponentials, sums, P, which takes the place of scores that have been read.
+                auto all_weights = [&](auto simple) {
+                    auto weights = [&](float (&s)[32], int w) {
+                        mask(simple, s, w);
+                        float2 f = pair_for(simple, factors, w, 1.f);
+                        const float2 v = pair_for(simple, by, w, 0.f);
+                        if (!decltype(simple)::value && scaled) {            // their products with the factors are rounded first, so that the maximum's weight is 1 however large m is
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float2 f = pair_for(factors, i, 1.f), h = pair_for(factors, 2 + i, 1.f);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            s[32 * i + e] = __fmul_rn(s[32 * i + e], e < 16 ? f.x : f.y);
-                            t[32 * i + e] = __fmul_rn(t[32 * i + e], e < 16 ? h.x : h.y);
+                            for (int e = 0; e < 32; e++) s[e] = __fmul_rn(s[e], e < 16 ? f.x : f.y);
+                            f = make_float2(1.f, 1.f);
                         }
-                    }
-                }
-                // A quarter of the keys: exponentials, sums, P.  The first half is signalled in front of the third quarter's stores, when its own are long done.
-                auto weights = [&](const float (&s)[64], int quarter, auto before_stores) {
-                    uint32_t p[16];
-                    const float2 both_f = pair_for(factors, quarter, 1.f), both_w = pair_for(by, quarter, 0.f);
+                        uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int at = quarter % 2 * 32 + 16 * i;
-                        const float f = scaled ? 1.f : i ? both_f.y : both_f.x, w = i ? both_w.y : both_w.x;
-                        const pair_t f2 = pair_of(f, f), w2 = pair_of(w, w);
+                        for (int i = 0; i < 2; i++) {
+                            const pair_t f2 = i ? pair_of(f.y, f.y) : pair_of(f.x, f.x), v2 = i ? pair_of(v.y, v.y) : pair_of(v.x, v.x);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            float x, y;
-                            parts_of(pair_fma(pair_of(s[at + 2 * e], s[at + 2 * e + 1]), f2, bases), x, y);
-                            x = exp2_fast(x);
-                            y = exp2_fast(y);
-                            const pair_t both = pair_of(x, y);
-                            sum[e & 1] = pair_add(sum[e & 1], both);
-                            parts_of(pair_mul(both, w2), x, y);
-                            p[8 * i + e] = pack<__half>(x, y);
+                            for (int e = 0; e < 8; e++) {
+                                float a0, a1;
+                                parts_of(pair_fma(pair_of(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]), f2, bases), a0, a1);
+                                const pair_t both = pair_of(exp2_fast(a0), exp2_fast(a1));
+                                sum[e & 1] = pair_add(sum[e & 1], both);
+                                parts_of(pair_mul(both, v2), a0, a1);
+                                p[8 * i + e] = pack<__half>(a0, a1);
+                            }
                         }
+                        tmem_st16(s_at + 16 * w, p);
+                    };
+#pragma unroll 1
+                    for (int h = 0; h < 2; h++) {
+                        wait_quarter(x);
+                        tmem_ld_quarter(s_at + 64 * h + 32, y);
+                        weights(x, 2 * h);
+                        wait_quarter(y);
+                        if (h == 0) tmem_ld_quarter(s_at + 64, x);
+                        weights(y, 2 * h + 1);
+                        if (h == 0) signal(&sh.p_half[tile]);
                     }
-                    before_stores();
-                    tmem_st16(s_at + 16 * quarter, p);
                 };
-                auto signal = [&](unsigned long long *bar) {
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar);
-                };
-                weights(s, 0, [] {});
-                weights(s, 1, [] {});
-                weights(t, 2, [&] { signal(&sh.p_half[tile]); });
-                weights(t, 3, [] {});
+                if (plain && !scaled) all_weights(std::true_type());
+                else                  all_weights(std::false_type());
+                float a0, a1;
+                parts_of(pair_add(sum[0], sum[1]), a0, a1);
+                l += a0 + a1;
                 leave_batch();
                 signal(&sh.p_full[tile]);
-                float x, y;
-                parts_of(pair_add(sum[0], sum[1]), x, y);
-                l += x + y;
             }
             finish();
             if (tile * kTile < pairs) {
