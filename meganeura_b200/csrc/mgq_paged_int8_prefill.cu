@@ -116,7 +116,7 @@ __device__ __forceinline__ void widen_rows(uint32_t codes, uint32_t operands, ui
     // eight lanes: rows r and r + 1, 64 dimensions each, of opposite halves where there are two
     const uint32_t half = D == 128 ? sub ^ (group & 1u) : 0u, first = row0 + sub + (D == 128 ? 2 * (group >> 1) : 2 * group);
     constexpr uint32_t kStep = D == 128 ? 4 : 8;
-#pragma unroll 2
+#pragma unroll 1
     for (uint32_t r = first; r < row0 + 32; r += kStep) {
         uint32_t w[4], o[8];
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(codes + r * D + half * 64 + j * 16) : "memory");
@@ -252,8 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
             if (!wait_all(&sh.code_full[from], from_round & 1u) || sh.last[from]) break;
             if (!wait_all(&sh.empty[slot], (round & 1u) ^ 1u)) break;
             const uint32_t src = smem_u32(codes) + from * kCodes, dst = smem_u32(ring) + slot * kStage;
-            if (what == 0) widen_rows<T, D>(src, dst, row0);
-            else           widen_rows<__half, D>(src, dst, row0);
+            if (std::is_same<T, __half>::value || what != 0) widen_rows<__half, D>(src, dst, row0);
+            else                                             widen_rows<T, D>(src, dst, row0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the products read it, and the next codes come
             __syncwarp();
             if (lane == 0) {
@@ -372,14 +372,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
             auto scores = [&](uint32_t tile, uint32_t at) {
                 const uint32_t q = q16 + tile * (kHalf / 16), k = ring16 + at * (kStage / 16);
                 umma_step<false>(tmem + tile * 128, q, k, kInstrS);
-#pragma unroll
+#pragma unroll 1
                 for (uint32_t i = 1; i < D / 16; i++) umma_step<true>(tmem + tile * 128, q + i / 4 * (2 * kHalf / 16) + i % 4 * 2, k + i / 4 * (kHalf / 16) + i % 4 * 2, kInstrS);
                 umma_commit(&sh.s_full[tile]);
             };
             // 64 keys, 16 per product
             auto values = [&](uint32_t tile, uint32_t at, uint32_t part, bool first) {
                 const uint32_t v = ring16 + at * (kStage / 16), o = tmem + 256 + tile * D, p = tmem + tile * 128;
-#pragma unroll
+#pragma unroll 1
                 for (uint32_t i = 0; i < kKeys / 32; i++) {
                     const uint32_t step = part * 4 + i;
                     umma_f16_ts_mn(o, p + step * 8, v + step * (2048 / 16), kHalf / 16, kInstrO, !first || i > 0 || part > 0);
@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                     const uint32_t k_slot = slot, k_round = round;
                     const bool more = kb + 1 < end;
                     if (more) advance();                     // to the next values
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t tile = 0; tile < 2; tile++) {
-                        const bool values_now = stop[tile] > kb;
+                        const bool values_now = (tile ? stop[1] : stop[0]) > kb;
                         if (values_now) {
                             if (!(ok = lane_wait(&sh.p_half[tile], p_seen >> tile & 1u))) break;
                             tc_fence_after();
@@ -424,9 +424,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                             p_seen ^= 1u << tile;
                             tc_fence_after();
                             values(tile, v_slot, 1, false);
-                            if (kb + 1 == stop[tile]) umma_commit(&sh.o_full[tile]);
+                            if (kb + 1 == (tile ? stop[1] : stop[0])) umma_commit(&sh.o_full[tile]);
                         }
-                        if (stop[tile] > kb + 1) scores(tile, k_slot);
+                        if ((tile ? stop[1] : stop[0]) > kb + 1) scores(tile, k_slot);
                     }
                     if (!ok) break;
                     if (kb + 2 == end) umma_commit(&sh.q_empty);    // no more scores of this unit
@@ -520,10 +520,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 // one that this row does not see must have no say.
                 const bool odd = !plain && sh.odd[sb][in_batch];
                 auto sees = [&](int w) { return sh.there[sb][in_batch][w] & bits(window ? pos - window + 1 : 0, pos + 1, key0 + 32 * w); };
-                auto pair_for = [&](auto simple, const float *p, int i, float otherwise) {
-                    float2 v = *reinterpret_cast<const float2 *>(p + 2 * i);
+                auto of_groups = [&](auto simple, const float *p, int w, float otherwise) {
+                    float2 v = *reinterpret_cast<const float2 *>(p + 2 * w);
                     if (!decltype(simple)::value && odd) {
-                        const uint32_t seen = sees(i);
+                        const uint32_t seen = sees(w);
                         if (!(seen & 0xFFFFu)) v.x = otherwise;
                         if (!(seen >> 16)) v.y = otherwise;
                     }
@@ -536,22 +536,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                     for (int e = 0; e < 32; e++) s[e] = seen >> e & 1u ? s[e] : -INFINITY;
                     __syncwarp();
                 };
-                float x[32], y[32], top = -INFINITY;
+                // Scores are read twice, for the maximum and for the weights, in loops that are short in the code; the next 32 are on their way as soon as these are used.
+                float s[32], top = -INFINITY;
+                tmem_ld_quarter(s_at, s);
                 auto find_top = [&](auto simple) {
-                    auto largest = [&](float (&s)[32], int w) {
-                        mask(simple, s, w);
-                        const float2 f = pair_for(simple, factors, w, 1.f);
-                        top = max3(top, max16(s) * f.x, max16(s + 16) * f.y);
-                    };
-                    tmem_ld_quarter(s_at, x);
 #pragma unroll 1
-                    for (int h = 0; h < 2; h++) {
-                        wait_quarter(x);
-                        tmem_ld_quarter(s_at + 64 * h + 32, y);
-                        largest(x, 2 * h);
-                        wait_quarter(y);
-                        tmem_ld_quarter(s_at + (h ? 0 : 64), x);             // in the end the first ones again
-                        largest(y, 2 * h + 1);
+                    for (int w = 0; w < 4; w++) {
+                        wait_quarter(s);
+                        mask(simple, s, w);
+                        const float2 f = of_groups(simple, factors, w, 1.f);
+                        const float a0 = max16(s), a1 = max16(s + 16);
+                        tmem_ld_quarter(s_at + (32 * w + 32) % 128, s);      // in the end the first ones again
+                        top = max3(top, a0 * f.x, a1 * f.y);
                     }
                 };
                 if (plain) find_top(std::true_type());
@@ -580,42 +576,35 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 const float base = m == -INFINITY ? 0.f : -m;
                 const pair_t bases = pair_of(base, base);
                 pair_t sum[2] = {0, 0};
-                // A quarter of the keys: exponentials, sums, P, which takes the place of scores that have been read.
+                // Exponentials, sums, P, which takes the place of scores that have been read.
                 auto all_weights = [&](auto simple) {
-                    auto weights = [&](float (&s)[32], int w) {
+#pragma unroll 1
+                    for (int w = 0; w < 4; w++) {
+                        wait_quarter(s);
                         mask(simple, s, w);
-                        float2 f = pair_for(simple, factors, w, 1.f);
-                        const float2 v = pair_for(simple, by, w, 0.f);
+                        float2 f = of_groups(simple, factors, w, 1.f);
+                        const float2 v = of_groups(simple, by, w, 0.f);
                         if (!decltype(simple)::value && scaled) {            // their products with the factors are rounded first, so that the maximum's weight is 1 however large m is
 #pragma unroll
                             for (int e = 0; e < 32; e++) s[e] = __fmul_rn(s[e], e < 16 ? f.x : f.y);
                             f = make_float2(1.f, 1.f);
                         }
+                        pair_t e[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) e[i] = pair_fma(pair_of(s[2 * i], s[2 * i + 1]), i < 8 ? pair_of(f.x, f.x) : pair_of(f.y, f.y), bases);
+                        if (w < 3) tmem_ld_quarter(s_at + 32 * w + 32, s);
                         uint32_t p[16];
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const pair_t f2 = i ? pair_of(f.y, f.y) : pair_of(f.x, f.x), v2 = i ? pair_of(v.y, v.y) : pair_of(v.x, v.x);
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                float a0, a1;
-                                parts_of(pair_fma(pair_of(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]), f2, bases), a0, a1);
-                                const pair_t both = pair_of(exp2_fast(a0), exp2_fast(a1));
-                                sum[e & 1] = pair_add(sum[e & 1], both);
-                                parts_of(pair_mul(both, v2), a0, a1);
-                                p[8 * i + e] = pack<__half>(a0, a1);
-                            }
+                        for (int i = 0; i < 16; i++) {
+                            float a0, a1;
+                            parts_of(e[i], a0, a1);
+                            const pair_t both = pair_of(exp2_fast(a0), exp2_fast(a1));
+                            sum[i & 1] = pair_add(sum[i & 1], both);
+                            parts_of(pair_mul(both, i < 8 ? pair_of(v.x, v.x) : pair_of(v.y, v.y)), a0, a1);
+                            p[i] = pack<__half>(a0, a1);
                         }
                         tmem_st16(s_at + 16 * w, p);
-                    };
-#pragma unroll 1
-                    for (int h = 0; h < 2; h++) {
-                        wait_quarter(x);
-                        tmem_ld_quarter(s_at + 64 * h + 32, y);
-                        weights(x, 2 * h);
-                        wait_quarter(y);
-                        if (h == 0) tmem_ld_quarter(s_at + 64, x);
-                        weights(y, 2 * h + 1);
-                        if (h == 0) signal(&sh.p_half[tile]);
+                        if (w == 1) signal(&sh.p_half[tile]);
                     }
                 };
                 if (plain && !scaled) all_weights(std::true_type());
