@@ -9,8 +9,9 @@
 // block's scale, as the sum of two f16, so that only the result is rounded.  They are relative to a maximum that may be 2^8 too low (kRoom), and to a power of
 // two of the blocks' scales (`e`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from the scores' layout to the right
 // operand's are transposed 8 x 8 at a time (movmatrix).
-// The four warps of a CTA split the keys: each takes 32 of a block of 128, has a ring of its own for their codes and scales, filled by TMA boxes of 16 keys
-// and 4-byte copies that run across the borders of units; nothing in the loop waits for another warp.  At a unit's end the four sums are joined in shared memory.
+// Four warps of a CTA split the keys: each takes 32 of a block of 128 and has a ring of its own for their codes and scales.  A fifth warp fills the rings, across the
+// borders of units: a lane brings 16 keys or values of a warp with a TMA box and their scale with a 4-byte copy.  (Where every warp filled its own, that was a
+// quarter of its instructions: 64 single tokens of the Qwen3-8B shape took 117 us.)  At a unit's end the four sums are joined in shared memory.
 #include <cstdint>
 
 #include "mgq_paged_int8.cuh"
@@ -19,7 +20,7 @@
 namespace mgq {
 namespace {
 
-constexpr int kThreads = 128, kWarps = 4, kStep = 32, kBlock = kWarps * kStep;      // keys of a warp's step, of all four
+constexpr int kThreads = 160, kWarps = 4, kStep = 32, kBlock = kWarps * kStep;      // keys of a warp's step, of all four
 constexpr int kGroups = kStep / 16;                      // 16 keys lie in one page and one block
 constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
 constexpr float kRoom = 8.f;
@@ -29,9 +30,9 @@ template <int D> __host__ __device__ constexpr uint32_t row_bytes() { return D <
 template <int D> __host__ __device__ constexpr uint32_t box_bytes() { return 16 * row_bytes<D>(); }
 template <int D> __host__ __device__ constexpr uint32_t group_bytes() { return D / row_bytes<D>() * box_bytes<D>(); }
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return 2 * kGroups * group_bytes<D>(); }   // keys of all groups, then values
-template <int D, int NP> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 4 : D == 128 ? (NP == 1 ? 3 : 2) : 1; }
-template <int D> __host__ __device__ constexpr int stages() { return D == 64 ? 3 : D == 128 ? 2 : 3; }
-constexpr int kJoin = 4;                                 // blocks of 16 columns joined at a time
+template <int D, int NP> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 3 : D == 128 ? 2 : 1; }
+template <int D> __host__ __device__ constexpr int stages() { return D == 64 ? 3 : 3; }
+constexpr int kJoin = 2;                                 // blocks of 16 columns joined at a time
 constexpr uint32_t kJoinPitch = kJoin * 16 + 2;
 template <int D, int NP> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * stages<D>() * stage_bytes<D>() + kWarps * NP * 8 * kJoinPitch * 4; }
 
@@ -40,29 +41,22 @@ __device__ unsigned int g_decode8_error;
 struct Maps {
     CUtensorMap k, v;
 };
+// Of a warp's keys in a ring's stage.
+struct __align__(8) Step {
+    int have[kGroups];                                   // how many of each 16 exist
+    float scale[kGroups][2];                             // of keys and values
+};
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose(uint32_t v)
 {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
-}
-__device__ __forceinline__ uint4 lds16(uint32_t addr)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t addr)
-{
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
 }
 constexpr uint32_t kBias = 0x80808080u, kHigh = 0x64646464u;
 // Two f16 whose bytes are 0x64 and a biased code each, less 1024 + 128.
@@ -91,19 +85,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     using Way = Walk<8 * NP, kBlock, kExtra>;
     extern __shared__ uint8_t s_raw[];
     __shared__ unsigned long long s_walk[40];
-    __shared__ __align__(8) unsigned long long s_full[kWarps][S];
-    __shared__ Way s_way[kWarps];
-    __shared__ Segment s_seg[kWarps][8];
-    __shared__ float s_scale[kWarps][S][kGroups][2];
-    __shared__ int s_have[kWarps][S][kGroups];
+    __shared__ __align__(8) unsigned long long s_full[kWarps][S], s_empty[kWarps][S];
+    __shared__ Way s_way;
+    __shared__ Segment s_seg[8];                         // the last units begun; no tokens behind the last
+    __shared__ Step s_step[kWarps][S];
     __shared__ float s_m[kWarps][8 * NP], s_l[kWarps][8 * NP];
     __shared__ volatile int s_failed;
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = __shfl_sync(0xffffffffu, t >> 5, 0), d = a.d;
     uint8_t *s_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t ring = smem_u32(s_mem) + warp * (S * kStage);
+    const uint8_t *codes = s_mem + warp * (S * kStage);
     float *s_join = reinterpret_cast<float *>(s_mem + (size_t)kWarps * S * kStage);
     if (t == 0) {
-        for (int i = 0; i < kWarps * S; i++) mbar_init(&s_full[i / S][i % S], 4 * kGroups);      // a box and a scale of keys and of values each
+        for (int i = 0; i < kWarps * S; i++) {
+            mbar_init(&s_full[i / S][i % S], 4 * kGroups);       // a box and a scale of keys and of values each
+            mbar_init(&s_empty[i / S][i % S], 1);
+        }
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -112,83 +108,91 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     {
         Way way;
         way.begin(a, blockIdx.x, gridDim.x, s_walk);
-        if (lane == 0) s_way[warp] = way;
+        if (t == kWarps * 32) s_way = way;
     }
     if (t == 0) clear_parts(a, blockIdx.x);
-    __syncwarp();
+    __syncthreads();
 
-    // ---- the producer's side of a warp: one step of 32 keys at a time, a segment without keys is a step without loads.  Lane = group of 16 keys * 2 + (keys or
-    // values) brings its box and scale; it has looked up its page a step ahead.
-    uint32_t p_seg = 0, p_block = 0, p_end = 0, p_slot = 0;      // segments begun, its next and last block, ring slot
-    bool p_live = true;
-    const uint32_t *p_table = nullptr;
-    int p_len = 0, p_kv = 0;
-    uint32_t p_page = 0xFFFFFFFFu;
-    const uint32_t p_group = lane >> 1 & (kGroups - 1);
-    auto look_up = [&]() {
-        const uint32_t key = p_block * kBlock + warp * kStep + p_group * 16;
-        p_page = p_block < p_end && (int)key < p_len ? p_table[key >> a.page_shift] : 0xFFFFFFFFu;
-    };
-    auto produce = [&]() {
-        if (p_live && p_block >= p_end) {                // the next segment
+    if (warp == kWarps) {
+        // lane = warp * 4 + group of 16 keys * 2 + (keys or values); a segment without keys is a step without loads, and so is the end
+        const uint32_t to = lane >> 2 & 3u, group = lane >> 1 & 1u, values = lane & 1u, within = (1u << a.page_shift) - 1;
+        const bool mine = lane < 16;
+        uint32_t seg = 0, slot = 0, round = 0, armed = 0;
+        bool ok = true, more = true;
+        while (more && ok) {
             if (lane == 0) {
                 Segment g;
-                const bool more = s_way[warp].next(a, g);
-                g.table = more ? g.table : nullptr;
-                s_seg[warp][p_seg & 7u] = g;
+                if (!s_way.next(a, g)) g.tokens = g.begin = g.end = 0;
+                s_seg[seg & 7u] = g;
             }
             __syncwarp();
-            const Segment &g = s_seg[warp][p_seg & 7u];
-            p_live = g.table != nullptr;
-            if (p_live) {
-                p_seg++;
-                p_table = g.table;
-                p_len = g.end <= g.begin ? 0 : g.len;
-                p_kv = (int)g.kv;
-                p_block = g.begin;
-                p_end = max(g.end, g.begin + 1);
-                look_up();
-            }
-        }
-        if (p_live) {
-            if (lane < 2 * kGroups) {
-                const uint32_t key = p_block * kBlock + warp * kStep + p_group * 16, within = (1u << a.page_shift) - 1;
-                const bool values = lane & 1u, real = p_page < a.pages;         // also: in front of the sequence's end
-                unsigned long long *bar = &s_full[warp][p_slot];
-                const uint32_t scale = smem_u32(&s_scale[warp][p_slot][p_group][values]);
-                if (!values) s_have[warp][p_slot][p_group] = real ? min(16, p_len - (int)key) : 0;       // written before the arrivals that publish it
-                if (real) {
-                    const uint32_t slot = (p_page << a.page_shift) + (key & within), dst = ring + p_slot * kStage + (values * kGroups + p_group) * kGroup;
-                    const float *from = (values ? a.v_scales : a.k_scales) + (size_t)(slot >> a.block_shift) * a.kv_heads + p_kv;
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale), "l"(from) : "memory");
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-                    mbar_arrive_expect_tx(bar, kGroup);
+            const Segment &g = s_seg[seg & 7u];
+            seg++;
+            more = g.tokens != 0;
+            const uint32_t *table = g.table;
+            const uint32_t begin = g.begin, end = max(g.end, g.begin + 1);
+            const int len = more && g.end > g.begin ? g.len : 0, kv = (int)g.kv;
+            uint32_t key = begin * kBlock + to * kStep + group * 16;
+            uint32_t page = mine && (int)key < len ? table[key >> a.page_shift] : 0xFFFFFFFFu;
+            for (uint32_t b = begin; b < end; b++) {
+                const uint32_t next_key = key + kBlock, next_page = mine && b + 1 < end && (int)next_key < len ? table[next_key >> a.page_shift] : 0xFFFFFFFFu;      // a step ahead
+                if (!(ok = mbar_wait_lanes(&s_empty[to][slot], (round & 1u) ^ 1u, mine, &s_failed, &g_decode8_error))) break;
+                if (mine) {
+                    const bool real = page < a.pages;            // also: in front of the sequence's end
+                    unsigned long long *bar = &s_full[to][slot];
+                    Step &step = s_step[to][slot];
+                    const uint32_t scale = smem_u32(&step.scale[group][values]);
+                    if (!values) step.have[group] = real ? min(16, len - (int)key) : 0;      // written before the arrivals that publish it
+                    if (real) {
+                        const uint32_t at = (page << a.page_shift) + (key & within), dst = smem_u32(s_mem) + (to * S + slot) * kStage + (values * kGroups + group) * kGroup;
+                        const float *from = (values ? a.v_scales : a.k_scales) + (size_t)(at >> a.block_shift) * a.kv_heads + kv;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale), "l"(from) : "memory");
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+                        mbar_arrive_expect_tx(bar, kGroup);
 #pragma unroll
-                    for (int c = 0; c < PARTS; c++) tma_load_3d(dst + c * kBox, values ? &maps.v : &maps.k, c * 128, p_kv, (int)slot, bar);
-                } else {
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale), "f"(0.f) : "memory");
-                    mbar_arrive(bar);
-                    mbar_arrive(bar);
+                        for (int c = 0; c < PARTS; c++) tma_load_3d(dst + c * kBox, values ? &maps.v : &maps.k, c * 128, kv, (int)at, bar);
+                    } else {
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale), "f"(0.f) : "memory");
+                        mbar_arrive(bar);
+                        mbar_arrive(bar);
+                    }
                 }
+                __syncwarp();
+                key = next_key;
+                page = next_page;
+                armed++;
+                if (++slot == S) { slot = 0; round++; }
             }
-            __syncwarp();
-            p_block++;
-            look_up();
-            p_slot = p_slot == S - 1 ? 0 : p_slot + 1;
         }
-    };
-#pragma unroll 1
-    for (int i = 0; i < S - 1; i++) produce();
+        // given up: the copies in flight land before the CTA exits
+        if (!ok && lane < kWarps)
+            for (uint32_t i = 0; i < min(armed, (uint32_t)S); i++) {
+                if (slot-- == 0) { slot = S - 1; round--; }
+                for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&s_full[lane][slot], round & 1u); w++) { }
+            }
+        return;
+    }
 
-    // ---- the consumer's side
+    // ---- the warps that use them
+    // A warp whose wait ran out meets the others once more, behind the unit, and all four leave: nobody waits for one that is gone.
+    auto meet = [] { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); };
+    auto any = [](bool mine) {
+        uint32_t r;
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)mine) : "memory");
+        return r != 0;
+    };
     uint32_t c_seg = 0, slot = 0, parity = 0;
     bool ok = true;
     const uint32_t row = lane >> 2, quad = lane & 3u;
     // byte `at` of row r of a box, as the swizzle of 64 or 128 bytes places its 16-byte pieces
     auto place = [](uint32_t r, uint32_t at) { return r * kRow + (at ^ (kRow == 128 ? (r & 7u) << 4 : (r >> 1 & 3u) << 4)); };
-    while (c_seg < p_seg) {
-        const Segment g = s_seg[warp][c_seg & 7u];
-        c_seg++;
+    for (;; c_seg++) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode8_error));
+        const Segment g = s_seg[c_seg & 7u];
+        if (!ok || g.tokens == 0) {
+            any(!ok);
+            break;
+        }
         const uint32_t pairs = g.tokens * g.heads;
         // queries of pair `row` of each block of 8: for part c of 128 dimensions those from c * 128 + quad * kPer on
         uint32_t q[NP][KT][2];
@@ -262,21 +266,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
         const uint32_t blocks = max(g.end, g.begin + 1) - g.begin;
         const int last_pos = g.pos0 + (int)g.tokens - 1;
         for (uint32_t b = 0; b < blocks; b++) {
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode8_error)))) break;
-            const uint32_t base = ring + slot * kStage;
+            if (b > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode8_error)))) break;
+            const uint8_t *base = codes + slot * kStage;
+            const Step &step = s_step[warp][slot];
+            unsigned long long *const empty = &s_empty[warp][slot];
             int have[kGroups];
             float ks[kGroups], vs[kGroups];
 #pragma unroll
             for (int i = 0; i < kGroups; i++) {
-                have[i] = s_have[warp][slot][i];
-                ks[i] = s_scale[warp][slot][i][0];
-                vs[i] = s_scale[warp][slot][i][1];
+                have[i] = step.have[i];
+                ks[i] = step.scale[i][0];
+                vs[i] = step.scale[i][1];
             }
             slot = slot == S - 1 ? 0 : slot + 1;
             parity ^= slot == 0;
-            produce();
+            auto leave = [&]() {                         // all lanes have read
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty);
+            };
             const int key0 = (int)((g.begin + b) * kBlock + warp * kStep);
-            if (have[0] + have[kGroups - 1] == 0 || key0 > last_pos) continue;
+            if (have[0] + have[kGroups - 1] == 0 || key0 > last_pos) {
+                leave();
+                continue;
+            }
             float s[kGroups][NP][4];
 #pragma unroll
             for (int i = 0; i < kGroups; i++) {
@@ -284,13 +296,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 for (int n = 0; n < NP; n++) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
 #pragma unroll
                 for (int c = 0; c < PARTS; c++) {
-                    const uint32_t k = base + i * kGroup + c * kBox;
+                    const uint8_t *k = base + i * kGroup + c * kBox;
                     uint32_t w[2][kWords];
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
                         for (uint32_t e = 0; e < kWords; e += 4) {
-                            const uint4 x = lds16(k + place(row + 8 * h, quad * kPer + 4 * e));
+                            const uint4 x = *reinterpret_cast<const uint4 *>(k + place(row + 8 * h, quad * kPer + 4 * e));
                             w[h][e] = x.x ^ kBias; w[h][e + 1] = x.y ^ kBias; w[h][e + 2] = x.z ^ kBias; w[h][e + 3] = x.w ^ kBias;
                         }
 #pragma unroll
@@ -377,16 +389,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 // values of keys 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9, dimensions row * kOwn on: a product's rows are two of them each
 #pragma unroll
                 for (int c = 0; c < PARTS; c++) {
-                    const uint32_t v = base + (kGroups + i) * kGroup + c * kBox;
+                    const uint8_t *v = base + (kGroups + i) * kGroup + c * kBox;
                     uint32_t w[4][kOwn / 4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const uint32_t at = v + place(2 * quad + (k & 1) + (k >> 1) * 8, row * kOwn);
+                        const uint8_t *at = v + place(2 * quad + (k & 1) + (k >> 1) * 8, row * kOwn);
                         if constexpr (kOwn == 16) {
-                            const uint4 x = lds16(at);
+                            const uint4 x = *reinterpret_cast<const uint4 *>(at);
                             w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
                         } else {
-                            const uint2 x = lds8(at);
+                            const uint2 x = *reinterpret_cast<const uint2 *>(at);
                             w[k][0] = x.x; w[k][1] = x.y;
                         }
                     }
@@ -410,9 +422,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     }
                 }
             }
+            leave();
         }
 
-        if (!ok) break;
+        if (any(!ok)) break;
 
         // ---- the four warps' sums
 #pragma unroll
@@ -427,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     s_l[warp][n * 8 + 2 * quad + e] = sum;
                 }
             }
-        __syncthreads();
+        meet();
         auto total = [&](uint32_t r, float &top) {
             top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
             float sum = 0.f;
@@ -462,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 #pragma unroll
                     for (int j = 0; j < kAt; j++) *reinterpret_cast<float2 *>(dst + 2 * j) = make_float2(o[n][j0 + j][e], o[n][j0 + j][e + 2]);
                 }
-            __syncthreads();
-            for (uint32_t i = t; i < pairs * 8; i += kThreads) {
+            meet();
+            for (uint32_t i = t; i < pairs * 8; i += kWarps * 32) {
                 const uint32_t r = i / 8, at = i % 8;
                 const uint32_t per = kOwn / 2, column = j0 / per * 128 + at * kOwn + j0 % per * 2;
                 if (column >= d) continue;
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     for (int c = 0; c < kSpan; c++) y[c] = rounded<T>(x[c] * inv);
                     if (wide) {
 #pragma unroll
-                        for (int c = 0; c < kSpan; c += 8) *reinterpret_cast<uint4 *>(dst + c) = *reinterpret_cast<const uint4 *>(y + c);
+                        for (int c = 0; c < kSpan; c += 4) *reinterpret_cast<uint2 *>(dst + c) = *reinterpret_cast<const uint2 *>(y + c);
                     } else {
 #pragma unroll
                         for (int c = 0; c < kSpan; c++) dst[c] = y[c];
@@ -498,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     for (int c = 0; c < kSpan; c += 2) *reinterpret_cast<float2 *>(part + r * d + column + c) = make_float2(x[c], x[c + 1]);
                 }
             }
-            __syncthreads();
+            meet();
         }
         if (!alone) {
             if (t < pairs) {
@@ -508,16 +521,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 part[8 * NP * d + 2 * t + 1] = sum;
             }
             if (t == 0) name_part(a, blockIdx.x, g);
-            __syncthreads();                             // before the next unit's maxima
+            meet();                             // before the next unit's maxima
         }
     }
-    // given up: the copies in flight land before the CTA exits
-    if (!ok && lane == 0)
-        for (int i = 0; i < S - 1; i++) {
-            for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&s_full[warp][slot], parity); w++) { }
-            slot = slot == S - 1 ? 0 : slot + 1;
-            parity ^= slot == 0;
-        }
 }
 
 template <typename T, int D, int NP>
