@@ -4,11 +4,13 @@
 // A unit's pairs of token and head (8 or 16: heads of one key / value head share its keys) are the columns of m16n8k16 products in f16 whose rows are 16 keys of a
 // head (scores) or 16 of its dimensions (results): codes are the left operand of both, eight pairs cost no more than they are, and the accumulators of eight
 // pairs of 128 are 32 registers.  The order of k inside a product, and of the results' rows, is free, so a lane takes 16 consecutive codes of a key with one
-// load.  A code becomes an f16 exactly: with 0x64 above its biased byte it reads 1024 + 128 + code.
+// load.  A biased byte code + 128 with a zero above it is an f16, subnormal and exact: (code + 128) 2^-24.  The bias is taken off by the tensor cores: scores
+// begin at -128 2^-24 times the sum of q, and behind each product of values comes one with -128 2^-24 in their place, so that no sum ever grows with the bias.
+// (Codes made whole by a subtraction per pair of them cost a seventh of the instructions, which are what this kernel has to save.)
 // Scores: q enters as f16, times a power of two that bf16 rows need to fit its range; a row's is undone in f32 with the block's scale.  Weights: times the
-// block's scale, as the sum of two f16, so that only the result is rounded.  They are relative to a maximum that may be 2^8 too low (kRoom), and to a power of
-// two of the blocks' scales (`e`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from the scores' layout to the right
-// operand's are transposed 8 x 8 at a time (movmatrix).
+// block's scale, rounded to f16, 2^-12 of each is lost at most; the low parts of it as a second operand took 5 % longer.  They are relative to a maximum that may be
+// 2^8 too low (kRoom), and to a power of two of the blocks' scales (`e2`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from
+// the scores' layout to the right operand's are transposed 8 x 8 at a time (movmatrix).
 // Four warps of a CTA split the keys: each takes 32 of a block of 128 and has a ring of its own for their codes and scales.  A fifth warp fills the rings, across the
 // borders of units: a lane brings 16 keys or values of a warp with a TMA box and their scale with a 4-byte copy.  (Where every warp filled its own, that was a
 // quarter of its instructions: 64 single tokens of the Qwen3-8B shape took 117 us.)  At a unit's end the four sums are joined in shared memory.
@@ -58,19 +60,8 @@ __device__ __forceinline__ uint32_t transpose(uint32_t v)
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-constexpr uint32_t kBias = 0x80808080u, kHigh = 0x64646464u;
-// Two f16 whose bytes are 0x64 and a biased code each, less 1024 + 128.
-__device__ __forceinline__ uint32_t unbiased(uint32_t v)
-{
-    const uint32_t off = 0x64806480u;
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&off));
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack_half(float x, float y)
-{
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
+constexpr uint32_t kBias = 0x80808080u;                  // of four bytes; as two f16 it reads -128 2^-24 twice
+constexpr float kUnit = 0x1p-24f;                        // of the codes as operands
 // 2^e for e from -126 to 127.
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -196,14 +187,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
         const uint32_t pairs = g.tokens * g.heads;
         // queries of pair `row` of each block of 8: for part c of 128 dimensions those from c * 128 + quad * kPer on
         uint32_t q[NP][KT][2];
-        float factor[NP][2];                             // of the pairs 2 quad and 2 quad + 1, whose scores this lane has
+        float factor[NP][2], bias[NP][2];                // of the pairs 2 quad and 2 quad + 1, whose scores this lane has
         int pos[NP][2];
 #pragma unroll
         for (int n = 0; n < NP; n++) {
             const uint32_t r = n * 8 + row, token = r / g.heads, head = r - token * g.heads;
             const bool live = r < pairs;
             const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + (live ? head : 0)) * d;
-            float up = 1.f;
+            float up = 1.f, total = 0.f;
             T v[PARTS][kPer];
 #pragma unroll
             for (int c = 0; c < PARTS; c++)
@@ -234,10 +225,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 const int exponent = min(max((int)(top >> 7) - 127 - 13, -100), 112);     // the largest becomes 2^13 to 2^14
                 up = power(-exponent);
                 const float f = power(exponent);
-                factor[n][0] = __shfl_sync(0xffffffffu, f, 8 * quad) * a.scale_log2;
-                factor[n][1] = __shfl_sync(0xffffffffu, f, 8 * quad + 4) * a.scale_log2;
+                factor[n][0] = __shfl_sync(0xffffffffu, f, 8 * quad) * (a.scale_log2 / kUnit);
+                factor[n][1] = __shfl_sync(0xffffffffu, f, 8 * quad + 4) * (a.scale_log2 / kUnit);
             } else {
-                factor[n][0] = factor[n][1] = a.scale_log2;
+                factor[n][0] = factor[n][1] = a.scale_log2 / kUnit;
             }
 #pragma unroll
             for (int c = 0; c < PARTS; c++)
@@ -246,8 +237,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const T x = v[c][4 * w + 2 * h], y = v[c][4 * w + 2 * h + 1];
-                        q[n][c * kWords + w][h] = pack_half(to_f32(x) * up, to_f32(y) * up);
+                        const __half2 both = __floats2half2_rn(to_f32(x) * up, to_f32(y) * up);
+                        q[n][c * kWords + w][h] = *reinterpret_cast<const uint32_t *>(&both);
+                        total += __low2float(both) + __high2float(both);
                     }
+            total += __shfl_xor_sync(0xffffffffu, total, 1);
+            total += __shfl_xor_sync(0xffffffffu, total, 2);
+            bias[n][0] = __shfl_sync(0xffffffffu, total, 8 * quad) * (-128.f * kUnit);
+            bias[n][1] = __shfl_sync(0xffffffffu, total, 8 * quad + 4) * (-128.f * kUnit);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const uint32_t p = n * 8 + 2 * quad + e;
@@ -255,7 +252,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
             }
         }
         float o[NP][KT][4], m[NP][2], l[NP][2];
-        int e2 = -1000;                                  // results are relative to 2^e2, the blocks' scales below it
+        int e2 = -124;                                   // results are relative to 2^e2, the blocks' scales below it; up1 * up2 = 2^(kUp - e2)
+        float limit = 0.f, up1 = 0.f, up2 = 0.f;
 #pragma unroll
         for (int n = 0; n < NP; n++) {
 #pragma unroll
@@ -293,7 +291,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 #pragma unroll
             for (int i = 0; i < kGroups; i++) {
 #pragma unroll
-                for (int n = 0; n < NP; n++) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
+                for (int n = 0; n < NP; n++) {
+                    s[i][n][0] = s[i][n][2] = bias[n][0];
+                    s[i][n][1] = s[i][n][3] = bias[n][1];
+                }
 #pragma unroll
                 for (int c = 0; c < PARTS; c++) {
                     const uint8_t *k = base + i * kGroup + c * kBox;
@@ -307,8 +308,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                         }
 #pragma unroll
                     for (uint32_t e = 0; e < kWords; e++) {
-                        const uint32_t f[4] = {unbiased(__byte_perm(w[0][e], kHigh, 0x4140)), unbiased(__byte_perm(w[1][e], kHigh, 0x4140)),
-                                               unbiased(__byte_perm(w[0][e], kHigh, 0x4342)), unbiased(__byte_perm(w[1][e], kHigh, 0x4342))};
+                        const uint32_t f[4] = {__byte_perm(w[0][e], 0, 0x4140), __byte_perm(w[1][e], 0, 0x4140), __byte_perm(w[0][e], 0, 0x4342), __byte_perm(w[1][e], 0, 0x4342)};
 #pragma unroll
                         for (int n = 0; n < NP; n++) mma(s[i][n], f, q[n][c * kWords + e][0], q[n][c * kWords + e][1]);
                     }
@@ -354,23 +354,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 #pragma unroll
             for (int i = 0; i < kGroups; i++) {
                 // the block's scale below 2^e2: from 2^-3 on where e2 follows it
-                const int exponent = (int)(__float_as_uint(vs[i]) >> 23 & 255u) - 126;              // vs < 2^exponent; 129 for one that is not finite
-                if (exponent > e2 && exponent < 129) {
-                    const int next = min(exponent + 2, 127);
-                    if (e2 > -1000) {
-                        const float keep = power(max(e2 - next, -126));
+                if (!(vs[i] < limit)) {
+                    const int exponent = (int)(__float_as_uint(vs[i]) >> 23 & 255u) - 126;          // vs < 2^exponent; 129 for one that is not finite, which has no say
+                    if (exponent < 129) {
+                        const int next = min(exponent + 2, 127);
+                        const float keep = limit > 0.f ? power(max(e2 - next, -126)) : 0.f;
 #pragma unroll
                         for (int n = 0; n < NP; n++)
 #pragma unroll
                             for (int j = 0; j < KT; j++)
 #pragma unroll
                                 for (int e = 0; e < 4; e++) o[n][j][e] *= keep;
+                        e2 = next;
+                        limit = power(e2);
+                        const int shift = kUp - e2;      // in two steps, as 2^shift alone may be out of range
+                        up1 = power(max(min(shift, 100), -126));
+                        up2 = power(max(shift - 100, 0));
                     }
-                    e2 = next;
                 }
-                const int shift = kUp - max(e2, -124);                       // vs * 2^shift in two steps, as 2^shift alone may be out of range
-                const float by = vs[i] * power(max(min(shift, 100), -126)) * power(max(shift - 100, 0));
-                uint32_t high[NP][2], low[NP][2];
+                const float by = vs[i] * up1 * up2;
+                uint32_t weight[NP][2];
 #pragma unroll
                 for (int n = 0; n < NP; n++)
 #pragma unroll
@@ -382,9 +385,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                             l[n][e] += p;
                             w[e] = whole || x != -INFINITY ? p * by : 0.f;                           // no product where nothing is seen: the scale may be anything
                         }
-                        const __half2 first = __floats2half2_rn(w[0], w[1]);
-                        high[n][h] = transpose(*reinterpret_cast<const uint32_t *>(&first));
-                        low[n][h] = transpose(pack_half(w[0] - __low2float(first), w[1] - __high2float(first)));
+                        const __half2 both = __floats2half2_rn(w[0], w[1]);
+                        weight[n][h] = transpose(*reinterpret_cast<const uint32_t *>(&both));
                     }
                 // values of keys 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9, dimensions row * kOwn on: a product's rows are two of them each
 #pragma unroll
@@ -407,17 +409,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                         // [a0 b0 a1 b1] and [a2 b2 a3 b3] of the keys a, b
                         const uint32_t x0 = __byte_perm(w[0][e], w[1][e], 0x5140) ^ kBias, x1 = __byte_perm(w[0][e], w[1][e], 0x7362) ^ kBias;
                         const uint32_t y0 = __byte_perm(w[2][e], w[3][e], 0x5140) ^ kBias, y1 = __byte_perm(w[2][e], w[3][e], 0x7362) ^ kBias;
-                        const uint32_t f[2][4] = {{unbiased(__byte_perm(x0, kHigh, 0x4140)), unbiased(__byte_perm(x0, kHigh, 0x4342)),
-                                                   unbiased(__byte_perm(y0, kHigh, 0x4140)), unbiased(__byte_perm(y0, kHigh, 0x4342))},
-                                                  {unbiased(__byte_perm(x1, kHigh, 0x4140)), unbiased(__byte_perm(x1, kHigh, 0x4342)),
-                                                   unbiased(__byte_perm(y1, kHigh, 0x4140)), unbiased(__byte_perm(y1, kHigh, 0x4342))}};
+                        const uint32_t f[2][4] = {{__byte_perm(x0, 0, 0x4140), __byte_perm(x0, 0, 0x4342), __byte_perm(y0, 0, 0x4140), __byte_perm(y0, 0, 0x4342)},
+                                                  {__byte_perm(x1, 0, 0x4140), __byte_perm(x1, 0, 0x4342), __byte_perm(y1, 0, 0x4140), __byte_perm(y1, 0, 0x4342)}};
+                        const uint32_t off[4] = {kBias, kBias, kBias, kBias};
 #pragma unroll
                         for (int n = 0; n < NP; n++)
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
                                 float (&acc)[4] = o[n][c * (kOwn / 2) + 2 * e + j];
-                                mma(acc, f[j], high[n][0], high[n][1]);
-                                mma(acc, f[j], low[n][0], low[n][1]);
+                                mma(acc, f[j], weight[n][0], weight[n][1]);
+                                mma(acc, off, weight[n][0], weight[n][1]);
                             }
                     }
                 }
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
             for (int w = 0; w < kWarps; w++) sum += s_l[w][r] != 0.f ? s_l[w][r] * exp2_fast(s_m[w][r] - top) : 0.f;
             return sum;
         };
-        const float scale2 = power(max(e2, -124)) * (1.f / (1 << kUp));
+        const float scale2 = power(e2) * (1.f / (1 << kUp) / kUnit);
 #pragma unroll
         for (int n = 0; n < NP; n++)
 #pragma unroll
