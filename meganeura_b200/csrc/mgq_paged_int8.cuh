@@ -13,7 +13,7 @@ struct Attend8Args : AttendArgs {
 
 // Few new tokens per sequence (mgq_paged_int8_decode.cu).
 uint32_t decode8_ctas(uint32_t head_dim);
-constexpr uint32_t kDecode8Rows = 16;                      // of a unit, at most
+constexpr uint32_t kDecode8Rows = 32;                      // of a unit, at most
 constexpr uint32_t kDecode8Pairs = 32;                     // of a sequence that is not yet many tokens'
 int launch_decode8(const Attend8Args &a, int dtype, uint32_t pairs, cudaStream_t stream);    // pairs: a bound of a sequence's tokens * heads per key / value head
 

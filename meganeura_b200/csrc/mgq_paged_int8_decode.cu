@@ -11,9 +11,11 @@
 // block's scale, rounded to f16, 2^-12 of each is lost at most; the low parts of it as a second operand took 5 % longer.  They are relative to a maximum that may be
 // 2^8 too low (kRoom), and to a power of two of the blocks' scales (`e2`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from
 // the scores' layout to the right operand's are transposed 8 x 8 at a time (movmatrix).
-// Four warps of a CTA split the keys: each takes 32 of a block of 128 and has a ring of its own for their codes and scales.  A fifth warp fills the rings, across the
-// borders of units: a lane brings 16 keys or values of a warp with a TMA box and their scale with a 4-byte copy.  (Where every warp filled its own, that was a
-// quarter of its instructions: 64 single tokens of the Qwen3-8B shape took 117 us.)  At a unit's end the four sums are joined in shared memory.
+// Four warps of a CTA split a unit, and each takes 32 keys of a block at a time, from a ring that a fifth warp fills across the borders of units: a lane brings 16
+// keys or values with a TMA box and their scales with 4-byte copies.  (Where every warp filled its own, that was a quarter of its instructions: 64 single
+// tokens of the Qwen3-8B shape took 117 us.)  At a unit's end the sums are joined in shared memory.
+// Heads of up to 128 in pairs (H = 2): a token's codes of one head are 128 bytes or less, a kilobyte apart, and HBM gives 5.0 TB/s of such pieces (107 us, as long without
+// any arithmetic).  So where it can be a unit is two neighbouring key / value heads, whose codes come in one box, and two warps work for either.
 #include <cstdint>
 
 #include "mgq_paged_int8.cuh"
@@ -22,7 +24,7 @@
 namespace mgq {
 namespace {
 
-constexpr int kThreads = 160, kWarps = 4, kStep = 32, kBlock = kWarps * kStep;      // keys of a warp's step, of all four
+constexpr int kThreads = 160, kWarps = 4, kStep = 32;             // keys of a warp's step
 constexpr int kGroups = kStep / 16;                      // 16 keys lie in one page and one block
 constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
 constexpr float kRoom = 8.f;
@@ -43,10 +45,10 @@ __device__ unsigned int g_decode8_error;
 struct Maps {
     CUtensorMap k, v;
 };
-// Of a warp's keys in a ring's stage.
-struct __align__(8) Step {
+// Of the keys in a ring's stage.
+template <int H> struct __align__(8) Step {
     int have[kGroups];                                   // how many of each 16 exist
-    float scale[kGroups][2];                             // of keys and values
+    float scale[H][kGroups][2];                          // of keys and values
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -65,7 +67,7 @@ constexpr float kUnit = 0x1p-24f;                        // of the codes as oper
 // 2^e for e from -126 to 127.
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-template <typename T, int D, int NP>                     // D: head size rounded up to 64, 128 or 256; NP: blocks of 8 pairs
+template <typename T, int D, int NP, int H>              // D: head size rounded up to 64, 128 or 256; NP: blocks of 8 pairs; H: key / value heads of a unit
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel(const __grid_constant__ Maps maps, const Attend8Args a, bool wide)
 {
     constexpr int KT = D / 16, S = stages<D>(), PARTS = D / row_bytes<D>();
@@ -73,23 +75,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     constexpr uint32_t kPer = kRow / 4;                  // consecutive codes of a key that a lane takes for the scores
     constexpr uint32_t kOwn = kRow / 8;                  // and of a value for the results
     constexpr uint32_t kWords = kPer / 4;
-    using Way = Walk<8 * NP, kBlock, kExtra>;
+    constexpr int kRings = kWarps / H, kBlock = kRings * kStep, kRows = 8 * NP * H;
+    static_assert(H == 1 || PARTS == 1, "two heads in one box");
+    using Way = Walk<kRows, kBlock, kExtra>;
     extern __shared__ uint8_t s_raw[];
     __shared__ unsigned long long s_walk[40];
-    __shared__ __align__(8) unsigned long long s_full[kWarps][S], s_empty[kWarps][S];
+    __shared__ __align__(8) unsigned long long s_full[kRings][S], s_empty[kRings][S];
     __shared__ Way s_way;
     __shared__ Segment s_seg[8];                         // the last units begun; no tokens behind the last
-    __shared__ Step s_step[kWarps][S];
+    __shared__ Step<H> s_step[kRings][S];
     __shared__ float s_m[kWarps][8 * NP], s_l[kWarps][8 * NP];
     __shared__ volatile int s_failed;
     const uint32_t t = threadIdx.x, lane = t & 31u, warp = __shfl_sync(0xffffffffu, t >> 5, 0), d = a.d;
     uint8_t *s_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~(uintptr_t)1023);
-    const uint8_t *codes = s_mem + warp * (S * kStage);
+    const uint32_t ring = warp % kRings, sub = warp / kRings;            // whose keys this warp takes, of which of the unit's heads
+    const uint8_t *codes = s_mem + ring * (S * H * kStage);
     float *s_join = reinterpret_cast<float *>(s_mem + (size_t)kWarps * S * kStage);
     if (t == 0) {
-        for (int i = 0; i < kWarps * S; i++) {
-            mbar_init(&s_full[i / S][i % S], 4 * kGroups);       // a box and a scale of keys and of values each
-            mbar_init(&s_empty[i / S][i % S], 1);
+        for (int i = 0; i < kRings * S; i++) {
+            mbar_init(&s_full[i / S][i % S], 4 * kGroups);       // a box and scales of keys and of values each
+            mbar_init(&s_empty[i / S][i % S], H);
         }
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -105,9 +110,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     __syncthreads();
 
     if (warp == kWarps) {
-        // lane = warp * 4 + group of 16 keys * 2 + (keys or values); a segment without keys is a step without loads, and so is the end
-        const uint32_t to = lane >> 2 & 3u, group = lane >> 1 & 1u, values = lane & 1u, within = (1u << a.page_shift) - 1;
-        const bool mine = lane < 16;
+        // lane = ring * 4 + group of 16 keys * 2 + (keys or values); a segment without keys is a step without loads, and so is the end
+        const uint32_t to = (lane >> 2) % kRings, group = lane >> 1 & 1u, values = lane & 1u, within = (1u << a.page_shift) - 1;
+        const bool mine = lane < 4 * kRings;
         uint32_t seg = 0, slot = 0, round = 0, armed = 0;
         bool ok = true, more = true;
         while (more && ok) {
@@ -122,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
             more = g.tokens != 0;
             const uint32_t *table = g.table;
             const uint32_t begin = g.begin, end = max(g.end, g.begin + 1);
-            const int len = more && g.end > g.begin ? g.len : 0, kv = (int)g.kv;
+            const int len = more && g.end > g.begin ? g.len : 0, kv = (int)g.kv * H;
             uint32_t key = begin * kBlock + to * kStep + group * 16;
             uint32_t page = mine && (int)key < len ? table[key >> a.page_shift] : 0xFFFFFFFFu;
             for (uint32_t b = begin; b < end; b++) {
@@ -131,19 +136,20 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 if (mine) {
                     const bool real = page < a.pages;            // also: in front of the sequence's end
                     unsigned long long *bar = &s_full[to][slot];
-                    Step &step = s_step[to][slot];
-                    const uint32_t scale = smem_u32(&step.scale[group][values]);
+                    Step<H> &step = s_step[to][slot];
                     if (!values) step.have[group] = real ? min(16, len - (int)key) : 0;      // written before the arrivals that publish it
                     if (real) {
-                        const uint32_t at = (page << a.page_shift) + (key & within), dst = smem_u32(s_mem) + (to * S + slot) * kStage + (values * kGroups + group) * kGroup;
-                        const float *from = (values ? a.v_scales : a.k_scales) + (size_t)(at >> a.block_shift) * a.kv_heads + kv;
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale), "l"(from) : "memory");
+                        const uint32_t at = (page << a.page_shift) + (key & within), dst = smem_u32(s_mem) + ((to * S + slot) * 2 * kGroups + values * kGroups + group) * (H * kGroup);
+                        const float *from = (values ? a.v_scales : a.k_scales) + (size_t)(at >> a.block_shift) * (a.kv_heads * H) + kv;
+#pragma unroll
+                        for (int h = 0; h < H; h++) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&step.scale[h][group][values])), "l"(from + h) : "memory");
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-                        mbar_arrive_expect_tx(bar, kGroup);
+                        mbar_arrive_expect_tx(bar, H * kGroup);
 #pragma unroll
                         for (int c = 0; c < PARTS; c++) tma_load_3d(dst + c * kBox, values ? &maps.v : &maps.k, c * 128, kv, (int)at, bar);
                     } else {
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale), "f"(0.f) : "memory");
+#pragma unroll
+                        for (int h = 0; h < H; h++) step.scale[h][group][values] = 0.f;
                         mbar_arrive(bar);
                         mbar_arrive(bar);
                     }
@@ -156,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
             }
         }
         // given up: the copies in flight land before the CTA exits
-        if (!ok && lane < kWarps)
+        if (!ok && lane < kRings)
             for (uint32_t i = 0; i < min(armed, (uint32_t)S); i++) {
                 if (slot-- == 0) { slot = S - 1; round--; }
                 for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(&s_full[lane][slot], round & 1u); w++) { }
@@ -175,23 +181,32 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     uint32_t c_seg = 0, slot = 0, parity = 0;
     bool ok = true;
     const uint32_t row = lane >> 2, quad = lane & 3u;
-    // byte `at` of row r of a box, as the swizzle of 64 or 128 bytes places its 16-byte pieces
-    auto place = [](uint32_t r, uint32_t at) { return r * kRow + (at ^ (kRow == 128 ? (r & 7u) << 4 : (r >> 1 & 3u) << 4)); };
+    // byte `at` of key r of this warp's head in a box, as the swizzle of 64 or 128 bytes places its 16-byte pieces
+    auto place = [&](uint32_t r, uint32_t at) {
+        const uint32_t line = r * H + sub;
+        return line * kRow + (at ^ (kRow == 128 ? (line & 7u) << 4 : (line >> 1 & 3u) << 4));
+    };
+    // The key of a product's row r (of 8), and the 16 codes that are a lane's c-th: any order will do that is the same for all operands.  With one head a
+    // quarter of a warp reads pieces of two lines that differ in their last bit, with two heads lines of one parity: keys 0 2 1 3 6 4 7 5 and a lane's pieces four
+    // apart leave no two pieces of eight lanes in the same banks, neither of keys nor of values (heads of 64 in pairs: two).
+    auto key_of = [](uint32_t r) { return H == 1 ? r : 0x57463120u >> (4 * r) & 7u; };
+    auto piece = [&](uint32_t c) { return H == 1 || kWords == 4 ? quad * (kPer / 16) + c : quad + 4 * c; };
+    const uint32_t my_key = key_of(row);
     for (;; c_seg++) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode8_error));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[ring][slot], parity, &s_failed, &g_decode8_error));
         const Segment g = s_seg[c_seg & 7u];
         if (!ok || g.tokens == 0) {
             any(!ok);
             break;
         }
-        const uint32_t pairs = g.tokens * g.heads;
+        const uint32_t heads = g.heads / H, pairs = g.tokens * heads;        // of a key / value head
         // queries of pair `row` of each block of 8: for part c of 128 dimensions those from c * 128 + quad * kPer on
         uint32_t q[NP][KT][2];
         float factor[NP][2], bias[NP][2];                // of the pairs 2 quad and 2 quad + 1, whose scores this lane has
         int pos[NP][2];
 #pragma unroll
         for (int n = 0; n < NP; n++) {
-            const uint32_t r = n * 8 + row, token = r / g.heads, head = r - token * g.heads;
+            const uint32_t r = n * 8 + row, token = r / heads, head = r - token * heads + sub * heads;
             const bool live = r < pairs;
             const T *src = static_cast<const T *>(a.q) + (size_t)(g.row0 + (live ? token : 0)) * a.q_pitch + (size_t)(g.head0 + (live ? head : 0)) * d;
             float up = 1.f, total = 0.f;
@@ -200,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
             for (int c = 0; c < PARTS; c++)
 #pragma unroll
                 for (uint32_t e = 0; e < kPer; e += 8) {
-                    const uint32_t at = c * 128 + quad * kPer + e;              // d is a multiple of 16: all eight or none
+                    const uint32_t at = c * 128 + piece(e / 16) * 16 + e % 16;   // d is a multiple of 16: all eight or none
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
                     if (live && at < d) {
                         if (wide) {
@@ -248,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const uint32_t p = n * 8 + 2 * quad + e;
-                pos[n][e] = p < pairs ? g.pos0 + (int)(p / g.heads) : -1;
+                pos[n][e] = p < pairs ? g.pos0 + (int)(p / heads) : -1;
             }
         }
         float o[NP][KT][4], m[NP][2], l[NP][2];
@@ -264,17 +279,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
         const uint32_t blocks = max(g.end, g.begin + 1) - g.begin;
         const int last_pos = g.pos0 + (int)g.tokens - 1;
         for (uint32_t b = 0; b < blocks; b++) {
-            if (b > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[warp][slot], parity, &s_failed, &g_decode8_error)))) break;
-            const uint8_t *base = codes + slot * kStage;
-            const Step &step = s_step[warp][slot];
-            unsigned long long *const empty = &s_empty[warp][slot];
+            if (b > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&s_full[ring][slot], parity, &s_failed, &g_decode8_error)))) break;
+            const uint8_t *base = codes + slot * (H * kStage);
+            const Step<H> &step = s_step[ring][slot];
+            unsigned long long *const empty = &s_empty[ring][slot];
             int have[kGroups];
             float ks[kGroups], vs[kGroups];
 #pragma unroll
             for (int i = 0; i < kGroups; i++) {
                 have[i] = step.have[i];
-                ks[i] = step.scale[i][0];
-                vs[i] = step.scale[i][1];
+                ks[i] = step.scale[sub][i][0];
+                vs[i] = step.scale[sub][i][1];
             }
             slot = slot == S - 1 ? 0 : slot + 1;
             parity ^= slot == 0;
@@ -282,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty);
             };
-            const int key0 = (int)((g.begin + b) * kBlock + warp * kStep);
+            const int key0 = (int)((g.begin + b) * kBlock + ring * kStep);
             if (have[0] + have[kGroups - 1] == 0 || key0 > last_pos) {
                 leave();
                 continue;
@@ -297,13 +312,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 }
 #pragma unroll
                 for (int c = 0; c < PARTS; c++) {
-                    const uint8_t *k = base + i * kGroup + c * kBox;
+                    const uint8_t *k = base + i * (H * kGroup) + c * kBox;
                     uint32_t w[2][kWords];
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
                         for (uint32_t e = 0; e < kWords; e += 4) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(k + place(row + 8 * h, quad * kPer + 4 * e));
+                            const uint4 x = *reinterpret_cast<const uint4 *>(k + place(my_key + 8 * h, piece(e / 4) * 16));
                             w[h][e] = x.x ^ kBias; w[h][e + 1] = x.y ^ kBias; w[h][e + 2] = x.z ^ kBias; w[h][e + 3] = x.w ^ kBias;
                         }
 #pragma unroll
@@ -314,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     }
                 }
             }
-            // keys `row` and `row` + 8 of a group by pairs 2 quad and 2 quad + 1
+            // keys my_key and my_key + 8 of a group by pairs 2 quad and 2 quad + 1
             const bool whole = have[0] + have[kGroups - 1] == kStep && key0 + kStep - 1 <= g.pos0 && (!a.window || key0 > last_pos - (int)a.window);
             bool up = false;
 #pragma unroll
@@ -325,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     for (int e = 0; e < 4; e++) {
                         float x = __fmul_rn(s[i][n][e], factor[n][e & 1] * ks[i]);
                         if (!whole) {
-                            const int at = (int)row + e / 2 * 8, key = key0 + i * 16 + at, p = pos[n][e & 1];
+                            const int at = (int)my_key + e / 2 * 8, key = key0 + i * 16 + at, p = pos[n][e & 1];
                             x = at < have[i] && key <= p && (!a.window || key > p - (int)a.window) ? x : -INFINITY;
                         }
                         s[i][n][e] = x;
@@ -388,14 +403,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                         const __half2 both = __floats2half2_rn(w[0], w[1]);
                         weight[n][h] = transpose(*reinterpret_cast<const uint32_t *>(&both));
                     }
-                // values of keys 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9, dimensions row * kOwn on: a product's rows are two of them each
+                // values of the keys of rows 2 quad, 2 quad + 1, and eight on, dimensions row * kOwn on: a product's rows are two of them each
 #pragma unroll
                 for (int c = 0; c < PARTS; c++) {
-                    const uint8_t *v = base + (kGroups + i) * kGroup + c * kBox;
+                    const uint8_t *v = base + (kGroups + i) * (H * kGroup) + c * kBox;
                     uint32_t w[4][kOwn / 4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const uint8_t *at = v + place(2 * quad + (k & 1) + (k >> 1) * 8, row * kOwn);
+                        const uint8_t *at = v + place(key_of(2 * quad + (k & 1)) + (k >> 1) * 8, row * kOwn);
                         if constexpr (kOwn == 16) {
                             const uint4 x = *reinterpret_cast<const uint4 *>(at);
                             w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
@@ -428,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 
         if (any(!ok)) break;
 
-        // ---- the four warps' sums
+        // ---- the sums of the warps of a head
 #pragma unroll
         for (int n = 0; n < NP; n++)
 #pragma unroll
@@ -442,11 +457,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 }
             }
         meet();
-        auto total = [&](uint32_t r, float &top) {
-            top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+        auto top_of = [&](uint32_t h, uint32_t r) {
+            float top = s_m[h * kRings][r];
+#pragma unroll
+            for (int w = 1; w < kRings; w++) top = fmaxf(top, s_m[h * kRings + w][r]);
+            return top;
+        };
+        auto total = [&](uint32_t h, uint32_t r, float &top) {
+            top = top_of(h, r);
             float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) sum += s_l[w][r] != 0.f ? s_l[w][r] * exp2_fast(s_m[w][r] - top) : 0.f;
+            for (int w = 0; w < kRings; w++) sum += s_l[h * kRings + w][r] != 0.f ? s_l[h * kRings + w][r] * exp2_fast(s_m[h * kRings + w][r] - top) : 0.f;
             return sum;
         };
         const float scale2 = power(e2) * (1.f / (1 << kUp) / kUnit);
@@ -455,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const uint32_t r = n * 8 + 2 * quad + e;
-                const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])), mine = s_l[warp][r] != 0.f ? exp2_fast(m[n][e] - top) : 0.f;
+                const float top = top_of(sub, r), mine = s_l[warp][r] != 0.f ? exp2_fast(m[n][e] - top) : 0.f;
 #pragma unroll
                 for (int j = 0; j < KT; j++) {
                     o[n][j][e] = mine != 0.f ? o[n][j][e] * mine * scale2 : 0.f;
@@ -463,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 }
             }
         const bool alone = g.first && g.last;
-        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * (8 * NP) * (d + 2);
+        float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kRows * (d + 2);
         // kJoin blocks of 16 results at a time: of every lane row's kOwn dimensions (of 128) those from c0 on
         constexpr int kAt = kJoin < KT ? kJoin : KT, kSpan = 2 * kAt;          // dimensions of a lane row joined at a time
 #pragma unroll
@@ -477,8 +498,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     for (int j = 0; j < kAt; j++) *reinterpret_cast<float2 *>(dst + 2 * j) = make_float2(o[n][j0 + j][e], o[n][j0 + j][e + 2]);
                 }
             meet();
-            for (uint32_t i = t; i < pairs * 8; i += kWarps * 32) {
-                const uint32_t r = i / 8, at = i % 8;
+            for (uint32_t i = t; i < H * pairs * 8; i += kWarps * 32) {
+                const uint32_t h = H == 1 ? 0u : i / (pairs * 8), r = i / 8 - h * pairs, at = i % 8, token = r / heads, head = h * heads + r - token * heads;
                 const uint32_t per = kOwn / 2, column = j0 / per * 128 + at * kOwn + j0 % per * 2;
                 if (column >= d) continue;
                 float x[kSpan];
@@ -486,16 +507,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                 for (int c = 0; c < kSpan; c += 2) {
                     x[c] = x[c + 1] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kWarps; w++) {
-                        const float2 v = *reinterpret_cast<const float2 *>(s_join + (w * (8 * NP) + r) * kJoinPitch + at * kSpan + c);
+                    for (int w = 0; w < kRings; w++) {
+                        const float2 v = *reinterpret_cast<const float2 *>(s_join + ((h * kRings + w) * (8 * NP) + r) * kJoinPitch + at * kSpan + c);
                         x[c] += v.x;
                         x[c + 1] += v.y;
                     }
                 }
                 if (alone) {
                     float top;
-                    const float sum = total(r, top), inv = sum == 0.f ? 0.f : 1.f / sum;
-                    const uint32_t token = r / g.heads, head = r - token * g.heads;
+                    const float sum = total(h, r, top), inv = sum == 0.f ? 0.f : 1.f / sum;
                     T *dst = static_cast<T *>(a.out) + (size_t)(g.row0 + token) * a.out_pitch + (size_t)(g.head0 + head) * d + column;
                     T y[kSpan];
 #pragma unroll
@@ -509,44 +529,57 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < kSpan; c += 2) *reinterpret_cast<float2 *>(part + r * d + column + c) = make_float2(x[c], x[c + 1]);
+                    for (int c = 0; c < kSpan; c += 2) *reinterpret_cast<float2 *>(part + (token * g.heads + head) * d + column + c) = make_float2(x[c], x[c + 1]);
                 }
             }
             meet();
         }
         if (!alone) {
-            if (t < pairs) {
+            if (t < H * pairs) {
+                const uint32_t token = t / g.heads, head = t - token * g.heads, h = head / heads;
                 float top;
-                const float sum = total(t, top);
-                part[8 * NP * d + 2 * t] = top;
-                part[8 * NP * d + 2 * t + 1] = sum;
+                const float sum = total(h, token * heads + head - h * heads, top);
+                part[kRows * d + 2 * t] = top;
+                part[kRows * d + 2 * t + 1] = sum;
             }
             if (t == 0) name_part(a, blockIdx.x, g);
-            meet();                             // before the next unit's maxima
+            meet();                                      // before the next unit's maxima
         }
     }
 }
 
-template <typename T, int D, int NP>
+template <typename T, int D, int NP, int H>
 int launch_sized(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pairs, cudaStream_t stream)
 {
     constexpr uint32_t ctas = 148 * ctas_per_sm<D, NP>();
-    auto *kernel = decode8_kernel<T, D, NP>;
+    auto *kernel = decode8_kernel<T, D, NP, H>;
     if (int rc = allow_smem(kernel, smem_bytes<D, NP>())) return rc;
     MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, NP>(), stream, maps, a, wide)) return rc;
-    return launch_merge<T, 8 * NP>(a, ctas, pairs, stream);
+    return launch_merge<T, 8 * NP * H>(a, ctas, H * pairs, stream);
 }
 
+template <typename T, int H>
+int launch_heads(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pairs, cudaStream_t stream)
+{
+    if (pairs <= 8) return a.d <= 64 ? launch_sized<T, 64, 1, H>(a, maps, wide, pairs, stream) : launch_sized<T, 128, 1, H>(a, maps, wide, pairs, stream);
+    return a.d <= 64 ? launch_sized<T, 64, 2, H>(a, maps, wide, pairs, stream) : launch_sized<T, 128, 2, H>(a, maps, wide, pairs, stream);
+}
+// Two key / value heads to a unit: as one with the query heads of both.
+bool in_pairs(const Attend8Args &a) { return a.d <= 128 && a.kv_heads % 2 == 0 && a.group <= 16; }
 template <typename T>
 int launch_typed(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pairs, cudaStream_t stream)
 {
-    if (a.d > 128) return launch_sized<T, 256, 1>(a, maps, wide, pairs, stream);
-    if (pairs <= 8) return a.d <= 64 ? launch_sized<T, 64, 1>(a, maps, wide, pairs, stream) : launch_sized<T, 128, 1>(a, maps, wide, pairs, stream);
-    return a.d <= 64 ? launch_sized<T, 64, 2>(a, maps, wide, pairs, stream) : launch_sized<T, 128, 2>(a, maps, wide, pairs, stream);
+    if (a.d > 128) return launch_sized<T, 256, 1, 1>(a, maps, wide, pairs, stream);
+    if (!in_pairs(a)) return launch_heads<T, 1>(a, maps, wide, pairs, stream);
+    Attend8Args b = a;
+    b.kv_heads /= 2;
+    b.group *= 2;
+    b.rows_to = a.rows_to < 0x80000000u ? 2 * a.rows_to + 1 : a.rows_to;
+    return launch_heads<T, 2>(b, maps, wide, pairs, stream);
 }
 
-// {head_dim, kv_heads, pages * page_size} of a cache, for boxes of 64 or 128 codes by 16 tokens of one head, in the swizzle of that size.  What lies outside
+// {head_dim, kv_heads, pages * page_size} of a cache, for boxes of 64 or 128 codes by 16 tokens of one head or two, in the swizzle of that size.  What lies outside
 // reads as zero.
 int encode_codes(CUtensorMap &map, const void *base, const Attend8Args &a)
 {
@@ -554,7 +587,7 @@ int encode_codes(CUtensorMap &map, const void *base, const Attend8Args &a)
     if (int rc = encode_fn(encode)) return rc;
     const cuuint64_t dims[3] = {a.d, a.kv_heads, (cuuint64_t)a.pages << a.page_shift};
     const cuuint64_t strides[2] = {a.d, (cuuint64_t)a.kv_heads * a.d};
-    const cuuint32_t box[3] = {a.d <= 64 ? 64u : 128u, 1, 16}, elem[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {a.d <= 64 ? 64u : 128u, in_pairs(a) ? 2u : 1u, 16}, elem[3] = {1, 1, 1};
     const CUresult cr = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                a.d <= 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                a.d % 128 == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
