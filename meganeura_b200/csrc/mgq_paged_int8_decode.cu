@@ -24,7 +24,7 @@
 namespace mgq {
 namespace {
 
-constexpr int kThreads = 160, kWarps = 4, kStep = 32;             // keys of a warp's step
+constexpr int kWarps = 4, kStep = 32;             // keys of a warp's step
 constexpr int kGroups = kStep / 16;                      // 16 keys lie in one page and one block
 constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
 constexpr float kRoom = 8.f;
@@ -34,11 +34,16 @@ template <int D> __host__ __device__ constexpr uint32_t row_bytes() { return D <
 template <int D> __host__ __device__ constexpr uint32_t box_bytes() { return 16 * row_bytes<D>(); }
 template <int D> __host__ __device__ constexpr uint32_t group_bytes() { return D / row_bytes<D>() * box_bytes<D>(); }
 template <int D> __host__ __device__ constexpr uint32_t stage_bytes() { return 2 * kGroups * group_bytes<D>(); }   // keys of all groups, then values
-template <int D, int NP> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 3 : D == 128 ? 2 : 1; }
-template <int D> __host__ __device__ constexpr int stages() { return D == 64 ? 3 : 3; }
+template <int D> __host__ __device__ constexpr int ctas_per_sm() { return D == 64 ? 3 : D == 128 ? 2 : 1; }
+constexpr int kStages = 3;
+// Heads of 128 by 16 pairs need more registers than the 168 that the ten warps of two CTAs of 160 threads leave each: 128 * 208 + 128 * 48 = 256 * 128, for the
+// warps that compute and for the one that fills the rings with three idle ones beside it.  32 sequences of up to 20 pairs take 59 us so, 64 with 90 bytes in local
+// memory; eight pairs are slower by it, 103 and 101 us.  (Three blocks of pairs, which would read the keys of 20 pairs once, took 77 us.)
+template <int D, int NP> __host__ __device__ constexpr bool splits_registers() { return D == 128 && NP == 2; }
+template <int D, int NP> __host__ __device__ constexpr int threads() { return splits_registers<D, NP>() ? 256 : 160; }
 constexpr int kJoin = 2;                                 // blocks of 16 columns joined at a time
 constexpr uint32_t kJoinPitch = kJoin * 16 + 2;
-template <int D, int NP> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * stages<D>() * stage_bytes<D>() + kWarps * NP * 8 * kJoinPitch * 4; }
+template <int D, int NP> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * kStages * stage_bytes<D>() + kWarps * NP * 8 * kJoinPitch * 4; }
 
 __device__ unsigned int g_decode8_error;
 
@@ -68,9 +73,9 @@ constexpr float kUnit = 0x1p-24f;                        // of the codes as oper
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 template <typename T, int D, int NP, int H>              // D: head size rounded up to 64, 128 or 256; NP: blocks of 8 pairs; H: key / value heads of a unit
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel(const __grid_constant__ Maps maps, const Attend8Args a, bool wide)
+__global__ void __launch_bounds__(threads<D, NP>(), ctas_per_sm<D>()) decode8_kernel(const __grid_constant__ Maps maps, const Attend8Args a, bool wide)
 {
-    constexpr int KT = D / 16, S = stages<D>(), PARTS = D / row_bytes<D>();
+    constexpr int KT = D / 16, S = kStages, PARTS = D / row_bytes<D>();
     constexpr uint32_t kStage = stage_bytes<D>(), kRow = row_bytes<D>(), kBox = box_bytes<D>(), kGroup = group_bytes<D>();
     constexpr uint32_t kPer = kRow / 4;                  // consecutive codes of a key that a lane takes for the scores
     constexpr uint32_t kOwn = kRow / 8;                  // and of a value for the results
@@ -109,7 +114,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     if (t == 0) clear_parts(a, blockIdx.x);
     __syncthreads();
 
-    if (warp == kWarps) {
+    if (warp >= kWarps) {
+        if constexpr (splits_registers<D, NP>()) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp > kWarps) return;
         // lane = ring * 4 + group of 16 keys * 2 + (keys or values); a segment without keys is a step without loads, and so is the end
         const uint32_t to = (lane >> 2) % kRings, group = lane >> 1 & 1u, values = lane & 1u, within = (1u << a.page_shift) - 1;
         const bool mine = lane < 4 * kRings;
@@ -171,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
     }
 
     // ---- the warps that use them
+    if constexpr (splits_registers<D, NP>()) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // A warp whose wait ran out meets the others once more, behind the unit, and all four leave: nobody waits for one that is gone.
     auto meet = [] { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); };
     auto any = [](bool mine) {
@@ -551,11 +559,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, NP>()) decode8_kernel
 template <typename T, int D, int NP, int H>
 int launch_sized(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pairs, cudaStream_t stream)
 {
-    constexpr uint32_t ctas = 148 * ctas_per_sm<D, NP>();
+    constexpr uint32_t ctas = 148 * ctas_per_sm<D>();
     auto *kernel = decode8_kernel<T, D, NP, H>;
     if (int rc = allow_smem(kernel, smem_bytes<D, NP>())) return rc;
     MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    if (int rc = launch(kernel, dim3(ctas), dim3(kThreads), smem_bytes<D, NP>(), stream, maps, a, wide)) return rc;
+    if (int rc = launch(kernel, dim3(ctas), dim3(threads<D, NP>()), smem_bytes<D, NP>(), stream, maps, a, wide)) return rc;
     return launch_merge<T, 8 * NP * H>(a, ctas, H * pairs, stream);
 }
 
@@ -596,7 +604,7 @@ int encode_codes(CUtensorMap &map, const void *base, const Attend8Args &a)
 
 }  // namespace
 
-uint32_t decode8_ctas(uint32_t head_dim) { return 148 * (head_dim <= 64 ? ctas_per_sm<64, 1>() : head_dim <= 128 ? ctas_per_sm<128, 1>() : ctas_per_sm<256, 1>()); }
+uint32_t decode8_ctas(uint32_t head_dim) { return 148 * (head_dim <= 64 ? ctas_per_sm<64>() : head_dim <= 128 ? ctas_per_sm<128>() : ctas_per_sm<256>()); }
 
 int launch_decode8(const Attend8Args &a, int dtype, uint32_t pairs, cudaStream_t stream)
 {
