@@ -4,13 +4,14 @@
 namespace mgq {
 namespace {
 
-// A block's scale is that of its largest value, so its rows belong together: those of a step that fall into one block stand one behind another, and the CTA of
-// the first of them takes all, for one head of the keys or of the values.  new = max(old, largest / 127), where old is 0 if the block's first slot is among
-// them: the block starts anew.  Codes that the block holds already become rint(code * old / new) where the scale grew.
-// Rotated values stay in registers between the pass for the largest and the one for the codes, kHold steps of 8 values a thread (64 rows of 128); what
-// lies behind is computed again.
-constexpr int kThreads = 256, kHold = 4;
-constexpr uint32_t kMostBlock = 1024;
+// A block's scale is that of its largest value, so its rows belong together: those of a step that fall into one block, a run, stand one behind another.  A CTA
+// takes the runs that begin in a window of rows, for one head of the keys or of the values: a run of more than kShort rows by all its threads, shorter ones by a
+// warp each.  new = max(old, largest / 127), where old is 0 if the block's first slot is among the rows: the block starts anew.  Codes that the block holds already
+// become rint(code * old / new) where the scale grew.  Rotated values stay in registers between the pass for the largest and the one for the codes, kHold
+// steps of 8 values a thread (64 rows of 128 for a CTA); what lies behind is computed again.
+// Loads that wait for one another bound it (slots, then scale and rows, then what is held): windows are as wide as leaves a few CTAs per SM.
+constexpr int kThreads = 256, kWarps = kThreads / 32, kHold = 4;
+constexpr uint32_t kMostBlock = 1024, kMostWindow = 32, kShort = 4;
 
 struct Append8Args {
     const void *q, *k, *v;
@@ -48,12 +49,126 @@ __device__ __forceinline__ void read4(const T *p, float (&f)[4], bool wide)
     }
 }
 
+// Rows [r0, r0 + n) into their block, by THREADS threads (a warp or the CTA).
+template <typename S, int THREADS, typename Slot>
+__device__ __forceinline__ void store_run(const Append8Args &a, const double *frequency, uint32_t *written, uint32_t *tops, uint32_t r0, uint32_t n, uint32_t head, bool values,
+                                          bool wide, Slot slot_of)
+{
+    auto meet = [] {
+        if constexpr (THREADS == 32) __syncwarp();
+        else                         __syncthreads();
+    };
+    const uint32_t t = threadIdx.x % THREADS, half = a.d / 2, steps = half / 4, block = 1u << a.block_shift, pitch = values ? a.v_pitch : a.k_pitch;
+    const bool rotate = a.rotate && !values;
+    const S *src = static_cast<const S *>(values ? a.v : a.k) + (size_t)head * a.d;
+    int8_t *cache = (values ? a.v_cache : a.k_cache) + (size_t)head * a.d;
+    const size_t row_bytes = (size_t)a.kv_heads * a.d;
+    const uint32_t id = slot_of(r0) >> a.block_shift;
+    float *scale_at = (values ? a.v_scales : a.k_scales) + (size_t)id * a.kv_heads + head;
+    const float was = *scale_at;
+    const uint32_t items = n * steps;                    // four pairs of a row each
+    auto fetch = [&](uint32_t i, float (&lo)[4], float (&hi)[4]) {
+        const uint32_t r = i / steps, p = (i - r * steps) * 4;
+        const S *row = src + (size_t)(r0 + r) * pitch + p;
+        read4(row, lo, wide);
+        read4(row + half, hi, wide);
+    };
+    auto turn = [&](uint32_t i, float (&lo)[4], float (&hi)[4]) {
+        if (!rotate) return;
+        const uint32_t r = i / steps, p = (i - r * steps) * 4, position = a.positions[r0 + r];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 w = turn_of(position, frequency[p + e]);
+            const float x = lo[e] * w.x - hi[e] * w.y;
+            hi[e] = lo[e] * w.y + hi[e] * w.x;
+            lo[e] = x;
+        }
+    };
+    // the rows' loads are on their way while their slots are noted
+    float lo[kHold][4], hi[kHold][4];
+#pragma unroll
+    for (int b = 0; b < kHold; b++)
+        if (b * THREADS + t < items) fetch(b * THREADS + t, lo[b], hi[b]);
+    for (uint32_t w = t; w < (block + 31) / 32; w += THREADS) written[w] = 0;
+    meet();
+    for (uint32_t r = t; r < n; r += THREADS) {
+        const uint32_t at = slot_of(r0 + r) & (block - 1);
+        atomicOr(&written[at / 32], 1u << (at & 31u));
+    }
+    uint32_t top = 0;
+    auto larger = [&](const float (&f)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+    };
+#pragma unroll
+    for (int b = 0; b < kHold; b++)
+        if (b * THREADS + t < items) {
+            turn(b * THREADS + t, lo[b], hi[b]);
+            larger(lo[b]);
+            larger(hi[b]);
+        }
+    for (uint32_t i = kHold * THREADS + t; i < items; i += THREADS) {
+        float x[4], y[4];
+        fetch(i, x, y);
+        turn(i, x, y);
+        larger(x);
+        larger(y);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (THREADS > 32) {
+        if (t % 32 == 0) tops[t / 32] = top;
+        meet();
+        for (uint32_t w = 0; w < THREADS / 32; w++) top = max(top, tops[w]);
+    } else {
+        meet();
+    }
+    const bool anew = written[0] & 1u;
+    const float old = anew ? 0.f : was;
+    // both are not negative or NaN: as bit patterns NaN is the largest
+    const uint32_t old_bits = __float_as_uint(old) & 0x7FFFFFFFu;
+    const float scale = __uint_as_float(max(old_bits, __float_as_uint(scale_of(top)))), inverse = inverse_of(scale);
+    auto put = [&](uint32_t i, const float (&x)[4], const float (&y)[4]) {
+        const uint32_t r = i / steps, p = (i - r * steps) * 4;
+        int8_t *dst = cache + (size_t)slot_of(r0 + r) * row_bytes + p;
+        *reinterpret_cast<uint32_t *>(dst) = codes_of(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
+        *reinterpret_cast<uint32_t *>(dst + half) = codes_of(y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse);
+    };
+#pragma unroll
+    for (int b = 0; b < kHold; b++)
+        if (b * THREADS + t < items) put(b * THREADS + t, lo[b], hi[b]);
+    for (uint32_t i = kHold * THREADS + t; i < items; i += THREADS) {
+        float x[4], y[4];
+        fetch(i, x, y);
+        turn(i, x, y);
+        put(i, x, y);
+    }
+    if (!anew && old_bits != __float_as_uint(scale)) {
+        const float ratio = inverse != 0.f ? old / scale : 0.f;
+        const uint32_t pieces = a.d / 16;
+        for (uint32_t i = t; i < block * pieces; i += THREADS) {
+            const uint32_t at = i / pieces;
+            if (written[at / 32] >> (at & 31u) & 1u) continue;
+            uint4 *p = reinterpret_cast<uint4 *>(cache + (((size_t)id << a.block_shift) + at) * row_bytes) + (i - at * pieces);
+            uint4 v = *p;
+            uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int8_t *c = reinterpret_cast<const int8_t *>(&w[e]);
+                w[e] = codes_of(c[0] * ratio, c[1] * ratio, c[2] * ratio, c[3] * ratio);
+            }
+            *p = v;
+        }
+    }
+    meet();                                              // the notes and the old scale have been read by all
+    if (t == 0) *scale_at = scale;
+}
+
 template <typename S, typename T>                        // source, rotated queries
 __global__ void __launch_bounds__(kThreads) append8_kernel(const Append8Args a, bool wide)
 {
     __shared__ double s_frequency[MGQ_PAGED_MAX_HEAD / 2];
     __shared__ float2 s_turn[MGQ_PAGED_MAX_HEAD / 2];
-    __shared__ uint32_t s_written[kMostBlock / 32], s_top[kThreads / 32];
+    __shared__ uint32_t s_written[kWarps][kMostBlock / 32], s_top[kWarps];
     const uint32_t t = threadIdx.x, half = a.d / 2, steps = half / 4;
     if (a.rotate && t < half) s_frequency[t] = exp2(-a.log2_theta * (double)t / (double)half);
     pdl_launch_dependents();
@@ -92,118 +207,47 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Append8Args a, 
         }
         return;
     }
-    const uint32_t job = blockIdx.x % (2 * a.kv_heads), head = job >> 1, block = 1u << a.block_shift;
-    const bool values = job & 1u, rotate = a.rotate && !values;
-    const uint32_t from = blockIdx.x / (2 * a.kv_heads) * a.window, pitch = values ? a.v_pitch : a.k_pitch;
-    const S *src = static_cast<const S *>(values ? a.v : a.k) + (size_t)head * a.d;
-    int8_t *cache = (values ? a.v_cache : a.k_cache) + (size_t)head * a.d;
-    float *scales = values ? a.v_scales : a.k_scales;
-    const size_t row_bytes = (size_t)a.kv_heads * a.d;
-    for (uint32_t r0 = from; r0 < min(from + a.window, a.rows); r0++) {
-        const uint32_t first = a.slots[r0], id = first >> a.block_shift;
-        if (first >= a.slots_end) continue;
-        if (r0 > 0) {                                    // another CTA's, or of this window's rows before
-            const uint32_t before = a.slots[r0 - 1];
-            if (before < a.slots_end && before >> a.block_shift == id) continue;
+    // the window's slots, the one in front and 256 behind
+    __shared__ uint32_t s_slots[1 + kMostWindow + kThreads], s_runs;
+    const uint32_t job = blockIdx.x % (2 * a.kv_heads), head = job >> 1, from = blockIdx.x / (2 * a.kv_heads) * a.window;
+    const bool values = job & 1u;
+    for (uint32_t i = t; i < 1 + kMostWindow + kThreads; i += kThreads) {
+        const uint32_t r = from + i - 1;                 // row -1 is none
+        s_slots[i] = r < a.rows ? a.slots[r] : 0xFFFFFFFFu;
+    }
+    __syncthreads();
+    if (t < 32) {
+        const uint32_t before = s_slots[t], slot = s_slots[t + 1];
+        const bool begins = t < a.window && slot < a.slots_end && !(before < a.slots_end && before >> a.block_shift == slot >> a.block_shift);
+        const uint32_t runs = __ballot_sync(0xffffffffu, begins);
+        if (t == 0) s_runs = runs;
+    }
+    __syncthreads();
+    const uint32_t lane = t & 31u, warp = t >> 5, runs = s_runs;
+    auto slot_of = [&](uint32_t r) { return r - from + 1 < 1 + kMostWindow + kThreads ? s_slots[r - from + 1] : r < a.rows ? a.slots[r] : 0xFFFFFFFFu; };
+    auto rows_of = [&](uint32_t r0) {                    // whole warps
+        const uint32_t id = slot_of(r0) >> a.block_shift;
+        for (uint32_t n = 0;; n += 32) {
+            const uint32_t slot = slot_of(r0 + n + lane), rest = __ballot_sync(0xffffffffu, !(slot < a.slots_end && slot >> a.block_shift == id));
+            if (rest) return n + __ffs(rest) - 1;
         }
-        // the rows of this block, and its slots that they fill
-        for (uint32_t w = t; w < (block + 31) / 32; w += kThreads) s_written[w] = 0;
-        __syncthreads();
-        uint32_t n = 0;
-        for (bool more = true; more;) {
-            const uint32_t r = r0 + n + t, slot = r < a.rows ? a.slots[r] : 0xFFFFFFFFu;
-            const bool here = slot < a.slots_end && slot >> a.block_shift == id;
-            const uint32_t rest = __ballot_sync(0xffffffffu, !here);
-            if (t % 32 == 0) s_top[t / 32] = rest ? (uint32_t)__ffs(rest) - 1 : 32u;
-            __syncthreads();
-            uint32_t count = 0;
-            for (uint32_t w = 0; w < kThreads / 32; w++) {
-                count += s_top[w];
-                if (s_top[w] < 32) break;
-            }
-            if (t < count) atomicOr(&s_written[(slot & (block - 1)) / 32], 1u << (slot & (block - 1) & 31u));
-            n += count;
-            more = count == kThreads;
-            __syncthreads();
-        }
-        const float old = s_written[0] & 1u ? 0.f : scales[(size_t)id * a.kv_heads + head];
-        const uint32_t items = n * steps;                // four pairs of a row each
-        auto fetch = [&](uint32_t i, float (&lo)[4], float (&hi)[4]) {
-            const uint32_t r = i / steps, p = (i - r * steps) * 4;
-            const S *row = src + (size_t)(r0 + r) * pitch + p;
-            read4(row, lo, wide);
-            read4(row + half, hi, wide);
-            if (!rotate) return;
-            const uint32_t position = a.positions[r0 + r];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float2 w = turn_of(position, s_frequency[p + e]);
-                const float x = lo[e] * w.x - hi[e] * w.y;
-                hi[e] = lo[e] * w.y + hi[e] * w.x;
-                lo[e] = x;
-            }
-        };
-        float lo[kHold][4], hi[kHold][4];
-        uint32_t top = 0;
-        auto larger = [&](const float (&f)[4]) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
-        };
-#pragma unroll
-        for (int b = 0; b < kHold; b++)
-            if (b * kThreads + t < items) {
-                fetch(b * kThreads + t, lo[b], hi[b]);
-                larger(lo[b]);
-                larger(hi[b]);
-            }
-        for (uint32_t i = kHold * kThreads + t; i < items; i += kThreads) {
-            float x[4], y[4];
-            fetch(i, x, y);
-            larger(x);
-            larger(y);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (t % 32 == 0) s_top[t / 32] = top;
-        __syncthreads();
-        for (uint32_t w = 0; w < kThreads / 32; w++) top = max(top, s_top[w]);
-        // both are not negative or NaN: as bit patterns NaN is the largest
-        const uint32_t old_bits = __float_as_uint(old) & 0x7FFFFFFFu;
-        const float scale = __uint_as_float(max(old_bits, __float_as_uint(scale_of(top)))), inverse = inverse_of(scale);
-        auto put = [&](uint32_t i, const float (&x)[4], const float (&y)[4]) {
-            const uint32_t r = i / steps, p = (i - r * steps) * 4;
-            int8_t *dst = cache + (size_t)a.slots[r0 + r] * row_bytes + p;
-            *reinterpret_cast<uint32_t *>(dst) = codes_of(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
-            *reinterpret_cast<uint32_t *>(dst + half) = codes_of(y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse);
-        };
-#pragma unroll
-        for (int b = 0; b < kHold; b++)
-            if (b * kThreads + t < items) put(b * kThreads + t, lo[b], hi[b]);
-        for (uint32_t i = kHold * kThreads + t; i < items; i += kThreads) {
-            float x[4], y[4];
-            fetch(i, x, y);
-            put(i, x, y);
-        }
-        if (!(s_written[0] & 1u) && old_bits != __float_as_uint(scale)) {
-            const float ratio = inverse != 0.f ? old / scale : 0.f;
-            const uint32_t words = a.d / 4;
-            for (uint32_t i = t; i < block * words; i += kThreads) {
-                const uint32_t at = i / words;
-                if (s_written[at / 32] >> (at & 31u) & 1u) continue;
-                uint32_t *p = reinterpret_cast<uint32_t *>(cache + (((size_t)id << a.block_shift) + at) * row_bytes) + (i - at * words);
-                const uint32_t w = *p;
-                const int8_t *c = reinterpret_cast<const int8_t *>(&w);
-                *p = codes_of(c[0] * ratio, c[1] * ratio, c[2] * ratio, c[3] * ratio);
-            }
-        }
-        __syncthreads();                                 // the old scale has been read by all
-        if (t == 0) scales[(size_t)id * a.kv_heads + head] = scale;
+    };
+    uint32_t shorter = 0;
+    for (uint32_t left = runs; left; left &= left - 1) {
+        const uint32_t r0 = from + __ffs(left) - 1, n = rows_of(r0);
+        if (n > kShort) store_run<S, kThreads>(a, s_frequency, s_written[0], s_top, r0, n, head, values, wide, slot_of);
+        else            shorter |= left & -left;
+    }
+    for (uint32_t i = 0; shorter; shorter &= shorter - 1, i++) {
+        const uint32_t r0 = from + __ffs(shorter) - 1;
+        if (i % kWarps == warp) store_run<S, 32>(a, s_frequency, s_written[warp], s_top, r0, rows_of(r0), head, values, wide, slot_of);
     }
 }
 
 template <typename S, typename T>
 int launch_typed(Append8Args &a, bool wide, cudaStream_t stream)
 {
-    a.window = a.rows <= 1024 ? 1 : 4;
+    a.window = min(max((uint32_t)((unsigned long long)a.rows * 2 * a.kv_heads / (148 * 8)), 1u), kMostWindow);
     a.cache_ctas = (a.rows + a.window - 1) / a.window * 2 * a.kv_heads;
     return launch(append8_kernel<S, T>, dim3(a.cache_ctas + (a.q ? min(a.rows, 148u * 4u) : 0u)), dim3(kThreads), 0, stream, a, wide);
 }
