@@ -8,9 +8,10 @@ namespace {
 // takes the runs that begin in a window of rows, for one head of the keys or of the values: a run of more than kShort rows by all its threads, shorter ones by a
 // warp each.  new = max(old, largest / 127), where old is 0 if the block's first slot is among the rows: the block starts anew.  Codes that the block holds already
 // become rint(code * old / new) where the scale grew.  Rotated values stay in registers between the pass for the largest and the one for the codes, kHold
-// steps of 8 values a thread (64 rows of 128 for a CTA); what lies behind is computed again.
-// Loads that wait for one another bound it (slots, then scale and rows, then what is held): windows are as wide as leaves a few CTAs per SM.
-constexpr int kThreads = 256, kWarps = kThreads / 32, kHold = 4;
+// steps of 16 values a thread (32 rows of 128 for a CTA); what lies behind is computed again.
+// Loads that wait for one another bound it (slots, then scale and rows, then what is held), so CTAs per SM count more than registers: 4096 rows of the Qwen3-8B shape
+// took 52, 45, 39 us with two, three, four; and windows are as wide as leaves eight CTAs per SM.
+constexpr int kThreads = 256, kWarps = kThreads / 32, kHold = 1, kCtas = 4;
 constexpr uint32_t kMostBlock = 1024, kMostWindow = 32, kShort = 4;
 
 struct Append8Args {
@@ -33,20 +34,18 @@ __device__ __forceinline__ float2 turn_of(uint32_t position, double frequency)
     return w;
 }
 template <typename T>
-__device__ __forceinline__ void read4(const T *p, float (&f)[4], bool wide)
+__device__ __forceinline__ void read8(const T *p, float (&f)[8], bool wide)
 {
-    if (!wide) {
+    T v[8];
+    if (wide) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = to_f32(p[i]);
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(p)[i];
     } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        const T *e = reinterpret_cast<const T *>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = to_f32(e[i]);
+        for (int i = 0; i < 8; i++) v[i] = p[i];
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = to_f32(v[i]);
 }
 
 // Rows [r0, r0 + n) into their block, by THREADS threads (a warp or the CTA).
@@ -58,7 +57,7 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
         if constexpr (THREADS == 32) __syncwarp();
         else                         __syncthreads();
     };
-    const uint32_t t = threadIdx.x % THREADS, half = a.d / 2, steps = half / 4, block = 1u << a.block_shift, pitch = values ? a.v_pitch : a.k_pitch;
+    const uint32_t t = threadIdx.x % THREADS, half = a.d / 2, steps = half / 8, block = 1u << a.block_shift, pitch = values ? a.v_pitch : a.k_pitch;
     const bool rotate = a.rotate && !values;
     const S *src = static_cast<const S *>(values ? a.v : a.k) + (size_t)head * a.d;
     int8_t *cache = (values ? a.v_cache : a.k_cache) + (size_t)head * a.d;
@@ -66,18 +65,18 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
     const uint32_t id = slot_of(r0) >> a.block_shift;
     float *scale_at = (values ? a.v_scales : a.k_scales) + (size_t)id * a.kv_heads + head;
     const float was = *scale_at;
-    const uint32_t items = n * steps;                    // four pairs of a row each
-    auto fetch = [&](uint32_t i, float (&lo)[4], float (&hi)[4]) {
-        const uint32_t r = i / steps, p = (i - r * steps) * 4;
+    const uint32_t items = n * steps;                    // eight pairs of a row each
+    auto fetch = [&](uint32_t i, float (&lo)[8], float (&hi)[8]) {
+        const uint32_t r = i / steps, p = (i - r * steps) * 8;
         const S *row = src + (size_t)(r0 + r) * pitch + p;
-        read4(row, lo, wide);
-        read4(row + half, hi, wide);
+        read8(row, lo, wide);
+        read8(row + half, hi, wide);
     };
-    auto turn = [&](uint32_t i, float (&lo)[4], float (&hi)[4]) {
+    auto turn = [&](uint32_t i, float (&lo)[8], float (&hi)[8]) {
         if (!rotate) return;
-        const uint32_t r = i / steps, p = (i - r * steps) * 4, position = a.positions[r0 + r];
+        const uint32_t r = i / steps, p = (i - r * steps) * 8, position = a.positions[r0 + r];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < 8; e++) {
             const float2 w = turn_of(position, frequency[p + e]);
             const float x = lo[e] * w.x - hi[e] * w.y;
             hi[e] = lo[e] * w.y + hi[e] * w.x;
@@ -85,7 +84,7 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
         }
     };
     // the rows' loads are on their way while their slots are noted
-    float lo[kHold][4], hi[kHold][4];
+    float lo[kHold][8], hi[kHold][8];
 #pragma unroll
     for (int b = 0; b < kHold; b++)
         if (b * THREADS + t < items) fetch(b * THREADS + t, lo[b], hi[b]);
@@ -96,9 +95,9 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
         atomicOr(&written[at / 32], 1u << (at & 31u));
     }
     uint32_t top = 0;
-    auto larger = [&](const float (&f)[4]) {
+    auto larger = [&](const float (&f)[8]) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
     };
 #pragma unroll
     for (int b = 0; b < kHold; b++)
@@ -108,7 +107,7 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
             larger(hi[b]);
         }
     for (uint32_t i = kHold * THREADS + t; i < items; i += THREADS) {
-        float x[4], y[4];
+        float x[8], y[8];
         fetch(i, x, y);
         turn(i, x, y);
         larger(x);
@@ -127,17 +126,19 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
     // both are not negative or NaN: as bit patterns NaN is the largest
     const uint32_t old_bits = __float_as_uint(old) & 0x7FFFFFFFu;
     const float scale = __uint_as_float(max(old_bits, __float_as_uint(scale_of(top)))), inverse = inverse_of(scale);
-    auto put = [&](uint32_t i, const float (&x)[4], const float (&y)[4]) {
-        const uint32_t r = i / steps, p = (i - r * steps) * 4;
+    auto put = [&](uint32_t i, const float (&x)[8], const float (&y)[8]) {
+        const uint32_t r = i / steps, p = (i - r * steps) * 8;
         int8_t *dst = cache + (size_t)slot_of(r0 + r) * row_bytes + p;
-        *reinterpret_cast<uint32_t *>(dst) = codes_of(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
-        *reinterpret_cast<uint32_t *>(dst + half) = codes_of(y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse);
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(codes_of(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse),
+                                                     codes_of(x[4] * inverse, x[5] * inverse, x[6] * inverse, x[7] * inverse));
+        *reinterpret_cast<uint2 *>(dst + half) = make_uint2(codes_of(y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse),
+                                                            codes_of(y[4] * inverse, y[5] * inverse, y[6] * inverse, y[7] * inverse));
     };
 #pragma unroll
     for (int b = 0; b < kHold; b++)
         if (b * THREADS + t < items) put(b * THREADS + t, lo[b], hi[b]);
     for (uint32_t i = kHold * THREADS + t; i < items; i += THREADS) {
-        float x[4], y[4];
+        float x[8], y[8];
         fetch(i, x, y);
         turn(i, x, y);
         put(i, x, y);
@@ -164,43 +165,52 @@ __device__ __forceinline__ void store_run(const Append8Args &a, const double *fr
 }
 
 template <typename S, typename T>                        // source, rotated queries
-__global__ void __launch_bounds__(kThreads) append8_kernel(const Append8Args a, bool wide)
+__global__ void __launch_bounds__(kThreads, kCtas) append8_kernel(const Append8Args a, bool wide)
 {
     __shared__ double s_frequency[MGQ_PAGED_MAX_HEAD / 2];
-    __shared__ float2 s_turn[MGQ_PAGED_MAX_HEAD / 2];
+    __shared__ float2 s_turn[kThreads];
     __shared__ uint32_t s_written[kWarps][kMostBlock / 32], s_top[kWarps];
-    const uint32_t t = threadIdx.x, half = a.d / 2, steps = half / 4;
+    const uint32_t t = threadIdx.x, half = a.d / 2, steps = half / 8;
     if (a.rotate && t < half) s_frequency[t] = exp2(-a.log2_theta * (double)t / (double)half);
     pdl_launch_dependents();
     pdl_wait();
     __syncthreads();
-    if (blockIdx.x >= a.cache_ctas) {                    // queries: a row at a time
-        for (uint32_t r = blockIdx.x - a.cache_ctas; r < a.rows; r += gridDim.x - a.cache_ctas) {
+    if (blockIdx.x >= a.cache_ctas) {                    // queries: as many rows at a time as have an angle for every thread
+        const uint32_t at_once = kThreads / half, row_items = a.q_heads * steps;
+        for (uint32_t r0 = (blockIdx.x - a.cache_ctas) * at_once; r0 < a.rows; r0 += (gridDim.x - a.cache_ctas) * at_once) {
+            const uint32_t rows = min(at_once, a.rows - r0);
+            float x[8], y[8];
+            auto fetch = [&](uint32_t i) {
+                const uint32_t r = i / row_items, in_row = i - r * row_items, head = in_row / steps;
+                const S *src = static_cast<const S *>(a.q) + (size_t)(r0 + r) * a.q_pitch + head * a.d + (in_row - head * steps) * 8;
+                read8(src, x, wide);
+                read8(src + half, y, wide);
+            };
+            if (t < rows * row_items) fetch(t);          // on its way while the angles are found
             if (a.rotate) {
-                if (t < half) s_turn[t] = turn_of(a.positions[r], s_frequency[t]);
+                if (t < rows * half) s_turn[t] = turn_of(a.positions[r0 + t / half], s_frequency[t % half]);
                 __syncthreads();
             }
-            for (uint32_t i = t; i < a.q_heads * steps; i += kThreads) {
-                const uint32_t head = i / steps, p = (i - head * steps) * 4;
-                const S *src = static_cast<const S *>(a.q) + (size_t)r * a.q_pitch + head * a.d + p;
-                T *dst = static_cast<T *>(a.q_out) + ((size_t)r * a.q_heads + head) * a.d + p;
-                float x[4], y[4];
-                read4(src, x, wide);
-                read4(src + half, y, wide);
-                T lo[4], hi[4];
+            for (uint32_t i = t; i < rows * row_items; i += kThreads) {
+                if (i != t) fetch(i);
+                const uint32_t r = i / row_items, in_row = i - r * row_items, head = in_row / steps, p = (in_row - head * steps) * 8;
+                T lo[8], hi[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float2 w = a.rotate ? s_turn[p + e] : make_float2(1.f, 0.f);
+                for (int e = 0; e < 8; e++) {
+                    const float2 w = a.rotate ? s_turn[r * half + p + e] : make_float2(1.f, 0.f);
                     lo[e] = rounded<T>(x[e] * w.x - y[e] * w.y);
                     hi[e] = rounded<T>(x[e] * w.y + y[e] * w.x);
-                    if (!wide) {
-                        dst[e] = lo[e];
-                        dst[half + e] = hi[e];
-                    }
                 }
+                T *to = static_cast<T *>(a.q_out) + ((size_t)(r0 + r) * a.q_heads + head) * a.d + p;
                 if (wide) {
-                    *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(lo);
-                    *reinterpret_cast<uint2 *>(dst + half) = *reinterpret_cast<const uint2 *>(hi);
+                    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(lo);
+                    *reinterpret_cast<uint4 *>(to + half) = *reinterpret_cast<const uint4 *>(hi);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        to[e] = lo[e];
+                        to[half + e] = hi[e];
+                    }
                 }
             }
             if (a.rotate) __syncthreads();
@@ -249,7 +259,8 @@ int launch_typed(Append8Args &a, bool wide, cudaStream_t stream)
 {
     a.window = min(max((uint32_t)((unsigned long long)a.rows * 2 * a.kv_heads / (148 * 8)), 1u), kMostWindow);
     a.cache_ctas = (a.rows + a.window - 1) / a.window * 2 * a.kv_heads;
-    return launch(append8_kernel<S, T>, dim3(a.cache_ctas + (a.q ? min(a.rows, 148u * 4u) : 0u)), dim3(kThreads), 0, stream, a, wide);
+    const uint32_t at_once = 2 * kThreads / a.d;         // rows of queries
+    return launch(append8_kernel<S, T>, dim3(a.cache_ctas + (a.q ? min((a.rows + at_once - 1) / at_once, 148u * 4u) : 0u)), dim3(kThreads), 0, stream, a, wide);
 }
 
 }  // namespace
@@ -260,7 +271,7 @@ int launch_paged_append_int8(const void *q, const void *k, const void *v, int sr
 {
     Append8Args a{q, k, v, positions, slots, q_out, k_cache, v_cache, k_scales, v_scales, rows, q ? q_heads : 0u, kv_heads, head_dim, q_pitch, k_pitch, v_pitch,
                   pages * page_size, page_shift(block), 1, 0, theta > 0.f ? log2((double)theta) : 0.0, theta > 0.f};
-    auto fits = [](const void *p, uint32_t pitch, int dtype) { return !p || (reinterpret_cast<uintptr_t>(p) % (4 * element_bytes(dtype)) == 0 && pitch % 4 == 0); };
+    auto fits = [](const void *p, uint32_t pitch, int dtype) { return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % (16 / element_bytes(dtype)) == 0); };
     const bool wide = fits(q, q_pitch, src_dtype) && fits(k, k_pitch, src_dtype) && fits(v, v_pitch, src_dtype) && fits(q_out, 0, q_dtype);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (src_dtype == MGQ_FMT_F32) return q_dtype == MGQ_FMT_F16 ? launch_typed<float, __half>(a, wide, s) : launch_typed<float, __nv_bfloat16>(a, wide, s);
