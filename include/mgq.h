@@ -322,8 +322,10 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
  *   to the nearest.  So a block keeps what it holds until its first slot is written again.  Rows of one block stand one behind another, as the plan
  *   writes them; a value that is not finite makes the block's scale so and its values NaN, until it starts anew.  q_dtype: the type of q_out, f16 or bf16;
  *   sources are f32 or of that type.
- * mgq_paged_attention_int8: as mgq_paged_attention with keys and values code * scale; q and out are f16 or bf16 (dtype).  The result is rounded once.  Scales are
- *   not negative, and values of more than 2^96 may come out infinite.  `workspace`: mgq_paged_attention_int8_workspace(...) bytes, as there. */
+ * mgq_paged_attention_int8: as mgq_paged_attention with keys and values code * scale; q and out are f16 or bf16 (dtype).  Scores and sums are f32, a weight times
+ *   its block's scale is rounded to f16 before it meets its code, the result to its type.  Of the largest weight times the largest scale that the call meets for
+ *   a head less than 2^-29 may be lost.  Scales are not negative, and values of more than 2^96 may come out infinite.  `workspace`:
+ *   mgq_paged_attention_int8_workspace(...) bytes, as there. */
 #define MGQ_INT8_MAX_K 131056
 int mgq_quantize_rows(const void *x, int dtype, uint32_t pitch, int8_t *codes, float *scales, uint32_t rows, uint32_t k, void *stream);
 int mgq_matmul_int8(const int8_t *a, const float *a_scales, const int8_t *w, const float *w_scales, const void *addend, void *out, int dtype, uint32_t m, uint32_t k,

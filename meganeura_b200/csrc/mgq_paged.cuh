@@ -35,6 +35,7 @@ struct AttendArgs {
     const uint32_t *starts, *lengths, *table;
     uint32_t sequences, rows, kv_heads, group, d, page_shift, pages, table_width, window, q_pitch, out_pitch;
     uint32_t rows_from, rows_to;         // sequences with this many pairs of token and head of a key / value head are this kernel's
+    uint32_t least;                      // key blocks of a piece, unless there is only one piece (0: one)
     float scale_log2;                    // scale * log2(e): scores are exponents of 2
     struct PartHead *heads;              // [CTAs][2]
     float *parts;                        // [CTAs][2]: sums [ROWS][d], then maximum and weight of each row [ROWS][2]
@@ -117,7 +118,7 @@ struct Walk {
             if (w < warp) base += scratch[w];
             total += scratch[w];
         }
-        const unsigned long long pieces = min((unsigned long long)ctas, max(total, 1ull));
+        const unsigned long long pieces = min((unsigned long long)ctas, max(a.least ? total / a.least : total, 1ull));
         const unsigned long long w0 = cta < pieces ? total * cta / pieces : total, w1 = cta < pieces ? total * (cta + 1) / pieces : total;
         if (w0 >= base && w0 < base + mine) {            // one thread at most
             unsigned long long rest = w0 - base, c = 0;

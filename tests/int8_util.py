@@ -29,8 +29,8 @@ def attention_bound(dtype, want, size, reach, d, floor=0.0):
 
     The result's rounding: half a step, 2^-25 where f16 is subnormal.  A weight is 2^(s - m) over their sum.  Its exponent: s is d products in f32 whose sizes sum to at most `reach`, each
     addition off by 2^-24 of a partial sum (twice that where tensor cores truncate), then two products by scales: off by (d + 8) 2^-23 reach in all, which the weight
-    carries relatively, numerator and sum alike; the exponential adds 2^-21.  Where a sequence has many new tokens a weight times its scale is rounded to f16 before it
-    meets its code: half a step, 2^-11.  The f32 sums of weights times codes add (1 + 64 joins) 2^-22 of `size`.
+    carries relatively, numerator and sum alike; the exponential adds 2^-21.  A weight times its scale is rounded to f16 before it meets its code: half a step,
+    2^-11.  The f32 sums of weights times codes add (1 + 64 joins) 2^-22 of `size`.
 
     `floor`, a row's keys times the cache's largest value: an f16 ends at 2^-24, so each weight is off by 2^-25 at least.  A row's largest is 2^7 times 1 or more
     (many tokens: 2^8), the block's scale over its power of two, which is at most 8 times the largest scale: 2^-25 * 2^-7 * 8 = 2^-29 of the largest value per key.  It shows
