@@ -44,9 +44,10 @@ constexpr int kStages = 3;
 // memory; eight pairs are slower by it, 103 and 101 us.  (Three blocks of pairs, which would read the keys of 20 pairs once, took 77 us.)
 template <int D, int NP> __host__ __device__ constexpr bool splits_registers() { return D == 128 && NP == 2; }
 template <int D, int NP> __host__ __device__ constexpr int threads() { return splits_registers<D, NP>() ? 256 : 160; }
-constexpr int kJoin = 2;                                 // blocks of 16 columns joined at a time
-constexpr uint32_t kJoinPitch = kJoin * 16 + 2;
-template <int D, int NP> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * kStages * stage_bytes<D>() + kWarps * NP * 8 * kJoinPitch * 4; }
+// Blocks of 16 columns joined at a time, as shared memory has room for.
+template <int D, int NP> __host__ __device__ constexpr int join_blocks() { return D == 128 && NP == 2 ? 2 : 4; }
+template <int D, int NP> __host__ __device__ constexpr uint32_t join_pitch() { return join_blocks<D, NP>() * 16 + 2; }
+template <int D, int NP> constexpr size_t smem_bytes() { return 1024 + (size_t)kWarps * kStages * stage_bytes<D>() + kWarps * NP * 8 * join_pitch<D, NP>() * 4; }
 
 __device__ unsigned int g_decode8_error;
 
@@ -496,8 +497,9 @@ __global__ void __launch_bounds__(threads<D, NP>(), ctas_per_sm<D>()) decode8_ke
             }
         const bool alone = g.first && g.last;
         float *part = a.parts + (size_t)part_index(blockIdx.x, g) * kRows * (d + 2);
-        // kJoin blocks of 16 results at a time: of every lane row's kOwn dimensions (of 128) those from c0 on
-        constexpr int kAt = kJoin < KT ? kJoin : KT, kSpan = 2 * kAt;          // dimensions of a lane row joined at a time
+        // of every lane row's kOwn dimensions (of 128) kSpan at a time
+        constexpr uint32_t kJoinPitch = join_pitch<D, NP>();
+        constexpr int kAt = join_blocks<D, NP>(), kSpan = 2 * kAt;
 #pragma unroll
         for (int j0 = 0; j0 < KT; j0 += kAt) {
 #pragma unroll
