@@ -88,6 +88,20 @@ def test_product_of_many_rows(dtype, m, k, n):
     check_product(np.random.default_rng(m * k * n), dtype, m, k, n, with_addend=bool(m % 2), pitch=m % 5)
 
 
+@pytest.mark.parametrize("m,k,n", [(2048, 144, 10240), (1900, 80, 10000), (600, 64, 19456), (300, 96, 19100)])
+def test_product_of_more_tiles_than_fit_at_once(m, k, n):
+    """Several rounds of tiles, the last of them cut."""
+    import torch
+    from meganeura_b200 import ops
+    rng = np.random.default_rng(m)
+    a, w = (rng.integers(-127, 128, s).astype(np.int8) for s in ((m, k), (n, k)))
+    sa, sw = (rng.random(s).astype(np.float32) + 0.01 for s in (m, n))
+    got = host(ops.matmul_int8(dev(a), dev(sa), dev(w), dev(sw), dtype=torch.float32))
+    for rows in np.array_split(np.arange(m), 8):
+        want = IO.matmul(a[rows], sa[rows], w, sw)
+        assert (np.abs(got[rows] - want) <= product_bound("f32", want, None)).all()
+
+
 @pytest.mark.parametrize("m", [1, 9, 40, 300])
 def test_product_at_the_largest_k(m):
     check_product(np.random.default_rng(m), "f32", m, 131056, 70, extreme=True)
