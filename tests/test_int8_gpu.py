@@ -259,6 +259,18 @@ def test_attention_of_many_tokens(dtype, heads, kv_heads, d, cached, fresh, page
     check_attention(dtype, *attention_inputs(rng, dtype, heads, kv_heads, d, page, block, cached, fresh, rows=sum(fresh) + 5, gain=1.5), window=window)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", HEADS)
+@pytest.mark.parametrize("cached,fresh,width,window", [([200, 0, 33, 700, 1, 90], [70, 1, 129, 2, 0, 40], 0, 0), ([700, 5, 40], [1, 100, 3], 1100, 150)])
+def test_attention_of_many_tokens_beside_few(dtype, heads, kv_heads, d, cached, fresh, width, window):
+    """More than four sequences, and tables that reach far: the sequences of few tokens have a launch of their own."""
+    rng = np.random.default_rng(heads * d)
+    q, k, v, ks, vs, table, *rest = attention_inputs(rng, dtype, heads, kv_heads, d, 16, 16, cached, fresh, rows=sum(fresh) + 5, gain=1.5)
+    if width:
+        table = np.concatenate([table, np.full((len(table), width - table.shape[1]), -1, table.dtype)], 1)
+    check_attention(dtype, q, k, v, ks, vs, table, *rest, window=window)
+
+
 @pytest.mark.parametrize("fresh", [1, 3, 150])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attention_of_scales_that_differ_widely(dtype, fresh):
