@@ -42,7 +42,9 @@ __device__ __forceinline__ void finish(const ProductArgs &a, uint32_t m, uint32_
     static_cast<T *>(a.out)[(size_t)m * a.out_pitch + n] = to_type<T>(y);
 }
 
-constexpr uint32_t kFewRows = 8;                           // of activations: mma.sync (mgq_int8.cu), beyond them tcgen05 (mgq_int8_tc.cu)
+// Activation rows up to which mma.sync (mgq_int8.cu) takes a product, with tcgen05 (mgq_int8_tc.cu) beyond.  8 rows of 4096 by 4096 and 24576 columns take 4.8 and 17.4 us
+// there; 9 to 16, two blocks of columns for mma.sync, took 10.4 and 24.5, on tcgen05 6.2 and 19.1.
+constexpr uint32_t kFewRows = 8;
 int launch_product_tc(const ProductArgs &a, int dtype, void *stream);
 
 }  // namespace mgq

@@ -7,6 +7,8 @@
 // pair_kernel: many tiles.  Two CTAs of a cluster share tiles of 256 weight rows by `tn` activation rows (cta_group::2): each holds its 128 weight rows and half of
 // the activation rows, and has its 128 rows' sums in its TMEM.  One CTA's copies would fill and feed its shared memory at 192 bytes per cycle with 128 x 256
 // tiles, a pair needs 128.  Persistent, one accumulator is read while the other is filled.
+// 2048 x 4096 by 12288 columns: 69 to 77 us, 2.7 to 3.0 POP/s where products alone from shared memory ran at 4.33.  Operands out of L2 bound it: 8192 cubed took 425 us and
+// without its loads 306.  Stages of 256 k, and smaller tiles for the last round alone, gave nothing.
 //   warp 0      TMA of this CTA's boxes, completing on full[s] of the pair's first CTA
 //   warp 1      (first CTA) issues the products, and gives stages and accumulators to both CTAs
 //   warps 2-9   epilogue: 32 rows by every other 32 columns each
@@ -381,7 +383,7 @@ int encode(CUtensorMap &map, const int8_t *base, uint32_t k, uint32_t rows, uint
     return cr == CUDA_SUCCESS ? MGQ_OK : fail(MGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
 }
 
-constexpr uint32_t kPairs = 74, kMostCtas = 296;          // two per SM
+constexpr uint32_t kPairs = 74, kMostCtas = 296;          // one and two per SM
 
 template <typename T>
 int launch_pair(const ProductArgs &a, uint32_t tn, cudaStream_t stream)
@@ -414,26 +416,26 @@ template <typename T>
 int launch_typed(const ProductArgs &a, cudaStream_t stream)
 {
     const uint32_t n_tiles = (a.n + kRows - 1) / kRows, chunks = (a.k + kChunk - 1) / kChunk;
-    // Few tiles: as few columns each (32 at least) as leave no more than two CTAs per SM, so that most SMs have work: 256 x 576 x 1536 with 32, 64, 128, 256 columns
-    // 3.7, 3.8, 4.7, 6.9 us, 203 x 1536 x 4100 with 32, 64, 128 5.9, 6.6, 8.4; against pairs 1024 x 1536 x 1536 6.7 and 7.4.  Where even so few SMs have work and k is long a cluster
-    // shares it out: 32 x 4096 x 4096 with 1, 2, 4, 8 CTAs 10.0, 9.2, 8.0, 8.0.  From k = 8192 on more columns and that (256 x 12288 x 4096: 128 by 4 CTAs 19.8 us,
-    // 32 alone 27.3).
+    // Few tiles: narrow ones, and a cluster for each that shares out a long k, as long as all run at once, two CTAs to an SM (in clusters 264 or so find room, of eight 256).
+    // Beyond that, and for many rows where wide tiles or a long k make reads from L2 count, pairs.  Some 1600 shapes of 9 to 2048 rows, k of 128 to 12288 and 100 to 24576
+    // columns were timed with all widths and splits; with these bounds they take 1 % longer than with the best for each.  256 x 576 x 1536 with 32, 64, 128 columns
+    // 3.7, 3.8, 4.7 us; 200 x 4096 x 576 with 32 columns by 8, 4, 2 CTAs 10.7 (more than fit at once), 6.1, 7.8; 256 x 12288 x 100 by 8, 4 7.2, 8.9, with 128 columns by 4 13.3;
+    // 512 x 256 x 8192 with 128 columns 5.2, in pairs 7.2; 512 x 2560 x 8192 12.5, 12.8, 512 x 8192 x 8192 31.8, 28.3.  Rows that begin in the middle of 32 bytes cost more
+    // reads: 355 x 1024 x 11008 with 128 columns 7.9, in pairs 9.5, of k = 1040 13.1 and 10.9.
+    const uint32_t least = a.m <= 16 ? 16 : 32, most = min(a.m <= 64 ? max((a.m + 15) / 16 * 16, least) : (a.m + 31) / 32 * 32, kMostCols), few_chunks = a.k % 32 ? 4 : 12;
     auto ctas = [&](uint32_t tn) { return (unsigned long long)n_tiles * ((a.m + tn - 1) / tn); };
-    uint32_t tn = a.m <= 16 ? 16 : 32, split = 1;
-    while (tn < kMostCols && ctas(tn) > kMostCtas) tn += tn < 64 ? 16 : 32;
-    if (ctas(tn) <= kMostCtas && (tn <= 64 || a.m <= kMostCols)) {
-        if (chunks >= 64 && a.m > 64 && ctas(128) * 4 <= kMostCtas) {
-            tn = min((a.m + 15) / 16 * 16, 128u);
-            split = 4;
-        } else if (chunks >= 16 && ctas(tn) <= kMostCtas / 4) {
-            while (split < kMostSplit && ctas(tn) * split * 2 <= kMostCtas && chunks >= split * 8) split *= 2;
-        }
-        return launch_split<T>(a, tn, split, stream);
+    for (uint32_t split = kMostSplit; split > 1; split /= 2) {
+        if (chunks < (split == 4 ? 16 : 32)) continue;
+        const uint32_t widest = min(most, split == 8 || chunks < 40 ? 32u : split == 4 ? 128u : 96u);
+        for (uint32_t tn = least; tn <= widest; tn += tn < 64 ? 16 : 32)
+            if (ctas(tn) * split <= (split == 8 ? 256 : 264)) return launch_split<T>(a, tn, split, stream);
     }
+    for (uint32_t tn = least; tn <= (a.m <= 256 ? most : kMostCols / 2); tn += tn < 64 ? 16 : 32)
+        if (ctas(tn) <= kMostCtas && (tn <= 64 || a.m <= 256 || chunks <= few_chunks) && (a.m < 96 || chunks < 40)) return launch_split<T>(a, tn, 1, stream);
     // The columns of a tile with the shortest rounds of tiles, which take as long as tn + 64 columns: 2048 x 12288 x 4096 with 128, 160, 192, 224, 256 took 101, 86, 95, 98,
     // 79 us, 300 x 4096 x 24576 47, 40, 42, 42, 44.
     uint32_t best = kMostCols, cost = 0xFFFFFFFFu;
-    for (uint32_t cols = kMostCols; cols >= 128; cols -= 32) {
+    for (uint32_t cols = kMostCols; cols >= min(max((a.m + 31) / 32 * 32, 64u), 128u); cols -= 32) {
         const uint32_t tiles = (a.m + cols - 1) / cols * ((a.n + 2 * kRows - 1) / (2 * kRows)), c = (tiles + kPairs - 1) / kPairs * (cols + 64);
         if (c < cost) {
             best = cols;

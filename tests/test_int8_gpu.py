@@ -81,6 +81,11 @@ def test_product_of_few_rows(dtype, m, k, n):
     check_product(np.random.default_rng(m * k * n), dtype, m, k, n, with_addend=bool(n % 2), pitch=n % 3)
 
 
+@pytest.mark.parametrize("m,k,n", [(8, 1040, 2380), (3, 80, 2369), (8, 576, 7001), (5, 1104, 7120), (1, 4096, 2368), (8, 1024, 2368)])
+def test_product_of_few_rows_by_many_columns(m, k, n):
+    check_product(np.random.default_rng(m * k * n), "bf16", m, k, n)
+
+
 @pytest.mark.parametrize("m,k,n", [(17, 64, 31), (33, 160, 65), (64, 4096, 200), (100, 1536, 130), (128, 128, 128), (129, 144, 257), (203, 1536, 300), (255, 2048, 127), (257, 528, 640),
                                    (300, 16, 300), (700, 1040, 90)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
