@@ -32,9 +32,9 @@ constexpr int kExtra = 2;                                // blocks of keys that 
 // Blocks of keys of a piece: with fewer the join of the parts takes longer than the blocks.  1, 2, 3, 4: one token over 8000 cached 25.7, 23.1, 21.8, 19.9 us, two
 // over 3000 19.0, 16.3, 17.4, 17.1, four of nine heads of 64 over up to 500 9.5, 9.8, 10.5, 11.7.
 constexpr uint32_t kLeastBlocks = 3;
-// The portion of a prompt by itself, and few sequences of many rows on average whose tables end early, are the other kernel's, those of a few tokens among them, too:
-// a launch of this one costs more than it saves (32 heads on 8 of 128, with it and without: 40 tokens over 500 32.2 and 25.4 us, 512 over none 37.6 and 30.6, four of 100
-// over 1000 45.7 and 38.6, three single tokens over 8000 beside 128 85.7 and 67.9), but for single tokens that are long (three over 32000 beside 512: 103 and 126).
+// Few sequences of many rows on average, a prompt's portion by itself among them, are the other kernel's, those of a few tokens too: a launch of this one costs more
+// than it saves (32 heads on 8 of 128, with it and without: 40 tokens over 500 32.2 and 25.4 us, 512 over none 37.6 and 30.6, four of 100 over 1000 45.7 and 38.6, three
+// single tokens over 8000 beside 128 85.7 and 67.9), but for single tokens that are long (three over 32000 beside 512: 103 and 126), which short tables rule out.
 constexpr uint32_t kFewSequences = 4, kManyRows = 32, kShortTables = 16384;
 constexpr float kRoom = 8.f;
 constexpr int kUp = 7;                                   // weights are 2^kUp times what they should be: 2^15 at most, and all of their bits down to 2^-21 of the largest
@@ -665,7 +665,7 @@ int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8
     a.parts = reinterpret_cast<float *>(a.heads + 2 * decode8_ctas(a.d));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (pairs <= kDecode8Pairs || !prefill8_takes(a)) return launch_decode8(a, dtype, pairs, s);
-    const bool alone = sequences == 1 || (sequences <= kFewSequences && rows >= kManyRows * sequences && (unsigned long long)table_width * page_size <= kShortTables);
+    const bool alone = sequences <= kFewSequences && rows >= kManyRows * sequences && (sequences == 1 || (unsigned long long)table_width * page_size <= kShortTables);
     if (!alone) {
         a.rows_to = kDecode8Pairs;
         if (int rc = launch_decode8(a, dtype, kDecode8Pairs, s)) return rc;

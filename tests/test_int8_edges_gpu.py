@@ -80,6 +80,34 @@ def test_queries_that_are_not_finite_stay_in_their_head_and_row(dtype, fresh):
     assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 128), (9, 3, 64), (8, 1, 256)])
+@pytest.mark.parametrize("fresh", [[1] * 6, [3, 1, 2, 5, 1, 4], [90, 1, 40, 3, 150, 33], [70, 65, 40, 33]])
+def test_attention_of_rows_that_see_nothing_and_of_lengths_that_cannot_be(dtype, heads, kv_heads, d, fresh):
+    """Sequences with fewer tokens than new ones, with none, longer than their table, and the last one's rows cut off behind the rows that are there."""
+    rng = np.random.default_rng(heads * d + len(fresh))
+    q, k, v, ks, vs, table, starts, lengths = attention_inputs(rng, dtype, heads, kv_heads, d, 32, 16, [200, 40, 0, 9, 64, 7][:len(fresh)], fresh)
+    lengths[0], lengths[1], lengths[2] = 0, 10 ** 9, max(1, fresh[2] - 1)
+    table[1, :] = np.arange(table.shape[1])
+    starts[-1] += 50
+    check_attention(dtype, q, k, v, ks, vs, table, starts, lengths, most=max(fresh))
+    check_attention(dtype, q, k, v, ks, vs, table, starts, np.zeros_like(lengths), most=max(fresh))
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,fresh", [(300, 1, 64, 1), (300, 1, 32, 5), (600, 2, 16, 2), (256, 1, 128, 3), (34, 2, 128, 2)])
+def test_attention_of_very_many_heads_per_key_head(heads, kv_heads, d, fresh):
+    rng = np.random.default_rng(heads + fresh)
+    check_attention("bf16", *attention_inputs(rng, "bf16", heads, kv_heads, d, 32, 32, [300, 0, 31], [fresh] * 3))
+
+
+@pytest.mark.parametrize("sequences", [1500, 4096])
+def test_attention_of_very_many_sequences(sequences):
+    rng = np.random.default_rng(sequences)
+    fresh = rng.integers(0, 3, sequences)
+    fresh[7] = 40
+    check_attention("f16", *attention_inputs(rng, "f16", 4, 2, 64, 16, 16, rng.integers(0, 20, sequences), fresh, rows=int(fresh.sum()) + 3))
+
+
 @pytest.mark.parametrize("most", [2, 40])
 def test_a_captured_attention_follows_the_lengths(most):
     """One graph, replayed with sequences of other lengths and numbers of new tokens, beside another graph of the same operator."""

@@ -107,6 +107,12 @@ def test_product_of_more_tiles_than_fit_at_once(m, k, n):
         assert (np.abs(got[rows] - want) <= product_bound("f32", want, None)).all()
 
 
+@pytest.mark.parametrize("m,k,n", [(128, 5120, 700), (300, 5120, 1000), (500, 5120, 1000), (700, 5120, 900), (1000, 5120, 1000), (1000, 5120, 1100), (1500, 2064, 100), (90, 4096, 1600),
+                                   (150, 64, 20000), (250, 64, 29000), (600, 528, 6000), (600, 336, 4000), (48, 64, 40000), (10, 32, 40000), (96, 144, 38016), (64, 48, 38100), (100, 5120, 9000)])
+def test_product_of_every_width_and_split(m, k, n):
+    check_product(np.random.default_rng(m * k + n), "bf16", m, k, n, with_addend=bool(n % 200))
+
+
 @pytest.mark.parametrize("m", [1, 9, 40, 300])
 def test_product_at_the_largest_k(m):
     check_product(np.random.default_rng(m), "f32", m, 131056, 70, extreme=True)
