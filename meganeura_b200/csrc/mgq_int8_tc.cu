@@ -7,8 +7,9 @@
 // pair_kernel: many tiles.  Two CTAs of a cluster share tiles of 256 weight rows by `tn` activation rows (cta_group::2): each holds its 128 weight rows and half of
 // the activation rows, and has its 128 rows' sums in its TMEM.  One CTA's copies would fill and feed its shared memory at 192 bytes per cycle with 128 x 256
 // tiles, a pair needs 128.  Persistent, one accumulator is read while the other is filled.
-// 2048 x 4096 by 12288 columns: 69 to 77 us, 2.7 to 3.0 POP/s where products alone from shared memory ran at 4.33.  Operands out of L2 bound it: 8192 cubed took 425 us and
-// without its loads 306.  Stages of 256 k, and smaller tiles for the last round alone, gave nothing.
+// 2048 x 4096 by 12288 columns: 69 to 82 us, 2.5 to 3.0 POP/s.  Power bounds it: codes of all the range hold the clock at 1.26 to 1.45 of 1.97 GHz, and 8192 cubed
+// takes 390 us (2.8 POP/s); with operands of zeros the same instructions take 250 (4.40), as fast as products alone out of shared memory (4.33).  So stages of 256 k, tiles of
+// 256 x 512, which read a quarter less from L2 (405 us), and smaller tiles for the last round gave nothing.
 //   warp 0      TMA of this CTA's boxes, completing on full[s] of the pair's first CTA
 //   warp 1      (first CTA) issues the products, and gives stages and accumulators to both CTAs
 //   warps 2-9   epilogue: 32 rows by every other 32 columns each
