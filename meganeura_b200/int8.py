@@ -37,10 +37,16 @@ def quantize_rows(x, out=None, stream=None):
         _refuse(device, codes=(out[0], _i8, (rows, k)), scales=(out[1], _f32, (rows,)))
 
     def call(sp):
-        codes, scales = (torch.empty((rows, k), dtype=_i8, device=x.device), torch.empty(rows, dtype=_f32, device=x.device)) if out is None else out
+        codes, scales = (x.new_empty((rows, k), dtype=_i8), x.new_empty(rows, dtype=_f32)) if out is None else out
         check(lib.mgq_quantize_rows(x.data_ptr(), _FORMATS[dtype], pitch, codes.data_ptr(), scales.data_ptr(), rows, k, sp))
         return codes, scales
     return _on(device, stream, call)
+
+
+def _result_pitch(name: str, t, dtype, device: int, m: int, n: int) -> int:
+    if t.dtype is not dtype or t.shape != (m, n):
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {(m, n)}, not {tuple(t.shape)} {t.dtype}")
+    return _pitch(name, t, device, n)
 
 
 def matmul_int8(a, a_scales, w, w_scales, addend=None, out=None, dtype=None, stream=None):
@@ -57,18 +63,16 @@ def matmul_int8(a, a_scales, w, w_scales, addend=None, out=None, dtype=None, str
         _refuse(device, a=(a, _i8, (m, k)), w=(w, _i8, (n, k)), a_scales=(a_scales, _f32, (m,)), w_scales=(w_scales, _f32, (n,)))
     if dtype is None:
         dtype = out.dtype if out is not None else addend.dtype if addend is not None else torch.bfloat16
-    if dtype not in _FORMATS:
+    form = _FORMATS.get(dtype)
+    if form is None:
         raise ValueError(f"the result must be float32, float16 or bfloat16, not {dtype}")
-    for name, t in (("out", out), ("addend", addend)):
-        if t is not None and (t.dtype is not dtype or t.shape != (m, n)):
-            raise ValueError(f"{name} must be a {dtype} tensor of shape {(m, n)}, not {tuple(t.shape)} {t.dtype}")
-    add_pitch = 0 if addend is None else _pitch("addend", addend, device, n)
-    out_pitch = n if out is None else _pitch("out", out, device, n)
+    out_pitch = n if out is None else _result_pitch("out", out, dtype, device, m, n)
+    add_pitch = 0 if addend is None else _result_pitch("addend", addend, dtype, device, m, n)
 
     def call(sp):
-        o = torch.empty((m, n), dtype=dtype, device=a.device) if out is None else out
+        o = a.new_empty((m, n), dtype=dtype) if out is None else out
         check(lib.mgq_matmul_int8(a.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), None if addend is None else addend.data_ptr(), o.data_ptr(),
-                                  _FORMATS[dtype], m, k, n, add_pitch, out_pitch, sp))
+                                  form, m, k, n, add_pitch, out_pitch, sp))
         return o
     return _on(device, stream, call)
 
@@ -77,13 +81,14 @@ def _caches(k_cache, v_cache, k_scales, v_scales):
     device, shape = k_cache.get_device(), k_cache.shape
     if device < 0:
         raise ValueError("a paged cache lives on the GPU; the library has no CPU path")
-    if len(shape) != 4 or not (_is(k_cache, _i8, device, shape) and _is(v_cache, _i8, device, shape)):
+    if len(shape) != 4 or k_cache.dtype is not _i8 or not (k_cache.is_contiguous() and _is(v_cache, _i8, device, shape)):
         raise ValueError("k_cache and v_cache must be alike: contiguous int8 [pages, page_size, kv_heads, head_dim] on one device")
-    pages, page_size, kv_heads, _ = shape
+    pages, page_size, kv_heads, d = shape
     blocks = k_scales.shape[1] if k_scales.dim() == 3 else 0
-    if blocks < 1 or page_size % blocks or not (_is(k_scales, _f32, device, (pages, blocks, kv_heads)) and _is(v_scales, _f32, device, (pages, blocks, kv_heads))):
+    scales = (pages, blocks, kv_heads)
+    if blocks < 1 or page_size % blocks or not (_is(k_scales, _f32, device, scales) and _is(v_scales, _f32, device, scales)):
         raise ValueError(f"k_scales and v_scales must be alike: contiguous float32 [{pages}, page_size / block, {kv_heads}] on cuda:{device}")
-    return device, *shape, page_size // blocks
+    return device, pages, page_size, kv_heads, d, page_size // blocks
 
 
 def paged_append_int8(q, k, v, positions, slots, k_cache, v_cache, k_scales, v_scales, theta: float = 0.0, q_out=None, q_dtype=None, stream=None):
@@ -108,7 +113,7 @@ def paged_append_int8(q, k, v, positions, slots, k_cache, v_cache, k_scales, v_s
         _refuse(device, q_out=(q_out, dst, (rows, heads, d)))
 
     def call(sp):
-        out = None if q is None else torch.empty((rows, heads, d), dtype=dst, device=k_cache.device) if q_out is None else q_out
+        out = None if q is None else k_cache.new_empty((rows, heads, d), dtype=dst) if q_out is None else q_out
         check(lib.mgq_paged_append_int8(None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), _FORMATS[src], positions.data_ptr(), slots.data_ptr(),
                                         None if out is None else out.data_ptr(), _HALF[dst], k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                                         rows, heads, kv_heads, d, q_pitch, k_pitch, v_pitch, page_size, pages, block, theta, sp))
@@ -139,8 +144,8 @@ def paged_attention_int8(q, k_cache, v_cache, k_scales, v_scales, table, starts,
         raise ValueError("out must have the shape and the type of q")
 
     def call(sp):
-        o = torch.zeros((rows, heads, d), dtype=dtype, device=q.device) if out is None else out
-        room = torch.empty(_attention_workspace(heads, kv_heads, d, most), dtype=torch.uint8, device=q.device)
+        o = q.new_zeros((rows, heads, d)) if out is None else out
+        room = q.new_empty(_attention_workspace(heads, kv_heads, d, most), dtype=torch.uint8)
         check(lib.mgq_paged_attention_int8(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), _HALF[dtype], table.data_ptr(),
                                            starts.data_ptr(), lengths.data_ptr(), o.data_ptr(), sequences, rows, most, heads, kv_heads, d, page_size, pages, block, width,
                                            q_pitch, _pitch("out", o, device, heads * d), d ** -0.5 if scale is None else scale, window, room.data_ptr(), sp))
