@@ -32,10 +32,14 @@ constexpr int kExtra = 2;                                // blocks of keys that 
 // Blocks of keys of a piece: with fewer the join of the parts takes longer than the blocks.  1, 2, 3, 4: one token over 8000 cached 25.7, 23.1, 21.8, 19.9 us, two
 // over 3000 19.0, 16.3, 17.4, 17.1, four of nine heads of 64 over up to 500 9.5, 9.8, 10.5, 11.7.
 constexpr uint32_t kLeastBlocks = 3;
-// Few sequences of many rows on average, a prompt's portion by itself among them, are the other kernel's, those of a few tokens too: a launch of this one costs more
-// than it saves (32 heads on 8 of 128, with it and without: 40 tokens over 500 32.2 and 25.4 us, 512 over none 37.6 and 30.6, four of 100 over 1000 45.7 and 38.6, three
-// single tokens over 8000 beside 128 85.7 and 67.9), but for single tokens that are long (three over 32000 beside 512: 103 and 126), which short tables rule out.
-constexpr uint32_t kFewSequences = 4, kManyRows = 32, kShortTables = 16384;
+// Which kernels serve more than kDecode8Pairs pairs.  The one for many tokens takes 20 us for the least, this one as long as it reads and joins: it takes everything where the
+// units, by what the tables let them read, are little work (kLittle: units of 16 pairs times keys, kPlace more for each), and no sequence has so many units that finding one's place
+// among them takes long (kMostUnits).  32 heads on 8 of 128, all here and all there, us: 9 tokens over 300 18.3 and 23.2, 40 over 1500 25.9 and 25.9, 12 times 9 over 1500 43.7 and 43.9, 12
+// times 40 over 300 49.9 and 32.5, 200 over 1500 59.3 and 34.2; 8 on 1, 500 over none 39.9 and 26.3.
+// Else each kernel takes its sequences, but where most have many tokens and none can be long the other one takes all, as a launch of this one costs more than it saves (12 times
+// 40 over 300 39.3 and 32.5, three single tokens over 8000 beside 128 85.7 and 67.9); single tokens over long sequences are slow there (three over 32000 beside 512 103 and 126).
+constexpr unsigned long long kLittle = 175000, kPlace = 100, kShort = 32768;
+constexpr uint32_t kMostUnits = 64, kManyRows = 32;
 constexpr float kRoom = 8.f;
 constexpr int kUp = 7;                                   // weights are 2^kUp times what they should be: 2^15 at most, and all of their bits down to 2^-21 of the largest
 
@@ -665,7 +669,10 @@ int launch_paged_attention_int8(const void *q, const int8_t *k_cache, const int8
     a.parts = reinterpret_cast<float *>(a.heads + 2 * decode8_ctas(a.d));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (pairs <= kDecode8Pairs || !prefill8_takes(a)) return launch_decode8(a, dtype, pairs, s);
-    const bool alone = sequences <= kFewSequences && rows >= kManyRows * sequences && (sequences == 1 || (unsigned long long)table_width * page_size <= kShortTables);
+    const unsigned long long reach = (unsigned long long)table_width * page_size, units = ((unsigned long long)rows * a.group / 16 + sequences) * kv_heads;
+    if (max_fresh <= kMostUnits * max(16 / a.group, 1u) && units <= kLittle / (reach + kPlace)) return launch_decode8(a, dtype, pairs, s);
+    const bool many = (unsigned long long)rows * a.group > (unsigned long long)kDecode8Pairs * sequences;
+    const bool alone = many && (sequences * reach <= kShort || (sequences == 1 && rows >= kManyRows));
     if (!alone) {
         a.rows_to = kDecode8Pairs;
         if (int rc = launch_decode8(a, dtype, kDecode8Pairs, s)) return rc;

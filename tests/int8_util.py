@@ -40,6 +40,11 @@ def attention_bound(dtype, want, size, reach, d, floor=0.0):
     return EPS[dtype] / 2 * np.abs(want) + np.minimum(weight, 1.0)[..., None] * size + (2.0 ** -25 if dtype == "f16" else 1e-30) + 2.0 ** -29 * floor
 
 
+def wider(table, page, reach):
+    """A table that goes on to `reach` tokens, which no sequence has: what the tables allow has a say in which kernels run."""
+    return np.concatenate([table, np.full((len(table), max(0, reach // page - table.shape[1])), -1, table.dtype)], 1)
+
+
 def check_attention(dtype, q, k, v, ks, vs, table, starts, lengths, scale=None, window=0, out=None, most=None, spread=None):
     """The operator on these inputs against the restatement; rows that belong to nobody against what was there before."""
     import torch
@@ -50,16 +55,23 @@ def check_attention(dtype, q, k, v, ks, vs, table, starts, lengths, scale=None, 
     before = host(out).copy()
     d = [torch.from_numpy(x).cuda() for x in (k, v, ks, vs)]
     most = most or max(1, int(np.diff(starts).max()))
-    ops.paged_attention_int8(q, *d, words(table), words(starts), words(lengths), most, scale=scale, window=window, out=out)
+    page = k.shape[1]
     want, size, reach = PO.attention(host(q), IO.values(k, ks), IO.values(v, vs), table, starts, lengths, scale, window)
     nobody = np.isnan(want).all((1, 2)) & (np.arange(len(want)) >= min(int(starts[-1]), len(want)))
-    got = host(out)
-    assert np.array_equal(got[nobody], before[nobody])
-    got, want = got[~nobody], want[~nobody]
-    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{np.isnan(got).sum()} NaN, {np.isnan(want).sum()} wanted"
+    want = want[~nobody]
     fine = ~np.isnan(want)
-    off, bound = np.abs(got - want)[fine], attention_bound(dtype, want, size[~nobody], reach[~nobody], q.shape[2], int(max(lengths)) * 127.0 * vs[np.isfinite(vs)].max())[fine]
-    assert np.isfinite(got[fine]).all()
-    worst = (off - bound).max() if off.size else 0
-    assert worst <= 0, f"off by {off.max():.3g}, {(off / bound).max():.2f} times the bound"
+    bound = attention_bound(dtype, want, size[~nobody], reach[~nobody], q.shape[2], int(max(lengths)) * 127.0 * vs[np.isfinite(vs)].max())[fine]
+    tables = [table]
+    if max(lengths) <= table.shape[1] * page and most * (q.shape[1] // k.shape[2]) > 32:      # more than one kernel may take them, and together
+        tables = [wider(table, page, 2 ** 20), wider(table, page, 2 ** 15 // len(table)), table]
+    for t in tables:
+        ops.paged_attention_int8(q, *d, words(t), words(starts), words(lengths), most, scale=scale, window=window, out=out)
+        got = host(out)
+        assert np.array_equal(got[nobody], before[nobody])
+        got = got[~nobody]
+        assert np.array_equal(np.isnan(got), np.isnan(want)), f"{np.isnan(got).sum()} NaN, {np.isnan(want).sum()} wanted"
+        off = np.abs(got - want)[fine]
+        assert np.isfinite(got[fine]).all()
+        worst = (off - bound).max() if off.size else 0
+        assert worst <= 0, f"off by {off.max():.3g}, {(off / bound).max():.2f} times the bound"
     return got

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from int8_util import attention_bound, attention_inputs, cache_of, check_attention
+from int8_util import attention_bound, attention_inputs, cache_of, check_attention, wider
 from oracle import int8_oracle as IO
 from oracle import paged_oracle as PO
 from paged_util import EPS, host, torch_type, words
@@ -39,9 +39,10 @@ def test_a_cache_of_more_than_4_gib(fresh):
     for t, want in ((ks, scales[0]), (vs, scales[1])):
         assert np.array_equal(host(t[held]), want)
     q = torch.from_numpy(rng.standard_normal((fresh, 32, d)).astype(np.float32)).cuda().to(torch.bfloat16)
-    got = ops.paged_attention_int8(q, k, v, ks, vs, words(table), words([0, fresh]), words([length]), fresh)
     want, size, reach = PO.attention(host(q), IO.values(codes[0], scales[0]), IO.values(codes[1], scales[1]), np.arange(4)[None], [0, fresh], [length], d ** -0.5)
-    assert (np.abs(host(got) - want) <= attention_bound("bf16", want, size, reach, d, length * 5.0)).all()
+    for t in (table, wider(table, page, 2 ** 20)):
+        got = ops.paged_attention_int8(q, k, v, ks, vs, words(t), words([0, fresh]), words([length]), fresh)
+        assert (np.abs(host(got) - want) <= attention_bound("bf16", want, size, reach, d, length * 5.0)).all()
 
 
 def test_products_into_rows_that_are_far_apart():
@@ -63,12 +64,13 @@ def test_products_into_rows_that_are_far_apart():
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("fresh", [1, 4, 70])
-def test_queries_that_are_not_finite_stay_in_their_head_and_row(dtype, fresh):
+@pytest.mark.parametrize("fresh,far", [(1, 0), (4, 0), (70, 0), (70, 2 ** 20), (70, 2 ** 14)])
+def test_queries_that_are_not_finite_stay_in_their_head_and_row(dtype, fresh, far):
     import torch
     from meganeura_b200 import ops
     rng = np.random.default_rng(fresh)
     q, k, v, ks, vs, table, starts, lengths = attention_inputs(rng, dtype, 8, 2, 64, 16, 16, [300, 40], [fresh, fresh])
+    table = wider(table, 16, far)
     args = [*(dev(x) for x in (k, v, ks, vs)), *(words(x) for x in (table, starts, lengths)), fresh]
     clean = host(ops.paged_attention_int8(q, *args))
     spoilt = q.clone()
@@ -92,6 +94,7 @@ def test_attention_of_rows_that_see_nothing_and_of_lengths_that_cannot_be(dtype,
     starts[-1] += 50
     check_attention(dtype, q, k, v, ks, vs, table, starts, lengths, most=max(fresh))
     check_attention(dtype, q, k, v, ks, vs, table, starts, np.zeros_like(lengths), most=max(fresh))
+    check_attention(dtype, q, k, v, ks, vs, table, starts, np.minimum(lengths, 30), most=max(fresh))
 
 
 @pytest.mark.parametrize("heads,kv_heads,d,fresh", [(300, 1, 64, 1), (300, 1, 32, 5), (600, 2, 16, 2), (256, 1, 128, 3), (34, 2, 128, 2)])
@@ -108,8 +111,8 @@ def test_attention_of_very_many_sequences(sequences):
     check_attention("f16", *attention_inputs(rng, "f16", 4, 2, 64, 16, 16, rng.integers(0, 20, sequences), fresh, rows=int(fresh.sum()) + 3))
 
 
-@pytest.mark.parametrize("most", [2, 40])
-def test_a_captured_attention_follows_the_lengths(most):
+@pytest.mark.parametrize("most,far", [(2, 0), (40, 0), (40, 2 ** 13), (40, 2 ** 20)])
+def test_a_captured_attention_follows_the_lengths(most, far):
     """One graph, replayed with sequences of other lengths and numbers of new tokens, beside another graph of the same operator."""
     import torch
     from meganeura_b200 import ops
@@ -118,7 +121,7 @@ def test_a_captured_attention_follows_the_lengths(most):
     k, ks = cache_of(rng, pages, page, block, 2, 64)
     v, vs = cache_of(rng, pages, page, block, 2, 64)
     d = [dev(x) for x in (k, v, ks, vs)]
-    table = rng.permutation(pages)[:S * 40].reshape(S, 40)
+    table = wider(rng.permutation(pages)[:S * 40].reshape(S, 40), page, far)
     q = torch.from_numpy(rng.standard_normal((rows, 8, 64)).astype(np.float32)).cuda().half()
     starts, lengths = words(np.zeros(S + 1)), words(np.zeros(S))
     outs = [torch.zeros_like(q) for _ in range(2)]
