@@ -307,9 +307,9 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
 
 /* 8-bit integers with scales in f32: a value is code * scale, codes -127 to 127.
  *
- * mgq_quantize_rows: rows of x (f32, f16 or bf16, `pitch` elements apart) as codes[rows, k] and scales[rows]: with top = max |x| of a row, scale = top / 127
- *   (0 where top < 2^-100) and code = x * (1 / scale) rounded to the nearest whole number, ties to even, every step in f32.  A row with an infinity or NaN has
- *   codes of 0 and a scale that is not finite, so its values are NaN.  Weights [n, k] are quantized with it, too, a scale per channel.
+ * mgq_quantize_rows: rows of x (f32, f16 or bf16, `pitch` elements apart) as codes[rows, k] and scales[rows]: with top = max |x| of a row, scale = top * (1 / 127)
+ *   (0 where top < 2^-100) and code = x * (1 / scale) rounded to the nearest whole number, ties to even, every step (1 / 127 too) rounded to f32.  A row with an
+ *   infinity or NaN has codes of 0 and a scale that is not finite, so its values are NaN.  Weights [n, k] are quantized with it, too, a scale per channel.
  * mgq_matmul_int8: out[m, n] = (sum over k of a[m, k] * w[n, k]) * a_scales[m] * w_scales[n] (+ addend[m, n]).  The sum is exact in 32 bits, so k is at most
  *   MGQ_INT8_MAX_K (codes of -128 included), the rest f32, rounded once to `dtype`, the type of out and addend (f32, f16 or bf16), whose rows are
  *   `pitch` elements apart.  k a multiple of 16, a and w dense and on 16 bytes.  out may be addend.

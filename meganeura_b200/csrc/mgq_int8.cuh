@@ -8,10 +8,11 @@ namespace mgq {
 
 // Rows and blocks whose largest magnitude is below are zeros: their scale's inverse would leave f32's range.
 constexpr float kLeast = 0x1p-100f;
-// From the largest magnitude's bit pattern.  Both divisions are rounded to nearest: the same scale and codes as the same formulas anywhere else.
-__device__ __forceinline__ float scale_of(uint32_t top) { return __uint_as_float(top) < kLeast ? 0.f : __uint_as_float(top) / 127.f; }
+// From the largest magnitude's bit pattern.  A 127th is a product with 1/127 as f32 rounds it, which is how torch divides a tensor by a number on the GPU (a true quotient is another
+// in 4 % of the rows, by 2^-24, which some codes near a tie show); the inverse is rounded to nearest.  So scale and codes are the same as those of the same formulas there.
+__device__ __forceinline__ float scale_of(uint32_t top) { return __uint_as_float(top) < kLeast ? 0.f : __uint_as_float(top) * (1.f / 127.f); }
 __device__ __forceinline__ float inverse_of(float scale) { return scale > 0.f && scale < INFINITY ? 1.f / scale : 0.f; }
-// Four values, in units of their scale, to the nearest whole numbers; NaN is 0.  At most 127 * (1 + 3 * 2^-24) comes in, so nothing is cut off.
+// Four values, in units of their scale, to the nearest whole numbers; NaN is 0.  At most 127 * (1 + 4 * 2^-24) comes in, so nothing is cut off.
 __device__ __forceinline__ uint32_t codes_of(float x, float y, float z, float w)
 {
     uint32_t v;

@@ -1,4 +1,4 @@
-"""Rows of 8-bit codes and paged caches of them, restated in numpy: one row, block and head at a time, in 64 bits but for the scales, whose f32 divisions are
+"""Rows of 8-bit codes and paged caches of them, restated in numpy: one row, block and head at a time, in 64 bits but for the scales, whose f32 roundings are
 part of the definition (a code is the rounding of a quotient by the scale that is stored)."""
 import numpy as np
 
@@ -7,7 +7,7 @@ LEAST = np.float32(2.0 ** -100)
 
 def scale_of(top):
     top = np.float32(top)
-    return np.float32(0) if top < LEAST else np.float32(top / np.float32(127))
+    return np.float32(0) if top < LEAST else np.float32(top * (np.float32(1) / np.float32(127)))
 
 
 def inverse_of(scale):

@@ -85,7 +85,7 @@ def test_rows_come_back_within_half_a_code():
     x = (rng.standard_normal((9, 333)) * np.exp2(rng.integers(-90, 100, (9, 1)))).astype(np.float32)
     x[3] = 0
     codes, scales = IO.quantize_rows(x)
-    # half a code, and the roundings of scale, inverse and product: 3 * 2^-24 of up to 127 codes
+    # half a code, and the roundings of 1/127 (half as much), scale, inverse and product: 3.5 * 2^-24 of up to 127 codes
     assert (np.abs(codes * scales[:, None].astype(np.float64) - x) <= scales[:, None] * (0.5 + 127 * 4 * 2.0 ** -24)).all()
     assert (np.abs(codes).max(1) == np.where(scales > 0, 127, 0)).all() and scales[3] == 0
 

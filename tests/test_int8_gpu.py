@@ -45,6 +45,17 @@ def test_quantize_rows_that_are_zero_tiny_huge_or_not_finite():
     assert scales[2] == 0 and scales[7] > 0 and np.isnan(scales[4]) and np.isinf(scales[5:7]).all() and codes[8, 1] == 0
 
 
+def test_codes_and_scales_are_those_of_the_formulas_in_torch():
+    """On the GPU, where torch divides by a number with a product: a large product of f32 rows may not show a code that fell to the other side of a tie."""
+    import torch
+    from meganeura_b200 import ops
+    x = torch.randn(2000, 4096, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    codes, scales = ops.quantize_rows(x)
+    scale = x.abs().amax(1) / 127
+    assert torch.equal(scales, scale)
+    assert torch.equal(codes.float(), (x * (1 / scale)[:, None]).round())
+
+
 # ---------------------------------------------------------------------------------------------- products
 
 def product_bound(dtype, want, addend):
