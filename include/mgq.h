@@ -312,7 +312,8 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
  *   infinity or NaN has codes of 0 and a scale that is not finite, so its values are NaN.  Weights [n, k] are quantized with it, too, a scale per channel.
  * mgq_matmul_int8: out[m, n] = (sum over k of a[m, k] * w[n, k]) * a_scales[m] * w_scales[n] (+ addend[m, n]).  The sum is exact in 32 bits, so k is at most
  *   MGQ_INT8_MAX_K (codes of -128 included), the rest f32, rounded once to `dtype`, the type of out and addend (f32, f16 or bf16), whose rows are
- *   `pitch` elements apart.  k a multiple of 16, a and w dense and on 16 bytes.  out may be addend.
+ *   `pitch` elements apart.  k a multiple of 16, a and w dense and on 16 bytes.  out may be addend, row by
+ *   row (the same pitch).
  *
  * Paged caches of such codes: k_cache, v_cache [pages][page_size][kv_heads][head_dim] with k_scales, v_scales [pages][page_size / block][kv_heads], a scale for `block`
  * consecutive tokens of a page and a head (block a power of two from 16 to page_size, head_dim a multiple of 16, pages * page_size below 2^31, caches

@@ -182,6 +182,8 @@ int mgq_matmul_int8(const int8_t *a, const float *a_scales, const int8_t *w, con
     if (m == 0 || m >= (1u << 31) || n == 0 || n >= (1u << 31)) return fail(MGQ_ERR_SHAPE, "matmul_int8: %u rows, %u columns", m, n);
     if (k == 0 || k % 16 || k > MGQ_INT8_MAX_K) return fail(MGQ_ERR_SHAPE, "matmul_int8: k = %u is not a multiple of 16 up to %d", k, MGQ_INT8_MAX_K);
     if (out_pitch < n || (addend && addend_pitch < n)) return fail(MGQ_ERR_SHAPE, "matmul_int8: rows %u and %u apart are shorter than %u", out_pitch, addend_pitch, n);
+    // rows that lie elsewhere as an addend than as a result would be written before others have read them
+    if (addend == out && m > 1 && addend_pitch != out_pitch) return fail(MGQ_ERR_SHAPE, "matmul_int8: an addend in place has rows %u apart, the result %u", addend_pitch, out_pitch);
     if (odd(a, 16) || odd(w, 16) || odd(out, element(dtype)) || odd(addend, element(dtype)) || odd_words(a_scales, w_scales))
         return fail(MGQ_ERR_ALIGN, "matmul_int8: misaligned pointer (codes begin on 16 bytes)");
     return launch_matmul_int8(a, a_scales, w, w_scales, addend, out, dtype, m, k, n, addend_pitch, out_pitch, stream);

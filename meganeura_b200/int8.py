@@ -53,7 +53,8 @@ def matmul_int8(a, a_scales, w, w_scales, addend=None, out=None, dtype=None, str
     """(a @ w.T) * a_scales[:, None] * w_scales (+ addend), the product in whole numbers (mgq_matmul_int8).
 
     a: [m, k] int8 codes of activations, a_scales: [m] float32; w: [n, k] int8, w_scales: [n] float32, as quantize_rows writes them.  k: a multiple
-    of 16.  The result [m, n] has the type of out or addend or `dtype` (bfloat16 where none is given); out and addend have one type and rows any distance apart.
+    of 16.  The result [m, n] has the type of out or addend or `dtype` (bfloat16 where none is given); out and addend have one type and rows any distance apart; out may be
+    addend.
     """
     device = a.get_device()
     if device < 0 or a.dim() != 2 or w.dim() != 2:
