@@ -310,7 +310,8 @@ __global__ void __launch_bounds__(threads<D, NP>(), ctas_per_sm<D>()) decode8_ke
 #pragma unroll
             for (int i = 0; i < kGroups; i++) {
                 have[i] = step.have[i];
-                ks[i] = step.scale[sub][i][0];
+                // An infinite one becomes NaN: where codes are zeros the bias leaves a rest of either sign, and -infinity would be a key that has no weight.
+                ks[i] = fmaf(step.scale[sub][i][0], 0.f, step.scale[sub][i][0]);
                 vs[i] = step.scale[sub][i][1];
             }
             slot = slot == S - 1 ? 0 : slot + 1;

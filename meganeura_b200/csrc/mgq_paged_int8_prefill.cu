@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 if (!(ok = wait_all(&sh.sc_empty[b], (batch >> 1 & 1u) ^ 1u))) break;
                 if (kb < kb_end) {
                     const uint32_t i = lane / 8;
-                    const float f = a.scale_log2 * ks;
+                    const float f = a.scale_log2 * fmaf(ks, 0.f, ks);      // NaN where the scale is infinite: its keys must not have scores of -infinity
                     sh.factor[b][i][group] = f < 1e-36f ? 1e-36f : f;      // a scale of 0 must not make -inf NaN
                     const int up = -mine;                // vs * 2^up in two steps, as 2^up alone may be out of range
                     sh.weight[b][i][group] = vs * power_of(max(min(up, 100), -126)) * power_of(max(up - 100, 0));
