@@ -323,9 +323,10 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
  *   to the nearest.  So a block keeps what it holds until its first slot is written again.  Rows of one block stand one behind another, as the plan
  *   writes them; a value that is not finite makes the block's scale so and its values NaN, until it starts anew.  q_dtype: the type of q_out, f16 or bf16;
  *   sources are f32 or of that type.
- * mgq_paged_attention_int8: as mgq_paged_attention with keys and values code * scale; q and out are f16 or bf16 (dtype).  Scores and sums are f32, a weight times
- *   its block's scale is rounded to f16 before it meets its code, the result to its type.  Of the largest weight times the largest scale that the call meets for
- *   a head less than 2^-29 may be lost.  Scales are not negative, and values of more than 2^96 may come out infinite.  `workspace`:
+ * mgq_paged_attention_int8: as mgq_paged_attention with keys and values code * scale; q and out are f16 or bf16 (dtype).  Scores and sums are f32, the result is rounded to
+ *   its type.  Where a sequence has more than 32 new tokens times heads per key / value head (head_dim up to 128) a weight times its block's scale may be rounded to f16 before it
+ *   meets its code, half a step, 2^-11 of it; else 2^-22 of it is lost at most.  Of the largest weight times the largest scale that the call meets for a head less than
+ *   2^-29 may be lost.  Scales are not negative; of queries, keys and values beyond 2^96 results may be infinite or NaN.  `workspace`:
  *   mgq_paged_attention_int8_workspace(...) bytes, as there. */
 #define MGQ_INT8_MAX_K 131056
 int mgq_quantize_rows(const void *x, int dtype, uint32_t pitch, int8_t *codes, float *scales, uint32_t rows, uint32_t k, void *stream);

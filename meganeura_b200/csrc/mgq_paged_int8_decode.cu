@@ -4,11 +4,13 @@
 // A unit's pairs of token and head (8 or 16: heads of one key / value head share its keys) are the columns of m16n8k16 products in f16 whose rows are 16 keys of a
 // head (scores) or 16 of its dimensions (results): codes are the left operand of both, eight pairs cost no more than they are, and the accumulators of eight
 // pairs of 128 are 32 registers.  The order of k inside a product, and of the results' rows, is free, so a lane takes 16 consecutive codes of a key with one
-// load.  A biased byte code + 128 with a zero above it is an f16, subnormal and exact: (code + 128) 2^-24.  The bias is taken off by the tensor cores: scores
-// begin at -128 2^-24 times the sum of q, and behind each product of values comes one with -128 2^-24 in their place, so that no sum ever grows with the bias.
-// (Codes made whole by a subtraction per pair of them cost a seventh of the instructions, which are what this kernel has to save.)
+// load.  A biased byte code + 128 with a zero above it is an f16, subnormal and exact: (code + 128) 2^-24.  From the scores the bias is taken off by where their sums begin, at
+// -128 2^-24 times the sum of q; from values by a subtraction per pair of them, so that no sum ever grows with the bias.  (The same for keys would cost a
+// fourteenth of the instructions, which are what this kernel has to save.)
 // Scores: q enters as f16, times a power of two that bf16 rows need to fit its range; a row's is undone in f32 with the block's scale.  Weights: times the
-// block's scale, rounded to f16, 2^-12 of each is lost at most; the low parts of it as a second operand took 5 % longer.  They are relative to a maximum that may be
+// block's scale, as the sum of two f16, 2^-22 of each is lost at most, so that only the result is rounded (2-norm against 64 bits: f16 0.00020, bf16 0.0016, as the rounded exact result).
+// One f16 alone, 2^-11, left 0.00026 to 0.00031 in f16, and with the products of second parts taking the bias off instead of the subtraction 64 single tokens of the Qwen3-8B shape took
+// 51.9 and not 52.3 us, 32 times 1 to 5 54.0 and not 55.2.  Weights are relative to a maximum that may be
 // 2^8 too low (kRoom), and to a power of two of the blocks' scales (`e2`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from
 // the scores' layout to the right operand's are transposed 8 x 8 at a time (movmatrix).
 // Four warps of a CTA split a unit, and each takes 32 keys of a block at a time, from a ring that a fifth warp fills across the borders of units: a lane brings 16
@@ -81,8 +83,15 @@ __device__ __forceinline__ uint32_t transpose(uint32_t v)
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-constexpr uint32_t kBias = 0x80808080u;                  // of four bytes; as two f16 it reads -128 2^-24 twice
+constexpr uint32_t kBias = 0x80808080u;                  // of four bytes
 constexpr float kUnit = 0x1p-24f;                        // of the codes as operands
+// Two codes as operands without their bias, exact as well.
+__device__ __forceinline__ uint32_t unbiased(uint32_t v)
+{
+    const uint32_t bias = 0x00800080u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&bias));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 // 2^e for e from -126 to 127.
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -411,7 +420,7 @@ __global__ void __launch_bounds__(threads<D, NP>(), ctas_per_sm<D>()) decode8_ke
                     }
                 }
                 const float by = vs[i] * up1 * up2;
-                uint32_t weight[NP][2];
+                uint32_t weight[NP][2], low[NP][2];
 #pragma unroll
                 for (int n = 0; n < NP; n++)
 #pragma unroll
@@ -425,6 +434,8 @@ __global__ void __launch_bounds__(threads<D, NP>(), ctas_per_sm<D>()) decode8_ke
                         }
                         const __half2 both = __floats2half2_rn(w[0], w[1]);
                         weight[n][h] = transpose(*reinterpret_cast<const uint32_t *>(&both));
+                        const __half2 rest = __floats2half2_rn(w[0] - __low2float(both), w[1] - __high2float(both));
+                        low[n][h] = transpose(*reinterpret_cast<const uint32_t *>(&rest));
                     }
                 // values of the keys of rows 2 quad, 2 quad + 1, and eight on, dimensions row * kOwn on: a product's rows are two of them each
 #pragma unroll
@@ -447,16 +458,16 @@ __global__ void __launch_bounds__(threads<D, NP>(), ctas_per_sm<D>()) decode8_ke
                         // [a0 b0 a1 b1] and [a2 b2 a3 b3] of the keys a, b
                         const uint32_t x0 = __byte_perm(w[0][e], w[1][e], 0x5140) ^ kBias, x1 = __byte_perm(w[0][e], w[1][e], 0x7362) ^ kBias;
                         const uint32_t y0 = __byte_perm(w[2][e], w[3][e], 0x5140) ^ kBias, y1 = __byte_perm(w[2][e], w[3][e], 0x7362) ^ kBias;
-                        const uint32_t f[2][4] = {{__byte_perm(x0, 0, 0x4140), __byte_perm(x0, 0, 0x4342), __byte_perm(y0, 0, 0x4140), __byte_perm(y0, 0, 0x4342)},
-                                                  {__byte_perm(x1, 0, 0x4140), __byte_perm(x1, 0, 0x4342), __byte_perm(y1, 0, 0x4140), __byte_perm(y1, 0, 0x4342)}};
-                        const uint32_t off[4] = {kBias, kBias, kBias, kBias};
+                        const uint32_t f[2][4] = {
+                            {unbiased(__byte_perm(x0, 0, 0x4140)), unbiased(__byte_perm(x0, 0, 0x4342)), unbiased(__byte_perm(y0, 0, 0x4140)), unbiased(__byte_perm(y0, 0, 0x4342))},
+                            {unbiased(__byte_perm(x1, 0, 0x4140)), unbiased(__byte_perm(x1, 0, 0x4342)), unbiased(__byte_perm(y1, 0, 0x4140)), unbiased(__byte_perm(y1, 0, 0x4342))}};
 #pragma unroll
                         for (int n = 0; n < NP; n++)
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
                                 float (&acc)[4] = o[n][c * (kOwn / 2) + 2 * e + j];
                                 mma(acc, f[j], weight[n][0], weight[n][1]);
-                                mma(acc, off, weight[n][0], weight[n][1]);
+                                mma(acc, f[j], low[n][0], low[n][1]);
                             }
                     }
                 }
