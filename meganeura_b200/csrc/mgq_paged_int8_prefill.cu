@@ -15,8 +15,8 @@
 //   warp 11         scales, two batches of four blocks, and which keys exist
 //   warps 12-15     codes to operands in the 128-byte swizzle: eight lanes take two rows' opposite halves, so that neither loads nor stores meet in a bank
 // Sums are kept relative to a maximum that may be 2^7 too low (2^15 where it has grown since): only where a row's maximum grows by more is O scaled.  Exponents are
-// score * factor - m in one rounding; rows whose scores pass 2^20 round before they subtract, and their m is the maximum itself, so that its weight is 1
-// however large m is.
+// score * factor - m in one rounding; rows whose scores pass 2^20 (huge) round before they subtract, and their m is the maximum itself, so that its weight is that of a whole
+// exponent however large m is: 2^8, added behind the subtraction, where m of other rows is the maximum less 8.
 // 4 x 2048 tokens over up to 6144, 32 heads of 128 on 8: 603 us in bf16 (912 TFLOP/s of the 1715 that a library product reaches), 640 in f16.  A tile's chain from scores to
 // weights bounds it, beside shared memory, where codes are read and operands written, and the instruction cache: the twelve warps run four different programs, so the
 // softmax reads its scores in short loops, twice (straight through with 208 registers 736 us, in 16 columns at a time 660), and what masks or huge scores need is apart.
@@ -558,11 +558,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 if (plain) find_top(std::true_type());
                 else       find_top(std::false_type());
                 // Nothing to do where the maximum stays at or below m + kRoom (finite behind the first block); -inf and NaN come here, too.
-                const bool calm = top <= m + kRoom && top >= -FLT_MAX && drop == 1.f;
+                const float room = m + (huge ? kRoom - kUnder : kRoom);
+                const bool calm = top <= room && top >= -FLT_MAX && drop == 1.f;
                 if (__any_sync(0xffffffffu, !calm)) {
-                    const bool up = !(top <= m + kRoom) && top > -INFINITY;                 // also where m is still -inf
+                    const bool up = !(top <= room) && top > -INFINITY;                      // also where m is still -inf
+                    const bool was = huge;
                     huge |= up && fabsf(top) > kHuge;
-                    const float under = up ? (huge ? top : top - kUnder) : m, keep = up ? exp2_fast(m - under) : 1.f;
+                    const float under = up ? (huge ? top : top - kUnder) : m, keep = up ? exp2_fast(m - under + (huge && !was ? kUnder : 0.f)) : 1.f;
                     l *= keep;
                     m = under;
                     if (kb != begin && __any_sync(0xffffffffu, up || drop != 1.f)) {
@@ -589,14 +591,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                         mask(simple, s, w);
                         float2 f = of_groups(simple, factors, w, 1.f);
                         const float2 v = of_groups(simple, by, w, 0.f);
-                        if (!decltype(simple)::value && scaled) {            // their products with the factors are rounded first, so that the maximum's weight is 1 however large m is
+                        pair_t minus = bases;
+                        if (!decltype(simple)::value && scaled) {            // the products with the factors are rounded first, so that the maximum's weight is 2^8 however large m is
+                            const float lift = huge ? kUnder : 0.f;
 #pragma unroll
-                            for (int e = 0; e < 32; e++) s[e] = __fmul_rn(s[e], e < 16 ? f.x : f.y);
+                            for (int e = 0; e < 32; e++) s[e] = __fadd_rn(__fadd_rn(__fmul_rn(s[e], e < 16 ? f.x : f.y), base), lift);
                             f = make_float2(1.f, 1.f);
+                            minus = 0;
                         }
                         pair_t e[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) e[i] = pair_fma(pair_of(s[2 * i], s[2 * i + 1]), i < 8 ? pair_of(f.x, f.x) : pair_of(f.y, f.y), bases);
+                        for (int i = 0; i < 16; i++) e[i] = pair_fma(pair_of(s[2 * i], s[2 * i + 1]), i < 8 ? pair_of(f.x, f.x) : pair_of(f.y, f.y), minus);
                         if (w < 3) tmem_ld_quarter(s_at + 32 * w + 32, s);
                         uint32_t p[16];
 #pragma unroll
@@ -621,6 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill8_kernel(const __grid_cons
                 signal(&sh.p_full[tile]);
             }
             finish();
+            if (huge) {                                  // sums and O are relative to m again, as parts are joined
+                l *= 1.f / (1 << (int)kUnder);
+                power *= 1.f / (1 << (int)kUnder);
+            }
             if (tile * kTile < pairs) {
                 // 128 bytes of eight rows at a time, turned so that a store covers whole lines of few rows
                 const bool alone = g.first && g.last;

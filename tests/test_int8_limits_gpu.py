@@ -2,10 +2,10 @@
 import numpy as np
 import pytest
 
-from int8_util import attention_bound, attention_inputs, check_attention
+from int8_util import attention_bound, attention_inputs, check_attention, wider
 from oracle import int8_oracle as IO
 from oracle import paged_oracle as PO
-from paged_util import host, words
+from paged_util import EPS, host, words
 
 pytestmark = pytest.mark.gpu
 
@@ -45,6 +45,49 @@ def test_results_of_few_tokens_are_rounded_once(dtype, heads, kv_heads, d, cache
     bound = attention_bound(dtype, want, size, reach, d, int(max(lengths)) * 127.0 * vs.max()) + (2.0 ** -22 - 2.0 ** -11) * size
     off = np.abs(got - want)
     assert (off <= bound).all(), f"off by {off.max():.3g}, {(off / bound).max():.2f} times the bound"
+
+
+def exact_scale(exponent):
+    """An f32 whose product with log2(e), as f32 rounds it, is 2^exponent."""
+    log2e, x = np.float32(1.4426950408889634), np.float32(2.0 ** exponent / 1.4426950408889634)
+    for _ in range(8):
+        if x * log2e == np.float32(2.0 ** exponent):
+            return float(x)
+        x = np.nextafter(x, np.float32(np.inf) if x * log2e < 2.0 ** exponent else np.float32(0))
+    raise AssertionError("no such number")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("cached,largest,others", [(60, 40, [3, 7, 50]), (300, 200, [3, 190, 260]), (300, 2, [130, 131, 299]), (5000, 4000, [10, 3000, 4500])])
+@pytest.mark.parametrize("fresh", [1, 60])
+def test_what_huge_scores_may_lose(dtype, cached, largest, others, fresh):
+    """Scores beyond 2^20 whose largest belongs to a value of zeros: weights of 2^-22, 2^-24 and 2^-26 of it are all that is left.
+
+    Every score is exact: its exponent is 2^14 (c0 + c1 2^-13) for a key's first two codes.  Weights and scales are powers of two, so that only what the operator says may be
+    lost: 2^-29 of the largest weight times the largest scale, for the three keys that have a weight, a code being 127 at most; and the result's rounding, 2^-20 for the f32 sums.
+    """
+    from meganeura_b200 import ops
+    rng = np.random.default_rng(cached)
+    q, k, v, ks, vs, table, starts, lengths = attention_inputs(rng, dtype, 2, 1, 64, 16, 16, [cached], [fresh])
+    q[:] = 0
+    q[..., 0], q[..., 1] = 1, 2.0 ** -13
+    k[:], ks[:], vs[:] = 0, 1, 4
+    at = lambda i: (table[0, i // 16], i % 16)
+    k[at(largest)][:, 0] = 100
+    v[at(largest)] = 0
+    want = np.zeros(64)
+    for i, key in enumerate(others):
+        k[at(key)][:, :2] = 100, -11 - i
+        want += 4.0 * v[at(key)][0] * 2.0 ** (-22 - 2 * i)
+    bound = (EPS[dtype] / 2 + 2.0 ** -20) * np.abs(want) + (2.0 ** -25 if dtype == "f16" else 0) + 3 * 2.0 ** -29 * 127 * 4
+    caches = [dev(x) for x in (k, v, ks, vs)]
+    for t in (table, wider(table, 16, 2 ** 15), wider(table, 16, 2 ** 20)):      # which kernels serve it depends on how far the table reaches
+        got = host(ops.paged_attention_int8(q, *caches, *(words(x) for x in (t, starts, lengths)), fresh, scale=exact_scale(14)))
+        off = np.abs(got - want)
+        assert (off <= bound).all(), f"off by {off.max():.3g}, {(off / bound).max():.2f} times the bound"
+    # beside rows whose scores are small
+    q[::2, 0, 0] = 2.0 ** -14
+    check_attention(dtype, q, k, v, ks, vs, table, starts, lengths, scale=exact_scale(14))
 
 
 def test_no_wait_ran_out():
