@@ -591,7 +591,7 @@ int launch_sized(const Attend8Args &a, const Maps &maps, bool wide, uint32_t pai
     if (int rc = allow_smem(kernel, smem_bytes<D, NP>())) return rc;
     MGQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     if (int rc = launch(kernel, dim3(ctas), dim3(threads<D, NP>()), smem_bytes<D, NP>(), stream, maps, a, wide)) return rc;
-    return launch_merge<T, 8 * NP * H>(a, ctas, H * pairs, stream);
+    return launch_merge<T, 8 * NP * H>(a, ctas, H * min(pairs, 8u * NP), stream);      // no unit has more; `pairs` may be any bound
 }
 
 template <typename T, int H>

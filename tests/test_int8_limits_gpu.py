@@ -90,6 +90,19 @@ def test_what_huge_scores_may_lose(dtype, cached, largest, others, fresh):
     check_attention(dtype, q, k, v, ks, vs, table, starts, lengths, scale=exact_scale(14))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (4, 2, 128), (6, 3, 64), (8, 1, 256)])
+@pytest.mark.parametrize("most", [2 ** 29, 2 ** 30, 2 ** 31, 2 ** 32 - 1])
+def test_a_bound_of_new_tokens_that_is_far_too_large(heads, kv_heads, d, most):
+    """Times the heads of a unit it passes 32 bits; rows off 16 bytes, so that the kernel of few tokens takes the call."""
+    import torch
+    rng = np.random.default_rng(d)
+    q, k, v, ks, vs, *rest = attention_inputs(rng, "bf16", heads, kv_heads, d, 32, 16, [900, 40], [5, 1])
+    wide = torch.zeros(q.shape[0], heads * d + 3, dtype=q.dtype, device="cuda")
+    view = wide[:, 1:1 + heads * d].unflatten(1, (heads, d))
+    view.copy_(q)
+    check_attention("bf16", view, k, v, ks, vs, *rest, out=torch.zeros_like(wide)[:, 1:1 + heads * d].unflatten(1, (heads, d)), most=most)
+
+
 def test_no_wait_ran_out():
     from meganeura_b200 import ops
     ops.device_status()
