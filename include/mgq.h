@@ -320,8 +320,8 @@ int mgq_paged_attention(const void *q, const void *k_cache, const void *v_cache,
  * on 16 bytes).  Pages, tables, slots and steps are those of the paged operators above, whose words and limits hold here as well.
  * mgq_paged_append_int8: as mgq_paged_append, for one block and head at a time: old = 0 if the block's first slot is among the rows, else its scale; scale =
  *   max(old, scale of the new rows' largest); the new rows' codes, and where the scale grew those of the slots that are not written, code * (old / scale)
- *   to the nearest.  So a block keeps what it holds until its first slot is written again.  Rows of one block stand one behind another, as the plan
- *   writes them; a value that is not finite makes the block's scale so and its values NaN, until it starts anew.  q_dtype: the type of q_out, f16 or bf16;
+ *   to the nearest.  So a block keeps what it holds until its first slot is written again.  Rows of one block may stand anywhere among the rows (one
+ *   behind another, as the plan writes them, is faster); a value that is not finite makes the block's scale so and its values NaN, until it starts anew.  q_dtype: the type of q_out, f16 or bf16;
  *   sources are f32 or of that type.
  * mgq_paged_attention_int8: as mgq_paged_attention with keys and values code * scale; q and out are f16 or bf16 (dtype).  Scores and sums are f32, the result is rounded to
  *   its type.  Where a sequence has more than 32 new tokens times heads per key / value head (head_dim up to 128) a weight times its block's scale may be rounded to f16 before it

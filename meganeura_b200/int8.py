@@ -96,7 +96,7 @@ def paged_append_int8(q, k, v, positions, slots, k_cache, v_cache, k_scales, v_s
     """Rows of keys (rotated where theta > 0) and values into a cache of 8-bit codes, and the rotated queries (mgq_paged_append_int8).
 
     As paged_append, but for the caches: int8 codes [pages, page_size, kv_heads, head_dim] and float32 scales [pages, page_size / block, kv_heads], updated
-    together.  Rows of one block of tokens stand one behind another, as in a PagedStep.  q, k, v: float32, float16 or bfloat16; returns
+    together.  Rows may stand in any order; fastest is a PagedStep's, where those of one block of tokens stand one behind another.  q, k, v: float32, float16 or bfloat16; returns
     q_out [rows, heads, head_dim], float16 or bfloat16 (q_dtype; the sources' type or bfloat16 where neither is given).
     """
     device, pages, page_size, kv_heads, d, block = _caches(k_cache, v_cache, k_scales, v_scales)

@@ -2,10 +2,10 @@
 import numpy as np
 import pytest
 
-from int8_util import attention_bound, attention_inputs, check_attention, wider
+from int8_util import attention_bound, attention_inputs, cache_of, check_attention, wider
 from oracle import int8_oracle as IO
 from oracle import paged_oracle as PO
-from paged_util import EPS, host, words
+from paged_util import EPS, block_table, host, words
 
 pytestmark = pytest.mark.gpu
 
@@ -101,6 +101,52 @@ def test_a_bound_of_new_tokens_that_is_far_too_large(heads, kv_heads, d, most):
     view = wide[:, 1:1 + heads * d].unflatten(1, (heads, d))
     view.copy_(q)
     check_attention("bf16", view, k, v, ks, vs, *rest, out=torch.zeros_like(wide)[:, 1:1 + heads * d].unflatten(1, (heads, d)), most=most)
+
+
+def orders(rng, rows):
+    """Ways in which a step's rows may stand: mixed, from the last to the first, as every seventh, one behind another but for the first, with pauses."""
+    yield rng.permutation(rows)
+    yield np.arange(rows)[::-1]
+    yield np.argsort(np.arange(rows) % 7, kind="stable")
+    yield np.roll(np.arange(rows), -1)
+    yield np.insert(np.arange(rows), np.sort(rng.integers(0, rows + 1, rows // 3 + 1)), -1)
+
+
+@pytest.mark.parametrize("kv_heads,d,page,block,cached,fresh", [
+    (2, 64, 16, 16, [3], [2]),
+    (2, 64, 32, 16, [0, 15, 40, 7, 16], [40, 1, 33, 2, 16]),
+    (8, 128, 64, 64, [10, 0, 63, 100], [300, 64, 1, 500]),
+    (1, 256, 32, 16, [5, 0], [700, 90]),
+    (3, 16, 1024, 1024, [0, 1000, 20], [1500, 30, 900]),
+    (2, 48, 256, 128, [1] * 50, [3] * 50),
+    (2, 32, 16, 16, [9] * 1500, [2] * 1500),
+])
+def test_append_of_rows_in_any_order(kv_heads, d, page, block, cached, fresh):
+    """Codes and scales are those of the rows in order, and the restatement's, wherever the rows of a block stand."""
+    import torch
+    from meganeura_b200 import ops
+    rng = np.random.default_rng(d * page + len(cached))
+    total = np.asarray(cached) + np.asarray(fresh)
+    pages = int(sum(-(-n // page) for n in total)) + 2
+    table = block_table(rng, total, page, pages)
+    slots = np.concatenate([table[s, np.arange(c, c + n) // page] * page + np.arange(c, c + n) % page for s, (c, n) in enumerate(zip(cached, fresh))])
+    positions, rows = np.concatenate([np.arange(c, c + n) for c, n in zip(cached, fresh)]), len(slots)
+    x = (rng.standard_normal((2, rows, kv_heads, d)) * np.exp(rng.standard_normal((1, rows, 1, 1)))).astype(np.float32)
+    before = [cache_of(rng, pages, page, block, kv_heads, d) for _ in range(2)]
+
+    def append(order, theta):
+        at = np.where(order < 0, 0, order)
+        c, s = [dev(b[0]) for b in before], [dev(b[1]) for b in before]
+        ops.paged_append_int8(None, dev(x[0, at]), dev(x[1, at]), words(positions[at]), words(np.where(order < 0, -1, slots[at])), *c, *s, theta=theta)
+        return [host(t) for t in (*c, *s)]
+
+    want = [IO.append(*b, y, slots) for b, y in zip(before, x)]
+    rotated = append(np.arange(rows), 1e4)
+    for order in orders(rng, rows):
+        got = append(order, 0.0)
+        for i in range(2):
+            assert np.array_equal(got[i], want[i][0]) and np.array_equal(got[2 + i], want[i][1])
+        assert all(np.array_equal(a, b) for a, b in zip(append(order, 1e4), rotated))
 
 
 def test_no_wait_ran_out():
