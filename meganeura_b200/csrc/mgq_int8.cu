@@ -8,7 +8,7 @@ namespace {
 // scale = max |x| / 127, code = rint(x / scale).  One pass over HBM: a CTA takes a row and keeps it in registers as it was read, 8 values a thread and step, up to
 // kHold steps (16384 values at 512 threads); what lies behind is read again, from L2.  The largest magnitude is found among the bit patterns without their
 // sign, whose order is that of the magnitudes with NaN above infinity, so that one that is not finite makes the scale so.
-// 2048 x 12288 in bf16: 11.2 us, 6.7 TB/s (HBM and L2); 8 x 4096: 1.8 us in a graph, a launch.
+// 2048 x 12288 in bf16: 13.8 us from HBM, 5.5 TB/s, 11.2 where L2 holds the rows; 8 x 4096: 1.9 us in a graph, a launch.
 constexpr int kHold = 4;
 constexpr uint32_t kMostThreads = 512;
 

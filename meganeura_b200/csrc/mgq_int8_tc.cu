@@ -8,7 +8,7 @@
 // the activation rows, and has its 128 rows' sums in its TMEM.  One CTA's copies would fill and feed its shared memory at 192 bytes per cycle with 128 x 256
 // tiles, a pair needs 128.  Persistent, one accumulator is read while the other is filled.
 // 2048 x 4096 by 12288 columns: 69 to 82 us, 2.5 to 3.0 POP/s.  Power bounds it: codes of all the range hold the clock at 1.26 to 1.45 of 1.97 GHz, and 8192 cubed
-// takes 390 us (2.8 POP/s); with operands of zeros the same instructions take 250 (4.40), as fast as products alone out of shared memory (4.33).  So stages of 256 k, tiles of
+// takes 340 to 390 us (2.8 to 3.2 POP/s); with operands of zeros the same instructions take 250 (4.40), as fast as products alone out of shared memory (4.33).  So stages of 256 k, tiles of
 // 256 x 512, which read a quarter less from L2 (405 us), and smaller tiles for the last round gave nothing.
 //   warp 0      TMA of this CTA's boxes, completing on full[s] of the pair's first CTA
 //   warp 1      (first CTA) issues the products, and gives stages and accumulators to both CTAs

@@ -35,7 +35,7 @@ struct AttendArgs {
     const uint32_t *starts, *lengths, *table;
     uint32_t sequences, rows, kv_heads, group, d, page_shift, pages, table_width, window, q_pitch, out_pitch;
     uint32_t rows_from, rows_to;         // sequences with this many pairs of token and head of a key / value head are this kernel's
-    uint32_t least;                      // key blocks of a piece, unless there is only one piece (0: one)
+    uint32_t least;                      // cost of a piece (Walk::cost: key blocks and EXTRA per unit), unless there is only one piece (0: any)
     float scale_log2;                    // scale * log2(e): scores are exponents of 2
     struct PartHead *heads;              // [CTAs][2]
     float *parts;                        // [CTAs][2]: sums [ROWS][d], then maximum and weight of each row [ROWS][2]

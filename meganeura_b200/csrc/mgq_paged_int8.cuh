@@ -14,8 +14,8 @@ struct Attend8Args : AttendArgs {
 // Few new tokens per sequence (mgq_paged_int8_decode.cu).
 uint32_t decode8_ctas(uint32_t head_dim);
 constexpr uint32_t kDecode8Rows = 32;                      // of a unit, at most
-// Pairs of a sequence that is not yet many tokens': 32 sequences of the Qwen3-8B shape with 32 pairs take 96 us with the kernel for few tokens and 117 with the other,
-// with 48 pairs 131 and 120.
+// Pairs of a sequence that is not yet many tokens': 32 sequences of the Qwen3-8B shape with 32 pairs take 90 us with the kernel for few tokens and 97 with the other,
+// with 48 pairs 131 and 98.
 constexpr uint32_t kDecode8Pairs = 32;
 int launch_decode8(const Attend8Args &a, int dtype, uint32_t pairs, cudaStream_t stream);    // pairs: a bound of a sequence's tokens * heads per key / value head
 

@@ -4,21 +4,20 @@
 // A unit's pairs of token and head (8 or 16: heads of one key / value head share its keys) are the columns of m16n8k16 products in f16 whose rows are 16 keys of a
 // head (scores) or 16 of its dimensions (results): codes are the left operand of both, eight pairs cost no more than they are, and the accumulators of eight
 // pairs of 128 are 32 registers.  The order of k inside a product, and of the results' rows, is free, so a lane takes 16 consecutive codes of a key with one
-// load.  A biased byte code + 128 with a zero above it is an f16, subnormal and exact: (code + 128) 2^-24.  From the scores the bias is taken off by where their sums begin, at
-// -128 2^-24 times the sum of q; from values by a subtraction per pair of them, so that no sum ever grows with the bias.  (The same for keys would cost a
-// fourteenth of the instructions, which are what this kernel has to save.)
+// load.  A biased byte code + 128 with a zero above it is an f16, subnormal and exact: (code + 128) 2^-24.  From the scores the bias is taken off by where their sums
+// begin, at -128 2^-24 times the sum of q; from values by a subtraction per pair of them, so that no sum ever grows with the bias.  (The same for keys would
+// cost a fourteenth of the instructions, which are what this kernel has to save.)
 // Scores: q enters as f16, times a power of two that bf16 rows need to fit its range; a row's is undone in f32 with the block's scale.  Weights: times the
-// block's scale, as the sum of two f16, 2^-22 of each is lost at most, so that only the result is rounded (2-norm against 64 bits: f16 0.00020, bf16 0.0016, as the rounded exact result).
-// One f16 alone, 2^-11, left 0.00026 to 0.00031 in f16, and with the products of second parts taking the bias off instead of the subtraction 64 single tokens of the Qwen3-8B shape took
-// 51.9 and not 52.3 us, 32 times 1 to 5 54.0 and not 55.2.  Weights are relative to a maximum that may be
-// 2^8 too low (kRoom), and to a power of two of the blocks' scales (`e2`) which rises when a larger scale comes; sums of weights are f32.  Weights that move from
-// the scores' layout to the right operand's are transposed 8 x 8 at a time (movmatrix).
+// block's scale, as the sum of two f16, 2^-22 of each is lost at most, so that only the result is rounded (2-norm against 64 bits: f16 0.00020, bf16 0.0016, as the rounded
+// exact result).  One f16 alone, 2^-11, left 0.00026 to 0.00031 in f16; with a product of the bias in the place of the second part's and of the subtraction 64 single tokens of the
+// Qwen3-8B shape took as long and 32 times 1 to 5 3 % less.  Weights are relative to a maximum that may be 2^8 too low (kRoom), and to a power of two of the blocks' scales (`e2`)
+// which rises when a larger scale comes; sums of weights are f32.  Weights that move from the scores' layout to the right operand's are transposed 8 x 8 at a time (movmatrix).
 // Four warps of a CTA split a unit, and each takes 32 keys of a block at a time, from a ring that a fifth warp fills across the borders of units: a lane brings 16
 // keys or values with a TMA box and their scales with 4-byte copies.  (Where every warp filled its own, that was a quarter of its instructions: 64 single
 // tokens of the Qwen3-8B shape took 117 us.)  At a unit's end the sums are joined in shared memory.
 // Heads of up to 128 in pairs (H = 2): a token's codes of one head are 128 bytes or less, a kilobyte apart, and HBM gives 5.0 TB/s of such pieces (107 us, as long without
 // any arithmetic).  So where it can be a unit is two neighbouring key / value heads, whose codes come in one box, and two warps work for either: 64 single tokens over
-// up to 8100 take 98 us, 5.5 TB/s with the join of the parts (5 us), 94 without any arithmetic.  32 times 1 to 5 tokens of four heads each over up to 4000 take 58:
+// up to 8100 take 97 us, 5.5 TB/s with the join of the parts (5 us), 94 without any arithmetic.  32 times 1 to 5 tokens of four heads each over up to 4000 take 58 to 62:
 // above 16 pairs two units read the same keys, and two warps of a scheduler do not hide each other's chains.
 #include <cstdint>
 
@@ -31,13 +30,14 @@ namespace {
 constexpr int kWarps = 4, kStep = 32;             // keys of a warp's step
 constexpr int kGroups = kStep / 16;                      // 16 keys lie in one page and one block
 constexpr int kExtra = 2;                                // blocks of keys that starting and ending a unit take as long as
-// Blocks of keys of a piece: with fewer the join of the parts takes longer than the blocks.  1, 2, 3, 4: one token over 8000 cached 25.7, 23.1, 21.8, 19.9 us, two
-// over 3000 19.0, 16.3, 17.4, 17.1, four of nine heads of 64 over up to 500 9.5, 9.8, 10.5, 11.7.
+// Cost of a piece, blocks of keys and kExtra for a unit: with less the join of the parts takes longer than the blocks.  1, 2, 3, 4: one token over 8000 cached 25.7, 23.1, 21.8, 19.9 us,
+// two over 3000 19.0, 16.3, 17.4, 17.1, four of nine heads of 64 over up to 500 9.5, 9.8, 10.5, 11.7.
 constexpr uint32_t kLeastBlocks = 3;
 // Which kernels serve more than kDecode8Pairs pairs.  The one for many tokens takes 20 us for the least, this one as long as it reads and joins: it takes everything where the
 // units, by what the tables let them read, are little work (kLittle: units of 16 pairs times keys, kPlace more for each), and no sequence has so many units that finding one's place
-// among them takes long (kMostUnits).  32 heads on 8 of 128, all here and all there, us: 9 tokens over 300 18.3 and 23.2, 40 over 1500 25.9 and 25.9, 12 times 9 over 1500 43.7 and 43.9, 12
-// times 40 over 300 49.9 and 32.5, 200 over 1500 59.3 and 34.2; 8 on 1, 500 over none 39.9 and 26.3.
+// among them takes long (kMostUnits).  32 heads on 8 of 128, all here and all there, us: 9 tokens over 300 19.7 and 23.3, 40 over 1500 26.2 and 26.0, 12 times 9 over 1500 45.8 and 44.5, 12
+// times 40 over 300 52.2 and 32.6, 200 over 1500 62.1 and 34.4; 8 on 1, 500 over none 41.0 and 26.8.  The tables' width is all that is known here of the lengths: with tables of 131072
+// tokens the first and the fourth of these take both kernels, 30 and 39.
 // Else each kernel takes its sequences, but where most have many tokens and none can be long the other one takes all, as a launch of this one costs more than it saves (12 times
 // 40 over 300 39.3 and 32.5, three single tokens over 8000 beside 128 85.7 and 67.9); single tokens over long sequences are slow there (three over 32000 beside 512 103 and 126).
 constexpr unsigned long long kLittle = 175000, kPlace = 100, kShort = 32768;

@@ -17,7 +17,7 @@
 // Sums are kept relative to a maximum that may be 2^7 too low (2^15 where it has grown since): only where a row's maximum grows by more is O scaled.  Exponents are
 // score * factor - m in one rounding; rows whose scores pass 2^20 (huge) round before they subtract, and their m is the maximum itself, so that its weight is that of a whole
 // exponent however large m is: 2^8, added behind the subtraction, where m of other rows is the maximum less 8.
-// 4 x 2048 tokens over up to 6144, 32 heads of 128 on 8: 603 us in bf16 (912 TFLOP/s of the 1715 that a library product reaches), 640 in f16.  A tile's chain from scores to
+// 4 x 2048 tokens over up to 6144, 32 heads of 128 on 8: 589 us in bf16 (932 TFLOP/s of the 1678 that a library product reaches), 587 in f16; over 16 bits 482.  A tile's chain from scores to
 // weights bounds it, beside shared memory, where codes are read and operands written, and the instruction cache: the twelve warps run four different programs, so the
 // softmax reads its scores in short loops, twice (straight through with 208 registers 736 us, in 16 columns at a time 660), and what masks or huge scores need is apart.
 // TMEM: S0, S1 (128 columns each, P in the first 64 of them), O0, O1.
